@@ -105,6 +105,15 @@ _SIGS = {
     "coli_hip_moe_forward_dev": ([_vp, _vp, _vp, _i], _i),
     "coli_hip_moe_forward": ([_vp, _f, _f, _i, _i32, _f, _i32], _i),
     "coli_hip_moe_last_union": ([_vp, _i32, _i32], _i),
+    "coli_hip_moe_last_balance_dev": ([_vp, _vp, _vp, _i, _vp, _vp, _vp], _i),
+    "coli_hip_lora_create": ([C.POINTER(_vp), _i, _i, _i, _i, _i, _i], _i),
+    "coli_hip_lora_free": ([_vp], None),
+    "coli_hip_lora_set_dev": ([_vp, _i, _vp, _vp, _i, C.c_float], _i),
+    "coli_hip_lora_gemm_dev": ([_tp, _vp, _vp, _vp, _i, _vp], _i),
+    "coli_hip_lora_grad_dev": ([_tp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp], _i),
+    "coli_hip_gemm_t_dev": ([_tp, _vp, _vp, _i], _i),
+    "coli_hip_balance_dev": ([_i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp], _i),
+    "coli_hip_balance_grad_dev": ([_i, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp], _i),
     "coli_hip_stream": ([_i], _vp),
     "coli_hip_tensor_upload_from_device": ([_tpp, _vp, _f, _u8, _i, _i, _i, _i, _i], _i),
     "coli_hip_fill_random_u8": ([_i, _vp, _sz, C.c_ulonglong], _i),

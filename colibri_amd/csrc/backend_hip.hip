@@ -99,6 +99,25 @@ int reserve(DevCtx *ctx, DevBuf *b, size_t bytes, int zero) {
     return 1;
 }
 
+// Grow-only device buffer whose outgrown allocations stay until shutdown: a
+// captured graph keeps the addresses it was captured with, and a larger call
+// after the capture must not free what a replay still reads and writes.
+int reserve_kept(DevCtx *ctx, DevBuf *b, size_t bytes, int zero) {
+    if (bytes <= b->cap) return 1;
+    if (b->p && ctx->n_outgrown == COLI_OUTGROWN) return 0;
+    const size_t want = std::max(bytes, 2 * b->cap) + 256;
+    void *p = nullptr;
+    if (!hip_check(hipMalloc(&p, want), "workspace allocation")) return 0;
+    if (zero && !hip_check(hipMemset(p, 0, want), "workspace clear")) {
+        (void)hipFree(p);
+        return 0;
+    }
+    if (b->p) ctx->outgrown[ctx->n_outgrown++] = b->p;
+    b->p = p;
+    b->cap = want;
+    return 1;
+}
+
 int reserve_pinned(DevCtx *ctx, PinBuf *b, size_t bytes) {
     if (bytes <= b->cap) return 1;
     if (b->h) {
@@ -187,8 +206,10 @@ extern "C" void coli_cuda_shutdown(void) {
         DevBuf *bufs[] = {&ctx->x, &ctx->h, &ctx->y, &ctx->g, &ctx->u, &ctx->partial, &ctx->sums,
                           &ctx->prob, &ctx->stage_w, &ctx->stage_s, &ctx->qdq, &ctx->flags,
                           &ctx->rslot, &ctx->rw, &ctx->tmp_tiles, &ctx->tmp_scales, &ctx->zeros,
-                          &ctx->split_cnt, &ctx->idot_y, &ctx->idot_sx};
+                          &ctx->split_cnt, &ctx->idot_y, &ctx->idot_sx, &ctx->lora_h, &ctx->lora_list,
+                          &ctx->gt, &ctx->bal, &ctx->bal_cnt};
         for (DevBuf *b : bufs) free_buf(b);
+        for (int k = 0; k < ctx->n_outgrown; k++) (void)hipFree(ctx->outgrown[k]);
         for (int f = 0; f < 4; f++) {
             free_buf(&ctx->frag[f].hi);
             free_buf(&ctx->frag[f].lo);
@@ -335,7 +356,8 @@ static int fill_tensor(DevCtx *ctx, ColiCudaTensor *t, const void *weights, cons
     }
     const uint8_t *wsrc_dev = w_on_device ? (const uint8_t *)weights : (const uint8_t *)ctx->stage_w.p;
     if (!hip_check(coli_launch_repack(t, wsrc_dev, ctx->stage_s.p, ctx->stream),
-                "tile repack"))
+                "tile repack") ||
+        !build_t_scales(ctx, t, true))
         return 0;
     return hip_check(hipStreamSynchronize(ctx->stream), "tile repack sync");
 }
@@ -493,6 +515,7 @@ extern "C" void coli_cuda_tensor_free(ColiCudaTensor *t) {
     if (t->sc) (void)hipFree(t->sc);
     if (t->desc) (void)hipFree(t->desc);
     if (t->sc_unit) (void)hipFree(t->sc_unit);
+    if (t->sct) (void)hipFree(t->sct);
     std::free(t);
 }
 

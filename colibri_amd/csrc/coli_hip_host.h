@@ -8,6 +8,8 @@
 #define COLI_PIPE_SLOTS 27
 // Batches larger than this run the grouped GEMM instead of the GEMV.
 #define COLI_GEMM_MIN_ROWS 32
+// Rows of one call of the adapter and input-gradient entry points.
+#define COLI_GRAD_MAX_ROWS 65535
 
 // The static scratch array behind coli_hip_pipe_gemm_noalloc (one copy per
 // device, held until the process ends): regions and the limits they imply.
@@ -30,6 +32,9 @@
 // larger then), the host's copy of one beside the transfer of another.
 #define COLI_PIECE_BYTES ((size_t)512 << 10)
 #define COLI_PIECES 32
+
+// Outgrown workspaces a device keeps (each at least doubles its buffer).
+#define COLI_OUTGROWN 256
 
 struct DevBuf {
     void *p = nullptr;
@@ -84,6 +89,11 @@ struct DevCtx {
     FragSet frag[4];                   // 0/1: inputs (int4 / fp4 order), 2/3: hidden rows
     int dense_set[2] = {0, 1};         // set the next coli_hip_gemm_run_dev reads, per order (gemm_prep)
     DevBuf pipe[COLI_PIPE_SLOTS];
+    // workspaces of the adapter, input-gradient and balance entry points
+    // (reserve_kept: outgrown ones live until shutdown)
+    DevBuf lora_h, lora_list, gt, bal, bal_cnt;
+    void *outgrown[COLI_OUTGROWN] = {};
+    int n_outgrown = 0;
     // pinned staging
     PinBuf host_x, host_y, host_prob, host_small;
     // this device's copy of the library's static scratch array (see
@@ -109,6 +119,7 @@ DevCtx *ctx_of(int device);
 int bind_ctx(DevCtx *ctx);
 int fault_injected(void);
 int reserve(DevCtx *ctx, DevBuf *b, size_t bytes, int zero);
+int reserve_kept(DevCtx *ctx, DevBuf *b, size_t bytes, int zero);
 int reserve_pinned(DevCtx *ctx, PinBuf *b, size_t bytes);
 void forget_emitted(DevCtx *ctx, const void *dst, size_t bytes);
 void note_group(DevCtx *ctx, int count, int total, double h2d, double ker, double d2h);
@@ -162,6 +173,17 @@ hipError_t coli_launch_weighted_sum_rows(float *out, const float *y, const float
                                          hipStream_t st);
 hipError_t coli_launch_sum_slots(float *dst, const float *slots, int n, int D, hipStream_t st);
 }
+
+// single-matrix products (expert.hip, gemm_t.hip)
+int tensor_computable(const ColiCudaTensor *t);
+int gemm_dev(DevCtx *ctx, ColiCudaTensor *t, float *y_dev, const float *x_dev, int S);
+int gemm_t_dev(DevCtx *ctx, ColiCudaTensor *t, float *dx, const float *dy, int S);
+int build_t_scales(DevCtx *ctx, ColiCudaTensor *t, bool update_only);
+// Counts and balance loss over router logits given as nch column-chunk
+// partials, chstride floats apart (balance.hip).
+int run_balance(DevCtx *ctx, const float *z, int nch, size_t chstride, const int *idx, const int *keff,
+                const uint8_t *mask, const int *off, int n, int T, int E, int K, int mode, float *loss, int *counts,
+                int *rows);
 
 // Expert path runner (expert.hip): one shared routine behind expert_group,
 // issue, expert_mlp, resident_issue and the MoE layer.

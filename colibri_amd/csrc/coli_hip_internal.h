@@ -46,6 +46,8 @@ struct ColiCudaTensor {
     size_t accounted;            // bytes charged to the device statistics
     struct ColiProb *desc;       // device: 64 descriptors, entry s-1 = this matrix on s rows
     void *sc_unit;               // fmt=2 int8-activation path: unit group scales (made on first use)
+    void *sct;                   // input gradients: scales by column group (made on first use, see gemm_t.hip)
+    int *sct_ge;                 // their column groups' exponents [4 nq], in the same allocation
     int e8_fold;                 // MXFP4: every e8m0 byte in [114, 140], so each e2m1 value times its
                                  // scale is a normal fp16 (the GEMM folds the scale into the operand)
 };

@@ -548,7 +548,7 @@ int frag_set_of(int kind, bool hidden) {
     return (hidden ? 2 : 0) + (kind == COLI_KIND_FP4 ? 1 : 0);
 }
 
-static int tensor_computable(const ColiCudaTensor *t) {
+int tensor_computable(const ColiCudaTensor *t) {
     if (!t) return 0;
     if (t->fmt == 4 && t->gs <= 0) return 0;   // c/backend_cuda.cu:1355-1359
     return t->fmt == 2 || t->fmt == 4 || t->fmt == 7;
@@ -1039,7 +1039,7 @@ static int gemm_run(DevCtx *ctx, ColiCudaTensor *t, float *y_dev, int S, const C
 }
 
 // y_dev[S, O] = x_dev[S, I] W^T on the stream (tensor already resident).
-static int gemm_dev(DevCtx *ctx, ColiCudaTensor *t, float *y_dev, const float *x_dev, int S) {
+int gemm_dev(DevCtx *ctx, ColiCudaTensor *t, float *y_dev, const float *x_dev, int S) {
     if (t->kind == COLI_KIND_GENERIC) {
         forget_emitted(ctx, y_dev, (size_t)S * t->O * sizeof(float));
         return hip_check(coli_launch_generic_i4(t, x_dev, t->I, y_dev, t->O, S, ctx->stream), "generic gemv");

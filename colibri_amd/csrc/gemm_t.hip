@@ -1,0 +1,486 @@
+// gemm_t.hip -- the input gradient of a resident projection: dx = dy W.
+//
+//   dx[s, i] = sum_o dy[s, o] n[o, i] sc[o, i / 32]
+//
+// The sum runs over O, along which the tiles hold one row a lane and the group
+// scales change, so neither the forward's operand layout nor its scaling of
+// results fits. Both are turned round in registers:
+//   * A wave takes half a tile quad, 64 columns: lane (o = lane % 16, c =
+//     lane / 16) loads dwords 2 h, 2 h + 1 of its 16 bytes, 8 nibbles of
+//     columns 64 h + 32 j + 8 c + t. An 8 x 8 nibble transpose among the eight
+//     lanes o % 8 (three exchanges: nibbles, bytes, halfwords with lanes ^1,
+//     ^2, ^4) makes t the lane and o % 8 the nibble; one exchange with lane ^8
+//     and one v_permlane32_swap then put o / 8 into lane bit 5 and the columns'
+//     j into lane bit 3. Lane l holds column 64 h + 32 (l / 8 % 2) + 16 r + 8 (l / 16 % 2)
+//     + l % 8 in register r, rows 8 (l / 32) + 0..7: the B operand of
+//     v_mfma_f32_32x32x16_f16. About 1.3 instructions a weight, no LDS.
+//   * A weight enters as n sc 2^-Eg in fp16 hi + lo, Eg the exponent of its
+//     column group's largest scale (exact for MXFP4, whose lo is zero and left
+//     out, and for int4 with fp16 scales; to 3 x 2^-22 with f32 scales, which
+//     enter as two fp16); dy as fp16 hi + lo under its row's exponent (2^-22). hi hi + hi lo + lo hi are summed in f32. The scales
+//     are kept a second time per tensor, by column group with eight rows' worth
+//     in 16 bytes (coli_t_scales, made on first use).
+#include "coli_hip_host.h"
+#include "coli_device.h"
+
+#include "coli_backend_abi.h"
+#include "coli_hip_ext.h"
+
+#include <algorithm>
+
+// Order of a lane's eight rows in the operands: the order the unpack leaves
+// nibbles in (int4: even ones, then odd ones).
+__host__ __device__ __forceinline__ int t_order(int int4, int e) { return !int4 ? e : e < 4 ? 2 * e : 2 * (e - 4) + 1; }
+
+// ---------------------------------------------------------------------------
+// scales by column group
+// ---------------------------------------------------------------------------
+// Workgroup q: the four column groups of tile quad q. sct[plane][4 q + j][octet]
+// holds eight rows' scales times 2^-Eg (int4: odd rows also / 16, their nibbles
+// unpack as 16 n; plane 1: the rest that fp16 leaves of an f32 scale).
+template <int KIND>
+__global__ __launch_bounds__(256) void coli_t_scales(const void *__restrict__ sc, int nrt, int nq, int noct,
+                                                     _Float16 *__restrict__ sct, int *__restrict__ ge) {
+    __shared__ float mx[256];
+    __shared__ int es[4];
+    const int q = blockIdx.x, tid = threadIdx.x;
+    auto scale = [&](int o, int j) -> float {
+        if (o >= nrt * 16) return 0.0f;
+        const size_t at = ((size_t)(o >> 4) * nq + q) * 64 + (o & 15) * 4 + j;
+        if constexpr (KIND == COLI_KIND_I4_H) return (float)((const _Float16 *)sc)[at];
+        else if constexpr (KIND == COLI_KIND_I4_F) return ((const float *)sc)[at];
+        else return __uint_as_float((uint32_t)((const uint8_t *)sc)[at] << 23);
+    };
+    float m = 0.0f;
+    for (int e = tid; e < nrt * 64; e += 256) {
+        const float s = fabsf(scale(e >> 2, e & 3));   // e & 3 == tid & 3
+        if (s < INFINITY) m = fmaxf(m, s);
+    }
+    mx[tid] = m;
+    __syncthreads();
+    if (tid < 4) {
+        for (int k = tid; k < 256; k += 4) m = fmaxf(m, mx[k]);
+        int E = 0;
+        if (m > 0.0f) {
+            frexpf(m, &E);       // m in [2^(E-1), 2^E)
+            // int4: |16 n| (s / 16) <= 128 * 2^8; e2m1: 6 * 2^12
+            E -= KIND == COLI_KIND_FP4 ? 13 : 12;
+        }
+        es[tid] = E;
+        ge[4 * q + tid] = E;
+    }
+    __syncthreads();
+    const size_t plane = (size_t)nq * 4 * noct * 8;
+    for (int e = tid; e < 4 * noct * 8; e += 256) {
+        const int j = e / (noct * 8), k = e - j * noct * 8;
+        const int o = (k & ~7) + t_order(KIND != COLI_KIND_FP4, k & 7);
+        float s = ldexpf(scale(o, j), -es[j]);
+        if (KIND != COLI_KIND_FP4 && (o & 1)) s *= 0.0625f;
+        const _Float16 h = (_Float16)s;
+        const size_t at = ((size_t)4 * q + j) * noct * 8 + k;
+        sct[at] = h;
+        if constexpr (KIND == COLI_KIND_I4_F) sct[plane + at] = (_Float16)(s - (float)h);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// dy as fp16 hi + lo
+// ---------------------------------------------------------------------------
+// [octet of K][row][8]: a step's operand is contiguous over the rows. Four rows
+// a workgroup (a wave each), gridDim.y chunks of the columns; every chunk takes
+// the row's maximum for itself. max |v| 2^-E lies in [2^14, 2^15).
+__global__ __launch_bounds__(256) void coli_t_prep(const float *__restrict__ dy, int S, int K, int noct, int int4, int vec,
+                                                   size_t Sp, _Float16 *__restrict__ hi, _Float16 *__restrict__ lo,
+                                                   int *__restrict__ exps) {
+    const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= S) return;
+    const float *xr = dy + (size_t)row * K;
+    auto oct = [&](int o, float (&v)[8]) {
+        if (vec && 8 * o + 8 <= K) {
+            const floatx4 a = *GPTR(floatx4, xr + 8 * o), b = *GPTR(floatx4, xr + 8 * o + 4);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                v[i] = a[i];
+                v[4 + i] = b[i];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = 8 * o + i < K ? xr[8 * o + i] : 0.0f;
+        }
+    };
+    float m = 0.0f;
+#pragma unroll 4
+    for (int o = lane; 8 * o < K; o += 64) {
+        float v[8];
+        oct(o, v);
+#pragma unroll
+        for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(v[i]));
+    }
+    m = wave_max64(m);
+    int E = 0;
+    if (m > 0.0f && isfinite(m)) {
+        frexpf(m, &E);
+        E -= 15;
+    }
+    if (lane == 0 && blockIdx.y == 0) exps[row] = E;
+    const int per = ((noct + gridDim.y - 1) / gridDim.y + 63) & ~63, o1 = min(noct, (int)(blockIdx.y + 1) * per);
+#pragma unroll 2
+    for (int o = blockIdx.y * per + lane; o < o1; o += 64) {
+        float v[8];
+        oct(o, v);
+        half8v h, l;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float y = ldexpf(v[t_order(int4, e)], -E);
+            h[e] = (_Float16)y;
+            l[e] = (_Float16)(y - (float)h[e]);
+        }
+        *(half8v *)(hi + ((size_t)o * Sp + row) * 8) = h;
+        *(half8v *)(lo + ((size_t)o * Sp + row) * 8) = l;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// the product
+// ---------------------------------------------------------------------------
+struct GemmTArgs {
+    const uint8_t *w;            // tiles [nrt][nq]
+    const _Float16 *sct;
+    const int *ge;               // [4 nq]
+    const _Float16 *hi, *lo;     // [noct][Sp][8]
+    const int *exps;             // [S]
+    size_t Sp;
+    int nrt, nq, noct, I, S;
+    int splits, per;             // K split: steps of 32 rows of W each
+    float *out;                  // [splits][S][I]
+};
+
+// 8 x 8 nibble transpose among lanes l ^ 0..7 (nibble t of lane o -> nibble o of lane t).
+struct NibT {
+    uint32_t rot, keep, bsel, hsel;
+};
+__device__ __forceinline__ NibT nib_consts(int lane) {
+    NibT c;
+    c.rot = lane & 1 ? 4u : 28u;                      // rotate right by
+    c.keep = lane & 1 ? 0xF0F0F0F0u : 0x0F0F0F0Fu;
+    // perm(x, y): bytes 4-7 are x's
+    c.bsel = lane & 2 ? 0x07030501u : 0x02060004u;
+    c.hsel = lane & 4 ? 0x07060302u : 0x01000504u;
+    return c;
+}
+__device__ __forceinline__ uint32_t nib_transpose(uint32_t x, const NibT &c) {
+    uint32_t y = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xF, 0xF, false);        // lane ^ 1
+    y = __builtin_amdgcn_alignbit(y, y, c.rot);
+    x = (x & c.keep) | (y & ~c.keep);
+    y = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xF, 0xF, false);                 // lane ^ 2
+    x = __builtin_amdgcn_perm(x, y, c.bsel);
+    y = (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, 0x104, 0xF, 0x5, false);           // lane + 4
+    y = (uint32_t)__builtin_amdgcn_update_dpp((int)y, (int)x, 0x114, 0xF, 0xA, false);           // lane - 4
+    return __builtin_amdgcn_perm(x, y, c.hsel);
+}
+
+// The two dwords (columns 32 j + ...) of a lane as two B operands' nibbles.
+__device__ __forceinline__ void half_quad(uint32_t d0, uint32_t d1, const NibT &c, uint32_t &b0, uint32_t &b1) {
+    d0 = nib_transpose(d0, c);
+    d1 = nib_transpose(d1, c);
+    // lane bit 3 <-> register (lane ^ 8), then lane bit 5 <-> register
+    const uint32_t e0 = (uint32_t)__builtin_amdgcn_update_dpp((int)d0, (int)d1, 0x128, 0xF, 0xC, false);
+    const uint32_t e1 = (uint32_t)__builtin_amdgcn_update_dpp((int)d1, (int)d0, 0x128, 0xF, 0x3, false);
+    const auto r = __builtin_amdgcn_permlane32_swap(e0, e1, false, false);
+    b0 = r[0];
+    b1 = r[1];
+}
+
+// hi (and lo) of eight weights from their nibbles and scales.
+template <int KIND>
+__device__ __forceinline__ void t_weights(uint32_t nib, half8v s, half8v s2, half8v &hi, half8v &lo) {
+    const half8v n = unpack_b<KIND>(nib);
+    hi = n * s;   // (pairs: v_pk_mul_f16)
+    if constexpr (KIND == COLI_KIND_FP4) {
+        (void)lo;
+    } else {
+#pragma unroll
+        for (int p = 0; p < 4; p++) {
+            const half2v nn = {n[2 * p], n[2 * p + 1]}, ss = {s[2 * p], s[2 * p + 1]}, hh = {hi[2 * p], hi[2 * p + 1]};
+            half2v l = __builtin_elementwise_fma(nn, ss, -hh);   // exact: 15 bits less 11
+            if constexpr (KIND == COLI_KIND_I4_F) {
+                const half2v s2p = {s2[2 * p], s2[2 * p + 1]};
+                l = __builtin_elementwise_fma(nn, s2p, l);
+            }
+            lo[2 * p] = l[0];
+            lo[2 * p + 1] = l[1];
+        }
+    }
+}
+
+// Workgroup (64 WN columns, 32 MT rows, K split); WK wave groups share its K
+// steps (32 rows of W: two row tiles) and are joined in LDS at the end. A
+// step's dy octets are staged in LDS (two buffers), the weights and scales of
+// the next step are requested before this one's products.
+template <int KIND, int MT, int WN, int WK>
+__global__ __launch_bounds__(64 * WN * WK) void coli_gemm_t(GemmTArgs a) {
+    constexpr int BM = 32 * MT, NT = 64 * WN, CH = 8 * BM;   // 16-byte chunks of a step: 2 parts x 4 octets x BM rows
+    constexpr int CPT = (CH + NT - 1) / NT;
+    constexpr int STAGE = CH * 16;
+    constexpr int JOIN = WK > 1 ? 64 * WN * 16 * 4 : 0;       // one accumulator of every wave of a group
+    constexpr int LDS = 2 * WK * STAGE > JOIN ? 2 * WK * STAGE : JOIN;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[LDS];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave % WN, wk = wave / WN;
+    const int gt = tid - wk * NT;                              // thread within its K group
+    const int hq = blockIdx.x * WN + wn, q = min(hq >> 1, a.nq - 1), h = hq & 1;   // half-quad
+    const int row0 = blockIdx.y * BM;
+    const int k0 = blockIdx.z * a.per, k1 = min((a.noct + 3) / 4, k0 + a.per);
+    const int nstep = (k1 - k0 + WK - 1) / WK;
+    const NibT nc = nib_consts(lane);
+    const uint8_t *wp = a.w + (size_t)q * COLI_TILE_BYTES + lane * 16 + 8 * h;
+    const size_t wstride = (size_t)a.nq * COLI_TILE_BYTES;
+    const size_t plane = (size_t)a.nq * 4 * a.noct * 8;
+    // lane bit 3: the column group, lane bit 5: the octet of a row tile
+    const _Float16 *sp = a.sct + (((size_t)4 * q + 2 * h + (lane >> 3 & 1)) * a.noct + (lane >> 5)) * 8;
+    floatx16 acc[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int r = 0; r < 2; r++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) acc[m][r][i] = 0.0f;
+    u32x2 wd[2];
+    half8v sc[2], sc2[2];
+    u32x4 ad[CPT];
+    auto load_w = [&](int step) {
+        step = min(step, k1 - 1);
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const int rt = min(2 * step + t, a.nrt - 1);   // (past the last row tile: zero scales)
+            wd[t] = *GPTR(u32x2, wp + rt * wstride);
+            sc[t] = *GPTR(half8v, sp + (size_t)(4 * step + 2 * t) * 8);
+            if constexpr (KIND == COLI_KIND_I4_F) sc2[t] = *GPTR(half8v, sp + plane + (size_t)(4 * step + 2 * t) * 8);
+        }
+    };
+    auto load_a = [&](int step) {
+        step = min(step, k1 - 1);
+#pragma unroll
+        for (int i = 0; i < CPT; i++) {
+            const int c = min(gt + i * NT, CH - 1), part = c / (4 * BM), oct = c / BM % 4, r = c % BM;
+            ad[i] = *GPTR(u32x4, (part ? a.lo : a.hi) + ((size_t)(4 * step + oct) * a.Sp + row0 + r) * 8);
+        }
+    };
+    auto store_a = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < CPT; i++)
+            if (CH % NT == 0 || gt + i * NT < CH)
+                *(u32x4 *)(lds + (size_t)(buf * WK + wk) * STAGE + (size_t)(gt + i * NT) * 16) = ad[i];
+    };
+    load_a(k0 + wk);
+    load_w(k0 + wk);
+    store_a(0);
+    __syncthreads();
+    for (int it = 0; it < nstep; it++) {
+        const int step = k0 + it * WK + wk;
+        u32x2 w0[2];
+        half8v s0[2], s1[2];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            w0[t] = wd[t];
+            s0[t] = sc[t];
+            s1[t] = sc2[t];
+        }
+        load_a(step + WK);
+        load_w(step + WK);
+        if (step < k1) {
+            const uint8_t *as = lds + (size_t)((it & 1) * WK + wk) * STAGE;
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                uint32_t b[2];
+                half_quad(w0[t][0], w0[t][1], nc, b[0], b[1]);
+                half8v bh[2], bl[2];
+#pragma unroll
+                for (int r = 0; r < 2; r++) t_weights<KIND>(b[r], s0[t], s1[t], bh[r], bl[r]);
+                const uint8_t *ap = as + (size_t)((2 * t + (lane >> 5)) * BM + (lane & 31)) * 16;
+#pragma unroll
+                for (int m = 0; m < MT; m++) {
+                    const half8v ah = *(const half8v *)(ap + m * 32 * 16);
+                    const half8v al = *(const half8v *)(ap + (4 * BM + m * 32) * 16);
+#pragma unroll
+                    for (int r = 0; r < 2; r++) {
+                        acc[m][r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh[r], acc[m][r], 0, 0, 0);
+                        acc[m][r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh[r], acc[m][r], 0, 0, 0);
+                        if constexpr (KIND != COLI_KIND_FP4)
+                            acc[m][r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl[r], acc[m][r], 0, 0, 0);
+                    }
+                }
+            }
+        }
+        if (it + 1 < nstep) store_a((it + 1) & 1);
+        __syncthreads();
+    }
+    if constexpr (WK > 1) {
+        // groups 1 .. WK - 1 hand their sums to group 0 in turn
+        float *js = (float *)lds;
+        for (int g = 1; g < WK; g++)
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int r = 0; r < 2; r++) {
+                    if (wk == g)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) js[i * NT + gt] = acc[m][r][i];
+                    __syncthreads();
+                    if (wk == 0)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) acc[m][r][i] += js[i * NT + gt];
+                    __syncthreads();
+                }
+        if (wk) return;
+    }
+    if (hq >= 2 * a.nq) return;
+    // lane: column l % 32 of the operand; register i: row 8 (i / 4) + 4 (l / 32) + i % 4
+    const int c0 = 128 * q + 64 * h + 32 * (lane >> 3 & 1) + 8 * (lane >> 4 & 1) + (lane & 7);
+    const int E = a.ge[4 * q + 2 * h + (lane >> 3 & 1)];
+    float *out = a.out + (size_t)blockIdx.z * a.S * a.I;
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const int row = row0 + 32 * m + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
+            if (row >= a.S) continue;
+            const int e = E + a.exps[row];
+#pragma unroll
+            for (int r = 0; r < 2; r++)
+                if (c0 + 16 * r < a.I) out[(size_t)row * a.I + c0 + 16 * r] = ldexpf(acc[m][r][i], e);
+        }
+}
+
+// Sum of the K splits, in order.
+__global__ __launch_bounds__(256) void coli_t_join(const float *__restrict__ part, float *__restrict__ out, size_t n,
+                                                   int splits) {
+    const size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i + 4 <= n && n % 4 == 0) {
+        floatx4 s = *GPTR(floatx4, part + i);
+        for (int p = 1; p < splits; p++) s += *GPTR(floatx4, part + p * n + i);
+        if (((uintptr_t)out & 15) == 0) {
+            *(floatx4 *)(out + i) = s;
+        } else {
+            for (int k = 0; k < 4; k++) out[i + k] = s[k];
+        }
+    } else {
+        for (size_t k = i; k < n && k < i + 4; k++) {
+            float s = part[k];
+            for (int p = 1; p < splits; p++) s += part[p * n + k];
+            out[k] = s;
+        }
+    }
+}
+
+// Source-layout int4 whose groups are not multiples of 32 columns: one thread
+// a column, rows of W in turn (the forward's scalar kernel, turned round).
+__global__ __launch_bounds__(256) void coli_t_generic(const uint8_t *__restrict__ w, const float *__restrict__ sc, int gs,
+                                                      int ng, int I, int O, const float *__restrict__ dy,
+                                                      float *__restrict__ dx) {
+    const int i = blockIdx.x * 256 + threadIdx.x, s = blockIdx.y;
+    if (i >= I) return;
+    const size_t rb = (size_t)(I + 1) / 2;
+    const float *d = dy + (size_t)s * O;
+    float acc = 0.0f;
+    for (int o = 0; o < O; o++) {
+        const int u = w[o * rb + (i >> 1)] >> (i & 1 ? 4 : 0) & 15;
+        acc += d[o] * ((float)(u - 8) * sc[(size_t)o * ng + i / gs]);
+    }
+    dx[(size_t)s * I + i] = acc;
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+static int t_octets(const ColiCudaTensor *t) { return (t->nrt + 1) / 2 * 4; }
+
+// The tensor's scales by column group: made on first use, rebuilt by
+// fill_tensor after an update.
+int build_t_scales(DevCtx *ctx, ColiCudaTensor *t, bool update_only) {
+    if (t->kind == COLI_KIND_GENERIC || (update_only && !t->sct)) return 1;
+    const int noct = t_octets(t), planes = t->kind == COLI_KIND_I4_F ? 2 : 1;
+    if (!t->sct) {
+        const size_t sb = (size_t)planes * t->nq * 4 * noct * 16;
+        if (!hip_check(hipMalloc(&t->sct, sb + (size_t)t->nq * 4 * sizeof(int)), "transposed scales")) return 0;
+        t->sct_ge = (int *)((uint8_t *)t->sct + sb);
+    }
+#define COLI_TS(KD)                                                                                            \
+    hipLaunchKernelGGL((coli_t_scales<KD>), dim3(t->nq), dim3(256), 0, ctx->stream, t->sc, t->nrt, t->nq, noct, \
+                       (_Float16 *)t->sct, t->sct_ge)
+    if (t->kind == COLI_KIND_I4_H) COLI_TS(COLI_KIND_I4_H);
+    else if (t->kind == COLI_KIND_I4_F) COLI_TS(COLI_KIND_I4_F);
+    else COLI_TS(COLI_KIND_FP4);
+#undef COLI_TS
+    return hip_check(hipGetLastError(), "transposed scales");
+}
+
+template <int KIND>
+static void launch_gemm_t(const GemmTArgs &a, int mt, hipStream_t st) {
+    const int rb = (a.S + 32 * mt - 1) / (32 * mt);
+    if (mt == 4) hipLaunchKernelGGL((coli_gemm_t<KIND, 4, 4, 1>), dim3((a.nq + 1) / 2, rb, a.splits), dim3(256), 0, st, a);
+    else if (mt == 2) hipLaunchKernelGGL((coli_gemm_t<KIND, 2, 4, 1>), dim3((a.nq + 1) / 2, rb, a.splits), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((coli_gemm_t<KIND, 1, 2, 4>), dim3(a.nq, rb, a.splits), dim3(512), 0, st, a);
+}
+
+int gemm_t_dev(DevCtx *ctx, ColiCudaTensor *t, float *dx, const float *dy, int S) {
+    forget_emitted(ctx, dx, (size_t)S * t->I * sizeof(float));
+    hipStream_t st = ctx->stream;
+    if (t->kind == COLI_KIND_GENERIC) {
+        hipLaunchKernelGGL(coli_t_generic, dim3((t->I + 255) / 256, S), dim3(256), 0, st, t->w, (const float *)t->sc, t->gs,
+                           t->ng_src, t->I, t->O, dy, dx);
+        return hip_check(hipGetLastError(), "generic gradient");
+    }
+    if (!t->sct && !build_t_scales(ctx, t, false)) return 0;
+    const int noct = t_octets(t), steps = noct / 4, mt = S <= 32 ? 1 : S <= 64 ? 2 : 4;
+    const size_t Sp = ((size_t)S + 127) & ~(size_t)127, fb = (size_t)noct * Sp * 16;
+    const int cus = ctx->cu_count ? ctx->cu_count : 256;
+    const long blocks = (long)((S + 32 * mt - 1) / (32 * mt)) * (mt == 1 ? t->nq : (t->nq + 1) / 2);
+    // workgroups for about two a CU, at least eight steps each
+    int splits = (int)std::max(1L, std::min((2L * cus + blocks - 1) / blocks, (long)std::max(1, steps / (mt == 1 ? 16 : 8))));
+    const int per = (steps + splits - 1) / splits;
+    splits = (steps + per - 1) / per;
+    const size_t eb = (Sp * sizeof(int) + 255) & ~(size_t)255;
+    const size_t pb = splits > 1 ? (size_t)splits * S * t->I * sizeof(float) : 0;
+    if (!reserve_kept(ctx, &ctx->gt, 2 * fb + eb + pb, 0)) return 0;
+    uint8_t *p = (uint8_t *)ctx->gt.p;
+    GemmTArgs a = {};
+    a.w = t->w;
+    a.sct = (const _Float16 *)t->sct;
+    a.ge = t->sct_ge;
+    a.hi = (_Float16 *)p;
+    a.lo = (_Float16 *)(p + fb);
+    a.exps = (int *)(p + 2 * fb);
+    a.Sp = Sp;
+    a.nrt = t->nrt;
+    a.nq = t->nq;
+    a.noct = noct;
+    a.I = t->I;
+    a.S = S;
+    a.splits = splits;
+    a.per = per;
+    a.out = splits > 1 ? (float *)(p + 2 * fb + eb) : dx;
+    const int vec = t->O % 4 == 0 && ((uintptr_t)dy & 15) == 0;
+    const int chunks = std::max(1, std::min(8, 2 * cus / ((S + 3) / 4)));
+    hipLaunchKernelGGL(coli_t_prep, dim3((S + 3) / 4, chunks), dim3(256), 0, st, dy, S, t->O, noct,
+                       (int)(t->kind != COLI_KIND_FP4), vec, Sp, (_Float16 *)a.hi, (_Float16 *)a.lo, (int *)a.exps);
+    if (!hip_check(hipGetLastError(), "gradient rows")) return 0;
+    if (t->kind == COLI_KIND_I4_H) launch_gemm_t<COLI_KIND_I4_H>(a, mt, st);
+    else if (t->kind == COLI_KIND_I4_F) launch_gemm_t<COLI_KIND_I4_F>(a, mt, st);
+    else launch_gemm_t<COLI_KIND_FP4>(a, mt, st);
+    if (!hip_check(hipGetLastError(), "input gradient")) return 0;
+    if (splits > 1) {
+        const size_t n = (size_t)S * t->I;
+        hipLaunchKernelGGL(coli_t_join, dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, st, a.out, dx, n, splits);
+        return hip_check(hipGetLastError(), "input gradient join");
+    }
+    return 1;
+}
+
+extern "C" int coli_hip_gemm_t_dev(ColiCudaTensor *t, float *dx_dev, const float *dy_dev, int S) {
+    if (fault_injected()) return 0;
+    if (!tensor_computable(t) || !dx_dev || !dy_dev || S < 1 || S > COLI_GRAD_MAX_ROWS) return 0;
+    DevCtx *ctx = ctx_of(t->device);
+    if (!bind_ctx(ctx)) return 0;
+    return gemm_t_dev(ctx, t, dx_dev, dy_dev, S);
+}

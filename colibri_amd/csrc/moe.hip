@@ -42,6 +42,7 @@ struct ColiHipMoe {
     int kind;                 // storage kind shared by every expert matrix
     std::vector<const ColiCudaTensor *> mats;   // every expert matrix (e8_fold is read per forward)
     int S_cap;
+    int S_last = 0;           // rows of the last forward
     float *rw = nullptr, *rb = nullptr;
     ColiProb *tab = nullptr;  // [E (+1 shared)][2]: dual template, down template
     // per-forward state (device)
@@ -1490,6 +1491,7 @@ extern "C" int coli_hip_moe_forward_dev(ColiHipMoe *m, const float *x_dev, float
     }
     forget_emitted(ctx, out_dev, (size_t)S * m->cfg.D * sizeof(float));
     const int ok = moe_forward_impl(m, ctx, x_dev, out_dev, S);
+    m->S_last = ok ? S : 0;
     if (!ok) m->route_cnt_dirty = true;
     return ok;
 }
@@ -1666,4 +1668,17 @@ extern "C" int coli_hip_moe_last_union(ColiHipMoe *m, int *nu, int *uniq) {
         !hip_check(hipMemcpy(uniq, m->uniq, (size_t)st[2] * sizeof(int), hipMemcpyDeviceToHost), "union ids"))
         return 0;
     return 1;
+}
+
+// The router's logits, indices and counts of live selections are still where
+// the last forward left them.
+extern "C" int coli_hip_moe_last_balance_dev(ColiHipMoe *m, const unsigned char *mask, const int *offsets, int n,
+                                             float *loss, int *counts, int *rows) {
+    if (fault_injected()) return 0;
+    if (!m || !m->S_last || !loss || !counts || !rows || (!offsets && n != 1)) return 0;
+    DevCtx *ctx = ctx_of(m->device);
+    if (!bind_ctx(ctx)) return 0;
+    const ColiHipMoeConfig &c = m->cfg;
+    return run_balance(ctx, m->logits, coli_router_chunks(c.D), (size_t)m->S_last * c.E, m->idx, m->keff, mask, offsets,
+                       n, m->S_last, c.E, c.K, c.route_mode, loss, counts, rows);
 }

@@ -125,6 +125,70 @@ int coli_hip_moe_last_union(ColiHipMoe *moe, int *nu, int *uniq);
  * threads, other streams) race. Returns 1 / 0. */
 int coli_hip_pipe_gemm_noalloc(ColiCudaTensor *tensor, float *y_dev, const float *x_dev, int S);
 
+/* ---- adapters beside a resident projection, and gradients through it --------
+ * For serving many fine-tuned variants of one quantized model, and for tuning
+ * them: the quantized matrix stays frozen. Device pointers, f32 rows, contiguous;
+ * asynchronous on the backend stream (an input written on another stream must
+ * be complete or waited for first). Workspaces grow on first use at a size and are
+ * shared by the calls of a device, which its one stream orders; a captured
+ * graph stays valid when later calls grow them, and must be replayed on that
+ * stream. S <= 65535. None of these has a counterpart in the reference. */
+
+/* A bank of low-rank adapters for one projection of width I -> O: slot a holds
+ * A [rank, I], B [O, rank] and a scale. dtype of the factors: 0 f32, 1 fp16,
+ * 2 bf16. slots <= 1024, max_rank <= 256. Slots start empty. */
+typedef struct ColiHipLora ColiHipLora;
+int coli_hip_lora_create(ColiHipLora **lora, int device, int I, int O, int slots, int max_rank, int dtype);
+void coli_hip_lora_free(ColiHipLora *lora);
+/* Copy an adapter into its slot (device pointers, row-major, of the bank's
+ * dtype; asynchronous: they must hold their values until the copy has run).
+ * rank 0 empties the slot; the factors are then not read. */
+int coli_hip_lora_set_dev(ColiHipLora *lora, int slot, const void *a_dev, const void *b_dev, int rank, float scale);
+/* y[s] = W x[s] + scale_a B_a (A_a x[s]) with a = slot_dev[s]: the projection
+ * of coli_cuda_pipe_gemm and each row's adapter in one call. A slot number
+ * outside the bank, or of an empty slot: no adapter. y must not overlap x. */
+int coli_hip_lora_gemm_dev(ColiCudaTensor *tensor, ColiHipLora *lora, float *y_dev, const float *x_dev, int S,
+                           const int *slot_dev);
+/* Gradients of that call from dy [S, O]: dx [S, I] (NULL: not wanted), and for
+ * every slot of the bank da [slots, max_rank, I] and db [slots, O, max_rank]
+ * (written whole: zeros past a slot's rank and where no row has the slot). */
+int coli_hip_lora_grad_dev(ColiCudaTensor *tensor, ColiHipLora *lora, const float *x_dev, const float *dy_dev, int S,
+                           const int *slot_dev, float *dx_dev, float *da_dev, float *db_dev);
+/* Input gradient of coli_cuda_pipe_gemm: dx[S, I] = dy[S, O] W. dx must not
+ * overlap dy. The first call on a tensor also lays out its scales a second
+ * time (freed with it; kept current by coli_cuda_tensor_update). */
+int coli_hip_gemm_t_dev(ColiCudaTensor *tensor, float *dx_dev, const float *dy_dev, int S);
+
+/* ---- load balance of routed rows -------------------------------------------
+ * Per-expert counts and the balance loss of T routed rows by sequence, and the
+ * gradient of the router's logits. Device pointers, asynchronous on the
+ * device's stream. None has a counterpart in the reference.
+ *
+ * Sequence i is the rows [offsets[i], offsets[i + 1]) (offsets [n + 1],
+ * ascending, int32; NULL with n = 1: all rows); rows whose mask byte is 0 count
+ * for nothing (mask [T]; NULL: all count). idx [T, K] are the selected experts,
+ * of which the first keff[t] are live (NULL: all K); an index outside 0..E-1 is
+ * not counted. p is the router's score of a row divided by its sum: softmax
+ * (route_mode 0), sigmoid (1, 2), sqrt-softplus (3), without the selection
+ * bias. With c_e the live selections of expert e in the sequence, C their sum
+ * and n_i its rows:
+ *   counts[i, e] = c_e, rows[i] = n_i,
+ *   loss[i] = sum_e (E c_e / C) (1 / n_i) sum_t p[t, e]      (0 where C or n_i is 0)
+ * 1.0 is balance (top-K of equal loads). E <= 1024, K <= 64, n <= 16384, T <= 2^24. */
+int coli_hip_balance_dev(int device, const float *logits, const int *idx, const int *keff, const unsigned char *mask,
+                         const int *offsets, int n, int T, int E, int K, int route_mode, float *loss, int *counts,
+                         int *rows);
+/* dlogits [T, E] from dloss [n] and the forward's counts and rows (the counts
+ * carry no gradient). Masked rows get zeros; rows of no sequence are left as
+ * they were. */
+int coli_hip_balance_grad_dev(int device, const float *logits, const unsigned char *mask, const int *offsets, int n,
+                              int T, int E, int route_mode, const float *dloss, const int *counts, const int *rows,
+                              float *dlogits);
+/* coli_hip_balance_dev over the last forward of a MoE layer (its rows, its own
+ * router logits, selections and route mode). Refused before the first one. */
+int coli_hip_moe_last_balance_dev(ColiHipMoe *moe, const unsigned char *mask, const int *offsets, int n, float *loss,
+                                  int *counts, int *rows);
+
 /* ---- plumbing for benchmarks and tests ----------------------------------- */
 /* coli_cuda_pipe_gemm in two halves, so a timer can bracket the GEMV kernel
  * alone: prep names the activations x_dev[S, I] for the tensor's storage

@@ -1,0 +1,279 @@
+"""Per-expert counts, the balance loss and the gradient of the router's logits
+(coli_hip_balance_dev, coli_hip_balance_grad_dev, coli_hip_moe_last_balance_dev)
+against the definition in 64 bits."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from balance_ref import balance, scores
+from colibri_amd import hiprt
+from colibri_amd.backend import ColiHipMoeConfig, f32p, i32p, tensor_array
+from moe_ref import Layer, make_router_inputs
+from op_util import Bufs
+
+pytestmark = pytest.mark.gpu
+
+
+def p_tol(z):
+    """Relative error of a score over the row's sum: the exponent's argument, up
+    to s = max |z| + |max z| of the row, is rounded before it is multiplied with
+    log2 e (1.45 s 2^-24, twice for the difference), and about sixteen roundings
+    of 2^-23 (exp2, log2, rcp, sqrt and the sums) follow; a sum shares that of
+    its largest terms."""
+    f = np.where(np.isfinite(z) & (np.abs(z) < 1e30), z, 0.0)
+    return (3.0 * float(np.abs(f).max(initial=0.0)) + 32.0) * 2.0 ** -23
+
+
+def run(session, z, idx, keff, mask, off, mode, dloss, dz0, n):
+    b = session.b
+    T, E = z.shape
+    with Bufs(b) as d:
+        pz, pi = d.up(z), d.up(idx)
+        pk, pm, po = (None if v is None else d.up(v) for v in (keff, mask, off))
+        pl, pc, pr = d.up(np.full(n, 7.0, np.float32)), d.up(np.full((n, E), 7, np.int32)), d.up(np.full(n, 7, np.int32))
+        pd, pg = d.up(dloss), d.up(dz0)
+        assert b.hip_balance_dev(0, pz, pi, pk, pm, po, n, T, E, idx.shape[1], mode, pl, pc, pr)
+        assert b.hip_balance_grad_dev(0, pz, pm, po, n, T, E, mode, pd, pc, pr, pg)
+        return d.down(pl, (n,)), d.down(pc, (n, E), np.int32), d.down(pr, (n,), np.int32), d.down(pg, (T, E))
+
+
+def check(session, z, idx, keff, mask, off, mode, seed=0):
+    rng = np.random.default_rng(seed)
+    T, E = z.shape
+    n = 1 if off is None else len(off) - 1
+    dloss = rng.standard_normal(n).astype(np.float32)
+    dz0 = np.full((T, E), 7.0, np.float32)
+    loss, counts, rows, dz = run(session, z, idx, keff, mask, off, mode, dloss, dz0, n)
+    rl, rc, rr, rg, mag = balance(z, idx, keff, mask, off, E, mode, dloss, dz0)
+    assert np.array_equal(counts, rc) and np.array_equal(rows, rr)
+    t = p_tol(z) + (T / 16 + 96) * 2.0 ** -24
+    assert (np.abs(loss - rl) <= t * np.abs(rl) + 1e-30).all(), (np.abs(loss - rl) / rl).max()
+    # a row of no sequence: as it was
+    inside = np.zeros(T, bool)
+    inside[0 if off is None else off[0]: T if off is None else off[-1]] = True
+    assert (dz[~inside] == 7.0).all()
+    err = np.abs(dz - rg)
+    # (2^-126: results below the normal range are flushed)
+    bad = inside[:, None] & ~(err <= 2 * p_tol(z) * mag + 2.0 ** -126)
+    assert not bad.any(), (int(bad.sum()), float((err[inside] / np.maximum(mag[inside], 1e-30)).max()))
+    return loss, dz
+
+
+def routed(rng, T, E, K, spread=1.0):
+    z = (rng.standard_normal((T, E)) * spread).astype(np.float32)
+    idx = np.argsort(-z, 1)[:, :K].astype(np.int32)
+    return z, np.ascontiguousarray(idx)
+
+
+SHAPES = [  # T, E, K, offsets
+    (1, 1, 1, None), (1, 8, 2, None), (3, 5, 2, [0, 0, 2, 2, 3]), (64, 64, 8, None), (128, 384, 8, [0, 100, 128]),
+    (129, 63, 3, None), (200, 130, 4, [5, 60, 60, 61, 180]), (777, 256, 8, [0, 1, 2, 3, 500, 770]),
+    (300, 1024, 6, [0, 300]), (1000, 7, 7, [0] + list(range(100, 1000, 3))), (5000, 96, 2, [0, 4990]),
+    (40000, 16, 1, None), (700, 512, 64, [0, 350, 700]),
+]
+
+
+@pytest.mark.parametrize("mode", [0, 1, 2, 3])
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "-".join(map(str, s[:3])))
+def test_matches_definition(session, mode, shape):
+    T, E, K, off = shape
+    rng = np.random.default_rng(T + E + mode)
+    z, idx = routed(rng, T, E, K)
+    off = None if off is None else np.asarray(off, np.int32)
+    keff = rng.integers(0, K + 1, T).astype(np.int32) if T % 2 else None
+    mask = (rng.random(T) < 0.8).astype(np.uint8) if E % 2 == 0 else None
+    check(session, z, idx, keff, mask, off, mode, T)
+
+
+@pytest.mark.parametrize("T", [40, 400])
+@pytest.mark.parametrize("mode", [0, 1, 3])
+def test_masked_places(session, mode, T):
+    """Sequences whose mask leaves no row, rows without selections, indices of no
+    expert, logits of -inf and of the type's lowest value, a row of nothing but
+    -inf, NaN and infinities in masked rows and behind the last sequence."""
+    rng = np.random.default_rng(mode + T)
+    E, K = 24, 4
+    z, idx = routed(rng, T, E, K, 3.0)
+    off = np.array([0, T // 4, T // 2, T // 2, T - 5], np.int32)
+    mask = np.ones(T, np.uint8)
+    mask[T // 4: T // 2] = 0                   # a sequence of masked rows
+    mask[3] = 0
+    z[3], z[T // 4], z[T - 1], z[T - 2] = np.nan, np.inf, np.nan, -np.inf
+    z[:, 7] = -np.inf
+    z[5:9, 2] = np.finfo(np.float32).min
+    z[10] = -np.inf
+    idx[12] = -1
+    idx[13, 1] = E
+    keff = np.full(T, K, np.int32)
+    keff[14], keff[15] = 0, -3
+    check(session, z, idx, keff, mask, off, mode)
+    keff[:] = 0                                 # no selection at all: loss and gradients 0
+    loss, dz = check(session, z, idx, keff, mask, off, mode)
+    assert not loss.any() and not dz[: T - 5].any()
+
+
+@pytest.mark.parametrize("mode", [0, 1, 3])
+def test_far_logits(session, mode):
+    """Rows whose scores all underflow in 32 bits (z to -300), rows of large ones."""
+    rng = np.random.default_rng(mode)
+    z, idx = routed(rng, 96, 40, 4)
+    z[:32] -= 200.0
+    z[32:48] -= 40.0
+    z[48:56] -= 27.5
+    z[64:] += 30.0
+    check(session, z, idx, None, None, np.array([0, 32, 64, 96], np.int32), mode)
+
+
+def test_nan_row_reaches_its_sequence_only(session):
+    rng = np.random.default_rng(4)
+    z, idx = routed(rng, 300, 32, 4)
+    z[150, 3] = np.nan
+    off = np.array([0, 100, 200, 300], np.int32)
+    loss, counts, rows, dz = run(session, z, idx, None, None, off, 0, np.ones(3, np.float32), np.zeros((300, 32), np.float32), 3)
+    assert np.isnan(loss[1]) and np.isfinite(loss[[0, 2]]).all()
+    assert np.isnan(dz[150]).all() and np.isfinite(np.delete(dz, 150, 0)).all()
+    assert (rows == 100).all() and (counts.sum(1) == 400).all()
+
+
+@pytest.mark.parametrize("mode", [0, 2, 3])
+def test_gradient_against_differences(session, mode):
+    """Central differences of the forward call's loss, the selections fixed.
+
+    With step h the difference is off by h^2 / 6 of the loss's third derivative
+    (a sum of f_e p_e / n, |p'''| <= 1 and the weights at most max f / n, two of
+    them) and by the two losses' own error over 2 h."""
+    rng = np.random.default_rng(8)
+    T, E, K, h = 5, 12, 3, 2.0 ** -5
+    z, idx = routed(rng, T, E, K)
+    off, one, dz0 = np.array([0, 5], np.int32), np.ones(1, np.float32), np.zeros((T, E), np.float32)
+    loss, counts, _, dz = run(session, z, idx, None, None, off, mode, one, dz0, 1)
+    f = counts[0] * E / counts.sum()
+    tol = h * h / 6 * 2 * f.max() / T + 2 * p_tol(z) * loss[0] / (2 * h)
+    for t, e in ((0, 0), (2, 5), (4, 11), (3, int(idx[3, 0]))):
+        v = []
+        for s in (1, -1):
+            zz = z.copy()
+            zz[t, e] += np.float32(s * h)
+            v.append((float(run(session, zz, idx, None, None, off, mode, one, dz0, 1)[0][0]), float(zz[t, e])))
+        assert abs((v[0][0] - v[1][0]) / (v[0][1] - v[1][1]) - dz[t, e]) <= tol
+
+
+def test_repeats_bitwise_and_unaligned(session):
+    b = session.b
+    rng = np.random.default_rng(12)
+    T, E, K = 3000, 64, 4
+    z, idx = routed(rng, T, E, K)
+    with Bufs(b) as d:
+        pz, pi = d.up(np.concatenate((np.zeros(1, np.float32), z.ravel()))), d.up(idx)
+        pa = d.up(z)
+        got = []
+        for p in (pa, pa, pz + 4):
+            pl, pc, pr, pg = (d.up(np.zeros(k, np.float32)) for k in (1, E, 1, T * E + 1))
+            pd = d.up(np.ones(1, np.float32))
+            g = pg + 4 if p == pz + 4 else pg
+            assert b.hip_balance_dev(0, p, pi, None, None, None, 1, T, E, K, 1, pl, pc, pr)
+            assert b.hip_balance_grad_dev(0, p, None, None, 1, T, E, 1, pd, pc, pr, g)
+            out = d.down(pg, (T * E + 1,))
+            got.append((d.down(pl, (1,)), d.down(pc, (E,), np.int32), out[1:] if g != pg else out[:-1]))
+        for other in got[1:]:
+            for u, v in zip(got[0], other):
+                assert np.array_equal(u.view(np.uint32), v.view(np.uint32))
+
+
+def test_balanced_loads_give_one(session):
+    """Every expert selected alike and scored alike: f_e = 1, P_e = 1 / E."""
+    T, E, K = 512, 32, 4
+    z = np.zeros((T, E), np.float32)
+    idx = ((np.arange(T)[:, None] * K + np.arange(K)) % E).astype(np.int32)
+    for mode in range(4):
+        loss, dz = check(session, z, idx, None, None, None, mode)
+        assert abs(float(loss[0]) - 1.0) <= 64 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("T", [50, 1500])
+def test_graph_replays(session, T):
+    b = session.b
+    rng = np.random.default_rng(T)
+    E, K, n = 48, 4, 3
+    z, idx = routed(rng, T, E, K)
+    z2, idx2 = routed(rng, 9000, 200, 8)
+    off = np.array([0, T // 3, T // 2, T - 1], np.int32)
+    with Bufs(b) as d:
+        pz, pi, po, pd = d.up(z), d.up(idx), d.up(off), d.up(np.ones(n, np.float32))
+        qz, qi, ql, qc, qr = d.up(z2), d.up(idx2), d.up(np.zeros(1, np.float32)), d.up(np.zeros(200, np.int32)), d.up(np.zeros(1, np.int32))
+        pl, pc, pr, pg = d.up(np.zeros(n, np.float32)), d.up(np.zeros((n, E), np.int32)), d.up(np.zeros(n, np.int32)), d.up(z * 0)
+
+        def step():
+            assert b.hip_balance_dev(0, pz, pi, None, None, po, n, T, E, K, 3, pl, pc, pr)
+            assert b.hip_balance_grad_dev(0, pz, None, po, n, T, E, 3, pd, pc, pr, pg)
+
+        def got():
+            return [d.down(p, s, np.uint32) for p, s in ((pl, (n,)), (pc, (n, E)), (pr, (n,)), (pg, (T - 1, E)))]
+
+        step()
+        eager = got()
+        with hiprt.Graph(b.hip_stream(0)) as g:
+            step()
+        for rep in range(3):
+            for p, k in ((pl, n), (pc, n * E), (pr, n), (pg, T * E)):
+                assert b.hip_fill_random_u8(0, p, k * 4, rep + 1)
+            g.launch()
+            for u, v in zip(eager, got()):
+                assert np.array_equal(u, v), rep
+            assert b.hip_balance_dev(0, qz, qi, None, None, None, 1, 9000 - rep, 200, 8, 0, ql, qc, qr)
+
+
+@pytest.mark.parametrize("mode,S,E,K,D", [(0, 1, 64, 8, 2048), (0, 9, 64, 8, 256), (2, 5, 128, 8, 1536), (1, 70, 33, 4, 640),
+                                          (3, 300, 96, 6, 384)])
+def test_last_forward_of_a_layer(session, mode, S, E, K, D):
+    """Counts and loss of the layer's own router after a forward."""
+    rng = np.random.default_rng(S + E)
+    b = session.b
+    layer = Layer(rng, 4, D, 128, E, shared=False)
+    x, W, bias = make_router_inputs(rng, S, D, E, K, mode, bias=mode != 0)
+    hs = layer.upload(session)
+    m = C.c_void_p()
+    try:
+        (g, _a), (u, _b), (w, _c) = (tensor_array([t[k] for t in hs[:E]]) for k in range(3))
+        cfg = ColiHipMoeConfig(D, 128, E, K, mode, 1, 0.0, 1.0, 0)
+        assert b.hip_moe_create(C.byref(m), 0, C.byref(cfg), f32p(W), None if bias is None else f32p(bias), g, u, w, None,
+                                None, None)
+        with Bufs(b) as d:
+            pl, pc, pr = d.up(np.zeros(2, np.float32)), d.up(np.zeros((2, E), np.int32)), d.up(np.zeros(2, np.int32))
+            assert not b.hip_moe_last_balance_dev(m, None, None, 1, pl, pc, pr)   # no forward yet
+            out, idx = np.zeros((S, D), np.float32), np.zeros((S, K), np.int32)
+            wt, keff = np.zeros((S, K), np.float32), np.zeros(S, np.int32)
+            assert b.hip_moe_forward(m, f32p(x), f32p(out), S, i32p(idx), f32p(wt), i32p(keff))
+            off = np.array([0, S // 2, S], np.int32)
+            assert b.hip_moe_last_balance_dev(m, None, d.up(off), 2, pl, pc, pr)
+            loss, counts, rows = d.down(pl, (2,)), d.down(pc, (2, E), np.int32), d.down(pr, (2,), np.int32)
+        z = x.astype(np.float64) @ W.astype(np.float64).T
+        rl, rc, rr, _, _ = balance(z, idx, keff, None, off, E, mode)
+        assert np.array_equal(counts, rc) and np.array_equal(rows, rr)
+        # a logit is an f32 sum of D products: off by (2 D + 16) 2^-24 of their
+        # magnitudes, and a score over its sum by twice that, relatively
+        dz = ((np.abs(x).astype(np.float64) @ np.abs(W).astype(np.float64).T).max() * (2 * D + 16)) * 2.0 ** -24
+        assert (np.abs(loss - rl) <= (p_tol(z) + (S / 16 + 96) * 2.0 ** -24 + 2 * dz) * rl).all()
+    finally:
+        if m:
+            b.hip_moe_free(m)
+        for t in hs:
+            for h in t:
+                session.free(h)
+
+
+def test_refusals(session):
+    b = session.b
+    with Bufs(b) as d:
+        p = d.up(np.zeros(4096, np.float32))
+        ok = (0, p, p, None, None, p, 1, 4, 8, 2, 0, p, p, p)
+        for k, bad in ((0, 9), (0, -1), (1, None), (2, None), (6, 0), (6, 16385), (7, 0), (7, (1 << 24) + 1), (8, 0), (8, 1025),
+                       (9, 0), (9, 9), (9, 65), (10, -1), (10, 4), (11, None), (12, None), (13, None)):
+            assert not b.hip_balance_dev(*(ok[:k] + (bad,) + ok[k + 1:])), (k, bad)
+        assert not b.hip_balance_dev(0, p, p, None, None, None, 2, 4, 8, 2, 0, p, p, p)   # sequences without offsets
+        ok = (0, p, None, p, 1, 4, 8, 0, p, p, p, p)
+        for k, bad in ((0, 9), (1, None), (4, 0), (5, 0), (6, 1025), (7, 4), (8, None), (9, None), (10, None), (11, None)):
+            assert not b.hip_balance_grad_dev(*(ok[:k] + (bad,) + ok[k + 1:])), (k, bad)
+        assert not b.hip_balance_grad_dev(0, p, None, None, 2, 4, 8, 0, p, p, p, p)
+        assert not b.hip_moe_last_balance_dev(None, None, None, 1, p, p, p)

@@ -1,0 +1,195 @@
+"""coli_hip_gemm_t_dev (dx = dy W over resident quantized weights) against a
+64-bit product with the dequantized matrix."""
+import numpy as np
+import pytest
+
+from colibri_amd import hiprt
+from op_util import KINDS, Bufs, close, gemm_tol, matrix, sum_tol
+from quant_util import deq_i4, deq_mxfp4, rand_i4, rand_mxfp4
+
+pytestmark = pytest.mark.gpu
+
+
+def run(session, h, dy, I):
+    with Bufs(session.b) as d:
+        py, px = d.up(dy), d.up(np.full((dy.shape[0], I), 7.0, np.float32))
+        assert session.b.hip_gemm_t_dev(h, px, py, dy.shape[0])
+        return d.down(px, (dy.shape[0], I))
+
+
+def tol(kind, O):
+    return sum_tol(2 * O) if kind == "gen" else gemm_tol(O)
+
+
+# O and I around the tiles (16 rows, 128 columns) and the K steps (32 rows),
+# rows around the tile heights 32 / 64 / 128 and the K splits
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("O,I,S", [(1, 1, 1), (16, 128, 1), (17, 33, 2), (33, 129, 5), (100, 200, 16), (31, 64, 31),
+                                   (96, 256, 32), (48, 130, 33), (640, 384, 64), (200, 515, 65), (1040, 260, 128),
+                                   (64, 128, 129), (2049, 131, 20), (300, 1000, 300)])
+def test_matches_dense(session, kind, O, I, S):
+    rng = np.random.default_rng(O * 7 + I * 3 + S + KINDS.index(kind))
+    h, w = matrix(session, rng, kind, O, I)
+    try:
+        dy = rng.standard_normal((S, O)).astype(np.float32)
+        close(run(session, h, dy, I), dy.astype(np.float64) @ w, np.abs(dy).astype(np.float64) @ np.abs(w), tol(kind, O))
+    finally:
+        session.free(h)
+
+
+def test_one_hot_rows_read_the_matrix(session):
+    """dy = e_o gives row o of W: every weight at its place, as exact as its
+    fp16 hi + lo: 3 x 2^-22 of an f32 scale's weight (see gemm_tol), else exact
+    down to fp16's last place under the column group's largest scale."""
+    rng = np.random.default_rng(3)
+    for kind in ("i4h", "i4f", "fp4"):
+        h, w = matrix(session, rng, kind, 80, 272)
+        try:
+            got = run(session, h, np.eye(80, dtype=np.float32), 272)
+            close(got, w, np.abs(w).max(0, keepdims=True) + 0 * w, 3 * 2.0 ** -22, kind)
+        finally:
+            session.free(h)
+
+
+@pytest.mark.parametrize("fmt", [4, 7])
+def test_wide_ranges(session, fmt):
+    """Scales 2^-20 .. 2^12 apart from one column group to the next and from row
+    to row, rows of dy 2^-60 .. 2^40, a zero row and a column group of zeros."""
+    rng = np.random.default_rng(11 + fmt)
+    O, I, S = 144, 320, 40
+    ng = I // 32
+    if fmt == 7:
+        q4, e8 = rand_mxfp4(rng, O, I)
+        e8 = (127 + rng.integers(-20, 13, (1, ng)) + rng.integers(-6, 1, (O, ng))).astype(np.uint8)
+        e8[:, 3] = 0
+        h, w = session.upload_mxfp4(q4, e8, I, O), deq_mxfp4(q4, e8, I)
+    else:
+        q4, sc = rand_i4(rng, O, I, 32, fp16_scales=False)
+        sc = (sc * 2.0 ** rng.integers(-20, 13, (1, ng)) * 2.0 ** rng.integers(-6, 1, (O, ng))).astype(np.float32)
+        sc[:, 3] = 0
+        h, w = session.upload(q4, sc, 4, I, O, 32), deq_i4(q4, sc, I, 32)
+    try:
+        dy = (rng.standard_normal((S, O)) * 2.0 ** rng.integers(-60, 41, (S, 1))).astype(np.float32)
+        dy[7] = 0
+        ref = dy.astype(np.float64) @ w
+        mag = np.abs(dy).astype(np.float64) @ np.abs(w)
+        got = run(session, h, dy, I)
+        close(got, ref, mag, gemm_tol(O))
+        assert not got[7].any() and not got[:, 96:128].any()
+    finally:
+        session.free(h)
+
+
+def test_scales_follow_an_update(session):
+    """The scales laid out for the gradient are those of the tensor's present weights."""
+    rng = np.random.default_rng(5)
+    O, I, S = 64, 256, 3
+    h, _ = matrix(session, rng, "i4h", O, I)
+    try:
+        dy = rng.standard_normal((S, O)).astype(np.float32)
+        run(session, h, dy, I)
+        q4, sc = rand_i4(rng, O, I, 32)
+        sc = sc * 4
+        assert session.b.cuda_tensor_update(h, q4.ctypes.data_as(__import__("ctypes").c_void_p),
+                                            sc.ctypes.data_as(__import__("ctypes").POINTER(__import__("ctypes").c_float)))
+        w = deq_i4(q4, sc, I, 32)
+        close(run(session, h, dy, I), dy.astype(np.float64) @ w, np.abs(dy).astype(np.float64) @ np.abs(w), gemm_tol(O))
+    finally:
+        session.free(h)
+
+
+def test_rows_do_not_mix(session):
+    """A row of infinities or NaN stays in its row, and what lies behind the last row is left as it was."""
+    rng = np.random.default_rng(9)
+    O, I, S = 70, 150, 37
+    h, w = matrix(session, rng, "i4h", O, I)
+    try:
+        dy = rng.standard_normal((S, O)).astype(np.float32)
+        dy[5, 3], dy[36, 0] = np.inf, np.nan
+        with Bufs(session.b) as d:
+            py, px = d.up(dy), d.up(np.full((S + 3, I), 7.0, np.float32))
+            assert session.b.hip_gemm_t_dev(h, px, py, S)
+            got = d.down(px, (S + 3, I))
+        assert (got[S:] == 7.0).all()
+        keep = [r for r in range(S) if r not in (5, 36)]
+        close(got[keep], dy[keep].astype(np.float64) @ w, np.abs(dy[keep]).astype(np.float64) @ np.abs(w), gemm_tol(O))
+        assert not np.isfinite(got[5]).all() and np.isnan(got[36]).any()
+    finally:
+        session.free(h)
+
+
+def test_unaligned_rows(session):
+    """Pointers that are only 4-byte aligned."""
+    rng = np.random.default_rng(13)
+    O, I, S = 128, 256, 18
+    h, w = matrix(session, rng, "fp4", O, I)
+    try:
+        dy = rng.standard_normal((S, O)).astype(np.float32)
+        with Bufs(session.b) as d:
+            py, px = d.up(np.concatenate((np.zeros(1, np.float32), dy.ravel()))), d.up(np.zeros(S * I + 1, np.float32))
+            assert session.b.hip_gemm_t_dev(h, px + 4, py + 4, S)
+            got = d.down(px, (S * I + 1,))[1:].reshape(S, I)
+        close(got, dy.astype(np.float64) @ w, np.abs(dy).astype(np.float64) @ np.abs(w), gemm_tol(O))
+    finally:
+        session.free(h)
+
+
+def test_adjoint_of_the_projection(session):
+    """<y, W x> = <W^T y, x>: the gradient belongs to coli_cuda_pipe_gemm's own matrix."""
+    rng = np.random.default_rng(17)
+    O, I, S = 272, 384, 24
+    for kind in ("i4h", "fp4", "gen"):
+        h, w = matrix(session, rng, kind, O, I)
+        try:
+            x, dy = rng.standard_normal((S, I)).astype(np.float32), rng.standard_normal((S, O)).astype(np.float32)
+            with Bufs(session.b) as d:
+                px, py = d.up(x), d.up(np.zeros((S, O), np.float32))
+                assert session.b.cuda_pipe_gemm(h, py, px, S)
+                y = d.down(py, (S, O)).astype(np.float64)
+            dx = run(session, h, dy, I).astype(np.float64)
+            lhs, rhs = (y * dy).sum(1), (dx * x).sum(1)
+            mag = ((np.abs(x).astype(np.float64) @ np.abs(w).T) * np.abs(dy)).sum(1)
+            assert (np.abs(lhs - rhs) <= (gemm_tol(O) + gemm_tol(I) + sum_tol(2 * max(O, I))) * mag).all()
+        finally:
+            session.free(h)
+
+
+@pytest.mark.parametrize("S", [3, 70])
+def test_graph_replays(session, S):
+    b = session.b
+    rng = np.random.default_rng(23 + S)
+    O, I = 1024, 384
+    h, _ = matrix(session, rng, "i4h", O, I)
+    try:
+        dy, other = rng.standard_normal((S, O)).astype(np.float32), rng.standard_normal((900, O)).astype(np.float32) * 3
+        with Bufs(b) as d:
+            py, px, po, pq = d.up(dy), d.up(np.zeros((S, I), np.float32)), d.up(other), d.up(np.zeros((900, I), np.float32))
+            assert b.hip_gemm_t_dev(h, px, py, S)
+            eager = d.down(px, (S, I))
+            with hiprt.Graph(b.hip_stream(0)) as g:
+                assert b.hip_gemm_t_dev(h, px, py, S)
+            for rep in range(3):
+                assert b.hip_fill_random_u8(0, px, S * I * 4, 5 + rep)
+                g.launch()
+                got = d.down(px, (S, I))
+                assert np.array_equal(got.view(np.uint32), eager.view(np.uint32)), rep
+                # eager work between the replays, larger than the capture's workspace
+                assert b.hip_gemm_t_dev(h, pq, po, 900 - rep)
+    finally:
+        session.free(h)
+
+
+def test_refusals(session):
+    b = session.b
+    rng = np.random.default_rng(1)
+    h, _ = matrix(session, rng, "i4h", 32, 32)
+    try:
+        with Bufs(b) as d:
+            p = d.up(np.zeros((1, 32), np.float32))
+            assert not b.hip_gemm_t_dev(None, p, p, 1)
+            assert not b.hip_gemm_t_dev(h, None, p, 1)
+            assert not b.hip_gemm_t_dev(h, p, None, 1)
+            assert not b.hip_gemm_t_dev(h, p, p, 0)
+            assert not b.hip_gemm_t_dev(h, p, p, 65536)
+    finally:
+        session.free(h)
