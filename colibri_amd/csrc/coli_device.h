@@ -269,6 +269,8 @@ __device__ __forceinline__ void dma_wait_tail(int pend) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));   // any 4-byte aligned address (one dwordx4 load)
+
 // ---------------------------------------------------------------------------
 // Activation-fragment build (the format and its reasons are described with
 // coli_prep_frag in gemv.hip), shared by that kernel and launches that run

@@ -177,7 +177,21 @@ hipError_t coli_launch_sum_slots(float *dst, const float *slots, int n, int D, h
 // single-matrix products (expert.hip, gemm_t.hip)
 int tensor_computable(const ColiCudaTensor *t);
 int gemm_dev(DevCtx *ctx, ColiCudaTensor *t, float *y_dev, const float *x_dev, int S);
-int gemm_t_dev(DevCtx *ctx, ColiCudaTensor *t, float *dx, const float *dy, int S);
+// gemm_dev in two halves: the rows' fragment build, if the product will read
+// fragments, as launch arguments for a launch that runs it beside other work
+// (a null: left for gemm_prepared to launch), then the product.
+int gemm_prep_beside(DevCtx *ctx, ColiCudaTensor *t, const float *x_dev, int S, ColiPrepArgs *a);
+int gemm_prepared(DevCtx *ctx, ColiCudaTensor *t, float *y_dev, const float *x_dev, int S);
+// dx = dy W: the decomposition, then the launches (with_join: the K splits'
+// sums into dx, else left in part [parts][S][I] when parts > 1).
+struct GemmTPlan {
+    ColiTPrepArgs prep;
+    int mt, splits, per;
+    float *part;
+    int parts;
+};
+int gemm_t_plan(DevCtx *ctx, ColiCudaTensor *t, const float *dy, int S, GemmTPlan *plan);
+int gemm_t_run(DevCtx *ctx, ColiCudaTensor *t, float *dx, const float *dy, int S, const GemmTPlan &plan, bool with_join);
 int build_t_scales(DevCtx *ctx, ColiCudaTensor *t, bool update_only);
 // Counts and balance loss over router logits given as nch column-chunk
 // partials, chstride floats apart (balance.hip).

@@ -76,6 +76,16 @@ struct ColiPrepArgs {
     int ldx, K, ngp, int4_order, gen, vec, nchunk, nblocks;
 };
 
+// One build of an input gradient's rows (coli_t_prep_rows):
+// dy [S, K] -> hi, lo [noct][Sp][8], one exponent a row.
+struct ColiTPrepArgs {
+    const float *dy;
+    _Float16 *hi, *lo;
+    int *exps;
+    size_t Sp;
+    int S, K, noct, int4;
+};
+
 struct ColiGemvArgs {
     const ColiProb *prob;     // device descriptors; null: the single problem prob0
     ColiProb prob0;

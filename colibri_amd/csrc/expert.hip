@@ -248,6 +248,15 @@ static bool xstage_enabled() {
     return !(e && e[0] == '0');
 }
 
+// Up to 32768 activations (rows x K) on the LDS-ring kernel are read as f32
+// and converted in the kernel, which saves the prep launch; beyond, every
+// workgroup staging the f32 rows costs more than the prep (the activations are
+// re-read by every workgroup, at twice the bytes of the hi fragments).
+static bool gemv_reads_f32(const GemvLaunchPlan &pl, int max_rows, int nq, const FragSet &f) {
+    return pl.dma && max_rows <= 4 && (long)max_rows * nq * 128 <= 32768 && f.px && !f.psrc && f.pK == nq * 128 &&
+           f.pld % 4 == 0 && (uintptr_t)f.px % 16 == 0 && xf32_enabled();
+}
+
 // Launch one tiled GEMV over `nprob` problems whose descriptors are on the device.
 int run_gemv(DevCtx *ctx, int kind, bool dual, const ColiProb *probs_dev, int nprob, const int *nprob_dev, int nrt,
              int nq, int O, int max_rows, int set, const int *xrows_dev, float *out, int ldo,
@@ -284,13 +293,7 @@ int run_gemv(DevCtx *ctx, int kind, bool dual, const ColiProb *probs_dev, int np
     const void *zero = ws ? ws->zero : ctx->zeros.p;
     ColiGemvArgs a;
     std::memset(&a, 0, sizeof(a));
-    // Up to 32768 activations (rows x K) on the LDS-ring kernel are read as
-    // f32 and converted in the kernel, which saves the prep launch; beyond,
-    // every workgroup staging the f32 rows costs more than the prep (the
-    // activations are re-read by every workgroup, at twice the bytes of the
-    // hi fragments).
-    if (pl.dma && max_rows <= 4 && (long)max_rows * nq * 128 <= 32768 && f.px && !f.psrc && f.pK == nq * 128 &&
-        f.pld % 4 == 0 && (uintptr_t)f.px % 16 == 0 && xf32_enabled()) {
+    if (gemv_reads_f32(pl, max_rows, nq, f)) {
         a.xf = f.px;
         a.ldx = f.pld;
         // one row tile over a long K: sixteen waves, twice the per-quad
@@ -1045,6 +1048,26 @@ int gemm_dev(DevCtx *ctx, ColiCudaTensor *t, float *y_dev, const float *x_dev, i
         return hip_check(coli_launch_generic_i4(t, x_dev, t->I, y_dev, t->O, S, ctx->stream), "generic gemv");
     }
     return gemm_prep(ctx, t, x_dev, S) && gemm_run(ctx, t, y_dev, S);
+}
+
+int gemm_prep_beside(DevCtx *ctx, ColiCudaTensor *t, const float *x_dev, int S, ColiPrepArgs *a) {
+    if (a) a->nblocks = 0;
+    if (t->kind == COLI_KIND_GENERIC) return 1;
+    if (!gemm_prep(ctx, t, x_dev, S)) return 0;
+    if (!a) return 1;
+    const int set = ctx->dense_set[t->kind == COLI_KIND_FP4 ? 1 : 0];
+    if (!dense_on_gemm(ctx, t, S)) {
+        // (the plan run_gemv makes for one matrix)
+        const int n_bt = (S + 15) / 16;
+        GemvLaunchPlan pl = plan_gemv(ctx, 1, n_bt, t->nrt, t->nq, false, S);
+        plan_dma(ctx, pl, t->kind, 1, n_bt, t->nrt, t->nq, false, S);
+        if (gemv_reads_f32(pl, S, t->nq, ctx->frag[set])) return 1;
+    }
+    return flush_frags_args(ctx, set, a);
+}
+
+int gemm_prepared(DevCtx *ctx, ColiCudaTensor *t, float *y_dev, const float *x_dev, int S) {
+    return t->kind == COLI_KIND_GENERIC ? gemm_dev(ctx, t, y_dev, x_dev, S) : gemm_run(ctx, t, y_dev, S);
 }
 
 extern "C" int coli_hip_gemm_prep_dev(ColiCudaTensor *t, const float *x_dev, int S) {

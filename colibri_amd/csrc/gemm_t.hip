@@ -32,6 +32,40 @@
 // nibbles in (int4: even ones, then odd ones).
 __host__ __device__ __forceinline__ int t_order(int int4, int e) { return !int4 ? e : e < 4 ? 2 * e : 2 * (e - 4) + 1; }
 
+// Octet o of a row, zeros past K.
+__device__ __forceinline__ void t_load8(const float *xr, int o, int K, float (&v)[8]) {
+    if (8 * o + 8 <= K) {
+        const f4u a = *GPTR(f4u, xr + 8 * o), b = *GPTR(f4u, xr + 8 * o + 4);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            v[i] = a[i];
+            v[4 + i] = b[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = 8 * o + i < K ? xr[8 * o + i] : 0.0f;
+    }
+}
+// As hi + lo under the exponent E, in operand order.
+__device__ __forceinline__ void t_split8(const float (&v)[8], int int4, int E, half8v &h, half8v &l) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        // (constant indices in both orders: a choice of registers, not of memory)
+        const float y = ldexpf(int4 ? v[t_order(1, e)] : v[e], -E);
+        h[e] = (_Float16)y;
+        l[e] = (_Float16)(y - (float)h[e]);
+    }
+}
+// E with max |v| 2^-E in [2^14, 2^15).
+__device__ __forceinline__ int t_exponent(float m) {
+    int E = 0;
+    if (m > 0.0f && isfinite(m)) {
+        frexpf(m, &E);
+        E -= 15;
+    }
+    return E;
+}
+
 // ---------------------------------------------------------------------------
 // scales by column group
 // ---------------------------------------------------------------------------
@@ -86,57 +120,52 @@ __global__ __launch_bounds__(256) void coli_t_scales(const void *__restrict__ sc
 // ---------------------------------------------------------------------------
 // dy as fp16 hi + lo
 // ---------------------------------------------------------------------------
-// [octet of K][row][8]: a step's operand is contiguous over the rows. Four rows
-// a workgroup (a wave each), gridDim.y chunks of the columns; every chunk takes
-// the row's maximum for itself. max |v| 2^-E lies in [2^14, 2^15).
-__global__ __launch_bounds__(256) void coli_t_prep(const float *__restrict__ dy, int S, int K, int noct, int int4, int vec,
-                                                   size_t Sp, _Float16 *__restrict__ hi, _Float16 *__restrict__ lo,
-                                                   int *__restrict__ exps) {
-    const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= S) return;
-    const float *xr = dy + (size_t)row * K;
-    auto oct = [&](int o, float (&v)[8]) {
-        if (vec && 8 * o + 8 <= K) {
-            const floatx4 a = *GPTR(floatx4, xr + 8 * o), b = *GPTR(floatx4, xr + 8 * o + 4);
+// [octet of K][row][8]: a step's operand is contiguous over the rows. Only for
+// more than 64 rows: fewer are converted by the product itself.
+//
+// Four rows a workgroup, thread (row = t % 4, octet t / 4 of each 256), so
+// that loads read 512 and stores write 64 contiguous bytes; a row of up to
+// 16384 columns is read once.
+#define COLI_T_SLOTS 8   // octets a thread holds
+__global__ __launch_bounds__(1024) void coli_t_prep_rows(ColiTPrepArgs a) {
+    __shared__ float wmax[16][4];
+    const int tid = threadIdx.x, lane = tid & 63, r = tid & 3, o0 = tid >> 2, row = blockIdx.x * 4 + r;
+    const float *xr = a.dy + (size_t)min(row, a.S - 1) * a.K;
+    float v[COLI_T_SLOTS][8], m = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                v[i] = a[i];
-                v[4 + i] = b[i];
-            }
-        } else {
+    for (int s = 0; s < COLI_T_SLOTS; s++) t_load8(xr, o0 + 256 * s, a.K, v[s]);
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = 8 * o + i < K ? xr[8 * o + i] : 0.0f;
-        }
-    };
-    float m = 0.0f;
-#pragma unroll 4
-    for (int o = lane; 8 * o < K; o += 64) {
-        float v[8];
-        oct(o, v);
+    for (int s = 0; s < COLI_T_SLOTS; s++)
 #pragma unroll
-        for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(v[i]));
+        for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(v[s][i]));
+    for (int o = o0 + 256 * COLI_T_SLOTS; o < a.noct; o += 256) {
+        float u[8];
+        t_load8(xr, o, a.K, u);
+#pragma unroll
+        for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(u[i]));
     }
-    m = wave_max64(m);
-    int E = 0;
-    if (m > 0.0f && isfinite(m)) {
-        frexpf(m, &E);
-        E -= 15;
-    }
-    if (lane == 0 && blockIdx.y == 0) exps[row] = E;
-    const int per = ((noct + gridDim.y - 1) / gridDim.y + 63) & ~63, o1 = min(noct, (int)(blockIdx.y + 1) * per);
-#pragma unroll 2
-    for (int o = blockIdx.y * per + lane; o < o1; o += 64) {
-        float v[8];
-        oct(o, v);
+#pragma unroll
+    for (int o = 4; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+    if (lane < 4) wmax[tid >> 6][lane] = m;
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 16; q++) m = fmaxf(m, wmax[q][r]);
+    if (row >= a.S) return;
+    const int E = t_exponent(m);
+    if (o0 == 0) a.exps[row] = E;
+    auto put = [&](int o, const float (&x)[8]) {
         half8v h, l;
+        t_split8(x, a.int4, E, h, l);
+        *(half8v *)(a.hi + ((size_t)o * a.Sp + row) * 8) = h;
+        *(half8v *)(a.lo + ((size_t)o * a.Sp + row) * 8) = l;
+    };
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float y = ldexpf(v[t_order(int4, e)], -E);
-            h[e] = (_Float16)y;
-            l[e] = (_Float16)(y - (float)h[e]);
-        }
-        *(half8v *)(hi + ((size_t)o * Sp + row) * 8) = h;
-        *(half8v *)(lo + ((size_t)o * Sp + row) * 8) = l;
+    for (int s = 0; s < COLI_T_SLOTS; s++)
+        if (o0 + 256 * s < a.noct) put(o0 + 256 * s, v[s]);
+    for (int o = o0 + 256 * COLI_T_SLOTS; o < a.noct; o += 256) {
+        float u[8];
+        t_load8(xr, o, a.K, u);
+        put(o, u);
     }
 }
 
@@ -147,9 +176,11 @@ struct GemmTArgs {
     const uint8_t *w;            // tiles [nrt][nq]
     const _Float16 *sct;
     const int *ge;               // [4 nq]
-    const _Float16 *hi, *lo;     // [noct][Sp][8]
+    const _Float16 *hi, *lo;     // [noct][Sp][8] (many rows)
     const int *exps;             // [S]
     size_t Sp;
+    const float *dy;             // [S][O] (few rows)
+    int O;
     int nrt, nq, noct, I, S;
     int splits, per;             // K split: steps of 32 rows of W each
     float *out;                  // [splits][S][I]
@@ -217,14 +248,19 @@ __device__ __forceinline__ void t_weights(uint32_t nib, half8v s, half8v s2, hal
 // steps (32 rows of W: two row tiles) and are joined in LDS at the end. A
 // step's dy octets are staged in LDS (two buffers), the weights and scales of
 // the next step are requested before this one's products.
-template <int KIND, int MT, int WN, int WK>
+// FEW (up to 64 rows): dy is read as f32 and converted on its way into LDS,
+// under the exponent of the row's part in this K split (the splits' sums are
+// f32 already), which saves the launch that would build the operands.
+template <int KIND, int MT, int WN, int WK, bool FEW>
 __global__ __launch_bounds__(64 * WN * WK) void coli_gemm_t(GemmTArgs a) {
-    constexpr int BM = 32 * MT, NT = 64 * WN, CH = 8 * BM;   // 16-byte chunks of a step: 2 parts x 4 octets x BM rows
-    constexpr int CPT = (CH + NT - 1) / NT;
-    constexpr int STAGE = CH * 16;
-    constexpr int JOIN = WK > 1 ? 64 * WN * 16 * 4 : 0;       // one accumulator of every wave of a group
+    constexpr int BM = 32 * MT, NT = 64 * WN, CH = (FEW ? 4 : 8) * BM;   // 8 (FEW: f32) values a chunk, 4 octets x BM rows
+    constexpr int CPT = CH / NT;
+    static_assert(CH % NT == 0, "whole chunks a thread");
+    constexpr int STAGE = 8 * BM * 16;
+    constexpr int JOIN = WK > 1 ? WK * (WK - 1) * (32 / WK) * NT * 4 : 0;
     constexpr int LDS = 2 * WK * STAGE > JOIN ? 2 * WK * STAGE : JOIN;
     __shared__ __attribute__((aligned(16))) uint8_t lds[LDS];
+    __shared__ int rexp[FEW ? BM : 1];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave % WN, wk = wave / WN;
     const int gt = tid - wk * NT;                              // thread within its K group
@@ -247,7 +283,9 @@ __global__ __launch_bounds__(64 * WN * WK) void coli_gemm_t(GemmTArgs a) {
             for (int i = 0; i < 16; i++) acc[m][r][i] = 0.0f;
     u32x2 wd[2];
     half8v sc[2], sc2[2];
-    u32x4 ad[CPT];
+    u32x4 ad[FEW ? 1 : CPT];
+    float af[FEW ? CPT : 1][8];
+    int ae[FEW ? CPT : 1];
     auto load_w = [&](int step) {
         step = min(step, k1 - 1);
 #pragma unroll
@@ -262,18 +300,56 @@ __global__ __launch_bounds__(64 * WN * WK) void coli_gemm_t(GemmTArgs a) {
         step = min(step, k1 - 1);
 #pragma unroll
         for (int i = 0; i < CPT; i++) {
-            const int c = min(gt + i * NT, CH - 1), part = c / (4 * BM), oct = c / BM % 4, r = c % BM;
-            ad[i] = *GPTR(u32x4, (part ? a.lo : a.hi) + ((size_t)(4 * step + oct) * a.Sp + row0 + r) * 8);
+            const int c = gt + i * NT;
+            if constexpr (FEW) {
+                const int r = row0 + (c >> 2), o = 4 * step + (c & 3);
+                t_load8(a.dy + (size_t)min(r, a.S - 1) * a.O, r < a.S ? o : a.noct, a.O, af[i]);
+            } else {
+                const int part = c / (4 * BM), oct = c / BM % 4, r = c % BM;
+                ad[i] = *GPTR(u32x4, (part ? a.lo : a.hi) + ((size_t)(4 * step + oct) * a.Sp + row0 + r) * 8);
+            }
         }
     };
     auto store_a = [&](int buf) {
+        uint8_t *to = lds + (size_t)(buf * WK + wk) * STAGE;
 #pragma unroll
-        for (int i = 0; i < CPT; i++)
-            if (CH % NT == 0 || gt + i * NT < CH)
-                *(u32x4 *)(lds + (size_t)(buf * WK + wk) * STAGE + (size_t)(gt + i * NT) * 16) = ad[i];
+        for (int i = 0; i < CPT; i++) {
+            const int c = gt + i * NT;
+            if constexpr (FEW) {
+                half8v hv, lv;
+                t_split8(af[i], KIND != COLI_KIND_FP4, ae[i], hv, lv);
+                *(half8v *)(to + ((c & 3) * BM + (c >> 2)) * 16) = hv;
+                *(half8v *)(to + ((4 + (c & 3)) * BM + (c >> 2)) * 16) = lv;
+            } else {
+                *(u32x4 *)(to + (size_t)c * 16) = ad[i];
+            }
+        }
     };
-    load_a(k0 + wk);
     load_w(k0 + wk);
+    load_a(k0 + wk);
+    if constexpr (FEW) {
+        // the rows' exponents over this split's columns
+        constexpr int TPR = 64 * WN * WK / BM;   // threads a row
+        const int r = tid / TPR, row = row0 + r;
+        float m = 0.0f;
+        if (row < a.S) {
+            const float *xr = a.dy + (size_t)row * a.O;
+            const int c1 = min(a.O, 32 * k1);
+            int c = 32 * k0 + 4 * (tid % TPR);
+#pragma unroll 4
+            for (; c + 4 <= c1; c += 4 * TPR) {
+                const f4u v = *GPTR(f4u, xr + c);
+                m = fmaxf(m, fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))));
+            }
+            for (; c < c1; c++) m = fmaxf(m, fabsf(xr[c]));   // (at most 3: the others are past c1)
+        }
+#pragma unroll
+        for (int o = 1; o < TPR; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+        if (tid % TPR == 0) rexp[r] = t_exponent(m);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < CPT; i++) ae[i] = rexp[(gt + i * NT) >> 2];
+    }
     store_a(0);
     __syncthreads();
     for (int it = 0; it < nstep; it++) {
@@ -315,41 +391,55 @@ __global__ __launch_bounds__(64 * WN * WK) void coli_gemm_t(GemmTArgs a) {
         if (it + 1 < nstep) store_a((it + 1) & 1);
         __syncthreads();
     }
-    if constexpr (WK > 1) {
-        // groups 1 .. WK - 1 hand their sums to group 0 in turn
-        float *js = (float *)lds;
-        for (int g = 1; g < WK; g++)
-#pragma unroll
-            for (int m = 0; m < MT; m++)
-#pragma unroll
-                for (int r = 0; r < 2; r++) {
-                    if (wk == g)
-#pragma unroll
-                        for (int i = 0; i < 16; i++) js[i * NT + gt] = acc[m][r][i];
-                    __syncthreads();
-                    if (wk == 0)
-#pragma unroll
-                        for (int i = 0; i < 16; i++) acc[m][r][i] += js[i * NT + gt];
-                    __syncthreads();
-                }
-        if (wk) return;
-    }
-    if (hq >= 2 * a.nq) return;
     // lane: column l % 32 of the operand; register i: row 8 (i / 4) + 4 (l / 32) + i % 4
     const int c0 = 128 * q + 64 * h + 32 * (lane >> 3 & 1) + 8 * (lane >> 4 & 1) + (lane & 7);
     const int E = a.ge[4 * q + 2 * h + (lane >> 3 & 1)];
     float *out = a.out + (size_t)blockIdx.z * a.S * a.I;
+    auto put = [&](int lrow, int r, float v) {
+        const int row = row0 + lrow;
+        if (row >= a.S || hq >= 2 * a.nq || c0 + 16 * r >= a.I) return;
+        out[(size_t)row * a.I + c0 + 16 * r] = ldexpf(v, E + (FEW ? rexp[FEW ? lrow : 0] : a.exps[row]));
+    };
+    if constexpr (WK == 1) {
 #pragma unroll
-    for (int m = 0; m < MT; m++)
+        for (int m = 0; m < MT; m++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const int row = row0 + 32 * m + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
-            if (row >= a.S) continue;
-            const int e = E + a.exps[row];
+            for (int i = 0; i < 16; i++)
 #pragma unroll
-            for (int r = 0; r < 2; r++)
-                if (c0 + 16 * r < a.I) out[(size_t)row * a.I + c0 + 16 * r] = ldexpf(acc[m][r][i], e);
+                for (int r = 0; r < 2; r++) put(32 * m + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3), r, acc[m][r][i]);
+    } else {
+        // group g finishes registers i with i / (16 / WK) == g: the others' are
+        // handed over through LDS, [g][the other][r][i][thread]
+        constexpr int NI = 16 / WK;
+        float *js = (float *)lds;
+        auto at = [&](int g, int s, int r, int i) { return (((g * (WK - 1) + (s < g ? s : s - 1)) * 2 + r) * NI + i) * NT + gt; };
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+            if (m) __syncthreads();
+#pragma unroll
+            for (int g = 0; g < WK; g++)
+                if (g != wk)
+#pragma unroll
+                    for (int r = 0; r < 2; r++)
+#pragma unroll
+                        for (int i = 0; i < NI; i++) js[at(g, wk, r, i)] = acc[m][r][g * NI + i];
+            __syncthreads();
+#pragma unroll
+            for (int g = 0; g < WK; g++)
+                if (g == wk)
+#pragma unroll
+                    for (int r = 0; r < 2; r++)
+#pragma unroll
+                        for (int i = 0; i < NI; i++) {
+                            float v = acc[m][r][g * NI + i];
+#pragma unroll
+                            for (int s = 0; s < WK; s++)
+                                if (s != g) v += js[at(g, s, r, i)];
+                            const int k = g * NI + i;
+                            put(32 * m + 8 * (k >> 2) + 4 * (lane >> 5) + (k & 3), r, v);
+                        }
         }
+    }
 }
 
 // Sum of the K splits, in order.
@@ -418,12 +508,50 @@ int build_t_scales(DevCtx *ctx, ColiCudaTensor *t, bool update_only) {
 template <int KIND>
 static void launch_gemm_t(const GemmTArgs &a, int mt, hipStream_t st) {
     const int rb = (a.S + 32 * mt - 1) / (32 * mt);
-    if (mt == 4) hipLaunchKernelGGL((coli_gemm_t<KIND, 4, 4, 1>), dim3((a.nq + 1) / 2, rb, a.splits), dim3(256), 0, st, a);
-    else if (mt == 2) hipLaunchKernelGGL((coli_gemm_t<KIND, 2, 4, 1>), dim3((a.nq + 1) / 2, rb, a.splits), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((coli_gemm_t<KIND, 1, 2, 4>), dim3(a.nq, rb, a.splits), dim3(512), 0, st, a);
+    if (mt == 4)
+        hipLaunchKernelGGL((coli_gemm_t<KIND, 4, 4, 1, false>), dim3((a.nq + 1) / 2, rb, a.splits), dim3(256), 0, st, a);
+    else if (mt == 2)
+        hipLaunchKernelGGL((coli_gemm_t<KIND, 2, 2, 4, true>), dim3(a.nq, rb, a.splits), dim3(512), 0, st, a);
+    else
+        hipLaunchKernelGGL((coli_gemm_t<KIND, 1, 2, 4, true>), dim3(a.nq, rb, a.splits), dim3(512), 0, st, a);
 }
 
-int gemm_t_dev(DevCtx *ctx, ColiCudaTensor *t, float *dx, const float *dy, int S) {
+int gemm_t_plan(DevCtx *ctx, ColiCudaTensor *t, const float *dy, int S, GemmTPlan *g) {
+    *g = GemmTPlan{};
+    if (t->kind == COLI_KIND_GENERIC) return 1;
+    if (!t->sct && !build_t_scales(ctx, t, false)) return 0;
+    const int noct = t_octets(t), steps = noct / 4, mt = S <= 32 ? 1 : S <= 64 ? 2 : 4;
+    const bool few = mt < 4;
+    const size_t Sp = few ? 0 : ((size_t)S + 127) & ~(size_t)127, fb = (size_t)noct * Sp * 16;
+    const int cus = ctx->cu_count ? ctx->cu_count : 256;
+    const long blocks = (long)((S + 32 * mt - 1) / (32 * mt)) * (few ? t->nq : (t->nq + 1) / 2);
+    // workgroups for about two a CU, at least eight steps each
+    int splits = (int)std::max(1L, std::min((2L * cus + blocks - 1) / blocks, (long)std::max(1, steps / 8)));
+    const int per = (steps + splits - 1) / splits;
+    splits = (steps + per - 1) / per;
+    const size_t eb = (Sp * sizeof(int) + 255) & ~(size_t)255;
+    const size_t pb = splits > 1 ? (size_t)splits * S * t->I * sizeof(float) : 0;
+    if (2 * fb + eb + pb && !reserve_kept(ctx, &ctx->gt, 2 * fb + eb + pb, 0)) return 0;
+    uint8_t *p = (uint8_t *)ctx->gt.p;
+    g->mt = mt;
+    g->splits = splits;
+    g->per = per;
+    g->part = (float *)(p + 2 * fb + eb);
+    g->parts = splits > 1 ? splits : 0;
+    ColiTPrepArgs &a = g->prep;
+    a.dy = dy;
+    a.hi = (_Float16 *)p;
+    a.lo = (_Float16 *)(p + fb);
+    a.exps = (int *)(p + 2 * fb);
+    a.Sp = Sp;
+    a.S = S;
+    a.K = t->O;
+    a.noct = noct;
+    a.int4 = t->kind != COLI_KIND_FP4;
+    return 1;
+}
+
+int gemm_t_run(DevCtx *ctx, ColiCudaTensor *t, float *dx, const float *dy, int S, const GemmTPlan &g, bool with_join) {
     forget_emitted(ctx, dx, (size_t)S * t->I * sizeof(float));
     hipStream_t st = ctx->stream;
     if (t->kind == COLI_KIND_GENERIC) {
@@ -431,50 +559,36 @@ int gemm_t_dev(DevCtx *ctx, ColiCudaTensor *t, float *dx, const float *dy, int S
                            t->ng_src, t->I, t->O, dy, dx);
         return hip_check(hipGetLastError(), "generic gradient");
     }
-    if (!t->sct && !build_t_scales(ctx, t, false)) return 0;
-    const int noct = t_octets(t), steps = noct / 4, mt = S <= 32 ? 1 : S <= 64 ? 2 : 4;
-    const size_t Sp = ((size_t)S + 127) & ~(size_t)127, fb = (size_t)noct * Sp * 16;
-    const int cus = ctx->cu_count ? ctx->cu_count : 256;
-    const long blocks = (long)((S + 32 * mt - 1) / (32 * mt)) * (mt == 1 ? t->nq : (t->nq + 1) / 2);
-    // workgroups for about two a CU, at least eight steps each
-    int splits = (int)std::max(1L, std::min((2L * cus + blocks - 1) / blocks, (long)std::max(1, steps / (mt == 1 ? 16 : 8))));
-    const int per = (steps + splits - 1) / splits;
-    splits = (steps + per - 1) / per;
-    const size_t eb = (Sp * sizeof(int) + 255) & ~(size_t)255;
-    const size_t pb = splits > 1 ? (size_t)splits * S * t->I * sizeof(float) : 0;
-    if (!reserve_kept(ctx, &ctx->gt, 2 * fb + eb + pb, 0)) return 0;
-    uint8_t *p = (uint8_t *)ctx->gt.p;
+    if (g.mt == 4) {
+        hipLaunchKernelGGL(coli_t_prep_rows, dim3((S + 3) / 4), dim3(1024), 0, st, g.prep);
+        if (!hip_check(hipGetLastError(), "gradient rows")) return 0;
+    }
     GemmTArgs a = {};
     a.w = t->w;
     a.sct = (const _Float16 *)t->sct;
     a.ge = t->sct_ge;
-    a.hi = (_Float16 *)p;
-    a.lo = (_Float16 *)(p + fb);
-    a.exps = (int *)(p + 2 * fb);
-    a.Sp = Sp;
+    a.hi = g.prep.hi;
+    a.lo = g.prep.lo;
+    a.exps = g.prep.exps;
+    a.Sp = g.prep.Sp;
+    a.dy = dy;
+    a.O = t->O;
     a.nrt = t->nrt;
     a.nq = t->nq;
-    a.noct = noct;
+    a.noct = g.prep.noct;
     a.I = t->I;
     a.S = S;
-    a.splits = splits;
-    a.per = per;
-    a.out = splits > 1 ? (float *)(p + 2 * fb + eb) : dx;
-    const int vec = t->O % 4 == 0 && ((uintptr_t)dy & 15) == 0;
-    const int chunks = std::max(1, std::min(8, 2 * cus / ((S + 3) / 4)));
-    hipLaunchKernelGGL(coli_t_prep, dim3((S + 3) / 4, chunks), dim3(256), 0, st, dy, S, t->O, noct,
-                       (int)(t->kind != COLI_KIND_FP4), vec, Sp, (_Float16 *)a.hi, (_Float16 *)a.lo, (int *)a.exps);
-    if (!hip_check(hipGetLastError(), "gradient rows")) return 0;
-    if (t->kind == COLI_KIND_I4_H) launch_gemm_t<COLI_KIND_I4_H>(a, mt, st);
-    else if (t->kind == COLI_KIND_I4_F) launch_gemm_t<COLI_KIND_I4_F>(a, mt, st);
-    else launch_gemm_t<COLI_KIND_FP4>(a, mt, st);
+    a.splits = g.splits;
+    a.per = g.per;
+    a.out = g.parts ? g.part : dx;
+    if (t->kind == COLI_KIND_I4_H) launch_gemm_t<COLI_KIND_I4_H>(a, g.mt, st);
+    else if (t->kind == COLI_KIND_I4_F) launch_gemm_t<COLI_KIND_I4_F>(a, g.mt, st);
+    else launch_gemm_t<COLI_KIND_FP4>(a, g.mt, st);
     if (!hip_check(hipGetLastError(), "input gradient")) return 0;
-    if (splits > 1) {
-        const size_t n = (size_t)S * t->I;
-        hipLaunchKernelGGL(coli_t_join, dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, st, a.out, dx, n, splits);
-        return hip_check(hipGetLastError(), "input gradient join");
-    }
-    return 1;
+    if (!with_join || !g.parts) return 1;
+    const size_t n = (size_t)S * t->I;
+    hipLaunchKernelGGL(coli_t_join, dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, st, a.out, dx, n, g.splits);
+    return hip_check(hipGetLastError(), "input gradient join");
 }
 
 extern "C" int coli_hip_gemm_t_dev(ColiCudaTensor *t, float *dx_dev, const float *dy_dev, int S) {
@@ -482,5 +596,6 @@ extern "C" int coli_hip_gemm_t_dev(ColiCudaTensor *t, float *dx_dev, const float
     if (!tensor_computable(t) || !dx_dev || !dy_dev || S < 1 || S > COLI_GRAD_MAX_ROWS) return 0;
     DevCtx *ctx = ctx_of(t->device);
     if (!bind_ctx(ctx)) return 0;
-    return gemm_t_dev(ctx, t, dx_dev, dy_dev, S);
+    GemmTPlan g;
+    return gemm_t_plan(ctx, t, dy_dev, S, &g) && gemm_t_run(ctx, t, dx_dev, dy_dev, S, g, true);
 }

@@ -43,30 +43,30 @@ struct ColiHipLora {
     LoraMeta *meta;              // [slots]; rank 0: nothing set
 };
 
-typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
-
-// Eight consecutive factors as f32 (16-byte aligned).
-__device__ __forceinline__ void load8(const float *p, float (&v)[8]) {
-    const floatx4 a = *GPTR(floatx4, p), b = *GPTR(floatx4, p + 4);
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        v[i] = a[i];
-        v[4 + i] = b[i];
-    }
-}
-__device__ __forceinline__ void load8(const _Float16 *p, float (&v)[8]) {
-    const half8v a = *GPTR(half8v, p);
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = (float)a[i];
-}
 struct bf16_t {
     uint16_t bits;
 };
-__device__ __forceinline__ void load8(const bf16_t *p, float (&v)[8]) {
-    const u16x8 a = *GPTR(u16x8, p);
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = __uint_as_float((uint32_t)a[i] << 16);
-}
+
+// Eight consecutive factors as loaded, and as f32.
+template <typename T> struct Raw8 {
+    u32x4 w;
+    __device__ void load(const T *p) { w = *GPTR(u32x4, p); }
+    __device__ float get(int i) const {
+        const uint32_t v = w[i >> 1];
+        if constexpr (sizeof(T) == 2 && !__is_same(T, _Float16))
+            return __uint_as_float(i & 1 ? v & 0xffff0000u : v << 16);
+        else
+            return (float)__builtin_bit_cast(half2v, v)[i & 1];
+    }
+};
+template <> struct Raw8<float> {
+    floatx4 a, b;
+    __device__ void load(const float *p) {
+        a = *GPTR(floatx4, p);
+        b = *GPTR(floatx4, p + 4);
+    }
+    __device__ float get(int i) const { return i < 4 ? a[i & 3] : b[i & 3]; }
+};
 
 // ---------------------------------------------------------------------------
 // the bank
@@ -81,20 +81,34 @@ __global__ __launch_bounds__(256) void coli_lora_set(const T *__restrict__ a, co
     if (blockIdx.x == 0 && tid == 0) *meta = {rank, scale};
     if ((int)blockIdx.x < na) {
         const int r = blockIdx.x / ca, c0 = (blockIdx.x - r * ca) * 2048;
-        for (int c = c0 + tid; c < min(Ip, c0 + 2048); c += 256)
-            va[(size_t)r * Ip + c] = r < rank && c < I ? a[(size_t)r * I + c] : T{};
+        T v[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int c = c0 + tid + 256 * k;
+            v[k] = r < rank && c < I ? a[(size_t)r * I + c] : T{};
+        }
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (c0 + tid + 256 * k < Ip) va[(size_t)r * Ip + c0 + tid + 256 * k] = v[k];
         return;
     }
     __shared__ T tile[64][66];
     const int nb = blockIdx.x - na, no = Op / 64, o0 = (nb % no) * 64, r0 = (nb / no) * 64;
-    for (int k = tid; k < 4096; k += 256) {
-        const int o = o0 + (k >> 6), r = r0 + (k & 63);
-        tile[k >> 6][k & 63] = o < O && r < rank ? b[(size_t)o * rank + r] : T{};
+    const int nr = min(64, Rp - r0);   // 16, 32 or 64: a wave's lanes cover 64 / nr rows of B
+    T v[16];
+#pragma unroll
+    for (int k = 0; k < 16; k++) {
+        const int e = tid + 256 * k, o = o0 + e / nr, r = r0 + e % nr;
+        v[k] = e < 64 * nr && o < O && r < rank ? b[(size_t)o * rank + r] : T{};
     }
+#pragma unroll
+    for (int k = 0; k < 16; k++)
+        if (tid + 256 * k < 64 * nr) tile[(tid + 256 * k) / nr][(tid + 256 * k) % nr] = v[k];
     __syncthreads();
-    for (int k = tid; k < 4096; k += 256) {
-        const int r = r0 + (k >> 6);
-        if (r < Rp) vb[(size_t)r * Op + o0 + (k & 63)] = tile[k & 63][k >> 6];
+#pragma unroll
+    for (int k = 0; k < 16; k++) {
+        const int e = tid + 256 * k, r = e >> 6;
+        if (r < nr) vb[(size_t)(r0 + r) * Op + o0 + (e & 63)] = tile[e & 63][r];
     }
 }
 
@@ -113,12 +127,13 @@ struct LoraRows {
     int *ntile;
 };
 
-__device__ __forceinline__ bool lora_live(const LoraRows &w, int s) {
-    return s >= 0 && s < w.slots && w.meta[s].rank > 0;
-}
+// (an empty slot counts: its rank of 0 is met where the factors are)
+__device__ __forceinline__ bool lora_live(const LoraRows &w, int s) { return s >= 0 && s < w.slots; }
 
 // Tile t of the call into LDS rows[]: the slot, and its rows' number (0: no
-// such tile). Every wave calls it; the caller synchronizes.
+// such tile). Every wave calls it; the caller synchronizes. ALL (at most
+// COLI_LORA_BALLOT rows): a row without an adapter is a tile of its own, slot -1.
+template <bool ALL = false>
 __device__ __forceinline__ int lora_tile(const LoraRows &w, int t, int *rows, int &slot) {
     const int lane = threadIdx.x & 63;
     if (w.S <= COLI_LORA_BALLOT) {
@@ -126,7 +141,10 @@ __device__ __forceinline__ int lora_tile(const LoraRows &w, int t, int *rows, in
         const int s = lane < w.S ? w.slot[lane] : -1;
         const bool live = lora_live(w, s);
         slot = __builtin_amdgcn_readlane(live ? s : -1, t);
-        if (slot < 0) return 0;
+        if (slot < 0) {
+            if (ALL) rows[0] = t;
+            return ALL ? 1 : 0;
+        }
         const unsigned long long m = __builtin_amdgcn_ballot_w64(live && s == slot);
         const int first = __popcll(m & ((1ull << t) - 1ull));
         if (first % COLI_LORA_TILE) return 0;
@@ -141,23 +159,26 @@ __device__ __forceinline__ int lora_tile(const LoraRows &w, int t, int *rows, in
     return e.z;
 }
 
-// Stable counting sort of the rows by slot: eight waves count and then place a
+// Stable counting sort of the rows by slot: NW waves count and then place a
 // run of rows each, 64 at a time, so a slot's rows keep their order (the sums
 // over them do not depend on timing).
-__global__ __launch_bounds__(512) void coli_lora_sort(LoraRows w) {
-    extern __shared__ int cnt[];   // [8][slots]
-    __shared__ int wsum[8][2];
+template <int NW>
+__global__ __launch_bounds__(64 * NW) void coli_lora_sort(LoraRows w) {
+    extern __shared__ int cnt[];   // [NW][slots]
+    __shared__ int wsum[NW][2];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nsl = w.slots;
-    const int per = ((w.S + 7) / 8 + 63) & ~63, r0 = wave * per, r1 = min(w.S, r0 + per);
-    for (int k = tid; k < 8 * nsl; k += 512) cnt[k] = 0;
+    const int per = ((w.S + NW - 1) / NW + 63) & ~63, r0 = wave * per, r1 = min(w.S, r0 + per);
+    for (int k = tid; k < NW * nsl; k += 64 * NW) cnt[k] = 0;
     __syncthreads();
     int *mine = cnt + wave * nsl;
     auto slot_of = [&](int r) {
         const int s = r < r1 ? w.slot[r] : -1;
         return lora_live(w, s) ? s : -1;
     };
+    int nx = slot_of(r0 + lane);
     for (int r = r0; r < r1; r += 64) {
-        const int s = slot_of(r + lane);
+        const int s = nx;
+        nx = slot_of(r + 64 + lane);   // (-1 past the run)
         unsigned long long todo = __builtin_amdgcn_ballot_w64(s >= 0);
         while (todo) {
             const int sl = __builtin_amdgcn_readlane(s, __builtin_ctzll(todo));
@@ -169,11 +190,11 @@ __global__ __launch_bounds__(512) void coli_lora_sort(LoraRows w) {
     __syncthreads();
     // exclusive sums over (slot, wave), of the rows and of the tiles
     int base = 0, tbase = 0;
-    for (int c0 = 0; c0 < nsl; c0 += 512) {
+    for (int c0 = 0; c0 < nsl; c0 += 64 * NW) {
         const int s = c0 + tid;
         int n = 0;
         if (s < nsl)
-            for (int v = 0; v < 8; v++) n += cnt[v * nsl + s];
+            for (int v = 0; v < NW; v++) n += cnt[v * nsl + s];
         const int nt = (n + COLI_LORA_TILE - 1) / COLI_LORA_TILE;
         int x = n, y = nt;
 #pragma unroll
@@ -190,7 +211,7 @@ __global__ __launch_bounds__(512) void coli_lora_sort(LoraRows w) {
         }
         __syncthreads();
         int bx = base, by = tbase;
-        for (int v = 0; v < 8; v++) {
+        for (int v = 0; v < NW; v++) {
             if (v < wave) {
                 bx += wsum[v][0];
                 by += wsum[v][1];
@@ -204,7 +225,7 @@ __global__ __launch_bounds__(512) void coli_lora_sort(LoraRows w) {
             for (int k = 0; k < nt; k++)
                 w.tile[t0 + k] = make_int4(s, first + k * COLI_LORA_TILE, min(COLI_LORA_TILE, n - k * COLI_LORA_TILE), 0);
             int at = first;
-            for (int v = 0; v < 8; v++) {
+            for (int v = 0; v < NW; v++) {
                 const int c = cnt[v * nsl + s];
                 cnt[v * nsl + s] = at;
                 at += c;
@@ -213,8 +234,10 @@ __global__ __launch_bounds__(512) void coli_lora_sort(LoraRows w) {
         __syncthreads();
     }
     if (tid == 0) *w.ntile = tbase;
+    nx = slot_of(r0 + lane);
     for (int r = r0; r < r1; r += 64) {
-        const int s = slot_of(r + lane);
+        const int s = nx;
+        nx = slot_of(r + 64 + lane);   // (-1 past the run)
         unsigned long long todo = __builtin_amdgcn_ballot_w64(s >= 0);
         while (todo) {
             const int sl = __builtin_amdgcn_readlane(s, __builtin_ctzll(todo));
@@ -232,236 +255,383 @@ __global__ __launch_bounds__(512) void coli_lora_sort(LoraRows w) {
 // the three products
 // ---------------------------------------------------------------------------
 template <typename T> struct LoraSide {
-    const float *x;              // [S][N] rows (shrink and outer: read; expand: y)
+    const float *x;              // [S][N] rows (shrink, outer)
     const T *v;                  // [slots][Rp][Np]
     float *h;                    // [splits][S][Rp] shrunk rows
     float *out;                  // expand: y [S][N]; outer: the gradient
+    const float *part;           // expand: y is the sum of these [parts][S][N] instead of what it holds
+    int parts;
     int N, Np, splits;
-    int vec;                     // N % 4 == 0 and rows 16-byte aligned
 };
 
-// Eight floats of a row from column n on, zeros past N.
-__device__ __forceinline__ void row8(const float *xr, int n, int N, int vec, float (&v)[8]) {
-    if (vec && n + 8 <= N) {
-        load8(xr + n, v);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = n + i < N ? xr[n + i] : 0.0f;
-    }
-}
-
-// shrink: workgroup (tile, column split, NR rank tiles of one side). The four
-// waves take 32 columns in turn: lane (m, k) reads eight columns of row m and
-// of factor m, which feed eight MFMAs (the order of the columns inside a sum
-// is free).
-template <typename T, int NR>
-__global__ __launch_bounds__(256) void coli_lora_shrink(LoraRows w, LoraSide<T> s0, LoraSide<T> s1, int Rp, int nz) {
+// shrink: workgroup (tile, column split, NR rank tiles of one side). The W
+// waves take 32 SUB columns in turn: lane (m, k) reads eight columns of row m
+// and of factor m, which feed eight MFMAs (the order of the columns inside a
+// sum is free); the next step is requested before this one's products. With
+// four waves, workgroups past nown build the projection's activation fragments.
+template <typename T, int NR, int W>
+__global__ __launch_bounds__(64 * W) void coli_lora_shrink(LoraRows w, LoraSide<T> s0, LoraSide<T> s1, int Rp, int nz,
+                                                           int tiles, int splits, int nown, ColiPrepArgs ride) {
+    constexpr int SUB = NR * sizeof(T) <= 8 ? 2 : 1, STEP = 32 * SUB;
     __shared__ int rows[COLI_LORA_TILE];
-    __shared__ float red[4][NR][16][17];
+    __shared__ float red[W][16][17];
+    const int b = blockIdx.x;
+    if constexpr (W == 4) {
+        if (b >= nown) {
+            prep_frag_block(ride, b - nown);
+            return;
+        }
+    }
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, kq = lane >> 4;
+    const int t = b % tiles, sp = b / tiles % splits, z = b / (tiles * splits);
     int slot = 0;
-    const int n = lora_tile(w, blockIdx.x, rows, slot);
+    const int n = lora_tile(w, t, rows, slot);
     if (n == 0) return;   // (uniform over the workgroup)
-    const LoraSide<T> s = (int)blockIdx.z < nz ? s0 : s1;
-    const int rt0 = (blockIdx.z % nz) * NR, sp = blockIdx.y;
+    const LoraSide<T> s = z < nz ? s0 : s1;
+    const int rt0 = (z % nz) * NR;
     if (sp >= s.splits || 16 * rt0 >= w.meta[slot].rank) return;
     __syncthreads();
-    const int steps = (s.N + 31) / 32, per = (steps + s.splits - 1) / s.splits;
-    const int k1 = min(steps, (sp + 1) * per);
-    const float *xr = s.x + (size_t)rows[min(m, n - 1)] * s.N;
-    const T *vr = s.v + ((size_t)slot * Rp + 16 * rt0 + m) * s.Np;
+    const int full = s.N / STEP, per = (full + s.splits - 1) / s.splits;
+    const int k1 = min(full, (sp + 1) * per);
+    const float *xr = s.x + (size_t)rows[min(m, n - 1)] * s.N + 8 * kq;
+    const T *vr = s.v + ((size_t)slot * Rp + 16 * rt0 + m) * s.Np + 8 * kq;
     floatx4 acc[NR];
 #pragma unroll
     for (int r = 0; r < NR; r++) acc[r] = (floatx4){0.f, 0.f, 0.f, 0.f};
-    for (int k = sp * per + wave; k < k1; k += 4) {
-        const int c = 32 * k + 8 * kq;
-        float xv[8], vv[NR][8];
-        row8(xr, c, s.N, s.vec, xv);
+    struct Step {
+        f4u x[SUB][2];
+        Raw8<T> v[SUB][NR];
+    };
+    auto load = [&](int k, Step &st) {
 #pragma unroll
-        for (int r = 0; r < NR; r++) load8(vr + (size_t)16 * r * s.Np + min(c, s.Np - 8), vv[r]);
+        for (int u = 0; u < SUB; u++) {
+            const float *p = xr + (size_t)STEP * k + 32 * u;
+            st.x[u][0] = *GPTR(f4u, p);
+            st.x[u][1] = *GPTR(f4u, p + 4);
 #pragma unroll
-        for (int r = 0; r < NR; r++)
+            for (int r = 0; r < NR; r++) st.v[u][r].load(vr + (size_t)16 * r * s.Np + (size_t)STEP * k + 32 * u);
+        }
+    };
+    Step cur, nxt;
+    int k = sp * per + wave;
+    if (k < k1) {
+        load(k, cur);
+        for (; k < k1; k += W) {
+            load(min(k + W, k1 - 1), nxt);
 #pragma unroll
-            for (int j = 0; j < 8; j++) acc[r] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[j], vv[r][j], acc[r], 0, 0, 0);
+            for (int u = 0; u < SUB; u++)
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+#pragma unroll
+                    for (int r = 0; r < NR; r++)
+                        acc[r] = __builtin_amdgcn_mfma_f32_16x16x4f32(cur.x[u][j >> 2][j & 3], cur.v[u][r].get(j), acc[r], 0, 0, 0);
+            cur = nxt;
+        }
     }
+    // columns past the last whole step: the last split, 32 a wave (the factors'
+    // padding is zero, the row is read as zero past N)
+    if (sp == s.splits - 1) {
+        for (int c = STEP * full + 32 * wave; c < s.N; c += 32 * W) {
+            float xv[8];
 #pragma unroll
-    for (int r = 0; r < NR; r++)
+            for (int j = 0; j < 8; j++) xv[j] = c + 8 * kq + j < s.N ? xr[c + j] : 0.0f;
+            Raw8<T> v[NR];
 #pragma unroll
-        for (int i = 0; i < 4; i++) red[wave][r][4 * kq + i][m] = acc[r][i];
-    __syncthreads();
-    for (int e = threadIdx.x; e < NR * 256; e += 256) {
-        const int r = e >> 8, row = (e >> 4) & 15, c = e & 15;
-        if (row < n)
-            s.h[((size_t)sp * w.S + rows[row]) * Rp + 16 * (rt0 + r) + c] =
-                (red[0][r][row][c] + red[1][r][row][c]) + (red[2][r][row][c] + red[3][r][row][c]);
+            for (int r = 0; r < NR; r++) v[r].load(vr + (size_t)16 * r * s.Np + c);
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+#pragma unroll
+                for (int r = 0; r < NR; r++) acc[r] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[j], v[r].get(j), acc[r], 0, 0, 0);
+        }
+    }
+    for (int r = 0; r < NR; r++) {
+        if (r) __syncthreads();
+#pragma unroll
+        for (int q = 0; q < NR; q++)
+            if (q == r)
+#pragma unroll
+                for (int i = 0; i < 4; i++) red[wave][4 * kq + i][m] = acc[q][i];
+        __syncthreads();
+        if (threadIdx.x < 256) {
+            const int row = threadIdx.x >> 4, c = threadIdx.x & 15;
+            float v = red[0][row][c];
+#pragma unroll
+            for (int q = 1; q < W; q++) v += red[q][row][c];
+            if (row < n) s.h[((size_t)sp * w.S + rows[row]) * Rp + 16 * (rt0 + r) + c] = v;
+        }
     }
 }
 
-// scale h of one row's rank r: the column splits joined in order; zero past
-// the adapter's rank.
-__device__ __forceinline__ float lora_h(const float *h, int splits, size_t pitch, int r, int rank, float scale) {
-    if (r >= rank) return 0.0f;
-    float v = h[r];
-    for (int p = 1; p < splits; p++) v += h[p * pitch + r];
-    return v * scale;
+// An element of h: the column splits joined in order, eight requested at once.
+__device__ __forceinline__ float lora_h(const float *h, int splits, size_t pitch) {
+    float v = 0.0f;
+    for (int p0 = 0; p0 < splits; p0 += 8) {
+        float t[8];
+#pragma unroll
+        for (int q = 0; q < 8; q++) t[q] = h[min(p0 + q, splits - 1) * pitch];
+#pragma unroll
+        for (int q = 0; q < 8; q++) v += p0 + q < splits ? t[q] : 0.0f;
+    }
+    return v;
 }
 
 // expand: workgroup (tile, 512 columns), a wave 128 of them: lane (m, k) holds
-// row m's h of rank 4 q + k and eight columns of the factor, eight MFMAs a
-// step of four ranks. The lane's results are eight consecutive columns of four
-// rows, added to y.
-template <typename T>
+// row m's h of rank 4 q + k and eight columns of the factor, eight MFMAs a step
+// of four ranks. The lane's results are eight consecutive columns of four
+// rows, added to y (JOIN: to the sum of y's partial sums, also in rows without
+// an adapter). Factors and y are requested before h is joined.
+template <typename T, bool JOIN>
 __global__ __launch_bounds__(256) void coli_lora_expand(LoraRows w, LoraSide<T> s, int Rp) {
     extern __shared__ float hs[];   // [16][Rp + 1]
     __shared__ int rows[COLI_LORA_TILE];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, kq = lane >> 4;
     int slot = 0;
-    const int n = lora_tile(w, blockIdx.x, rows, slot);
+    const int n = lora_tile<JOIN>(w, blockIdx.x, rows, slot);
     if (n == 0) return;   // (uniform over the workgroup)
-    __syncthreads();
+    const bool none = slot < 0;
+    if (none) slot = 0;
+    const int c0 = blockIdx.y * 512 + wave * 128, c = c0 + 8 * m;
+    const T *vr = s.v + (size_t)slot * Rp * s.Np + (size_t)kq * s.Np + min(c, s.Np - 8);
+    Raw8<T> v[4];
+#pragma unroll
+    for (int q = 0; q < 4; q++) v[q].load(vr + (size_t)4 * q * s.Np);   // (Rp >= 16)
     const LoraMeta meta = w.meta[slot];
-    const int rank = min(meta.rank, Rp), r4 = (rank + 3) & ~3;
-    for (int e = threadIdx.x; e < 16 * r4; e += 256) {
-        const int row = e / r4, r = e - row * r4;
-        hs[row * (Rp + 1) + r] = row < n ? lora_h(s.h + (size_t)rows[row] * Rp, s.splits, (size_t)w.S * Rp, r, rank, meta.scale) : 0.0f;
+    const int rank = none ? 0 : min(meta.rank, Rp), r16 = (rank + 15) & ~15;
+    if (!JOIN && rank == 0) return;
+    __syncthreads();
+    const bool whole = c + 8 <= s.N;
+    const float *yr[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) yr[i] = (JOIN ? s.part : s.out) + (size_t)rows[min(4 * kq + i, n - 1)] * s.N + c;
+    f4u y[4][2];
+    auto load_y = [&](f4u (&v)[4][2]) {
+        if (whole) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                v[i][0] = *GPTR(f4u, yr[i]);
+                v[i][1] = *GPTR(f4u, yr[i] + 4);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[i][j >> 2][j & 3] = c + j < s.N ? yr[i][j] : 0.0f;
+        }
+    };
+    load_y(y);
+    if constexpr (JOIN) {
+        for (int p = 1; p < s.parts; p++) {
+            f4u z[4][2];
+#pragma unroll
+            for (int i = 0; i < 4; i++) yr[i] += (size_t)w.S * s.N;
+            load_y(z);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) y[i][e] += z[i][e];
+        }
+    }
+    for (int e = threadIdx.x; e < 16 * r16; e += 256) {
+        const int row = e / r16, r = e - row * r16;
+        // (past the rank: zeros, also where a row of infinities shrank to NaN)
+        const float hv = lora_h(s.h + (size_t)rows[min(row, n - 1)] * Rp + min(r, rank - 1), s.splits, (size_t)w.S * Rp);
+        hs[row * (Rp + 1) + r] = row < n && r < rank ? meta.scale * hv : 0.0f;
     }
     __syncthreads();
-    const int c = blockIdx.y * 512 + wave * 128 + 8 * m;
-    if (blockIdx.y * 512 + wave * 128 >= s.Np) return;
-    const T *vr = s.v + (size_t)slot * Rp * s.Np + min(c, s.Np - 8);
+    if (c0 >= s.Np) return;
     floatx4 acc[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) acc[j] = (floatx4){0.f, 0.f, 0.f, 0.f};
-    for (int r = 0; r < r4; r += 4) {
-        float vv[8];
-        load8(vr + (size_t)(r + kq) * s.Np, vv);
-        const float hv = hs[m * (Rp + 1) + r + kq];
+    for (int r = 0; r < r16; r += 16) {
+        Raw8<T> nx[4];
+        const int rn = r + 16 < r16 ? r + 16 : r;
 #pragma unroll
-        for (int j = 0; j < 8; j++) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(hv, vv[j], acc[j], 0, 0, 0);
+        for (int q = 0; q < 4; q++) nx[q].load(vr + (size_t)(rn + 4 * q) * s.Np);
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const float hv = hs[m * (Rp + 1) + r + 4 * q + kq];
+#pragma unroll
+            for (int j = 0; j < 8; j++) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(hv, v[q].get(j), acc[j], 0, 0, 0);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; q++) v[q] = nx[q];
     }
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const int row = 4 * kq + i;
         if (row >= n || c >= s.N) continue;
-        float *yr = s.out + (size_t)rows[row] * s.N + c;
-        if (s.vec && c + 8 <= s.N) {
-            floatx4 y0 = *(const floatx4 *)yr, y1 = *(const floatx4 *)(yr + 4);
+        float *to = s.out + (size_t)rows[row] * s.N + c;
+        f4u y0 = y[i][0], y1 = y[i][1];
+        if (rank) {
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 y0[j] += acc[j][i];
                 y1[j] += acc[4 + j][i];
             }
-            *(floatx4 *)yr = y0;
-            *(floatx4 *)(yr + 4) = y1;
+        }
+        if (whole) {
+            *(f4u *)to = y0;
+            *(f4u *)(to + 4) = y1;
         } else {
 #pragma unroll
             for (int j = 0; j < 8; j++)
-                if (c + j < s.N) yr[j] += acc[j][i];
+                if (c + j < s.N) to[j] = j < 4 ? y0[j & 3] : y1[j & 3];
         }
     }
 }
 
-// outer: workgroup (64 columns, slot and NR rank tiles, side); the four waves
-// take 16 rows of the slot in turn, four MFMA steps of four rows, and their
-// sums are joined in LDS. Side 0: dA [slots][max_rank][N]; side 1 (dB): stored
-// transposed, [slots][N][max_rank]. Every element is written, zeros where a
-// slot has no rows or rank.
-template <typename T, int NR>
-__global__ __launch_bounds__(256) void coli_lora_outer(LoraRows w, LoraSide<T> s0, LoraSide<T> s1, int Rp, int max_rank) {
+// outer: workgroup (64 columns, slot and NR rank tiles, side); the W waves take
+// 16 rows of the slot in turn, four MFMA steps of four rows, the next 16 rows
+// requested before this step's products and their numbers a step earlier; the
+// waves' sums are joined in LDS. Side 0: dA [slots][max_rank][N]; side 1 (dB):
+// stored transposed, [slots][N][max_rank]. Every element is written, zeros
+// where a slot has no rows or rank.
+template <typename T, int NR, int W>
+__global__ __launch_bounds__(64 * W) void coli_lora_outer(LoraRows w, LoraSide<T> s0, LoraSide<T> s1, int Rp, int max_rank) {
+    constexpr int RW = W > 8 ? 8 : W;   // waves of the LDS join
+    constexpr bool LIST = W > 4;        // beyond COLI_LORA_BALLOT rows
     __shared__ int rows[COLI_LORA_BALLOT];
-    __shared__ float red[4][64][17];
+    __shared__ float hl[LIST ? 1 : COLI_LORA_BALLOT][LIST ? 1 : 16 * NR + 1];
+    __shared__ float red[RW][64][17];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, kq = lane >> 4;
     const int nrp = (Rp / 16 + NR - 1) / NR, slot = blockIdx.y / nrp, rt0 = (blockIdx.y - slot * nrp) * NR;
     const bool side1 = blockIdx.z != 0;
     // (h of one side meets the rows of the other)
     const float *x = side1 ? s1.x : s0.x;
-    const int N = side1 ? s1.N : s0.N, vec = side1 ? s1.vec : s0.vec;
-    const float *h = side1 ? s0.h : s1.h;
+    const int N = side1 ? s1.N : s0.N;
+    const float *h = (side1 ? s0.h : s1.h) + 16 * rt0;
     const int splits = side1 ? s0.splits : s1.splits;
     float *out = side1 ? s1.out : s0.out;
     const int c0 = blockIdx.x * 64, c = c0 + 4 * m;
     if (c0 >= N) return;
     const LoraMeta meta = w.meta[slot];
     const int rank = min(meta.rank, Rp);
-    int cnt = 0, first = 0;
-    if (rank > 0) {
-        if (w.S <= COLI_LORA_BALLOT) {
-            const unsigned long long mk = __builtin_amdgcn_ballot_w64(lane < w.S && w.slot[min(lane, w.S - 1)] == slot);
-            if (mk >> lane & 1) rows[__popcll(mk & ((1ull << lane) - 1ull))] = lane;
-            cnt = __popcll(mk);
-        } else {
-            const int2 rn = w.run[slot];
-            first = rn.x;
-            cnt = rn.y;
-        }
+    int cnt = 0;
+    const int *list = rows;
+    if constexpr (!LIST) {
+        const unsigned long long mk = __builtin_amdgcn_ballot_w64(lane < w.S && w.slot[min(lane, w.S - 1)] == slot);
+        if (mk >> lane & 1) rows[__popcll(mk & ((1ull << lane) - 1ull))] = lane;
+        cnt = __popcll(mk);
+    } else {
+        const int2 rn = w.run[slot];
+        list = w.perm + rn.x;
+        cnt = rn.y;
     }
+    if (rank <= 16 * rt0) cnt = 0;
     __syncthreads();
+    const size_t pitch = (size_t)w.S * Rp;
+    if constexpr (!LIST) {
+        for (int e = threadIdx.x; e < cnt * 16 * NR; e += 64 * W) {
+            const int p = e / (16 * NR), r = e % (16 * NR);
+            hl[p][r] = lora_h(h + (size_t)rows[p] * Rp + r, splits, pitch);
+        }
+        __syncthreads();
+    }
     floatx4 acc[NR][4];
 #pragma unroll
     for (int r = 0; r < NR; r++)
 #pragma unroll
         for (int j = 0; j < 4; j++) acc[r][j] = (floatx4){0.f, 0.f, 0.f, 0.f};
-    const size_t pitch = (size_t)w.S * Rp;
-    for (int p0 = 16 * wave; p0 < cnt; p0 += 64) {
-        float xv[4][4], hv[4][NR];
+    const bool whole = c + 4 <= N;
+    struct Step {
+        f4u x[4];
+        float h[4][NR];
+    };
+    auto numbers = [&](int p0, int (&rw)[4]) {
+#pragma unroll
+        for (int u = 0; u < 4; u++) rw[u] = list[min(p0 + 4 * u + kq, cnt - 1)];
+    };
+    auto load = [&](int p0, const int (&rw)[4], Step &st) {
 #pragma unroll
         for (int u = 0; u < 4; u++) {
-            const int p = p0 + 4 * u + kq;
-            const bool live = p < cnt;
-            const int pc = live ? p : cnt - 1;
-            const int row = w.S <= COLI_LORA_BALLOT ? rows[pc] : w.perm[first + pc];
-            const float *xr = x + (size_t)row * N;
-            if (vec && c + 4 <= N) {
-                const floatx4 t = *GPTR(floatx4, xr + c);
-#pragma unroll
-                for (int j = 0; j < 4; j++) xv[u][j] = live ? t[j] : 0.0f;
+            const float *xr = x + (size_t)rw[u] * N + c;
+            if (whole) {
+                st.x[u] = *GPTR(f4u, xr);
             } else {
 #pragma unroll
-                for (int j = 0; j < 4; j++) xv[u][j] = live && c + j < N ? xr[c + j] : 0.0f;
+                for (int j = 0; j < 4; j++) st.x[u][j] = c + j < N ? xr[j] : 0.0f;
             }
 #pragma unroll
             for (int r = 0; r < NR; r++) {
-                const int rk = 16 * (rt0 + r) + m;
-                hv[u][r] = live ? lora_h(h + (size_t)row * Rp, splits, pitch, rk, rank, meta.scale) : 0.0f;
+                if constexpr (LIST) {
+                    const float *hr = h + (size_t)rw[u] * Rp + 16 * r + m;
+                    float v = hr[0];
+                    if (splits > 1) v += hr[pitch];
+                    if (splits > 2) v += hr[2 * pitch];
+                    if (splits > 3) v += hr[3 * pitch];
+                    st.h[u][r] = v;
+                } else {
+                    st.h[u][r] = hl[min(p0 + 4 * u + kq, cnt - 1)][16 * r + m];
+                }
+            }
+            if (p0 + 4 * u + kq >= cnt) {
+                st.x[u] = (f4u){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int r = 0; r < NR; r++) st.h[u][r] = 0.0f;
             }
         }
+    };
+    int p0 = 16 * wave;
+    if (p0 < cnt) {
+        int rw[4];
+        Step cur, nxt;
+        numbers(p0, rw);
+        load(p0, rw, cur);
+        numbers(p0 + 16 * W, rw);
+        for (; p0 < cnt; p0 += 16 * W) {
+            int rn[4];
+            numbers(p0 + 32 * W, rn);
+            load(p0 + 16 * W, rw, nxt);
 #pragma unroll
-        for (int u = 0; u < 4; u++)
+            for (int u = 0; u < 4; u++)
 #pragma unroll
-            for (int r = 0; r < NR; r++)
+                for (int r = 0; r < NR; r++)
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    acc[r][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(hv[u][r], xv[u][j], acc[r][j], 0, 0, 0);
+                    for (int j = 0; j < 4; j++)
+                        acc[r][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(cur.h[u][r], cur.x[u][j], acc[r][j], 0, 0, 0);
+            cur = nxt;
+#pragma unroll
+            for (int u = 0; u < 4; u++) rw[u] = rn[u];
+        }
     }
-#pragma unroll
     for (int r = 0; r < NR; r++) {
         __syncthreads();
+        // lane (m, kq): columns 4 m + j, ranks 4 kq + i
+        if (W > RW && wave >= RW) {
 #pragma unroll
-        for (int j = 0; j < 4; j++)
+            for (int q = 0; q < NR; q++)
+                if (q == r)
 #pragma unroll
-            for (int i = 0; i < 4; i++) red[wave][lane][4 * i + j] = acc[r][j][i];
+                    for (int j = 0; j < 4; j++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) red[wave - RW][lane][4 * i + j] = acc[q][j][i];
+        }
+        if (W > RW) __syncthreads();
+        if (wave < RW) {
+#pragma unroll
+            for (int q = 0; q < NR; q++)
+                if (q == r)
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            float v = acc[q][j][i];
+                            if (W > RW) v += red[wave][lane][4 * i + j];
+                            red[wave][lane][4 * i + j] = v;
+                        }
+        }
         __syncthreads();
-        // wave i finishes rank 4 kq + i of the tile
-        float v[4];
+        for (int e = threadIdx.x; e < 1024; e += 64 * W) {
+            const int rk = side1 ? e & 15 : e >> 6, col = side1 ? e >> 4 : e & 63;
+            const int ln = (col >> 2) + 16 * (rk >> 2), at = 4 * (rk & 3) + (col & 3);
+            float v = red[0][ln][at];
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            v[j] = (red[0][lane][4 * wave + j] + red[1][lane][4 * wave + j]) +
-                   (red[2][lane][4 * wave + j] + red[3][lane][4 * wave + j]);
-        const int rk = 16 * (rt0 + r) + 4 * kq + wave;
-        if (rk >= max_rank) continue;
-        if (side1) {
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (c + j < N) out[((size_t)slot * N + c + j) * max_rank + rk] = v[j];
-        } else {
-            float *o = out + ((size_t)slot * max_rank + rk) * N + c;
-            if (vec && c + 4 <= N) {
-                *(floatx4 *)o = (floatx4){v[0], v[1], v[2], v[3]};
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (c + j < N) o[j] = v[j];
-            }
+            for (int q = 1; q < RW; q++) v += red[q][ln][at];
+            const int k = 16 * (rt0 + r) + rk;
+            // (past the rank: zeros, also where a row of infinities shrank to NaN)
+            v = k < rank ? v * meta.scale : 0.0f;
+            if (k < max_rank && c0 + col < N)
+                out[side1 ? ((size_t)slot * N + c0 + col) * max_rank + k : ((size_t)slot * max_rank + k) * N + c0 + col] = v;
         }
     }
 }
@@ -469,11 +639,15 @@ __global__ __launch_bounds__(256) void coli_lora_outer(LoraRows w, LoraSide<T> s
 // ---------------------------------------------------------------------------
 // launches
 // ---------------------------------------------------------------------------
-// Column splits of the shrink: enough workgroups for two a CU, each of at
-// least 256 columns (two steps of its waves).
-static int shrink_splits(const DevCtx *ctx, int tiles, int N) {
-    const int want = (2 * (ctx->cu_count ? ctx->cu_count : 256) + tiles - 1) / tiles;
-    return std::max(1, std::min(std::min(want, 32), (N + 255) / 256));
+// Column splits of one side's shrink: workgroups of `cols` columns such that
+// all of them are about two a CU (four waves each up to COLI_LORA_BALLOT rows:
+// at least a step a wave; eight waves beyond, where every product over h adds
+// the splits again: at most four).
+static int shrink_splits(const DevCtx *ctx, int S, long columns, int N) {
+    const int cus = ctx->cu_count ? ctx->cu_count : 256;
+    const bool few = S <= COLI_LORA_BALLOT;
+    const long cols = std::max(few ? 256L : 512L, columns / (2 * cus));
+    return (int)std::max(1L, std::min((N + cols / 2) / cols, few ? 16L : 4L));
 }
 
 static int lora_tiles(int S, int slots) {
@@ -496,13 +670,17 @@ static int lora_rows(DevCtx *ctx, const ColiHipLora *l, const int *slot_dev, int
     w->run = (int2 *)(p + tb);
     w->perm = (int *)(p + tb + rb);
     w->ntile = (int *)(p + tb + rb + pb);
-    hipLaunchKernelGGL(coli_lora_sort, dim3(1), dim3(512), (size_t)8 * l->slots * sizeof(int), ctx->stream, *w);
+    // (a counter for each wave and slot: 32 KiB of LDS)
+    if (l->slots <= 512)
+        hipLaunchKernelGGL((coli_lora_sort<16>), dim3(1), dim3(1024), (size_t)16 * l->slots * sizeof(int), ctx->stream, *w);
+    else
+        hipLaunchKernelGGL((coli_lora_sort<8>), dim3(1), dim3(512), (size_t)8 * l->slots * sizeof(int), ctx->stream, *w);
     return hip_check(hipGetLastError(), "adapter rows");
 }
 
 template <typename T>
 static LoraSide<T> lora_side(const ColiHipLora *l, bool b, const float *x, float *h, float *out, int splits) {
-    LoraSide<T> s;
+    LoraSide<T> s = {};
     s.x = x;
     s.v = (const T *)(b ? l->bt : l->a);
     s.h = h;
@@ -510,40 +688,54 @@ static LoraSide<T> lora_side(const ColiHipLora *l, bool b, const float *x, float
     s.N = b ? l->O : l->I;
     s.Np = b ? l->Op : l->Ip;
     s.splits = splits;
-    s.vec = s.N % 4 == 0 && (((uintptr_t)x | (uintptr_t)out) & 15) == 0;
     return s;
 }
 
+// Up to COLI_LORA_BALLOT rows the launch also runs `ride`; beyond, its
+// workgroups have eight waves and the projection launches that build itself.
 template <typename T>
 static int launch_shrink(DevCtx *ctx, const ColiHipLora *l, const LoraRows &w, const LoraSide<T> &s0,
-                         const LoraSide<T> &s1, int sides) {
+                         const LoraSide<T> &s1, int sides, const ColiPrepArgs &ride) {
     const int tiles = lora_tiles(w.S, l->slots), nrt = l->Rp / 16, sp = std::max(s0.splits, sides > 1 ? s1.splits : 1);
-#define COLI_SHRINK(NR)                                                                                              \
-    hipLaunchKernelGGL((coli_lora_shrink<T, NR>), dim3(tiles, sp, sides *((nrt + NR - 1) / NR)), dim3(256), 0,         \
-                       ctx->stream, w, s0, s1, l->Rp, (nrt + NR - 1) / NR)
-    if (nrt == 1) COLI_SHRINK(1);
-    else if (nrt == 2) COLI_SHRINK(2);
-    else COLI_SHRINK(4);
+    const int nr = nrt >= 4 ? 4 : nrt, nz = nrt / nr, nown = tiles * sp * sides * nz;
+#define COLI_SHRINK(NR, W)                                                                                            hipLaunchKernelGGL((coli_lora_shrink<T, NR, W>), dim3(nown + ride.nblocks), dim3(64 * W), 0,                               ctx->stream, w, s0, s1, l->Rp, nz, tiles, sp, nown, ride)
+    if (w.S <= COLI_LORA_BALLOT) {
+        if (nr == 1) COLI_SHRINK(1, 4);
+        else if (nr == 2) COLI_SHRINK(2, 4);
+        else COLI_SHRINK(4, 4);
+    } else {
+        if (nr == 1) COLI_SHRINK(1, 8);
+        else if (nr == 2) COLI_SHRINK(2, 8);
+        else COLI_SHRINK(4, 8);
+    }
 #undef COLI_SHRINK
     return hip_check(hipGetLastError(), "adapter shrink");
 }
 
 template <typename T>
 static int launch_expand(DevCtx *ctx, const ColiHipLora *l, const LoraRows &w, const LoraSide<T> &s) {
-    hipLaunchKernelGGL((coli_lora_expand<T>), dim3(lora_tiles(w.S, l->slots), (s.Np + 511) / 512), dim3(256),
-                       (size_t)16 * (l->Rp + 1) * sizeof(float), ctx->stream, w, s, l->Rp);
+    const dim3 grid(lora_tiles(w.S, l->slots), (s.Np + 511) / 512);
+    const size_t shm = (size_t)16 * (l->Rp + 1) * sizeof(float);
+    if (s.parts)
+        hipLaunchKernelGGL((coli_lora_expand<T, true>), grid, dim3(256), shm, ctx->stream, w, s, l->Rp);
+    else
+        hipLaunchKernelGGL((coli_lora_expand<T, false>), grid, dim3(256), shm, ctx->stream, w, s, l->Rp);
     return hip_check(hipGetLastError(), "adapter expand");
 }
 
 template <typename T>
 static int launch_outer(DevCtx *ctx, const ColiHipLora *l, const LoraRows &w, const LoraSide<T> &s0, const LoraSide<T> &s1) {
-    const int nrt = l->Rp / 16, cols = (std::max(l->I, l->O) + 63) / 64;
-#define COLI_OUTER(NR)                                                                                             \
-    hipLaunchKernelGGL((coli_lora_outer<T, NR>), dim3(cols, l->slots *((nrt + NR - 1) / NR), 2), dim3(256), 0,       \
-                       ctx->stream, w, s0, s1, l->Rp, l->max_rank)
-    if (nrt == 1) COLI_OUTER(1);
-    else if (nrt == 2) COLI_OUTER(2);
-    else COLI_OUTER(4);
+    const int nrt = l->Rp / 16, cols = (std::max(l->I, l->O) + 63) / 64, nr = nrt >= 4 ? 4 : nrt;
+#define COLI_OUTER(NR, W)                                                                                           hipLaunchKernelGGL((coli_lora_outer<T, NR, W>), dim3(cols, l->slots *(nrt / nr), 2), dim3(64 * W), 0,                                ctx->stream, w, s0, s1, l->Rp, l->max_rank)
+    if (w.S <= COLI_LORA_BALLOT) {
+        if (nr == 1) COLI_OUTER(1, 4);
+        else if (nr == 2) COLI_OUTER(2, 4);
+        else COLI_OUTER(4, 4);
+    } else {
+        if (nr == 1) COLI_OUTER(1, 16);
+        else if (nr == 2) COLI_OUTER(2, 16);
+        else COLI_OUTER(4, 16);
+    }
 #undef COLI_OUTER
     return hip_check(hipGetLastError(), "adapter gradients");
 }
@@ -552,30 +744,38 @@ template <typename T>
 static int lora_forward(DevCtx *ctx, ColiCudaTensor *t, const ColiHipLora *l, float *y, const float *x, int S,
                         const int *slot_dev) {
     LoraRows w;
-    const int splits = shrink_splits(ctx, lora_tiles(S, l->slots), l->I);
+    const int splits = shrink_splits(ctx, S, (long)lora_tiles(S, l->slots) * l->I, l->I);
     if (!reserve_kept(ctx, &ctx->lora_h, (size_t)splits * S * l->Rp * sizeof(float), 0) ||
         !lora_rows(ctx, l, slot_dev, S, &w))
         return 0;
     float *h = (float *)ctx->lora_h.p;
     const LoraSide<T> a = lora_side<T>(l, false, x, h, nullptr, splits);
-    LoraSide<T> b = lora_side<T>(l, true, nullptr, h, y, splits);
-    return launch_shrink<T>(ctx, l, w, a, a, 1) && gemm_dev(ctx, t, y, x, S) && launch_expand<T>(ctx, l, w, b);
+    const LoraSide<T> b = lora_side<T>(l, true, nullptr, h, y, splits);
+    ColiPrepArgs ride = {};
+    if (!gemm_prep_beside(ctx, t, x, S, S <= COLI_LORA_BALLOT ? &ride : nullptr)) return 0;
+    return launch_shrink<T>(ctx, l, w, a, a, 1, ride) && gemm_prepared(ctx, t, y, x, S) && launch_expand<T>(ctx, l, w, b);
 }
 
 template <typename T>
 static int lora_backward(DevCtx *ctx, ColiCudaTensor *t, const ColiHipLora *l, const float *x, const float *dy, int S,
                          const int *slot_dev, float *dx, float *da, float *db) {
     LoraRows w;
-    const int tiles = lora_tiles(S, l->slots);
-    const int spa = shrink_splits(ctx, 2 * tiles, l->I), spb = shrink_splits(ctx, 2 * tiles, l->O);
+    const long columns = (long)lora_tiles(S, l->slots) * (l->I + l->O);
+    const int spa = shrink_splits(ctx, S, columns, l->I), spb = shrink_splits(ctx, S, columns, l->O);
     const size_t hb = (size_t)S * l->Rp * sizeof(float);
     if (!reserve_kept(ctx, &ctx->lora_h, (spa + spb) * hb, 0) || !lora_rows(ctx, l, slot_dev, S, &w)) return 0;
-    float *ha = (float *)ctx->lora_h.p, *hb_ = (float *)((uint8_t *)ctx->lora_h.p + spa * hb);
-    const LoraSide<T> sa = lora_side<T>(l, false, x, ha, da, spa), sb = lora_side<T>(l, true, dy, hb_, db, spb);
-    if (!launch_shrink<T>(ctx, l, w, sa, sb, 2) || !launch_outer<T>(ctx, l, w, sa, sb)) return 0;
+    float *h0 = (float *)ctx->lora_h.p, *h1 = (float *)((uint8_t *)ctx->lora_h.p + spa * hb);
+    const LoraSide<T> sa = lora_side<T>(l, false, x, h0, da, spa), sb = lora_side<T>(l, true, dy, h1, db, spb);
+    GemmTPlan plan = {};
+    if (dx && !gemm_t_plan(ctx, t, dy, S, &plan)) return 0;
+    if (!launch_shrink<T>(ctx, l, w, sa, sb, 2, ColiPrepArgs{}) || !launch_outer<T>(ctx, l, w, sa, sb)) return 0;
     if (!dx) return 1;
-    LoraSide<T> e = lora_side<T>(l, false, nullptr, hb_, dx, spb);
-    return gemm_t_dev(ctx, t, dx, dy, S) && launch_expand<T>(ctx, l, w, e);
+    LoraSide<T> e = lora_side<T>(l, false, nullptr, h1, dx, spb);
+    if (S <= COLI_LORA_BALLOT && plan.parts) {   // every row is a tile's: the expand joins the splits
+        e.part = plan.part;
+        e.parts = plan.parts;
+    }
+    return gemm_t_run(ctx, t, dx, dy, S, plan, !e.parts) && launch_expand<T>(ctx, l, w, e);
 }
 
 // ---------------------------------------------------------------------------
