@@ -25,8 +25,6 @@
 
 #define COLI_BAL_MAX_SEQS 16384
 #define COLI_BAL_MAX_ROWS (1 << 24)
-// Rows one workgroup finishes alone, loss included.
-#define COLI_BAL_SINGLE 128
 
 struct BalanceArgs {
     const float *z;            // [nch][T][E]: logits, or column-chunk partials added in chunk order
@@ -35,8 +33,7 @@ struct BalanceArgs {
     const int *idx, *keff;     // [T][K], [T] or null
     const uint8_t *mask;       // [T] or null
     const int *off;            // [n + 1] or null: one sequence of all rows
-    int n, T, E, K, mode, R;   // R: rows per workgroup
-    int vec;                   // E % 4 == 0 and every row 16-byte aligned
+    int n, T, E, K, R;         // R: rows per workgroup
     float *loss;               // [n]
     int *counts, *rows;        // [n][E], [n]
     // partial sums of workgroup b's rows of sequence i, slot b + i (the pairs
@@ -69,137 +66,161 @@ __device__ __forceinline__ int dpp_sum16i(int v) {
 // The row's logits; columns past E read -inf, which every score maps to 0.
 template <int NV>
 __device__ __forceinline__ void bal_load(const BalanceArgs &a, int row, int l, float (&v)[4 * NV]) {
-    const float *zr = a.z + (size_t)row * a.E;
+    const float *zr = a.z + (size_t)row * a.E + 4 * l;
+    auto piece = [&](const float *p, int e, float fill) -> floatx4 {
+        if (e + 4 <= a.E) return *GPTR(f4u, p);
+        floatx4 t = {fill, fill, fill, fill};
+#pragma unroll
+        for (int k = 0; k < 3; k++)
+            if (e + k < a.E) t[k] = p[k];
+        return t;
+    };
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-        const int e = 64 * i + 4 * l;
-        if (a.vec) {
-            const floatx4 t = e < a.E ? *GPTR(floatx4, zr + e) : (floatx4){-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        const floatx4 t = piece(zr + 64 * i, 64 * i + 4 * l, -INFINITY);
 #pragma unroll
-            for (int k = 0; k < 4; k++) v[4 * i + k] = t[k];
-        } else {
+        for (int k = 0; k < 4; k++) v[4 * i + k] = t[k];
+    }
+    for (int ch = 1; ch < a.nch; ch++)
 #pragma unroll
-            for (int k = 0; k < 4; k++) v[4 * i + k] = e + k < a.E ? zr[e + k] : -INFINITY;
+        for (int i = 0; i < NV; i++) {
+            const floatx4 t = piece(zr + (size_t)ch * a.chstride + 64 * i, 64 * i + 4 * l, 0.0f);
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[4 * i + k] += t[k];
         }
-    }
-    for (int ch = 1; ch < a.nch; ch++) {
-        const float *zc = zr + (size_t)ch * a.chstride;
-#pragma unroll
-        for (int i = 0; i < NV; i++)
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-                if (64 * i + 4 * l + k < a.E) v[4 * i + k] += zc[64 * i + 4 * l + k];
-    }
 }
 
-// v: logits in, p out; with GRAD, up: u'(z). The hardware's exp2, log2, rcp and
-// sqrt (1 ulp each) are used: a p is off by a few 2^-23. Scores so small that
-// their sum would lose bits (every z below about -27) go by their logarithm
-// instead, where both u are linear to within f32: z, or z / 2 in mode 3. A row
-// of nothing but -inf has p = 0.
-template <int NV, bool GRAD>
-__device__ __forceinline__ void bal_prob(int mode, float (&v)[4 * NV], float (&up)[4 * NV]) {
-    float z[4 * NV], sum = 0.0f;
-#pragma unroll
-    for (int k = 0; k < 4 * NV; k++) z[k] = v[k];
-    if (mode) {
+// v: the row's logits in; out, scores whose sum over the row (`sum`) they are to
+// be divided by: p = v / sum. GRAD: v u'(z) instead, and ws = sum_e w_e v_e, so
+// that the row is held once. The hardware's exp2, log2, rcp and rsq (1 ulp each)
+// are used: a p is off by a few 2^-23. Scores so small that their sum would lose
+// bits (every z below about -27) go by their logarithm instead, where both u are
+// linear to within f32: z, or z / 2 in mode 3. A row of nothing but -inf has
+// p = 0.
+template <int NV, int MODE, bool GRAD>
+__device__ __forceinline__ void bal_scores(const BalanceArgs &a, int row, int l, const float *w, float (&v)[4 * NV],
+                                           float &sum, float &ws) {
+    sum = ws = 0.0f;
+    auto add = [&](int k, float s, float up) {
+        sum += s;
+        if constexpr (GRAD) ws += w[k] * s;
+        v[k] = GRAD ? s * up : s;
+    };
+    if constexpr (MODE == 3) {
 #pragma unroll
         for (int k = 0; k < 4 * NV; k++) {
-            const float t = __expf(-fabsf(z[k])), w = 1.0f + t, r = __builtin_amdgcn_rcpf(w);
-            const bool pos = z[k] >= 0.0f;
-            const float sg = pos ? r : t * r;
-            if (mode == 3) {
-                // log(1 + t) = t log(w) / (w - 1): the rounding of w cancels
-                const float d = w - 1.0f, lg = d > 0.0f ? t * (__logf(w) * __builtin_amdgcn_rcpf(d)) : t;
-                const float sp = (pos ? z[k] : 0.0f) + lg;
-                v[k] = __builtin_amdgcn_sqrtf(sp);
-                if constexpr (GRAD) up[k] = z[k] < -15.0f ? 0.5f : 0.5f * sg * __builtin_amdgcn_rcpf(sp);
-            } else {
-                v[k] = sg;
-                if constexpr (GRAD) up[k] = pos ? t * r : r;
+            const float z = v[k], t = __expf(-fabsf(z)), o = 1.0f + t;
+            // log(1 + t) = log o + (t - (o - 1)) / o but for the square of o's
+            // rounding; 1 / o <= 1 is left out of that last place
+            const float sp = fmaxf(z, 0.0f) + (__logf(o) + (t - (o - 1.0f)));
+            const float q = __builtin_amdgcn_rsqf(fmaxf(sp, 1e-37f));
+            float up = 1.0f;
+            if constexpr (GRAD) {
+                const float r = __builtin_amdgcn_rcpf(o);
+                up = z < -15.0f ? 0.5f : 0.5f * (z >= 0.0f ? r : t * r) * (q * q);
             }
-            if (z[k] != z[k]) v[k] = z[k];
-            sum += v[k];
+            add(k, z == z ? sp * q : z, up);
+        }
+    } else if constexpr (MODE == 1) {
+#pragma unroll
+        for (int k = 0; k < 4 * NV; k++) {
+            const float z = v[k], t = __expf(-fabsf(z)), r = __builtin_amdgcn_rcpf(1.0f + t);
+            add(k, z >= 0.0f ? r : t * r, z >= 0.0f ? t * r : r);
+        }
+    }
+    if (MODE) sum = dpp_sum16(sum);
+    if (MODE == 0 || sum < 1e-12f) {
+        if (MODE) bal_load<NV>(a, row, l, v);
+        float m = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < 4 * NV; k++) m = fmaxf(m, v[k]);
+        m = dpp_max16(m);
+        sum = ws = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4 * NV; k++) {
+            // (m = -inf: only -inf and NaN in the row; NaN stays). u' where every
+            // score is small: 1, or 1 / 2 in mode 3.
+            const float c = MODE == 3 ? 0.5f : 1.0f;
+            add(k, v[k] == -INFINITY ? 0.0f : __expf(c * (v[k] - m)), c);
         }
         sum = dpp_sum16(sum);
     }
-    if (!mode || sum < 1e-12f) {
-        float m = -INFINITY;
-#pragma unroll
-        for (int k = 0; k < 4 * NV; k++) m = fmaxf(m, z[k]);
-        m = dpp_max16(m);
-        const float c = mode == 3 ? 0.5f : 1.0f;
-        float s = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 4 * NV; k++) {
-            // (m = -inf: only -inf and NaN in the row; NaN stays)
-            v[k] = z[k] == -INFINITY ? 0.0f : __expf(c * (z[k] - m));
-            if constexpr (GRAD)
-                if (!mode) up[k] = 1.0f;
-            s += v[k];
-        }
-        sum = dpp_sum16(s);
-    }
-    const float r = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-    for (int k = 0; k < 4 * NV; k++) v[k] *= r;
+    if constexpr (GRAD) ws = dpp_sum16(ws);
 }
 
+// The sequences' offsets, clamped to the rows; in LDS where they fit (each
+// lookup of a row's sequence reads a few, one after the other).
+#define COLI_BAL_OFF 1024
+struct BalOff {
+    const int *lds, *off;
+    int n, T;
+    __device__ int get(int i) const {
+        if (!off) return i ? T : 0;
+        return min(max(n < COLI_BAL_OFF ? lds[i] : off[i], 0), T);
+    }
+};
 // First sequence that ends after `row`: the offsets up to it, counted by the block.
-__device__ __forceinline__ int bal_first(const BalanceArgs &a, int row) {
+__device__ __forceinline__ int bal_first(const BalanceArgs &a, int row, int *s_off) {
     if (!a.off) return 0;
     int c = 0;
+    if (threadIdx.x == 0) s_off[0] = a.off[0];
     for (int j0 = 0; j0 < a.n; j0 += blockDim.x) {
         const int j = j0 + threadIdx.x;
-        c += __syncthreads_count(j < a.n && a.off[j + 1] <= row);
+        const int o = j < a.n ? a.off[j + 1] : 0;
+        if (j < a.n && a.n < COLI_BAL_OFF) s_off[j + 1] = o;
+        c += __syncthreads_count(j < a.n && o <= row);
     }
     return c;
 }
-__device__ __forceinline__ int bal_begin(const BalanceArgs &a, int i) {
-    return a.off ? min(max(a.off[i], 0), a.T) : 0;
-}
-__device__ __forceinline__ int bal_end(const BalanceArgs &a, int i) {
-    return a.off ? min(max(a.off[i + 1], 0), a.T) : a.T;
-}
+
+// Waves of the workgroup that finishes all rows alone.
+template <int NV> constexpr int bal_single_waves() { return NV <= 4 ? 16 : NV <= 8 ? 8 : 4; }
 
 // Sums of each workgroup's R rows by sequence; with SINGLE (one workgroup for
-// all rows) the outputs themselves.
-template <int NV, bool SINGLE>
-__global__ __launch_bounds__(256) void coli_balance_rows(BalanceArgs a) {
-    __shared__ float red[4][64 * NV];
+// all rows) the outputs themselves. A wave takes four rows of each step of 4 W
+// rows from the workgroup's first; the first step's logits are requested before
+// the rows' sequences are known.
+template <int NV, int MODE, bool SINGLE>
+__global__ __launch_bounds__(SINGLE ? 64 * bal_single_waves<NV>() : 256, NV <= 6 ? 4 : NV <= 8 ? 3 : 1) void coli_balance_rows(BalanceArgs a) {
+    constexpr int W = SINGLE ? bal_single_waves<NV>() : 4, NT = 64 * W, RS = 4 * W;
+    __shared__ float red[W][64 * NV];
     __shared__ int cnt[64 * NV];
-    __shared__ int seg_n[2];
-    __shared__ float wsum[4];
+    __shared__ int seg_n[2], s_off[COLI_BAL_OFF];
+    __shared__ float wsum[W];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l = lane & 15, g = lane >> 4;
     const int b = blockIdx.x, r0 = b * a.R, r1 = min(a.T, r0 + a.R);
+    float v[4 * NV];
+    int have = 0;   // the step whose rows v holds
+    bal_load<NV>(a, min(r0 + 4 * wave + g, r1 - 1), l, v);
     if constexpr (SINGLE) {
-        for (size_t e = tid; e < (size_t)a.n * a.E; e += 256) a.counts[e] = 0;
-        for (int i = tid; i < a.n; i += 256) {
+        for (int e = tid; e < a.n * a.E; e += NT) a.counts[e] = 0;
+        for (int i = tid; i < a.n; i += NT) {
             a.loss[i] = 0.0f;
             a.rows[i] = 0;
         }
     }
-    int i = bal_first(a, r0);
-    int row = i < a.n ? max(r0, bal_begin(a, 0)) : r1;
-    if constexpr (SINGLE) __syncthreads();
+    int i = bal_first(a, r0, s_off);
+    const BalOff off = {s_off, a.off, a.n, a.T};
+    if (!a.off || SINGLE) __syncthreads();
+    int row = i < a.n ? max(r0, off.get(0)) : r1;
     while (row < r1 && i < a.n) {
-        const int end = bal_end(a, i);
+        const int end = off.get(i + 1);
         if (end <= row) {
             i++;
             continue;
         }
         const int hi = min(end, r1);
-        for (int e = tid; e < 64 * NV; e += 256) cnt[e] = 0;
+        for (int e = tid; e < 64 * NV; e += NT) cnt[e] = 0;
         if (tid < 2) seg_n[tid] = 0;
         __syncthreads();
         // selections: (row, slot) pairs over the threads
         int nsel = 0, nrow = 0;
         const int npair = (hi - row) * a.K;
-        for (int s = tid; s < npair; s += 256) {
+        for (int s = tid; s < npair; s += NT) {
             const int t = row + s / a.K, kk = s - s / a.K * a.K;
-            if (a.mask && !a.mask[t]) continue;
-            const int e = a.idx[(size_t)t * a.K + kk];
-            if (kk < (a.keff ? a.keff[t] : a.K) && e >= 0 && e < a.E) {
+            const int e = a.idx[(size_t)t * a.K + kk], ke = a.keff ? a.keff[t] : a.K;
+            const bool live = !a.mask || a.mask[t];
+            if (live && kk < ke && e >= 0 && e < a.E) {
                 atomicAdd(cnt + e, 1);
                 nsel++;
             }
@@ -207,17 +228,21 @@ __global__ __launch_bounds__(256) void coli_balance_rows(BalanceArgs a) {
         float acc[4 * NV];
 #pragma unroll
         for (int k = 0; k < 4 * NV; k++) acc[k] = 0.0f;
-        for (int t0 = row + 4 * wave; t0 < hi; t0 += 16) {
-            const int t = t0 + g;
-            const bool live = t < hi && (!a.mask || a.mask[t]);
-            float v[4 * NV], none[4 * NV];
-            bal_load<NV>(a, t < hi ? t : t0, l, v);
-            bal_prob<NV, false>(a.mode, v, none);
+        for (int s = (row - r0) / RS; r0 + RS * s < hi; s++) {
+            const int t = r0 + RS * s + 4 * wave + g;
+            const bool in = t >= row && t < hi, live = in && (!a.mask || a.mask[t]);
+            float sum, ws;
+            if (have != s) bal_load<NV>(a, min(t, r1 - 1), l, v);
+            bal_scores<NV, MODE, false>(a, min(t, r1 - 1), l, nullptr, v, sum, ws);
             if (live) {
+                const float r = sum == 0.0f ? 0.0f : 1.0f / sum;
                 nrow += l == 0;
 #pragma unroll
-                for (int k = 0; k < 4 * NV; k++) acc[k] += v[k];
+                for (int k = 0; k < 4 * NV; k++) acc[k] += v[k] * r;
             }
+            have = s + 1;
+            if (r0 + RS * have < r1) bal_load<NV>(a, min(t + RS, r1 - 1), l, v);
+            else have = -1;
         }
         if (nsel) atomicAdd(seg_n + 1, nsel);
         if (nrow) atomicAdd(seg_n, nrow);
@@ -232,26 +257,32 @@ __global__ __launch_bounds__(256) void coli_balance_rows(BalanceArgs a) {
                 *(floatx4 *)&red[wave][64 * v + 4 * l] =
                     (floatx4){acc[4 * v], acc[4 * v + 1], acc[4 * v + 2], acc[4 * v + 3]};
         __syncthreads();
-        const int n = seg_n[0], C = seg_n[1];
+        auto total = [&](int e) {
+            float v = red[0][e];
+#pragma unroll
+            for (int q = 1; q < W; q++) v += red[q][e];
+            return v;
+        };
         if constexpr (SINGLE) {
+            const int n = seg_n[0], C = seg_n[1];
             float d = 0.0f;
-            for (int e = tid; e < a.E; e += 256) {
-                const float P = (red[0][e] + red[1][e]) + (red[2][e] + red[3][e]);
+            for (int e = tid; e < a.E; e += NT) {
                 a.counts[(size_t)i * a.E + e] = cnt[e];
-                d += (float)cnt[e] * P;
+                d += (float)cnt[e] * total(e);
             }
 #pragma unroll
             for (int o = 32; o; o >>= 1) d += __shfl_xor(d, o);
             if (lane == 0) wsum[wave] = d;
             __syncthreads();
             if (tid == 0) {
+                for (int q = 1; q < W; q++) d += wsum[q];
                 a.rows[i] = n;
-                a.loss[i] = C && n ? ((wsum[0] + wsum[1]) + (wsum[2] + wsum[3])) * ((float)a.E / (float)C / (float)n) : 0.0f;
+                a.loss[i] = C && n ? d * ((float)a.E / (float)C / (float)n) : 0.0f;
             }
         } else {
             const size_t slot = (size_t)(b + i);
-            for (int e = tid; e < a.Ep; e += 256) {
-                a.ps[slot * a.Ep + e] = (red[0][e] + red[1][e]) + (red[2][e] + red[3][e]);
+            for (int e = tid; e < a.Ep; e += NT) {
+                a.ps[slot * a.Ep + e] = total(e);
                 a.pc[slot * a.Ep + e] = cnt[e];
             }
             if (tid < 2) a.pn[2 * slot + tid] = seg_n[tid];
@@ -262,83 +293,109 @@ __global__ __launch_bounds__(256) void coli_balance_rows(BalanceArgs a) {
     }
 }
 
-// Joins a sequence's partial sums, 64 columns a workgroup (16 lanes of four
-// columns x blockDim / 16 groups of slots); the workgroup that arrives last
-// adds the loss's pieces in column order.
-template <int NT>
-__global__ __launch_bounds__(NT) void coli_balance_join(BalanceArgs a) {
-    constexpr int G = NT / 16;
-    __shared__ floatx4 sp[G][16];
-    __shared__ int sc[G][64], sn[G][2];
-    const int i = blockIdx.x, eb = blockIdx.y, neb = gridDim.y, tid = threadIdx.x, l = tid & 15, g = tid >> 4;
-    const int lo = bal_begin(a, i), hi = bal_end(a, i);
+// Joins a sequence's partial sums. A workgroup (sequence, 64 NB columns) has
+// 1024 / (16 NB) groups of slots, each of 16 NB lanes of four columns. With
+// all columns in one workgroup the loss is complete; else (a long sequence) the
+// one that arrives last adds the pieces in column order.
+template <int NB>
+__global__ __launch_bounds__(1024) void coli_balance_join(BalanceArgs a) {
+    constexpr int L = 16 * NB, G = 1024 / L;
+    __shared__ floatx4 sp[G][L];
+    __shared__ __attribute__((aligned(16))) int sc[G][4 * L];
+    __shared__ int sn[G][2];
+    __shared__ float wsum[16];
+    const int i = blockIdx.x, eb = blockIdx.y, neb = gridDim.y, tid = threadIdx.x, l = tid % L, g = tid / L;
+    const BalOff off = {nullptr, a.off, COLI_BAL_OFF, a.T};
+    const int lo = off.get(i), hi = off.get(i + 1);
     const int b0 = lo / a.R, b1 = hi > lo ? (hi - 1) / a.R : b0 - 1;
+    const int col = 4 * (L * eb + l);
     floatx4 s = (floatx4){0.f, 0.f, 0.f, 0.f};
-    int c[4] = {0, 0, 0, 0}, n0 = 0, n1 = 0;
-#pragma unroll 4
-    for (int b = b0 + g; b <= b1; b += G) {
-        const size_t slot = (size_t)(b + i);
-        const floatx4 x = *GPTR(floatx4, a.ps + slot * a.Ep + 64 * eb + 4 * l);
-        const u32x4 y = *GPTR(u32x4, a.pc + slot * a.Ep + 64 * eb + 4 * l);
-        n0 += a.pn[2 * slot];
-        n1 += a.pn[2 * slot + 1];
-        s += x;
+    u32x4 c = (u32x4){0u, 0u, 0u, 0u};
+    int n0 = 0, n1 = 0;
+    if (g < G && col < a.Ep) {
+        for (int b = b0 + g; b <= b1; b += 4 * G) {
+            floatx4 x[4];
+            u32x4 y[4];
+            int m0[4], m1[4];
 #pragma unroll
-        for (int k = 0; k < 4; k++) c[k] += (int)y[k];
+            for (int u = 0; u < 4; u++) {
+                const size_t slot = (size_t)(min(b + u * G, b1) + i);
+                x[u] = *GPTR(floatx4, a.ps + slot * a.Ep + col);
+                y[u] = *GPTR(u32x4, a.pc + slot * a.Ep + col);
+                m0[u] = a.pn[2 * slot];
+                m1[u] = a.pn[2 * slot + 1];
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                if (b + u * G <= b1) {
+                    s += x[u];
+                    c += y[u];
+                    n0 += m0[u];
+                    n1 += m1[u];
+                }
+        }
     }
-    sp[g][l] = s;
-#pragma unroll
-    for (int k = 0; k < 4; k++) sc[g][4 * l + k] = c[k];
-    if (l == 0) {
-        sn[g][0] = n0;
-        sn[g][1] = n1;
+    if (g < G) {
+        sp[g][l] = s;
+        *(u32x4 *)&sc[g][4 * l] = c;
+        if (l == 0) {
+            sn[g][0] = n0;
+            sn[g][1] = n1;
+        }
     }
     __syncthreads();
-    if (tid < 64) {
-        const int e = 64 * eb + tid;
+    float d = 0.0f;
+    for (int e = tid; e < 4 * L; e += 1024) {
         float P = 0.0f;
-        int C = 0, n = 0, cn = 0;
-        for (int q = 0; q < G; q++) {
-            P += sp[q][tid >> 2][tid & 3];
-            cn += sc[q][tid];
-            n += sn[q][0];
-            C += sn[q][1];
-        }
-        if (e < a.E) a.counts[(size_t)i * a.E + e] = cn;
-        float d = (float)cn * P;
+        int cn = 0;
 #pragma unroll
-        for (int o = 32; o; o >>= 1) d += __shfl_xor(d, o);
-        if (tid == 0) {
-            const float f = C && n ? (float)a.E / (float)C / (float)n : 0.0f;
-            // the first workgroup of the sequence writes the row count; every
-            // one publishes its piece and counts itself in
-            if (eb == 0) a.rows[i] = n;
-            if (neb == 1) {
-                a.loss[i] = f != 0.0f ? d * f : 0.0f;
-            } else {
-                __hip_atomic_store(a.lossp + (size_t)i * neb + eb, d, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                const int at = __hip_atomic_fetch_add(a.arrive + i, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
-                if (at == neb - 1) {
-                    float t = 0.0f;
-                    for (int q = 0; q < neb; q++)
-                        t += __hip_atomic_load(a.lossp + (size_t)i * neb + q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                    a.loss[i] = f != 0.0f ? t * f : 0.0f;
-                    __hip_atomic_store(a.arrive + i, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                }
-            }
+        for (int q = 0; q < G; q++) {
+            P += ((const float *)sp[q])[e];
+            cn += sc[q][e];
         }
+        if (4 * L * eb + e < a.E) a.counts[(size_t)i * a.E + 4 * L * eb + e] = cn;
+        d += (float)cn * P;
     }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) d += __shfl_xor(d, o);
+    if ((tid & 63) == 0) wsum[tid >> 6] = d;
+    __syncthreads();
+    if (tid) return;
+    int n = 0, C = 0;
+    for (int q = 0; q < G; q++) {
+        n += sn[q][0];
+        C += sn[q][1];
+    }
+    for (int q = 1; q < 16; q++) d += wsum[q];
+    const float f = C && n ? (float)a.E / (float)C / (float)n : 0.0f;
+    if (eb == 0) a.rows[i] = n;
+    if (neb > 1) {
+        // publish the piece where every XCD sees it, then count it in
+        __hip_atomic_store(a.lossp + (size_t)i * neb + eb, d, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const int at = __hip_atomic_fetch_add(a.arrive + i, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+        if (at != neb - 1) return;
+        d = 0.0f;
+        for (int q = 0; q < neb; q++)
+            d += __hip_atomic_load(a.lossp + (size_t)i * neb + q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(a.arrive + i, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    a.loss[i] = f != 0.0f ? d * f : 0.0f;
 }
 
 // dz of each workgroup's R rows; rows of no sequence are left as they were.
-template <int NV>
-__global__ __launch_bounds__(256) void coli_balance_grad(BalanceArgs a) {
+template <int NV, int MODE>
+__global__ __launch_bounds__(256, NV <= 8 ? 4 : 1) void coli_balance_grad(BalanceArgs a) {
+    __shared__ int s_off[COLI_BAL_OFF];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l = lane & 15, g = lane >> 4;
     const int r0 = blockIdx.x * a.R, r1 = min(a.T, r0 + a.R);
-    int i = bal_first(a, r0);
-    int row = i < a.n ? max(r0, bal_begin(a, 0)) : r1;
+    float v[4 * NV];
+    int have = 0;   // the step whose rows v holds
+    bal_load<NV>(a, min(r0 + 4 * wave + g, r1 - 1), l, v);
+    int i = bal_first(a, r0, s_off);
+    const BalOff off = {s_off, a.off, a.n, a.T};
+    int row = i < a.n ? max(r0, off.get(0)) : r1;
     while (row < r1 && i < a.n) {
-        const int end = bal_end(a, i);
+        const int end = off.get(i + 1);
         if (end <= row) {
             i++;
             continue;
@@ -360,29 +417,27 @@ __global__ __launch_bounds__(256) void coli_balance_grad(BalanceArgs a) {
         const float f = C > 0 && n > 0 ? a.dloss[i] * ((float)a.E / (float)C / (float)n) : 0.0f;
 #pragma unroll
         for (int k = 0; k < 4 * NV; k++) w[k] *= f;
-        for (int t0 = row + 4 * wave; t0 < hi; t0 += 16) {
-            const int t = t0 + g;
-            float v[4 * NV], up[4 * NV];
-            bal_load<NV>(a, t < hi ? t : t0, l, v);
-            bal_prob<NV, true>(a.mode, v, up);
-            float d = 0.0f;
-#pragma unroll
-            for (int k = 0; k < 4 * NV; k++) d += w[k] * v[k];
-            d = dpp_sum16(d);
-            const bool live = t < hi && f != 0.0f && (!a.mask || a.mask[t]);
-            if (t >= hi) continue;
+        for (int s = (row - r0) / 16; r0 + 16 * s < hi; s++) {
+            const int t = r0 + 16 * s + 4 * wave + g;
+            const bool in = t >= row && t < hi, live = in && f != 0.0f && (!a.mask || a.mask[t]);
+            float sum, ws;
+            if (have != s) bal_load<NV>(a, min(t, r1 - 1), l, v);
+            have = -1;
+            bal_scores<NV, MODE, true>(a, min(t, r1 - 1), l, w, v, sum, ws);
+            const float r = sum == 0.0f ? 0.0f : 1.0f / sum, d = ws * r;
+            if (!in) continue;
             float *dr = a.dz + (size_t)t * a.E;
 #pragma unroll
             for (int q = 0; q < NV; q++) {
                 const int e = 64 * q + 4 * l;
                 floatx4 o;
 #pragma unroll
-                for (int k = 0; k < 4; k++) o[k] = live ? v[4 * q + k] * (w[4 * q + k] - d) * up[4 * q + k] : 0.0f;
-                if (a.vec) {
-                    if (e < a.E) *(floatx4 *)(dr + e) = o;
+                for (int k = 0; k < 4; k++) o[k] = live ? v[4 * q + k] * r * (w[4 * q + k] - d) : 0.0f;
+                if (e + 4 <= a.E) {
+                    *(f4u *)(dr + e) = o;
                 } else {
 #pragma unroll
-                    for (int k = 0; k < 4; k++)
+                    for (int k = 0; k < 3; k++)
                         if (e + k < a.E) dr[e + k] = o[k];
                 }
             }
@@ -393,6 +448,11 @@ __global__ __launch_bounds__(256) void coli_balance_grad(BalanceArgs a) {
 }
 
 static int nv_of(int E) { return E <= 64 ? 1 : E <= 128 ? 2 : E <= 256 ? 4 : E <= 384 ? 6 : E <= 512 ? 8 : 16; }
+// (modes 1 and 2 score alike)
+#define COLI_BAL_MODE(mode, CALL, NV) \
+    if ((mode) == 0) CALL(NV, 0);     \
+    else if ((mode) == 3) CALL(NV, 3); \
+    else CALL(NV, 1)
 #define COLI_BAL_NV(E, CALL)          \
     switch (nv_of(E)) {               \
     case 1: CALL(1); break;           \
@@ -424,8 +484,6 @@ int run_balance(DevCtx *ctx, const float *z, int nch, size_t chstride, const int
     a.T = T;
     a.E = E;
     a.K = K;
-    a.mode = mode;
-    a.vec = E % 4 == 0 && ((uintptr_t)z & 15) == 0;
     a.loss = loss;
     a.counts = counts;
     a.rows = rows;
@@ -433,11 +491,15 @@ int run_balance(DevCtx *ctx, const float *z, int nch, size_t chstride, const int
     forget_emitted(ctx, counts, (size_t)n * E * sizeof(int));
     forget_emitted(ctx, rows, (size_t)n * sizeof(int));
     hipStream_t st = ctx->stream;
-    if (T <= COLI_BAL_SINGLE && n <= 64) {
+    // up to four steps of one workgroup: one launch, loss included
+    if (T <= (E <= 256 ? 256 : E <= 512 ? 128 : 64) && n <= 64) {
         a.R = T;
-#define COLI_BAL_ONE(NV) hipLaunchKernelGGL((coli_balance_rows<NV, true>), dim3(1), dim3(256), 0, st, a)
+#define COLI_BAL_ONE_M(NV, M) \
+    hipLaunchKernelGGL((coli_balance_rows<NV, M, true>), dim3(1), dim3(64 * bal_single_waves<NV>()), 0, st, a)
+#define COLI_BAL_ONE(NV) COLI_BAL_MODE(mode, COLI_BAL_ONE_M, NV)
         COLI_BAL_NV(E, COLI_BAL_ONE)
 #undef COLI_BAL_ONE
+#undef COLI_BAL_ONE_M
         return hip_check(hipGetLastError(), "balance");
     }
     // 16 rows a step of a workgroup; about 1024 workgroups once there are rows for them
@@ -445,7 +507,9 @@ int run_balance(DevCtx *ctx, const float *z, int nch, size_t chstride, const int
     const int nb = (T + a.R - 1) / a.R;
     const size_t slots = (size_t)nb + n;
     a.Ep = (E + 63) / 64 * 64;
-    const int neb = a.Ep / 64;
+    // slots of a sequence: few, one workgroup adds all its columns; many, one for each 64
+    const bool many = nb / n > 64;
+    const int neb = many ? a.Ep / 64 : 1;
     const size_t ps_b = slots * a.Ep * 4, pn_b = (slots * 8 + 255) & ~(size_t)255, lp_b = ((size_t)n * neb * 4 + 255) & ~(size_t)255;
     if (!reserve_kept(ctx, &ctx->bal, 2 * ps_b + pn_b + lp_b, 0) ||
         !reserve_kept(ctx, &ctx->bal_cnt, (size_t)COLI_BAL_MAX_SEQS * sizeof(int), 1))
@@ -456,14 +520,16 @@ int run_balance(DevCtx *ctx, const float *z, int nch, size_t chstride, const int
     a.pn = (int *)(p + 2 * ps_b);
     a.lossp = (float *)(p + 2 * ps_b + pn_b);
     a.arrive = (int *)ctx->bal_cnt.p;
-#define COLI_BAL_ROWS(NV) hipLaunchKernelGGL((coli_balance_rows<NV, false>), dim3(nb), dim3(256), 0, st, a)
+#define COLI_BAL_ROWS_M(NV, M) hipLaunchKernelGGL((coli_balance_rows<NV, M, false>), dim3(nb), dim3(256), 0, st, a)
+#define COLI_BAL_ROWS(NV) COLI_BAL_MODE(mode, COLI_BAL_ROWS_M, NV)
     COLI_BAL_NV(E, COLI_BAL_ROWS)
 #undef COLI_BAL_ROWS
+#undef COLI_BAL_ROWS_M
     if (!hip_check(hipGetLastError(), "balance rows")) return 0;
-    if (nb / n > 16)
-        hipLaunchKernelGGL((coli_balance_join<1024>), dim3(n, neb), dim3(1024), 0, st, a);
-    else
-        hipLaunchKernelGGL((coli_balance_join<256>), dim3(n, neb), dim3(256), 0, st, a);
+#define COLI_BAL_JOIN(NB) hipLaunchKernelGGL((coli_balance_join<NB>), dim3(n, neb), dim3(1024), 0, st, a)
+    if (many) COLI_BAL_JOIN(1);
+    else COLI_BAL_NV(E, COLI_BAL_JOIN)
+#undef COLI_BAL_JOIN
     return hip_check(hipGetLastError(), "balance join");
 }
 
@@ -495,16 +561,16 @@ extern "C" int coli_hip_balance_grad_dev(int device, const float *logits, const 
     a.n = n;
     a.T = T;
     a.E = E;
-    a.mode = route_mode;
-    a.vec = E % 4 == 0 && (((uintptr_t)logits | (uintptr_t)dlogits) & 15) == 0;
     a.counts = (int *)counts;
     a.rows = (int *)rows;
     a.dloss = dloss;
     a.dz = dlogits;
     a.R = std::max(16, (T + 2047) / 2048 + 15 & ~15);
     const int nb = (T + a.R - 1) / a.R;
-#define COLI_BAL_GRAD(NV) hipLaunchKernelGGL((coli_balance_grad<NV>), dim3(nb), dim3(256), 0, ctx->stream, a)
+#define COLI_BAL_GRAD_M(NV, M) hipLaunchKernelGGL((coli_balance_grad<NV, M>), dim3(nb), dim3(256), 0, ctx->stream, a)
+#define COLI_BAL_GRAD(NV) COLI_BAL_MODE(route_mode, COLI_BAL_GRAD_M, NV)
     COLI_BAL_NV(E, COLI_BAL_GRAD)
 #undef COLI_BAL_GRAD
+#undef COLI_BAL_GRAD_M
     return hip_check(hipGetLastError(), "balance gradient");
 }

@@ -272,6 +272,97 @@ __device__ __forceinline__ void dma_wait_tail(int pend) {
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));   // any 4-byte aligned address (one dwordx4 load)
 
 // ---------------------------------------------------------------------------
+// Operands of an input gradient (gemm_t.hip): rows of dy as fp16 hi + lo. The
+// build runs alone or beside other work (lora.hip).
+// ---------------------------------------------------------------------------
+// Order of a lane's eight rows in the operands: the order the unpack leaves
+// nibbles in (int4: even ones, then odd ones).
+__host__ __device__ __forceinline__ int t_order(int int4, int e) { return !int4 ? e : e < 4 ? 2 * e : 2 * (e - 4) + 1; }
+
+// Octet o of a row, zeros past K.
+__device__ __forceinline__ void t_load8(const float *xr, int o, int K, float (&v)[8]) {
+    if (8 * o + 8 <= K) {
+        const f4u a = *GPTR(f4u, xr + 8 * o), b = *GPTR(f4u, xr + 8 * o + 4);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            v[i] = a[i];
+            v[4 + i] = b[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = 8 * o + i < K ? xr[8 * o + i] : 0.0f;
+    }
+}
+// As hi + lo under the exponent E, in operand order.
+__device__ __forceinline__ void t_split8(const float (&v)[8], int int4, int E, half8v &h, half8v &l) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        // (constant indices in both orders: a choice of registers, not of memory)
+        const float y = ldexpf(int4 ? v[t_order(1, e)] : v[e], -E);
+        h[e] = (_Float16)y;
+        l[e] = (_Float16)(y - (float)h[e]);
+    }
+}
+// E with max |v| 2^-E in [2^14, 2^15).
+__device__ __forceinline__ int t_exponent(float m) {
+    int E = 0;
+    if (m > 0.0f && isfinite(m)) {
+        frexpf(m, &E);
+        E -= 15;
+    }
+    return E;
+}
+
+// [octet of K][row][8]: a step's operand is contiguous over the rows. Only for
+// more than 64 rows: fewer are converted by the product itself.
+//
+// Four rows a workgroup, thread (row = t % 4, octet t / 4 of each 256), so
+// that loads read 512 and stores write 64 contiguous bytes; a row of up to
+// 16384 columns is read once.
+#define COLI_T_SLOTS 8   // octets a thread holds
+__device__ __forceinline__ void coli_t_prep_block(const ColiTPrepArgs &a, int blk) {
+    __shared__ float wmax[16][4];
+    const int tid = threadIdx.x, lane = tid & 63, r = tid & 3, o0 = tid >> 2, row = blk * 4 + r;
+    const float *xr = a.dy + (size_t)min(row, a.S - 1) * a.K;
+    float v[COLI_T_SLOTS][8], m = 0.0f;
+#pragma unroll
+    for (int s = 0; s < COLI_T_SLOTS; s++) t_load8(xr, o0 + 256 * s, a.K, v[s]);
+#pragma unroll
+    for (int s = 0; s < COLI_T_SLOTS; s++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(v[s][i]));
+    for (int o = o0 + 256 * COLI_T_SLOTS; o < a.noct; o += 256) {
+        float u[8];
+        t_load8(xr, o, a.K, u);
+#pragma unroll
+        for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(u[i]));
+    }
+#pragma unroll
+    for (int o = 4; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+    if (lane < 4) wmax[tid >> 6][lane] = m;
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 16; q++) m = fmaxf(m, wmax[q][r]);
+    if (row >= a.S) return;
+    const int E = t_exponent(m);
+    if (o0 == 0) a.exps[row] = E;
+    auto put = [&](int o, const float (&x)[8]) {
+        half8v h, l;
+        t_split8(x, a.int4, E, h, l);
+        *(half8v *)(a.hi + ((size_t)o * a.Sp + row) * 8) = h;
+        *(half8v *)(a.lo + ((size_t)o * a.Sp + row) * 8) = l;
+    };
+#pragma unroll
+    for (int s = 0; s < COLI_T_SLOTS; s++)
+        if (o0 + 256 * s < a.noct) put(o0 + 256 * s, v[s]);
+    for (int o = o0 + 256 * COLI_T_SLOTS; o < a.noct; o += 256) {
+        float u[8];
+        t_load8(xr, o, a.K, u);
+        put(o, u);
+    }
+}
+
+// ---------------------------------------------------------------------------
 // Activation-fragment build (the format and its reasons are described with
 // coli_prep_frag in gemv.hip), shared by that kernel and launches that run
 // the build beside other work.

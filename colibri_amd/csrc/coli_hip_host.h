@@ -182,8 +182,9 @@ int gemm_dev(DevCtx *ctx, ColiCudaTensor *t, float *y_dev, const float *x_dev, i
 // (a null: left for gemm_prepared to launch), then the product.
 int gemm_prep_beside(DevCtx *ctx, ColiCudaTensor *t, const float *x_dev, int S, ColiPrepArgs *a);
 int gemm_prepared(DevCtx *ctx, ColiCudaTensor *t, float *y_dev, const float *x_dev, int S);
-// dx = dy W: the decomposition, then the launches (with_join: the K splits'
-// sums into dx, else left in part [parts][S][I] when parts > 1).
+// dx = dy W: the decomposition, then the launches (with_prep: the rows' operands
+// too, where plan.prep.nblocks asks for them; with_join: the K splits' sums into
+// dx, else left in part [parts][S][I] where parts is not 0).
 struct GemmTPlan {
     ColiTPrepArgs prep;
     int mt, splits, per;
@@ -191,7 +192,8 @@ struct GemmTPlan {
     int parts;
 };
 int gemm_t_plan(DevCtx *ctx, ColiCudaTensor *t, const float *dy, int S, GemmTPlan *plan);
-int gemm_t_run(DevCtx *ctx, ColiCudaTensor *t, float *dx, const float *dy, int S, const GemmTPlan &plan, bool with_join);
+int gemm_t_run(DevCtx *ctx, ColiCudaTensor *t, float *dx, const float *dy, int S, const GemmTPlan &plan, bool with_prep,
+               bool with_join);
 int build_t_scales(DevCtx *ctx, ColiCudaTensor *t, bool update_only);
 // Counts and balance loss over router logits given as nch column-chunk
 // partials, chstride floats apart (balance.hip).

@@ -76,14 +76,14 @@ struct ColiPrepArgs {
     int ldx, K, ngp, int4_order, gen, vec, nchunk, nblocks;
 };
 
-// One build of an input gradient's rows (coli_t_prep_rows):
-// dy [S, K] -> hi, lo [noct][Sp][8], one exponent a row.
+// One build of an input gradient's rows (coli_t_prep_block): dy [S, K] -> hi,
+// lo [noct][Sp][8], one exponent a row; nblocks 1024-thread blocks.
 struct ColiTPrepArgs {
     const float *dy;
     _Float16 *hi, *lo;
     int *exps;
     size_t Sp;
-    int S, K, noct, int4;
+    int S, K, noct, int4, nblocks;
 };
 
 struct ColiGemvArgs {

@@ -28,44 +28,6 @@
 
 #include <algorithm>
 
-// Order of a lane's eight rows in the operands: the order the unpack leaves
-// nibbles in (int4: even ones, then odd ones).
-__host__ __device__ __forceinline__ int t_order(int int4, int e) { return !int4 ? e : e < 4 ? 2 * e : 2 * (e - 4) + 1; }
-
-// Octet o of a row, zeros past K.
-__device__ __forceinline__ void t_load8(const float *xr, int o, int K, float (&v)[8]) {
-    if (8 * o + 8 <= K) {
-        const f4u a = *GPTR(f4u, xr + 8 * o), b = *GPTR(f4u, xr + 8 * o + 4);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            v[i] = a[i];
-            v[4 + i] = b[i];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = 8 * o + i < K ? xr[8 * o + i] : 0.0f;
-    }
-}
-// As hi + lo under the exponent E, in operand order.
-__device__ __forceinline__ void t_split8(const float (&v)[8], int int4, int E, half8v &h, half8v &l) {
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-        // (constant indices in both orders: a choice of registers, not of memory)
-        const float y = ldexpf(int4 ? v[t_order(1, e)] : v[e], -E);
-        h[e] = (_Float16)y;
-        l[e] = (_Float16)(y - (float)h[e]);
-    }
-}
-// E with max |v| 2^-E in [2^14, 2^15).
-__device__ __forceinline__ int t_exponent(float m) {
-    int E = 0;
-    if (m > 0.0f && isfinite(m)) {
-        frexpf(m, &E);
-        E -= 15;
-    }
-    return E;
-}
-
 // ---------------------------------------------------------------------------
 // scales by column group
 // ---------------------------------------------------------------------------
@@ -120,54 +82,7 @@ __global__ __launch_bounds__(256) void coli_t_scales(const void *__restrict__ sc
 // ---------------------------------------------------------------------------
 // dy as fp16 hi + lo
 // ---------------------------------------------------------------------------
-// [octet of K][row][8]: a step's operand is contiguous over the rows. Only for
-// more than 64 rows: fewer are converted by the product itself.
-//
-// Four rows a workgroup, thread (row = t % 4, octet t / 4 of each 256), so
-// that loads read 512 and stores write 64 contiguous bytes; a row of up to
-// 16384 columns is read once.
-#define COLI_T_SLOTS 8   // octets a thread holds
-__global__ __launch_bounds__(1024) void coli_t_prep_rows(ColiTPrepArgs a) {
-    __shared__ float wmax[16][4];
-    const int tid = threadIdx.x, lane = tid & 63, r = tid & 3, o0 = tid >> 2, row = blockIdx.x * 4 + r;
-    const float *xr = a.dy + (size_t)min(row, a.S - 1) * a.K;
-    float v[COLI_T_SLOTS][8], m = 0.0f;
-#pragma unroll
-    for (int s = 0; s < COLI_T_SLOTS; s++) t_load8(xr, o0 + 256 * s, a.K, v[s]);
-#pragma unroll
-    for (int s = 0; s < COLI_T_SLOTS; s++)
-#pragma unroll
-        for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(v[s][i]));
-    for (int o = o0 + 256 * COLI_T_SLOTS; o < a.noct; o += 256) {
-        float u[8];
-        t_load8(xr, o, a.K, u);
-#pragma unroll
-        for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(u[i]));
-    }
-#pragma unroll
-    for (int o = 4; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
-    if (lane < 4) wmax[tid >> 6][lane] = m;
-    __syncthreads();
-#pragma unroll
-    for (int q = 0; q < 16; q++) m = fmaxf(m, wmax[q][r]);
-    if (row >= a.S) return;
-    const int E = t_exponent(m);
-    if (o0 == 0) a.exps[row] = E;
-    auto put = [&](int o, const float (&x)[8]) {
-        half8v h, l;
-        t_split8(x, a.int4, E, h, l);
-        *(half8v *)(a.hi + ((size_t)o * a.Sp + row) * 8) = h;
-        *(half8v *)(a.lo + ((size_t)o * a.Sp + row) * 8) = l;
-    };
-#pragma unroll
-    for (int s = 0; s < COLI_T_SLOTS; s++)
-        if (o0 + 256 * s < a.noct) put(o0 + 256 * s, v[s]);
-    for (int o = o0 + 256 * COLI_T_SLOTS; o < a.noct; o += 256) {
-        float u[8];
-        t_load8(xr, o, a.K, u);
-        put(o, u);
-    }
-}
+__global__ __launch_bounds__(1024) void coli_t_prep_rows(ColiTPrepArgs a) { coli_t_prep_block(a, blockIdx.x); }
 
 // ---------------------------------------------------------------------------
 // the product
@@ -252,7 +167,7 @@ __device__ __forceinline__ void t_weights(uint32_t nib, half8v s, half8v s2, hal
 // under the exponent of the row's part in this K split (the splits' sums are
 // f32 already), which saves the launch that would build the operands.
 template <int KIND, int MT, int WN, int WK, bool FEW>
-__global__ __launch_bounds__(64 * WN * WK) void coli_gemm_t(GemmTArgs a) {
+__global__ __launch_bounds__(64 * WN * WK, 2) void coli_gemm_t(GemmTArgs a) {
     constexpr int BM = 32 * MT, NT = 64 * WN, CH = (FEW ? 4 : 8) * BM;   // 8 (FEW: f32) values a chunk, 4 octets x BM rows
     constexpr int CPT = CH / NT;
     static_assert(CH % NT == 0, "whole chunks a thread");
@@ -509,11 +424,32 @@ template <int KIND>
 static void launch_gemm_t(const GemmTArgs &a, int mt, hipStream_t st) {
     const int rb = (a.S + 32 * mt - 1) / (32 * mt);
     if (mt == 4)
-        hipLaunchKernelGGL((coli_gemm_t<KIND, 4, 4, 1, false>), dim3((a.nq + 1) / 2, rb, a.splits), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((coli_gemm_t<KIND, 4, 4, 2, false>), dim3((a.nq + 1) / 2, rb, a.splits), dim3(512), 0, st, a);
     else if (mt == 2)
         hipLaunchKernelGGL((coli_gemm_t<KIND, 2, 2, 4, true>), dim3(a.nq, rb, a.splits), dim3(512), 0, st, a);
     else
         hipLaunchKernelGGL((coli_gemm_t<KIND, 1, 2, 4, true>), dim3(a.nq, rb, a.splits), dim3(512), 0, st, a);
+}
+
+// K splits of many rows: the modelled time, in steps of 32 rows of W. A
+// workgroup (eight waves of about 240 registers) has a CU to itself, so rounds
+// of workgroups, each about eight steps longer than its products; a split adds
+// its sums written and read again, and a launch to join them. A step takes 1.4
+// us with three products (int4), 0.9 with two (measured, all CUs busy: 2048 x
+// 4096 x 14336 and 512 x 7168 x 2048). Splits measured: 512 x 4096 x 14336 2 /
+// 4 / 8: 285 / 196 / 213 us; 512 x 7168 x 2048 MXFP4 1 / 2 / 3: 83 / 65 / 85.
+static int t_splits(const ColiCudaTensor *t, int S, int cus, long blocks, int steps) {
+    const double step = t->kind == COLI_KIND_FP4 ? 0.9 : 1.4, mb = (double)S * t->I * 4e-6;
+    int best = 1;
+    double least = 1e30;
+    for (int s = 1; s <= 32 && s * 8 <= std::max(8, steps); s++) {
+        const double us = step * (double)((blocks * s + cus - 1) / cus) * ((steps + s - 1) / s + 8) + (s > 1 ? (s + 1) * mb / 4 + 3 : 0);
+        if (us < least) {
+            least = us;
+            best = s;
+        }
+    }
+    return best;
 }
 
 int gemm_t_plan(DevCtx *ctx, ColiCudaTensor *t, const float *dy, int S, GemmTPlan *g) {
@@ -525,8 +461,8 @@ int gemm_t_plan(DevCtx *ctx, ColiCudaTensor *t, const float *dy, int S, GemmTPla
     const size_t Sp = few ? 0 : ((size_t)S + 127) & ~(size_t)127, fb = (size_t)noct * Sp * 16;
     const int cus = ctx->cu_count ? ctx->cu_count : 256;
     const long blocks = (long)((S + 32 * mt - 1) / (32 * mt)) * (few ? t->nq : (t->nq + 1) / 2);
-    // workgroups for about two a CU, at least eight steps each
-    int splits = (int)std::max(1L, std::min((2L * cus + blocks - 1) / blocks, (long)std::max(1, steps / 8)));
+    int splits = few ? (int)std::max(1L, std::min((2L * cus + blocks - 1) / blocks, (long)std::max(1, steps / 8)))
+                     : t_splits(t, S, cus, blocks, steps);
     const int per = (steps + splits - 1) / splits;
     splits = (steps + per - 1) / per;
     const size_t eb = (Sp * sizeof(int) + 255) & ~(size_t)255;
@@ -548,10 +484,12 @@ int gemm_t_plan(DevCtx *ctx, ColiCudaTensor *t, const float *dy, int S, GemmTPla
     a.K = t->O;
     a.noct = noct;
     a.int4 = t->kind != COLI_KIND_FP4;
+    a.nblocks = few ? 0 : (S + 3) / 4;
     return 1;
 }
 
-int gemm_t_run(DevCtx *ctx, ColiCudaTensor *t, float *dx, const float *dy, int S, const GemmTPlan &g, bool with_join) {
+int gemm_t_run(DevCtx *ctx, ColiCudaTensor *t, float *dx, const float *dy, int S, const GemmTPlan &g, bool with_prep,
+               bool with_join) {
     forget_emitted(ctx, dx, (size_t)S * t->I * sizeof(float));
     hipStream_t st = ctx->stream;
     if (t->kind == COLI_KIND_GENERIC) {
@@ -559,8 +497,8 @@ int gemm_t_run(DevCtx *ctx, ColiCudaTensor *t, float *dx, const float *dy, int S
                            t->ng_src, t->I, t->O, dy, dx);
         return hip_check(hipGetLastError(), "generic gradient");
     }
-    if (g.mt == 4) {
-        hipLaunchKernelGGL(coli_t_prep_rows, dim3((S + 3) / 4), dim3(1024), 0, st, g.prep);
+    if (with_prep && g.prep.nblocks) {
+        hipLaunchKernelGGL(coli_t_prep_rows, dim3(g.prep.nblocks), dim3(1024), 0, st, g.prep);
         if (!hip_check(hipGetLastError(), "gradient rows")) return 0;
     }
     GemmTArgs a = {};
@@ -597,5 +535,5 @@ extern "C" int coli_hip_gemm_t_dev(ColiCudaTensor *t, float *dx_dev, const float
     DevCtx *ctx = ctx_of(t->device);
     if (!bind_ctx(ctx)) return 0;
     GemmTPlan g;
-    return gemm_t_plan(ctx, t, dy_dev, S, &g) && gemm_t_run(ctx, t, dx_dev, dy_dev, S, g, true);
+    return gemm_t_plan(ctx, t, dy_dev, S, &g) && gemm_t_run(ctx, t, dx_dev, dy_dev, S, g, true, true);
 }

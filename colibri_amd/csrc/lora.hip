@@ -51,6 +51,7 @@ struct bf16_t {
 template <typename T> struct Raw8 {
     u32x4 w;
     __device__ void load(const T *p) { w = *GPTR(u32x4, p); }
+    __device__ void set(const T *p) { w = *(const u32x4 *)p; }
     __device__ float get(int i) const {
         const uint32_t v = w[i >> 1];
         if constexpr (sizeof(T) == 2 && !__is_same(T, _Float16))
@@ -64,6 +65,10 @@ template <> struct Raw8<float> {
     __device__ void load(const float *p) {
         a = *GPTR(floatx4, p);
         b = *GPTR(floatx4, p + 4);
+    }
+    __device__ void set(const float *p, const float *q) {
+        a = *(const floatx4 *)p;
+        b = *(const floatx4 *)q;
     }
     __device__ float get(int i) const { return i < 4 ? a[i & 3] : b[i & 3]; }
 };
@@ -122,8 +127,8 @@ struct LoraRows {
     // beyond COLI_LORA_BALLOT rows (coli_lora_sort): rows in slot order, each
     // slot's run in it, and the tiles (slot, first, rows)
     int *perm;                   // [S]
-    int2 *run;                   // [slots]: first, rows
-    int4 *tile;                  // [ntile]
+    int2 *run;                   // [slots + 1]: first, rows; the last: rows without an adapter
+    int4 *tile;                  // [ntile[1]], the first ntile[0] of them of slots
     int *ntile;
 };
 
@@ -131,8 +136,8 @@ struct LoraRows {
 __device__ __forceinline__ bool lora_live(const LoraRows &w, int s) { return s >= 0 && s < w.slots; }
 
 // Tile t of the call into LDS rows[]: the slot, and its rows' number (0: no
-// such tile). Every wave calls it; the caller synchronizes. ALL (at most
-// COLI_LORA_BALLOT rows): a row without an adapter is a tile of its own, slot -1.
+// such tile). Every wave calls it; the caller synchronizes. ALL: rows without
+// an adapter make tiles too (up to COLI_LORA_BALLOT rows one each), of slot -1.
 template <bool ALL = false>
 __device__ __forceinline__ int lora_tile(const LoraRows &w, int t, int *rows, int &slot) {
     const int lane = threadIdx.x & 63;
@@ -152,9 +157,9 @@ __device__ __forceinline__ int lora_tile(const LoraRows &w, int t, int *rows, in
         if ((m >> lane & 1) && at >= 0 && at < COLI_LORA_TILE) rows[at] = lane;
         return min(COLI_LORA_TILE, __popcll(m) - first);
     }
-    if (t >= *w.ntile) return 0;
+    if (t >= w.ntile[ALL]) return 0;
     const int4 e = w.tile[t];
-    slot = e.x;
+    slot = e.x < w.slots ? e.x : -1;
     if (lane < e.z) rows[lane] = w.perm[e.y + lane];
     return e.z;
 }
@@ -164,16 +169,17 @@ __device__ __forceinline__ int lora_tile(const LoraRows &w, int t, int *rows, in
 // over them do not depend on timing).
 template <int NW>
 __global__ __launch_bounds__(64 * NW) void coli_lora_sort(LoraRows w) {
-    extern __shared__ int cnt[];   // [NW][slots]
+    extern __shared__ int cnt[];   // [NW][slots + 1]
     __shared__ int wsum[NW][2];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nsl = w.slots;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nsl = w.slots + 1;
     const int per = ((w.S + NW - 1) / NW + 63) & ~63, r0 = wave * per, r1 = min(w.S, r0 + per);
     for (int k = tid; k < NW * nsl; k += 64 * NW) cnt[k] = 0;
     __syncthreads();
     int *mine = cnt + wave * nsl;
     auto slot_of = [&](int r) {
-        const int s = r < r1 ? w.slot[r] : -1;
-        return lora_live(w, s) ? s : -1;
+        if (r >= r1) return -1;
+        const int s = w.slot[r];
+        return lora_live(w, s) ? s : w.slots;
     };
     int nx = slot_of(r0 + lane);
     for (int r = r0; r < r1; r += 64) {
@@ -222,6 +228,10 @@ __global__ __launch_bounds__(64 * NW) void coli_lora_sort(LoraRows w) {
         if (s < nsl) {
             const int first = bx + x - n, t0 = by + y - nt;
             w.run[s] = make_int2(first, n);
+            if (s == w.slots) {
+                w.ntile[0] = t0;
+                w.ntile[1] = t0 + nt;
+            }
             for (int k = 0; k < nt; k++)
                 w.tile[t0 + k] = make_int4(s, first + k * COLI_LORA_TILE, min(COLI_LORA_TILE, n - k * COLI_LORA_TILE), 0);
             int at = first;
@@ -233,7 +243,6 @@ __global__ __launch_bounds__(64 * NW) void coli_lora_sort(LoraRows w) {
         }
         __syncthreads();
     }
-    if (tid == 0) *w.ntile = tbase;
     nx = slot_of(r0 + lane);
     for (int r = r0; r < r1; r += 64) {
         const int s = nx;
@@ -262,18 +271,32 @@ template <typename T> struct LoraSide {
     const float *part;           // expand: y is the sum of these [parts][S][N] instead of what it holds
     int parts;
     int N, Np, splits;
+    int sorted;                  // h rows are in slot order (coli_lora_join), not the call's
 };
 
 // shrink: workgroup (tile, column split, NR rank tiles of one side). The W
-// waves take 32 SUB columns in turn: lane (m, k) reads eight columns of row m
-// and of factor m, which feed eight MFMAs (the order of the columns inside a
-// sum is free); the next step is requested before this one's products. With
-// four waves, workgroups past nown build the projection's activation fragments.
+// waves take COLS columns in turn: a lane loads 16 bytes of a row of x or of
+// the factor, neighbours next to each other (lanes of one MFMA operand lie in
+// sixteen rows: loaded that way every 16 bytes were a cache line of their own,
+// 151 MB in 70 us), and the wave turns them round in its own LDS, 16-byte
+// pieces xored with their row so that the operand reads meet no bank twice.
+// Lane (m, k) then holds eight columns of row m and of factor m, which feed
+// eight MFMAs (the order of the columns inside a sum is free). The next step is
+// requested before this one's products. With four waves, workgroups past nown
+// build the projection's activation fragments.
+template <typename T, int NR> struct ShrinkGeom {
+    static constexpr int COLS = NR * sizeof(T) <= 8 ? 64 : 32;
+    static constexpr int XP = COLS / 4, VP = COLS * (int)sizeof(T) / 16;   // 16-byte pieces a row
+    static constexpr int XI = 16 * XP / 64, VI = 16 * VP / 64;             // loads of 64 lanes: x, a rank tile
+    static constexpr int BYTES = 16 * 16 * (XP + NR * VP);                 // a wave's LDS
+};
 template <typename T, int NR, int W>
 __global__ __launch_bounds__(64 * W) void coli_lora_shrink(LoraRows w, LoraSide<T> s0, LoraSide<T> s1, int Rp, int nz,
                                                            int tiles, int splits, int nown, ColiPrepArgs ride) {
-    constexpr int SUB = NR * sizeof(T) <= 8 ? 2 : 1, STEP = 32 * SUB;
+    using G = ShrinkGeom<T, NR>;
+    constexpr int STEP = G::COLS;
     __shared__ int rows[COLI_LORA_TILE];
+    __shared__ __attribute__((aligned(16))) uint8_t turn[W][G::BYTES];
     __shared__ float red[W][16][17];
     const int b = blockIdx.x;
     if constexpr (W == 4) {
@@ -292,45 +315,80 @@ __global__ __launch_bounds__(64 * W) void coli_lora_shrink(LoraRows w, LoraSide<
     if (sp >= s.splits || 16 * rt0 >= w.meta[slot].rank) return;
     __syncthreads();
     const int full = s.N / STEP, per = (full + s.splits - 1) / s.splits;
-    const int k1 = min(full, (sp + 1) * per);
-    const float *xr = s.x + (size_t)rows[min(m, n - 1)] * s.N + 8 * kq;
-    const T *vr = s.v + ((size_t)slot * Rp + 16 * rt0 + m) * s.Np + 8 * kq;
+    const int k0 = sp * per, k1 = min(full, k0 + per);
+    const T *vs = s.v + ((size_t)slot * Rp + 16 * rt0) * s.Np;
     floatx4 acc[NR];
 #pragma unroll
     for (int r = 0; r < NR; r++) acc[r] = (floatx4){0.f, 0.f, 0.f, 0.f};
+    // the lane's places in a load: row lane / pieces of each 64 / pieces rows
+    const float *xp[G::XI];
+    const T *vp[G::VI];
+    uint8_t *xw[G::XI], *vw[G::VI];
+    uint8_t *mine = turn[wave];
+#pragma unroll
+    for (int i = 0; i < G::XI; i++) {
+        const int r = i * (64 / G::XP) + lane / G::XP, p = lane % G::XP;
+        xp[i] = s.x + (size_t)rows[min(r, n - 1)] * s.N + 4 * p;
+        xw[i] = mine + (r * G::XP + (p ^ (r & (G::XP - 1)))) * 16;
+    }
+#pragma unroll
+    for (int i = 0; i < G::VI; i++) {
+        const int r = i * (64 / G::VP) + lane / G::VP, p = lane % G::VP;
+        vp[i] = vs + (size_t)r * s.Np + p * (16 / (int)sizeof(T));
+        vw[i] = mine + 16 * 16 * G::XP + (r * G::VP + (p ^ (r & (G::VP - 1)))) * 16;
+    }
     struct Step {
-        f4u x[SUB][2];
-        Raw8<T> v[SUB][NR];
+        f4u x[G::XI];
+        u32x4 v[NR][G::VI];
     };
     auto load = [&](int k, Step &st) {
+        const size_t c = (size_t)STEP * k;
 #pragma unroll
-        for (int u = 0; u < SUB; u++) {
-            const float *p = xr + (size_t)STEP * k + 32 * u;
-            st.x[u][0] = *GPTR(f4u, p);
-            st.x[u][1] = *GPTR(f4u, p + 4);
+        for (int i = 0; i < G::XI; i++) st.x[i] = *GPTR(f4u, xp[i] + c);
 #pragma unroll
-            for (int r = 0; r < NR; r++) st.v[u][r].load(vr + (size_t)16 * r * s.Np + (size_t)STEP * k + 32 * u);
-        }
+        for (int r = 0; r < NR; r++)
+#pragma unroll
+            for (int i = 0; i < G::VI; i++) st.v[r][i] = *GPTR(u32x4, vp[i] + (size_t)16 * r * s.Np + c);
     };
-    Step cur, nxt;
-    int k = sp * per + wave;
-    if (k < k1) {
-        load(k, cur);
-        for (; k < k1; k += W) {
-            load(min(k + W, k1 - 1), nxt);
+    Step st;
+    if (k0 + wave < k1) load(k0 + wave, st);
+    for (int k = k0 + wave; k < k1; k += W) {
 #pragma unroll
-            for (int u = 0; u < SUB; u++)
+        for (int i = 0; i < G::XI; i++) *(f4u *)xw[i] = st.x[i];
 #pragma unroll
-                for (int j = 0; j < 8; j++)
+        for (int r = 0; r < NR; r++)
 #pragma unroll
-                    for (int r = 0; r < NR; r++)
-                        acc[r] = __builtin_amdgcn_mfma_f32_16x16x4f32(cur.x[u][j >> 2][j & 3], cur.v[u][r].get(j), acc[r], 0, 0, 0);
-            cur = nxt;
+            for (int i = 0; i < G::VI; i++) *(u32x4 *)(vw[i] + r * 16 * 16 * G::VP) = st.v[r][i];
+        load(min(k + W, k1 - 1), st);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the wave's other lanes' pieces
+#pragma unroll
+        for (int u = 0; u < STEP / 32; u++) {
+            // columns 32 u + 8 kq + 0..7
+            floatx4 x[2];
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+                x[e] = *(const floatx4 *)(mine + (m * G::XP + ((8 * u + 2 * kq + e) ^ (m & (G::XP - 1)))) * 16);
+            Raw8<T> v[NR];
+#pragma unroll
+            for (int r = 0; r < NR; r++) {
+                const uint8_t *vr = mine + 16 * 16 * (G::XP + r * G::VP) + m * G::VP * 16;
+                auto piece = [&](int p) { return (const T *)(vr + (p ^ (m & (G::VP - 1))) * 16); };
+                if constexpr (sizeof(T) == 4) v[r].set(piece(8 * u + 2 * kq), piece(8 * u + 2 * kq + 1));
+                else v[r].set(piece(4 * u + kq));
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+#pragma unroll
+                for (int r = 0; r < NR; r++)
+                    acc[r] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j >> 2][j & 3], v[r].get(j), acc[r], 0, 0, 0);
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // read before the next step's writes
     }
     // columns past the last whole step: the last split, 32 a wave (the factors'
     // padding is zero, the row is read as zero past N)
     if (sp == s.splits - 1) {
+        const float *xr = s.x + (size_t)rows[min(m, n - 1)] * s.N + 8 * kq;
+        const T *vr = vs + (size_t)m * s.Np + 8 * kq;
         for (int c = STEP * full + 32 * wave; c < s.N; c += 32 * W) {
             float xv[8];
 #pragma unroll
@@ -360,6 +418,38 @@ __global__ __launch_bounds__(64 * W) void coli_lora_shrink(LoraRows w, LoraSide<
             if (row < n) s.h[((size_t)sp * w.S + rows[row]) * Rp + 16 * (rt0 + r) + c] = v;
         }
     }
+}
+
+// The column splits of h joined, the rows in slot order: [S][Rp] a side, 4 ranks
+// a thread.
+struct LoraJoin {
+    const float *h[2];
+    float *to[2];
+    int splits[2];
+    const int *perm;
+    int S, Rp, nblocks;          // nblocks workgroups of 1024 threads a side
+};
+__device__ __forceinline__ void lora_join_block(const LoraJoin &j, int b) {
+    const int side = b >= j.nblocks, r4 = j.Rp / 4;
+    const size_t e = (size_t)(b - side * j.nblocks) * 1024 + threadIdx.x, p = e / r4, n = (size_t)j.S * r4;
+    if (e >= n) return;
+    const floatx4 *h = (const floatx4 *)(side ? j.h[1] : j.h[0]) + (size_t)j.perm[p] * r4 + e % r4;
+    const int splits = side ? j.splits[1] : j.splits[0];
+    floatx4 t[4];
+#pragma unroll
+    for (int q = 0; q < 4; q++) t[q] = h[min(q, splits - 1) * n];   // (at most four)
+    floatx4 v = t[0];
+#pragma unroll
+    for (int q = 1; q < 4; q++)
+        if (q < splits) v += t[q];
+    ((floatx4 *)(side ? j.to[1] : j.to[0]))[e] = v;
+}
+
+// The join, with the input gradient's operand build (gemm_t.hip) beside it.
+__global__ __launch_bounds__(1024) void coli_lora_join(LoraJoin j, ColiTPrepArgs prep) {
+    const int b = blockIdx.x;
+    if (b < 2 * j.nblocks) lora_join_block(j, b);
+    else coli_t_prep_block(prep, b - 2 * j.nblocks);
 }
 
 // An element of h: the column splits joined in order, eight requested at once.
@@ -434,7 +524,8 @@ __global__ __launch_bounds__(256) void coli_lora_expand(LoraRows w, LoraSide<T> 
     for (int e = threadIdx.x; e < 16 * r16; e += 256) {
         const int row = e / r16, r = e - row * r16;
         // (past the rank: zeros, also where a row of infinities shrank to NaN)
-        const float hv = lora_h(s.h + (size_t)rows[min(row, n - 1)] * Rp + min(r, rank - 1), s.splits, (size_t)w.S * Rp);
+        const int hr = s.sorted ? w.tile[blockIdx.x].y + min(row, n - 1) : rows[min(row, n - 1)];
+        const float hv = lora_h(s.h + (size_t)hr * Rp + min(r, rank - 1), s.splits, (size_t)w.S * Rp);
         hs[row * (Rp + 1) + r] = row < n && r < rank ? meta.scale * hv : 0.0f;
     }
     __syncthreads();
@@ -483,7 +574,9 @@ __global__ __launch_bounds__(256) void coli_lora_expand(LoraRows w, LoraSide<T> 
 // outer: workgroup (64 columns, slot and NR rank tiles, side); the W waves take
 // 16 rows of the slot in turn, four MFMA steps of four rows, the next 16 rows
 // requested before this step's products and their numbers a step earlier; the
-// waves' sums are joined in LDS. Side 0: dA [slots][max_rank][N]; side 1 (dB):
+// waves' sums are joined in LDS. h: up to COLI_LORA_BALLOT rows its column
+// splits, joined here in LDS; beyond, joined and in slot order already
+// (coli_lora_join). Side 0: dA [slots][max_rank][N]; side 1 (dB):
 // stored transposed, [slots][N][max_rank]. Every element is written, zeros
 // where a slot has no rows or rank.
 template <typename T, int NR, int W>
@@ -506,7 +599,7 @@ __global__ __launch_bounds__(64 * W) void coli_lora_outer(LoraRows w, LoraSide<T
     if (c0 >= N) return;
     const LoraMeta meta = w.meta[slot];
     const int rank = min(meta.rank, Rp);
-    int cnt = 0;
+    int cnt = 0, first = 0;
     const int *list = rows;
     if constexpr (!LIST) {
         const unsigned long long mk = __builtin_amdgcn_ballot_w64(lane < w.S && w.slot[min(lane, w.S - 1)] == slot);
@@ -514,13 +607,14 @@ __global__ __launch_bounds__(64 * W) void coli_lora_outer(LoraRows w, LoraSide<T
         cnt = __popcll(mk);
     } else {
         const int2 rn = w.run[slot];
-        list = w.perm + rn.x;
+        first = rn.x;
+        list = w.perm + first;
         cnt = rn.y;
     }
     if (rank <= 16 * rt0) cnt = 0;
     __syncthreads();
-    const size_t pitch = (size_t)w.S * Rp;
     if constexpr (!LIST) {
+        const size_t pitch = (size_t)w.S * Rp;
         for (int e = threadIdx.x; e < cnt * 16 * NR; e += 64 * W) {
             const int p = e / (16 * NR), r = e % (16 * NR);
             hl[p][r] = lora_h(h + (size_t)rows[p] * Rp + r, splits, pitch);
@@ -553,16 +647,9 @@ __global__ __launch_bounds__(64 * W) void coli_lora_outer(LoraRows w, LoraSide<T
             }
 #pragma unroll
             for (int r = 0; r < NR; r++) {
-                if constexpr (LIST) {
-                    const float *hr = h + (size_t)rw[u] * Rp + 16 * r + m;
-                    float v = hr[0];
-                    if (splits > 1) v += hr[pitch];
-                    if (splits > 2) v += hr[2 * pitch];
-                    if (splits > 3) v += hr[3 * pitch];
-                    st.h[u][r] = v;
-                } else {
-                    st.h[u][r] = hl[min(p0 + 4 * u + kq, cnt - 1)][16 * r + m];
-                }
+                const int p = min(p0 + 4 * u + kq, cnt - 1);
+                if constexpr (LIST) st.h[u][r] = h[(size_t)(first + p) * Rp + 16 * r + m];
+                else st.h[u][r] = hl[p][16 * r + m];
             }
             if (p0 + 4 * u + kq >= cnt) {
                 st.x[u] = (f4u){0.f, 0.f, 0.f, 0.f};
@@ -641,17 +728,16 @@ __global__ __launch_bounds__(64 * W) void coli_lora_outer(LoraRows w, LoraSide<T
 // ---------------------------------------------------------------------------
 // Column splits of one side's shrink: workgroups of `cols` columns such that
 // all of them are about two a CU (four waves each up to COLI_LORA_BALLOT rows:
-// at least a step a wave; eight waves beyond, where every product over h adds
-// the splits again: at most four).
-static int shrink_splits(const DevCtx *ctx, int S, long columns, int N) {
+// at least a step a wave; eight waves beyond, at most `most` splits).
+static int shrink_splits(const DevCtx *ctx, int S, long columns, int N, long most) {
     const int cus = ctx->cu_count ? ctx->cu_count : 256;
     const bool few = S <= COLI_LORA_BALLOT;
     const long cols = std::max(few ? 256L : 512L, columns / (2 * cus));
-    return (int)std::max(1L, std::min((N + cols / 2) / cols, few ? 16L : 4L));
+    return (int)std::max(1L, std::min((N + cols / 2) / cols, few ? 16L : most));
 }
 
 static int lora_tiles(int S, int slots) {
-    return S <= COLI_LORA_BALLOT ? S : S / COLI_LORA_TILE + std::min(S, slots);
+    return S <= COLI_LORA_BALLOT ? S : S / COLI_LORA_TILE + std::min(S, slots + 1);
 }
 
 // The rows' grouping, and (beyond COLI_LORA_BALLOT rows) the launch that makes it.
@@ -663,18 +749,19 @@ static int lora_rows(DevCtx *ctx, const ColiHipLora *l, const int *slot_dev, int
     w->slots = l->slots;
     if (S <= COLI_LORA_BALLOT) return 1;
     const size_t nt = (size_t)lora_tiles(S, l->slots);
-    const size_t tb = nt * sizeof(int4), rb = (size_t)l->slots * sizeof(int2), pb = (size_t)S * sizeof(int);
-    if (!reserve_kept(ctx, &ctx->lora_list, tb + rb + pb + sizeof(int), 0)) return 0;
+    const size_t tb = nt * sizeof(int4), rb = (size_t)(l->slots + 1) * sizeof(int2), pb = (size_t)S * sizeof(int);
+    if (!reserve_kept(ctx, &ctx->lora_list, tb + rb + pb + 2 * sizeof(int), 0)) return 0;
     uint8_t *p = (uint8_t *)ctx->lora_list.p;
     w->tile = (int4 *)p;
     w->run = (int2 *)(p + tb);
     w->perm = (int *)(p + tb + rb);
     w->ntile = (int *)(p + tb + rb + pb);
-    // (a counter for each wave and slot: 32 KiB of LDS)
+    // (a counter for each wave and slot: about 32 KiB of LDS at most)
+    const size_t bins = (size_t)l->slots + 1;
     if (l->slots <= 512)
-        hipLaunchKernelGGL((coli_lora_sort<16>), dim3(1), dim3(1024), (size_t)16 * l->slots * sizeof(int), ctx->stream, *w);
+        hipLaunchKernelGGL((coli_lora_sort<16>), dim3(1), dim3(1024), 16 * bins * sizeof(int), ctx->stream, *w);
     else
-        hipLaunchKernelGGL((coli_lora_sort<8>), dim3(1), dim3(512), (size_t)8 * l->slots * sizeof(int), ctx->stream, *w);
+        hipLaunchKernelGGL((coli_lora_sort<8>), dim3(1), dim3(512), 8 * bins * sizeof(int), ctx->stream, *w);
     return hip_check(hipGetLastError(), "adapter rows");
 }
 
@@ -744,7 +831,7 @@ template <typename T>
 static int lora_forward(DevCtx *ctx, ColiCudaTensor *t, const ColiHipLora *l, float *y, const float *x, int S,
                         const int *slot_dev) {
     LoraRows w;
-    const int splits = shrink_splits(ctx, S, (long)lora_tiles(S, l->slots) * l->I, l->I);
+    const int splits = shrink_splits(ctx, S, (long)lora_tiles(S, l->slots) * l->I, l->I, 8);
     if (!reserve_kept(ctx, &ctx->lora_h, (size_t)splits * S * l->Rp * sizeof(float), 0) ||
         !lora_rows(ctx, l, slot_dev, S, &w))
         return 0;
@@ -761,21 +848,34 @@ static int lora_backward(DevCtx *ctx, ColiCudaTensor *t, const ColiHipLora *l, c
                          const int *slot_dev, float *dx, float *da, float *db) {
     LoraRows w;
     const long columns = (long)lora_tiles(S, l->slots) * (l->I + l->O);
-    const int spa = shrink_splits(ctx, S, columns, l->I), spb = shrink_splits(ctx, S, columns, l->O);
-    const size_t hb = (size_t)S * l->Rp * sizeof(float);
-    if (!reserve_kept(ctx, &ctx->lora_h, (spa + spb) * hb, 0) || !lora_rows(ctx, l, slot_dev, S, &w)) return 0;
-    float *h0 = (float *)ctx->lora_h.p, *h1 = (float *)((uint8_t *)ctx->lora_h.p + spa * hb);
-    const LoraSide<T> sa = lora_side<T>(l, false, x, h0, da, spa), sb = lora_side<T>(l, true, dy, h1, db, spb);
+    const int spa = shrink_splits(ctx, S, columns, l->I, 4), spb = shrink_splits(ctx, S, columns, l->O, 4);
+    const bool few = S <= COLI_LORA_BALLOT;
+    const size_t hn = (size_t)S * l->Rp;
+    if (!reserve_kept(ctx, &ctx->lora_h, (spa + spb + (few ? 0 : 2)) * hn * sizeof(float), 0) ||
+        !lora_rows(ctx, l, slot_dev, S, &w))
+        return 0;
+    float *h0 = (float *)ctx->lora_h.p, *h1 = h0 + spa * hn;
+    LoraSide<T> sa = lora_side<T>(l, false, x, h0, da, spa), sb = lora_side<T>(l, true, dy, h1, db, spb);
     GemmTPlan plan = {};
     if (dx && !gemm_t_plan(ctx, t, dy, S, &plan)) return 0;
-    if (!launch_shrink<T>(ctx, l, w, sa, sb, 2, ColiPrepArgs{}) || !launch_outer<T>(ctx, l, w, sa, sb)) return 0;
+    if (!launch_shrink<T>(ctx, l, w, sa, sb, 2, ColiPrepArgs{})) return 0;
+    if (!few) {
+        LoraJoin j = {{h0, h1}, {h1 + spb * hn, h1 + (spb + 1) * hn}, {spa, spb}, w.perm, S, l->Rp, (int)((hn / 4 + 1023) / 1024)};
+        hipLaunchKernelGGL(coli_lora_join, dim3(2 * j.nblocks + plan.prep.nblocks), dim3(1024), 0, ctx->stream, j, plan.prep);
+        if (!hip_check(hipGetLastError(), "adapter rows join")) return 0;
+        sa.h = j.to[0];
+        sb.h = j.to[1];
+        sa.splits = sb.splits = 1;
+    }
+    if (!launch_outer<T>(ctx, l, w, sa, sb)) return 0;
     if (!dx) return 1;
-    LoraSide<T> e = lora_side<T>(l, false, nullptr, h1, dx, spb);
-    if (S <= COLI_LORA_BALLOT && plan.parts) {   // every row is a tile's: the expand joins the splits
+    LoraSide<T> e = lora_side<T>(l, false, nullptr, sb.h, dx, sb.splits);
+    e.sorted = !few;
+    if (plan.parts) {   // the expand joins the K splits
         e.part = plan.part;
         e.parts = plan.parts;
     }
-    return gemm_t_run(ctx, t, dx, dy, S, plan, !e.parts) && launch_expand<T>(ctx, l, w, e);
+    return gemm_t_run(ctx, t, dx, dy, S, plan, few, !e.parts) && launch_expand<T>(ctx, l, w, e);
 }
 
 // ---------------------------------------------------------------------------
