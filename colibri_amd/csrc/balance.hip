@@ -11,9 +11,9 @@
 // (the counts carry no gradient). Both passes are bound by the logits' bytes:
 // T E 4 read forward, read and written backward.
 //
-// A row is held by 16 lanes (float4 v of lane l: columns 64 v + 4 l), so a wave
-// runs four rows at once, every reduction of a row is four DPP steps, and one
-// load instruction of a row group reads 256 contiguous bytes. All sums are f32,
+// A row is held by L = 16, 32 or 64 lanes (float4 v of lane l: columns 4 L v +
+// 4 l), at most sixteen columns a lane, so a wave runs four rows at once up to
+// 256 experts, and the reductions of a row are lane permutes on the VALU. All sums are f32,
 // the counts integers; they are joined in a fixed order (no float atomics).
 #include "coli_hip_host.h"
 #include "coli_device.h"
@@ -56,37 +56,80 @@ __device__ __forceinline__ float dpp_sum16(float v) {
     v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xF, 0xF, false));
     return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x140, 0xF, 0xF, false));
 }
-__device__ __forceinline__ int dpp_sum16i(int v) {
+// Sum, maximum over the L lanes of a row.
+template <int L> __device__ __forceinline__ float bal_sum(float v) {
+    v = dpp_sum16(v);
+    if constexpr (L >= 32) {
+        const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    }
+    if constexpr (L >= 64) {
+        const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(b[0]) + __uint_as_float(b[1]);
+    }
+    return v;
+}
+template <int L> __device__ __forceinline__ float bal_max(float v) {
+    v = dpp_max16(v);
+    if constexpr (L >= 32) v = fmaxf(v, __shfl_xor(v, 16));
+    if constexpr (L >= 64) v = fmaxf(v, __shfl_xor(v, 32));
+    return v;
+}
+template <int L> __device__ __forceinline__ int bal_sumi(int v) {
     v += __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, false);
     v += __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, false);
     v += __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, false);
-    return v + __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, false);
+    if constexpr (L >= 32) v += __shfl_xor(v, 16);
+    if constexpr (L >= 64) v += __shfl_xor(v, 32);
+    return v;
 }
 
-// The row's logits; columns past E read -inf, which every score maps to 0.
-template <int NV>
+// Columns that every E taking this form has (nv_of): its blocks up to there are whole.
+template <int L, int NV> constexpr int bal_whole() {
+    return L == 16 ? (NV == 1 ? 0 : 32 * NV) : L == 32 ? (NV == 3 ? 256 : 384) : 512;
+}
+
+// The row's logits; columns past E read -inf, which every score maps to 0. No
+// lane takes a branch of its own (see row4): four columns a load, moved back
+// where they would pass E, and with ROW 1 (E % 4 != 0) shifted to their places
+// again; ROW 2 (E < 4): one column a load.
+template <int L, int NV, int ROW>
 __device__ __forceinline__ void bal_load(const BalanceArgs &a, int row, int l, float (&v)[4 * NV]) {
-    const float *zr = a.z + (size_t)row * a.E + 4 * l;
-    auto piece = [&](const float *p, int e, float fill) -> floatx4 {
-        if (e + 4 <= a.E) return *GPTR(f4u, p);
-        floatx4 t = {fill, fill, fill, fill};
-#pragma unroll
-        for (int k = 0; k < 3; k++)
-            if (e + k < a.E) t[k] = p[k];
+    const float *zr = a.z + (size_t)row * a.E;
+    auto block = [&](const float *p, int i) -> floatx4 {
+        const int e = 4 * L * i + 4 * l;
+        if constexpr (ROW == 2)
+            return (floatx4){p[min(e, a.E - 1)], p[min(e + 1, a.E - 1)], p[min(e + 2, a.E - 1)], p[min(e + 3, a.E - 1)]};
+        floatx4 t = *GPTR(f4u, p + min(e, a.E - 4));
+        if constexpr (ROW == 1) {
+            if (4 * L * (i + 1) > bal_whole<L, NV>()) {
+                const int d = e - min(e, a.E - 4);
+                const bool d1 = d & 1, d2 = d & 2;
+                t = (floatx4){d1 ? t[1] : t[0], d1 ? t[2] : t[1], d1 ? t[3] : t[2], t[3]};
+                t = (floatx4){d2 ? t[2] : t[0], d2 ? t[3] : t[1], t[2], t[3]};
+            }
+        }
         return t;
     };
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-        const floatx4 t = piece(zr + 64 * i, 64 * i + 4 * l, -INFINITY);
+        const floatx4 t = block(zr, i);
 #pragma unroll
         for (int k = 0; k < 4; k++) v[4 * i + k] = t[k];
     }
     for (int ch = 1; ch < a.nch; ch++)
 #pragma unroll
         for (int i = 0; i < NV; i++) {
-            const floatx4 t = piece(zr + (size_t)ch * a.chstride + 64 * i, 64 * i + 4 * l, 0.0f);
+            const floatx4 t = block(zr + (size_t)ch * a.chstride, i);
 #pragma unroll
             for (int k = 0; k < 4; k++) v[4 * i + k] += t[k];
+        }
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+        if (4 * L * (i + 1) > bal_whole<L, NV>()) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[4 * i + k] = 4 * L * i + 4 * l + (ROW ? k : 0) < a.E ? v[4 * i + k] : -INFINITY;
         }
 }
 
@@ -97,7 +140,7 @@ __device__ __forceinline__ void bal_load(const BalanceArgs &a, int row, int l, f
 // bits (every z below about -27) go by their logarithm instead, where both u are
 // linear to within f32: z, or z / 2 in mode 3. A row of nothing but -inf has
 // p = 0.
-template <int NV, int MODE, bool GRAD>
+template <int L, int NV, int MODE, int ROW, bool GRAD>
 __device__ __forceinline__ void bal_scores(const BalanceArgs &a, int row, int l, const float *w, float (&v)[4 * NV],
                                            float &sum, float &ws) {
     sum = ws = 0.0f;
@@ -128,13 +171,13 @@ __device__ __forceinline__ void bal_scores(const BalanceArgs &a, int row, int l,
             add(k, z >= 0.0f ? r : t * r, z >= 0.0f ? t * r : r);
         }
     }
-    if (MODE) sum = dpp_sum16(sum);
+    if (MODE) sum = bal_sum<L>(sum);
     if (MODE == 0 || sum < 1e-12f) {
-        if (MODE) bal_load<NV>(a, row, l, v);
+        if (MODE) bal_load<L, NV, ROW>(a, row, l, v);
         float m = -INFINITY;
 #pragma unroll
         for (int k = 0; k < 4 * NV; k++) m = fmaxf(m, v[k]);
-        m = dpp_max16(m);
+        m = bal_max<L>(m);
         sum = ws = 0.0f;
 #pragma unroll
         for (int k = 0; k < 4 * NV; k++) {
@@ -143,9 +186,9 @@ __device__ __forceinline__ void bal_scores(const BalanceArgs &a, int row, int l,
             const float c = MODE == 3 ? 0.5f : 1.0f;
             add(k, v[k] == -INFINITY ? 0.0f : __expf(c * (v[k] - m)), c);
         }
-        sum = dpp_sum16(sum);
+        sum = bal_sum<L>(sum);
     }
-    if constexpr (GRAD) ws = dpp_sum16(ws);
+    if constexpr (GRAD) ws = bal_sum<L>(ws);
 }
 
 // The sequences' offsets, clamped to the rows; in LDS where they fit (each
@@ -173,25 +216,22 @@ __device__ __forceinline__ int bal_first(const BalanceArgs &a, int row, int *s_o
     return c;
 }
 
-// Waves of the workgroup that finishes all rows alone.
-template <int NV> constexpr int bal_single_waves() { return NV <= 4 ? 16 : NV <= 8 ? 8 : 4; }
-
 // Sums of each workgroup's R rows by sequence; with SINGLE (one workgroup for
-// all rows) the outputs themselves. A wave takes four rows of each step of 4 W
-// rows from the workgroup's first; the first step's logits are requested before
+// all rows, sixteen waves) the outputs themselves. A wave takes 64 / L rows of each
+// step from the workgroup's first; the first step's logits are requested before
 // the rows' sequences are known.
-template <int NV, int MODE, bool SINGLE>
-__global__ __launch_bounds__(SINGLE ? 64 * bal_single_waves<NV>() : 256, NV <= 6 ? 4 : NV <= 8 ? 3 : 1) void coli_balance_rows(BalanceArgs a) {
-    constexpr int W = SINGLE ? bal_single_waves<NV>() : 4, NT = 64 * W, RS = 4 * W;
-    __shared__ float red[W][64 * NV];
-    __shared__ int cnt[64 * NV];
+template <int L, int NV, int MODE, int ROW, bool SINGLE>
+__global__ __launch_bounds__(SINGLE ? 1024 : 256, 4) void coli_balance_rows(BalanceArgs a) {
+    constexpr int W = SINGLE ? 16 : 4, NT = 64 * W, RW = 64 / L, RS = RW * W, COLS = 4 * L * NV;
+    __shared__ float red[W][COLS];
+    __shared__ int cnt[COLS];
     __shared__ int seg_n[2], s_off[COLI_BAL_OFF];
     __shared__ float wsum[W];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l = lane % L, g = lane / L;
     const int b = blockIdx.x, r0 = b * a.R, r1 = min(a.T, r0 + a.R);
     float v[4 * NV];
     int have = 0;   // the step whose rows v holds
-    bal_load<NV>(a, min(r0 + 4 * wave + g, r1 - 1), l, v);
+    bal_load<L, NV, ROW>(a, min(r0 + RW * wave + g, r1 - 1), l, v);
     if constexpr (SINGLE) {
         for (int e = tid; e < a.n * a.E; e += NT) a.counts[e] = 0;
         for (int i = tid; i < a.n; i += NT) {
@@ -210,7 +250,7 @@ __global__ __launch_bounds__(SINGLE ? 64 * bal_single_waves<NV>() : 256, NV <= 6
             continue;
         }
         const int hi = min(end, r1);
-        for (int e = tid; e < 64 * NV; e += NT) cnt[e] = 0;
+        for (int e = tid; e < COLS; e += NT) cnt[e] = 0;
         if (tid < 2) seg_n[tid] = 0;
         __syncthreads();
         // selections: (row, slot) pairs over the threads
@@ -229,11 +269,11 @@ __global__ __launch_bounds__(SINGLE ? 64 * bal_single_waves<NV>() : 256, NV <= 6
 #pragma unroll
         for (int k = 0; k < 4 * NV; k++) acc[k] = 0.0f;
         for (int s = (row - r0) / RS; r0 + RS * s < hi; s++) {
-            const int t = r0 + RS * s + 4 * wave + g;
+            const int t = r0 + RS * s + RW * wave + g;
             const bool in = t >= row && t < hi, live = in && (!a.mask || a.mask[t]);
             float sum, ws;
-            if (have != s) bal_load<NV>(a, min(t, r1 - 1), l, v);
-            bal_scores<NV, MODE, false>(a, min(t, r1 - 1), l, nullptr, v, sum, ws);
+            if (have != s) bal_load<L, NV, ROW>(a, min(t, r1 - 1), l, v);
+            bal_scores<L, NV, MODE, ROW, false>(a, min(t, r1 - 1), l, nullptr, v, sum, ws);
             if (live) {
                 const float r = sum == 0.0f ? 0.0f : 1.0f / sum;
                 nrow += l == 0;
@@ -241,20 +281,20 @@ __global__ __launch_bounds__(SINGLE ? 64 * bal_single_waves<NV>() : 256, NV <= 6
                 for (int k = 0; k < 4 * NV; k++) acc[k] += v[k] * r;
             }
             have = s + 1;
-            if (r0 + RS * have < r1) bal_load<NV>(a, min(t + RS, r1 - 1), l, v);
+            if (r0 + RS * have < r1) bal_load<L, NV, ROW>(a, min(t + RS, r1 - 1), l, v);
             else have = -1;
         }
         if (nsel) atomicAdd(seg_n + 1, nsel);
         if (nrow) atomicAdd(seg_n, nrow);
 #pragma unroll
         for (int k = 0; k < 4 * NV; k++) {
-            acc[k] += __shfl_xor(acc[k], 16);
-            acc[k] += __shfl_xor(acc[k], 32);
+            if (L < 32) acc[k] += __shfl_xor(acc[k], 16);
+            if (L < 64) acc[k] += __shfl_xor(acc[k], 32);
         }
         if (g == 0)
 #pragma unroll
             for (int v = 0; v < NV; v++)
-                *(floatx4 *)&red[wave][64 * v + 4 * l] =
+                *(floatx4 *)&red[wave][4 * L * v + 4 * l] =
                     (floatx4){acc[4 * v], acc[4 * v + 1], acc[4 * v + 2], acc[4 * v + 3]};
         __syncthreads();
         auto total = [&](int e) {
@@ -383,14 +423,15 @@ __global__ __launch_bounds__(1024) void coli_balance_join(BalanceArgs a) {
 }
 
 // dz of each workgroup's R rows; rows of no sequence are left as they were.
-template <int NV, int MODE>
-__global__ __launch_bounds__(256, NV <= 8 ? 4 : 1) void coli_balance_grad(BalanceArgs a) {
+template <int L, int NV, int MODE, int ROW>
+__global__ __launch_bounds__(256, 4) void coli_balance_grad(BalanceArgs a) {
+    constexpr int RW = 64 / L, RS = 4 * RW;
     __shared__ int s_off[COLI_BAL_OFF];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l = lane % L, g = lane / L;
     const int r0 = blockIdx.x * a.R, r1 = min(a.T, r0 + a.R);
     float v[4 * NV];
     int have = 0;   // the step whose rows v holds
-    bal_load<NV>(a, min(r0 + 4 * wave + g, r1 - 1), l, v);
+    bal_load<L, NV, ROW>(a, min(r0 + RW * wave + g, r1 - 1), l, v);
     int i = bal_first(a, r0, s_off);
     const BalOff off = {s_off, a.off, a.n, a.T};
     int row = i < a.n ? max(r0, off.get(0)) : r1;
@@ -407,29 +448,29 @@ __global__ __launch_bounds__(256, NV <= 8 ? 4 : 1) void coli_balance_grad(Balanc
         for (int v = 0; v < NV; v++)
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                const int e = 64 * v + 4 * l + k;
+                const int e = 4 * L * v + 4 * l + k;
                 const int c = e < a.E ? a.counts[(size_t)i * a.E + e] : 0;
                 w[4 * v + k] = (float)c;
                 C += c;
             }
-        C = dpp_sum16i(C);
+        C = bal_sumi<L>(C);
         const int n = a.rows[i];
         const float f = C > 0 && n > 0 ? a.dloss[i] * ((float)a.E / (float)C / (float)n) : 0.0f;
 #pragma unroll
         for (int k = 0; k < 4 * NV; k++) w[k] *= f;
-        for (int s = (row - r0) / 16; r0 + 16 * s < hi; s++) {
-            const int t = r0 + 16 * s + 4 * wave + g;
+        for (int s = (row - r0) / RS; r0 + RS * s < hi; s++) {
+            const int t = r0 + RS * s + RW * wave + g;
             const bool in = t >= row && t < hi, live = in && f != 0.0f && (!a.mask || a.mask[t]);
             float sum, ws;
-            if (have != s) bal_load<NV>(a, min(t, r1 - 1), l, v);
+            if (have != s) bal_load<L, NV, ROW>(a, min(t, r1 - 1), l, v);
             have = -1;
-            bal_scores<NV, MODE, true>(a, min(t, r1 - 1), l, w, v, sum, ws);
+            bal_scores<L, NV, MODE, ROW, true>(a, min(t, r1 - 1), l, w, v, sum, ws);
             const float r = sum == 0.0f ? 0.0f : 1.0f / sum, d = ws * r;
             if (!in) continue;
             float *dr = a.dz + (size_t)t * a.E;
 #pragma unroll
             for (int q = 0; q < NV; q++) {
-                const int e = 64 * q + 4 * l;
+                const int e = 4 * L * q + 4 * l;
                 floatx4 o;
 #pragma unroll
                 for (int k = 0; k < 4; k++) o[k] = live ? v[4 * q + k] * r * (w[4 * q + k] - d) : 0.0f;
@@ -447,21 +488,23 @@ __global__ __launch_bounds__(256, NV <= 8 ? 4 : 1) void coli_balance_grad(Balanc
     }
 }
 
-static int nv_of(int E) { return E <= 64 ? 1 : E <= 128 ? 2 : E <= 256 ? 4 : E <= 384 ? 6 : E <= 512 ? 8 : 16; }
 // (modes 1 and 2 score alike)
-#define COLI_BAL_MODE(mode, CALL, NV) \
-    if ((mode) == 0) CALL(NV, 0);     \
-    else if ((mode) == 3) CALL(NV, 3); \
-    else CALL(NV, 1)
-#define COLI_BAL_NV(E, CALL)          \
-    switch (nv_of(E)) {               \
-    case 1: CALL(1); break;           \
-    case 2: CALL(2); break;           \
-    case 4: CALL(4); break;           \
-    case 6: CALL(6); break;           \
-    case 8: CALL(8); break;           \
-    default: CALL(16); break;         \
-    }
+#define COLI_BAL_SCORE(mode, CALL, L, NV, ROW) \
+    if ((mode) == 0) CALL(L, NV, 0, ROW);      \
+    else if ((mode) == 3) CALL(L, NV, 3, ROW); \
+    else CALL(L, NV, 1, ROW)
+#define COLI_BAL_MODE(mode, CALL, L, NV)                           \
+    if (a.E % 4 == 0) { COLI_BAL_SCORE(mode, CALL, L, NV, 0); }    \
+    else { COLI_BAL_SCORE(mode, CALL, L, NV, 1); }
+// lanes a row and float4 a lane (bal_whole knows the ranges)
+#define COLI_BAL_CALL(mode, CALL)                                                    \
+    if (a.E < 4) { COLI_BAL_SCORE(mode, CALL, 16, 1, 2); }                           \
+    else if (a.E <= 64) { COLI_BAL_MODE(mode, CALL, 16, 1) }                         \
+    else if (a.E <= 128) { COLI_BAL_MODE(mode, CALL, 16, 2) }                        \
+    else if (a.E <= 256) { COLI_BAL_MODE(mode, CALL, 16, 4) }                        \
+    else if (a.E <= 384) { COLI_BAL_MODE(mode, CALL, 32, 3) }                        \
+    else if (a.E <= 512) { COLI_BAL_MODE(mode, CALL, 32, 4) }                        \
+    else { COLI_BAL_MODE(mode, CALL, 64, 4) }
 
 static bool balance_shape_ok(int n, int T, int E, int mode) {
     return n >= 1 && n <= COLI_BAL_MAX_SEQS && T >= 1 && T <= COLI_BAL_MAX_ROWS && E >= 1 && E <= 1024 && mode >= 0 &&
@@ -494,12 +537,9 @@ int run_balance(DevCtx *ctx, const float *z, int nch, size_t chstride, const int
     // up to four steps of one workgroup: one launch, loss included
     if (T <= (E <= 256 ? 256 : E <= 512 ? 128 : 64) && n <= 64) {
         a.R = T;
-#define COLI_BAL_ONE_M(NV, M) \
-    hipLaunchKernelGGL((coli_balance_rows<NV, M, true>), dim3(1), dim3(64 * bal_single_waves<NV>()), 0, st, a)
-#define COLI_BAL_ONE(NV) COLI_BAL_MODE(mode, COLI_BAL_ONE_M, NV)
-        COLI_BAL_NV(E, COLI_BAL_ONE)
+#define COLI_BAL_ONE(L, NV, M, ROW) hipLaunchKernelGGL((coli_balance_rows<L, NV, M, ROW, true>), dim3(1), dim3(1024), 0, st, a)
+        COLI_BAL_CALL(mode, COLI_BAL_ONE)
 #undef COLI_BAL_ONE
-#undef COLI_BAL_ONE_M
         return hip_check(hipGetLastError(), "balance");
     }
     // 16 rows a step of a workgroup; about 1024 workgroups once there are rows for them
@@ -520,15 +560,17 @@ int run_balance(DevCtx *ctx, const float *z, int nch, size_t chstride, const int
     a.pn = (int *)(p + 2 * ps_b);
     a.lossp = (float *)(p + 2 * ps_b + pn_b);
     a.arrive = (int *)ctx->bal_cnt.p;
-#define COLI_BAL_ROWS_M(NV, M) hipLaunchKernelGGL((coli_balance_rows<NV, M, false>), dim3(nb), dim3(256), 0, st, a)
-#define COLI_BAL_ROWS(NV) COLI_BAL_MODE(mode, COLI_BAL_ROWS_M, NV)
-    COLI_BAL_NV(E, COLI_BAL_ROWS)
+#define COLI_BAL_ROWS(L, NV, M, ROW) hipLaunchKernelGGL((coli_balance_rows<L, NV, M, ROW, false>), dim3(nb), dim3(256), 0, st, a)
+    COLI_BAL_CALL(mode, COLI_BAL_ROWS)
 #undef COLI_BAL_ROWS
-#undef COLI_BAL_ROWS_M
     if (!hip_check(hipGetLastError(), "balance rows")) return 0;
 #define COLI_BAL_JOIN(NB) hipLaunchKernelGGL((coli_balance_join<NB>), dim3(n, neb), dim3(1024), 0, st, a)
-    if (many) COLI_BAL_JOIN(1);
-    else COLI_BAL_NV(E, COLI_BAL_JOIN)
+    if (many || E <= 64) COLI_BAL_JOIN(1);
+    else if (E <= 128) COLI_BAL_JOIN(2);
+    else if (E <= 256) COLI_BAL_JOIN(4);
+    else if (E <= 384) COLI_BAL_JOIN(6);
+    else if (E <= 512) COLI_BAL_JOIN(8);
+    else COLI_BAL_JOIN(16);
 #undef COLI_BAL_JOIN
     return hip_check(hipGetLastError(), "balance join");
 }
@@ -567,10 +609,8 @@ extern "C" int coli_hip_balance_grad_dev(int device, const float *logits, const 
     a.dz = dlogits;
     a.R = std::max(16, (T + 2047) / 2048 + 15 & ~15);
     const int nb = (T + a.R - 1) / a.R;
-#define COLI_BAL_GRAD_M(NV, M) hipLaunchKernelGGL((coli_balance_grad<NV, M>), dim3(nb), dim3(256), 0, ctx->stream, a)
-#define COLI_BAL_GRAD(NV) COLI_BAL_MODE(route_mode, COLI_BAL_GRAD_M, NV)
-    COLI_BAL_NV(E, COLI_BAL_GRAD)
+#define COLI_BAL_GRAD(L, NV, M, ROW) hipLaunchKernelGGL((coli_balance_grad<L, NV, M, ROW>), dim3(nb), dim3(256), 0, ctx->stream, a)
+    COLI_BAL_CALL(route_mode, COLI_BAL_GRAD)
 #undef COLI_BAL_GRAD
-#undef COLI_BAL_GRAD_M
     return hip_check(hipGetLastError(), "balance gradient");
 }

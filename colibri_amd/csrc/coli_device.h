@@ -279,18 +279,30 @@ typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));   // any 4-by
 // nibbles in (int4: even ones, then odd ones).
 __host__ __device__ __forceinline__ int t_order(int int4, int e) { return !int4 ? e : e < 4 ? 2 * e : 2 * (e - 4) + 1; }
 
-// Octet o of a row, zeros past K.
-__device__ __forceinline__ void t_load8(const float *xr, int o, int K, float (&v)[8]) {
-    if (8 * o + 8 <= K) {
-        const f4u a = *GPTR(f4u, xr + 8 * o), b = *GPTR(f4u, xr + 8 * o + 4);
+// Four elements of a row of n >= 4 from element c on (past its end: some element
+// of the row), by one load moved back where it would pass the end; ODD (n % 4 !=
+// 0): and shifted to their places again. No lane takes a branch of its own: a
+// vector load and element loads merged under divergent control flow were
+// miscompiled in one kernel here (hipcc 7.2: elements of the vector overwritten
+// between the load and a later loop), and a uniform branch would keep the loads
+// of one step from being requested together.
+template <bool ODD> __device__ __forceinline__ floatx4 row4(const float *xr, int c, int n) {
+    const int p = min(c, n - 4);
+    floatx4 t = *GPTR(f4u, xr + p);
+    if constexpr (ODD) {
+        const bool d1 = (c - p) & 1, d2 = (c - p) & 2;
+        t = (floatx4){d1 ? t[1] : t[0], d1 ? t[2] : t[1], d1 ? t[3] : t[2], t[3]};
+        t = (floatx4){d2 ? t[2] : t[0], d2 ? t[3] : t[1], t[2], t[3]};
+    }
+    return t;
+}
+// Octet o of a row of K (past its end the weights' scales are zero).
+template <bool ODD> __device__ __forceinline__ void t_load8(const float *xr, int o, int K, float (&v)[8]) {
+    const floatx4 a = row4<ODD>(xr, 8 * o, K), b = row4<ODD>(xr, 8 * o + 4, K);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            v[i] = a[i];
-            v[4 + i] = b[i];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = 8 * o + i < K ? xr[8 * o + i] : 0.0f;
+    for (int i = 0; i < 4; i++) {
+        v[i] = a[i];
+        v[4 + i] = b[i];
     }
 }
 // As hi + lo under the exponent E, in operand order.
@@ -320,20 +332,19 @@ __device__ __forceinline__ int t_exponent(float m) {
 // that loads read 512 and stores write 64 contiguous bytes; a row of up to
 // 16384 columns is read once.
 #define COLI_T_SLOTS 8   // octets a thread holds
-__device__ __forceinline__ void coli_t_prep_block(const ColiTPrepArgs &a, int blk) {
-    __shared__ float wmax[16][4];
+template <bool ODD> __device__ __forceinline__ void t_prep_block(const ColiTPrepArgs &a, int blk, float (*wmax)[4]) {
     const int tid = threadIdx.x, lane = tid & 63, r = tid & 3, o0 = tid >> 2, row = blk * 4 + r;
     const float *xr = a.dy + (size_t)min(row, a.S - 1) * a.K;
     float v[COLI_T_SLOTS][8], m = 0.0f;
 #pragma unroll
-    for (int s = 0; s < COLI_T_SLOTS; s++) t_load8(xr, o0 + 256 * s, a.K, v[s]);
+    for (int s = 0; s < COLI_T_SLOTS; s++) t_load8<ODD>(xr, o0 + 256 * s, a.K, v[s]);
 #pragma unroll
     for (int s = 0; s < COLI_T_SLOTS; s++)
 #pragma unroll
         for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(v[s][i]));
     for (int o = o0 + 256 * COLI_T_SLOTS; o < a.noct; o += 256) {
         float u[8];
-        t_load8(xr, o, a.K, u);
+        t_load8<ODD>(xr, o, a.K, u);
 #pragma unroll
         for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(u[i]));
     }
@@ -357,9 +368,14 @@ __device__ __forceinline__ void coli_t_prep_block(const ColiTPrepArgs &a, int bl
         if (o0 + 256 * s < a.noct) put(o0 + 256 * s, v[s]);
     for (int o = o0 + 256 * COLI_T_SLOTS; o < a.noct; o += 256) {
         float u[8];
-        t_load8(xr, o, a.K, u);
+        t_load8<ODD>(xr, o, a.K, u);
         put(o, u);
     }
+}
+__device__ __forceinline__ void coli_t_prep_block(const ColiTPrepArgs &a, int blk) {
+    __shared__ float wmax[16][4];
+    if (a.K % 4 == 0) t_prep_block<false>(a, blk, wmax);
+    else t_prep_block<true>(a, blk, wmax);
 }
 
 // ---------------------------------------------------------------------------

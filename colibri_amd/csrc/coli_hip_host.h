@@ -187,7 +187,7 @@ int gemm_prepared(DevCtx *ctx, ColiCudaTensor *t, float *y_dev, const float *x_d
 // dx, else left in part [parts][S][I] where parts is not 0).
 struct GemmTPlan {
     ColiTPrepArgs prep;
-    int mt, splits, per;
+    int splits, per;
     float *part;
     int parts;
 };

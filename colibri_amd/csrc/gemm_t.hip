@@ -87,6 +87,10 @@ __global__ __launch_bounds__(1024) void coli_t_prep_rows(ColiTPrepArgs a) { coli
 // ---------------------------------------------------------------------------
 // the product
 // ---------------------------------------------------------------------------
+// Rows that convert dy inside the product (measured, product and build: 64 rows
+// of 4096 x 14336 int4 45 us, on the many-row kernel 52).
+#define COLI_T_FEW 64
+
 struct GemmTArgs {
     const uint8_t *w;            // tiles [nrt][nq]
     const _Float16 *sct;
@@ -95,7 +99,7 @@ struct GemmTArgs {
     const int *exps;             // [S]
     size_t Sp;
     const float *dy;             // [S][O] (few rows)
-    int O;
+    int O;                       // its columns, at least 4
     int nrt, nq, noct, I, S;
     int splits, per;             // K split: steps of 32 rows of W each
     float *out;                  // [splits][S][I]
@@ -159,23 +163,51 @@ __device__ __forceinline__ void t_weights(uint32_t nib, half8v s, half8v s2, hal
     }
 }
 
-// Workgroup (64 WN columns, 32 MT rows, K split); WK wave groups share its K
-// steps (32 rows of W: two row tiles) and are joined in LDS at the end. A
-// step's dy octets are staged in LDS (two buffers), the weights and scales of
-// the next step are requested before this one's products.
-// FEW (up to 64 rows): dy is read as f32 and converted on its way into LDS,
-// under the exponent of the row's part in this K split (the splits' sums are
-// f32 already), which saves the launch that would build the operands.
-template <int KIND, int MT, int WN, int WK, bool FEW>
+// One K step's products: a lane's dwords d of two row tiles' half-quad, their
+// scales, and dy's octets in LDS ([part][octet][BM rows][8]).
+template <int KIND, int MT>
+__device__ __forceinline__ void t_products(const uint32_t (&d)[2][2], const half8v (&sc)[2], const half8v (&sc2)[2],
+                                           const NibT &nc, const uint8_t *as, int lane, floatx16 (&acc)[MT][2]) {
+    constexpr int BM = 32 * MT;
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+        uint32_t b[2];
+        half_quad(d[t][0], d[t][1], nc, b[0], b[1]);
+        half8v bh[2], bl[2];
+#pragma unroll
+        for (int r = 0; r < 2; r++) t_weights<KIND>(b[r], sc[t], sc2[t], bh[r], bl[r]);
+        const uint8_t *ap = as + (size_t)((2 * t + (lane >> 5)) * BM + (lane & 31)) * 16;
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+            const half8v ah = *(const half8v *)(ap + m * 32 * 16);
+            const half8v al = *(const half8v *)(ap + (4 * BM + m * 32) * 16);
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                acc[m][r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh[r], acc[m][r], 0, 0, 0);
+                acc[m][r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh[r], acc[m][r], 0, 0, 0);
+                if constexpr (KIND != COLI_KIND_FP4)
+                    acc[m][r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl[r], acc[m][r], 0, 0, 0);
+            }
+        }
+    }
+}
+
+// Many rows: workgroup (64 WN columns, 32 MT rows, K split); WK wave groups
+// share its K steps (32 rows of W: two row tiles) and are joined in LDS at the
+// end. A step's dy octets are staged in LDS (two buffers), the weights and
+// scales of the next step are requested before this one's products. Bound by
+// the matrix cores: int4 runs three products, at 2048 x 4096 x 14336 617 us or
+// 1.17 PFLOP/s of fp16 (the library's large fp16 product: 1.07 on the same
+// card); with one wave group, one wave a SIMD, 686 us.
+template <int KIND, int MT, int WN, int WK>
 __global__ __launch_bounds__(64 * WN * WK, 2) void coli_gemm_t(GemmTArgs a) {
-    constexpr int BM = 32 * MT, NT = 64 * WN, CH = (FEW ? 4 : 8) * BM;   // 8 (FEW: f32) values a chunk, 4 octets x BM rows
+    constexpr int BM = 32 * MT, NT = 64 * WN, CH = 8 * BM;   // 16-byte chunks of a step: 2 parts x 4 octets x BM rows
     constexpr int CPT = CH / NT;
     static_assert(CH % NT == 0, "whole chunks a thread");
     constexpr int STAGE = 8 * BM * 16;
-    constexpr int JOIN = WK > 1 ? WK * (WK - 1) * (32 / WK) * NT * 4 : 0;
+    constexpr int JOIN = WK * (WK - 1) * (32 / WK) * NT * 4;
     constexpr int LDS = 2 * WK * STAGE > JOIN ? 2 * WK * STAGE : JOIN;
     __shared__ __attribute__((aligned(16))) uint8_t lds[LDS];
-    __shared__ int rexp[FEW ? BM : 1];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave % WN, wk = wave / WN;
     const int gt = tid - wk * NT;                              // thread within its K group
@@ -184,11 +216,15 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void coli_gemm_t(GemmTArgs a) {
     const int k0 = blockIdx.z * a.per, k1 = min((a.noct + 3) / 4, k0 + a.per);
     const int nstep = (k1 - k0 + WK - 1) / WK;
     const NibT nc = nib_consts(lane);
-    const uint8_t *wp = a.w + (size_t)q * COLI_TILE_BYTES + lane * 16 + 8 * h;
+    // (a base of the whole wave and a 32-bit offset of the lane: no address
+    // arithmetic on the VALU)
+    const uint8_t *wp = a.w + (size_t)q * COLI_TILE_BYTES + 8 * h;
+    const uint32_t wo = lane * 16;
     const size_t wstride = (size_t)a.nq * COLI_TILE_BYTES;
-    const size_t plane = (size_t)a.nq * 4 * a.noct * 8;
+    const size_t plane = (size_t)a.nq * 4 * a.noct * 16;
     // lane bit 3: the column group, lane bit 5: the octet of a row tile
-    const _Float16 *sp = a.sct + (((size_t)4 * q + 2 * h + (lane >> 3 & 1)) * a.noct + (lane >> 5)) * 8;
+    const uint8_t *sp = (const uint8_t *)a.sct + ((size_t)4 * q + 2 * h) * a.noct * 16;
+    const uint32_t so = (uint32_t)((lane >> 3 & 1) * a.noct + (lane >> 5)) * 16;
     floatx16 acc[MT][2];
 #pragma unroll
     for (int m = 0; m < MT; m++)
@@ -198,111 +234,51 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void coli_gemm_t(GemmTArgs a) {
             for (int i = 0; i < 16; i++) acc[m][r][i] = 0.0f;
     u32x2 wd[2];
     half8v sc[2], sc2[2];
-    u32x4 ad[FEW ? 1 : CPT];
-    float af[FEW ? CPT : 1][8];
-    int ae[FEW ? CPT : 1];
+    u32x4 ad[CPT];
     auto load_w = [&](int step) {
         step = min(step, k1 - 1);
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            const int rt = min(2 * step + t, a.nrt - 1);   // (past the last row tile: zero scales)
-            wd[t] = *GPTR(u32x2, wp + rt * wstride);
-            sc[t] = *GPTR(half8v, sp + (size_t)(4 * step + 2 * t) * 8);
-            if constexpr (KIND == COLI_KIND_I4_F) sc2[t] = *GPTR(half8v, sp + plane + (size_t)(4 * step + 2 * t) * 8);
+            const uint8_t *wb = wp + min(2 * step + t, a.nrt - 1) * wstride;   // (past the last row tile: zero scales)
+            const uint8_t *sb = sp + (size_t)(4 * step + 2 * t) * 16;
+            wd[t] = *GPTR(u32x2, wb + wo);
+            sc[t] = *GPTR(half8v, sb + so);
+            if constexpr (KIND == COLI_KIND_I4_F) sc2[t] = *GPTR(half8v, sb + plane + so);
         }
     };
     auto load_a = [&](int step) {
         step = min(step, k1 - 1);
 #pragma unroll
         for (int i = 0; i < CPT; i++) {
+            // chunk c: part c / (4 BM) (the same for the whole workgroup), octet c / BM % 4, row c % BM
+            static_assert(4 * BM % NT == 0, "a load is of one part");
             const int c = gt + i * NT;
-            if constexpr (FEW) {
-                const int r = row0 + (c >> 2), o = 4 * step + (c & 3);
-                t_load8(a.dy + (size_t)min(r, a.S - 1) * a.O, r < a.S ? o : a.noct, a.O, af[i]);
-            } else {
-                const int part = c / (4 * BM), oct = c / BM % 4, r = c % BM;
-                ad[i] = *GPTR(u32x4, (part ? a.lo : a.hi) + ((size_t)(4 * step + oct) * a.Sp + row0 + r) * 8);
-            }
+            const uint8_t *ab = (const uint8_t *)(i * NT >= 4 * BM ? a.lo : a.hi) + ((size_t)4 * step * a.Sp + row0) * 16;
+            ad[i] = *GPTR(u32x4, ab + (uint32_t)((c / BM % 4) * (uint32_t)a.Sp + c % BM) * 16);
         }
     };
     auto store_a = [&](int buf) {
-        uint8_t *to = lds + (size_t)(buf * WK + wk) * STAGE;
 #pragma unroll
-        for (int i = 0; i < CPT; i++) {
-            const int c = gt + i * NT;
-            if constexpr (FEW) {
-                half8v hv, lv;
-                t_split8(af[i], KIND != COLI_KIND_FP4, ae[i], hv, lv);
-                *(half8v *)(to + ((c & 3) * BM + (c >> 2)) * 16) = hv;
-                *(half8v *)(to + ((4 + (c & 3)) * BM + (c >> 2)) * 16) = lv;
-            } else {
-                *(u32x4 *)(to + (size_t)c * 16) = ad[i];
-            }
-        }
+        for (int i = 0; i < CPT; i++) *(u32x4 *)(lds + (size_t)(buf * WK + wk) * STAGE + (size_t)(gt + i * NT) * 16) = ad[i];
     };
     load_w(k0 + wk);
     load_a(k0 + wk);
-    if constexpr (FEW) {
-        // the rows' exponents over this split's columns
-        constexpr int TPR = 64 * WN * WK / BM;   // threads a row
-        const int r = tid / TPR, row = row0 + r;
-        float m = 0.0f;
-        if (row < a.S) {
-            const float *xr = a.dy + (size_t)row * a.O;
-            const int c1 = min(a.O, 32 * k1);
-            int c = 32 * k0 + 4 * (tid % TPR);
-#pragma unroll 4
-            for (; c + 4 <= c1; c += 4 * TPR) {
-                const f4u v = *GPTR(f4u, xr + c);
-                m = fmaxf(m, fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))));
-            }
-            for (; c < c1; c++) m = fmaxf(m, fabsf(xr[c]));   // (at most 3: the others are past c1)
-        }
-#pragma unroll
-        for (int o = 1; o < TPR; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
-        if (tid % TPR == 0) rexp[r] = t_exponent(m);
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < CPT; i++) ae[i] = rexp[(gt + i * NT) >> 2];
-    }
     store_a(0);
     __syncthreads();
     for (int it = 0; it < nstep; it++) {
         const int step = k0 + it * WK + wk;
-        u32x2 w0[2];
+        uint32_t w0[2][2];
         half8v s0[2], s1[2];
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            w0[t] = wd[t];
+            w0[t][0] = wd[t][0];
+            w0[t][1] = wd[t][1];
             s0[t] = sc[t];
             s1[t] = sc2[t];
         }
         load_a(step + WK);
         load_w(step + WK);
-        if (step < k1) {
-            const uint8_t *as = lds + (size_t)((it & 1) * WK + wk) * STAGE;
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                uint32_t b[2];
-                half_quad(w0[t][0], w0[t][1], nc, b[0], b[1]);
-                half8v bh[2], bl[2];
-#pragma unroll
-                for (int r = 0; r < 2; r++) t_weights<KIND>(b[r], s0[t], s1[t], bh[r], bl[r]);
-                const uint8_t *ap = as + (size_t)((2 * t + (lane >> 5)) * BM + (lane & 31)) * 16;
-#pragma unroll
-                for (int m = 0; m < MT; m++) {
-                    const half8v ah = *(const half8v *)(ap + m * 32 * 16);
-                    const half8v al = *(const half8v *)(ap + (4 * BM + m * 32) * 16);
-#pragma unroll
-                    for (int r = 0; r < 2; r++) {
-                        acc[m][r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh[r], acc[m][r], 0, 0, 0);
-                        acc[m][r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh[r], acc[m][r], 0, 0, 0);
-                        if constexpr (KIND != COLI_KIND_FP4)
-                            acc[m][r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl[r], acc[m][r], 0, 0, 0);
-                    }
-                }
-            }
-        }
+        if (step < k1) t_products<KIND, MT>(w0, s0, s1, nc, lds + (size_t)((it & 1) * WK + wk) * STAGE, lane, acc);
         if (it + 1 < nstep) store_a((it + 1) & 1);
         __syncthreads();
     }
@@ -310,51 +286,197 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void coli_gemm_t(GemmTArgs a) {
     const int c0 = 128 * q + 64 * h + 32 * (lane >> 3 & 1) + 8 * (lane >> 4 & 1) + (lane & 7);
     const int E = a.ge[4 * q + 2 * h + (lane >> 3 & 1)];
     float *out = a.out + (size_t)blockIdx.z * a.S * a.I;
-    auto put = [&](int lrow, int r, float v) {
-        const int row = row0 + lrow;
-        if (row >= a.S || hq >= 2 * a.nq || c0 + 16 * r >= a.I) return;
-        out[(size_t)row * a.I + c0 + 16 * r] = ldexpf(v, E + (FEW ? rexp[FEW ? lrow : 0] : a.exps[row]));
+    // group g finishes registers i with i / (16 / WK) == g: the others' are
+    // handed over through LDS, [g][the other][r][i][thread]
+    constexpr int NI = 16 / WK;
+    float *js = (float *)lds;
+    auto at = [&](int g, int s, int r, int i) { return (((g * (WK - 1) + (s < g ? s : s - 1)) * 2 + r) * NI + i) * NT + gt; };
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
+        if (m) __syncthreads();
+#pragma unroll
+        for (int g = 0; g < WK; g++)
+            if (g != wk)
+#pragma unroll
+                for (int r = 0; r < 2; r++)
+#pragma unroll
+                    for (int i = 0; i < NI; i++) js[at(g, wk, r, i)] = acc[m][r][g * NI + i];
+        __syncthreads();
+#pragma unroll
+        for (int g = 0; g < WK; g++)
+            if (g == wk)
+#pragma unroll
+                for (int i = 0; i < NI; i++) {
+                    const int k = g * NI + i, row = row0 + 32 * m + 8 * (k >> 2) + 4 * (lane >> 5) + (k & 3);
+                    const int e = E + a.exps[min(row, a.S - 1)];
+#pragma unroll
+                    for (int r = 0; r < 2; r++) {
+                        float v = acc[m][r][k];
+#pragma unroll
+                        for (int s = 0; s < WK; s++)
+                            if (s != g) v += js[at(g, s, r, i)];
+                        if (row < a.S && hq < 2 * a.nq && c0 + 16 * r < a.I)
+                            out[(size_t)row * a.I + c0 + 16 * r] = ldexpf(v, e);
+                    }
+                }
+    }
+}
+
+// Up to 64 rows: workgroup (tile quad, 32 rows, K split), eight waves that take
+// its K steps in turn, each with all 128 columns and its own copy of the step's
+// dy: read as f32 and converted on its way into the wave's LDS, under the
+// exponent of the row's part in this split (the splits' sums are f32 already).
+// No launch builds operands, and no barrier holds the waves together before
+// their sums are joined. Bound by the VALU (transpose, unpack and conversion,
+// about 450 instructions a step of 4096 weights); a 64-row form spilled its
+// accumulators, so 33 to 64 rows read and unpack the weights twice.
+template <int KIND, bool ODD>
+__global__ __launch_bounds__(512, 2) void coli_gemm_t_few(GemmTArgs a) {
+    constexpr int BM = 32, W = 8, CPT = 4 * BM / 64, STAGE = 8 * BM * 16, PD = 2;
+    // the join: two accumulators of every wave at a time
+    constexpr int LDS = 2 * W * 16 * 64 * 4;
+    static_assert(W * STAGE <= LDS, "the waves' stages");
+    __shared__ __attribute__((aligned(16))) uint8_t lds[LDS];
+    __shared__ int rexp[BM];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int q = blockIdx.x, row0 = blockIdx.y * BM, live = min(BM, a.S - row0);
+    const int k0 = blockIdx.z * a.per, k1 = min((a.noct + 3) / 4, k0 + a.per);
+    const NibT nc = nib_consts(lane);
+    // (a base of the whole wave and a 32-bit offset of the lane: no address
+    // arithmetic on the VALU)
+    const uint8_t *wp = a.w + (size_t)q * COLI_TILE_BYTES;
+    const uint32_t wo = lane * 16;
+    const size_t wstride = (size_t)a.nq * COLI_TILE_BYTES;
+    const size_t plane = (size_t)a.nq * 4 * a.noct * 16;
+    // lane bit 3: the column group of a half, lane bit 5: the octet of a row tile
+    const uint8_t *sp = (const uint8_t *)a.sct + (size_t)4 * q * a.noct * 16;
+    const uint32_t so = (uint32_t)((lane >> 3 & 1) * a.noct + (lane >> 5)) * 16;
+    const float *dy = a.dy + (size_t)row0 * a.O;
+    floatx16 acc[2][1][2];
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int r = 0; r < 2; r++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) acc[h][0][r][i] = 0.0f;
+    struct Step {
+        u32x4 w[2];
+        half8v s[2][2], s2[2][2];   // [half][row tile]
     };
-    if constexpr (WK == 1) {
+    Step st[PD];
+    float af[CPT][8];
+    int ae[CPT];
+    auto load_w = [&](int step, Step &p) {
+        step = min(step, k1 - 1);
 #pragma unroll
-        for (int m = 0; m < MT; m++)
+        for (int t = 0; t < 2; t++) {
+            const uint8_t *wb = wp + min(2 * step + t, a.nrt - 1) * wstride;   // (past the last row tile: zero scales)
+            p.w[t] = *GPTR(u32x4, wb + wo);
 #pragma unroll
-            for (int i = 0; i < 16; i++)
+            for (int h = 0; h < 2; h++) {
+                const uint8_t *sb = sp + ((size_t)2 * h * a.noct + 4 * step + 2 * t) * 16;
+                p.s[h][t] = *GPTR(half8v, sb + so);
+                if constexpr (KIND == COLI_KIND_I4_F) p.s2[h][t] = *GPTR(half8v, sb + plane + so);
+            }
+        }
+    };
+    // chunk c of a step: octet c % 4 of row c / 4 (a chunk of rows past S: skipped
+    // where all of a load's are, else some row's, not kept)
+    auto load_a = [&](int step) {
+        step = min(step, k1 - 1);
 #pragma unroll
-                for (int r = 0; r < 2; r++) put(32 * m + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3), r, acc[m][r][i]);
-    } else {
-        // group g finishes registers i with i / (16 / WK) == g: the others' are
-        // handed over through LDS, [g][the other][r][i][thread]
-        constexpr int NI = 16 / WK;
-        float *js = (float *)lds;
-        auto at = [&](int g, int s, int r, int i) { return (((g * (WK - 1) + (s < g ? s : s - 1)) * 2 + r) * NI + i) * NT + gt; };
+        for (int i = 0; i < CPT; i++) {
+            if (16 * i >= live) continue;
+            const int c = lane + i * 64;
+            t_load8<ODD>(dy + (uint32_t)(min(c >> 2, live - 1) * a.O), 4 * step + (c & 3), a.O, af[i]);
+        }
+    };
 #pragma unroll
-        for (int m = 0; m < MT; m++) {
-            if (m) __syncthreads();
+    for (int p = 0; p < PD; p++) load_w(k0 + wave + p * W, st[p]);
 #pragma unroll
-            for (int g = 0; g < WK; g++)
-                if (g != wk)
+    for (int i = 0; i < CPT; i++)
 #pragma unroll
-                    for (int r = 0; r < 2; r++)
+        for (int e = 0; e < 8; e++) af[i][e] = 0.0f;
+    load_a(k0 + wave);
+    {
+        // the rows' exponents over this split's columns
+        constexpr int TPR = 64 * W / BM;   // threads a row
+        const int r = tid / TPR;
+        float m = 0.0f;
+        const float *xr = dy + (size_t)min(r, live - 1) * a.O;
+        // (requested eight at a time: the split's first products wait for this)
+        for (int c = 32 * k0 + 4 * (tid % TPR); c < 32 * k1; c += 32 * TPR) {
+            floatx4 v[8];
 #pragma unroll
-                        for (int i = 0; i < NI; i++) js[at(g, wk, r, i)] = acc[m][r][g * NI + i];
-            __syncthreads();
+            for (int u = 0; u < 8; u++) v[u] = row4<ODD>(xr, min(c + 4 * u * TPR, 32 * k1 - 4), a.O);
 #pragma unroll
-            for (int g = 0; g < WK; g++)
-                if (g == wk)
+            for (int u = 0; u < 8; u++)
+                m = fmaxf(m, fmaxf(fmaxf(fabsf(v[u][0]), fabsf(v[u][1])), fmaxf(fabsf(v[u][2]), fabsf(v[u][3]))));
+        }
 #pragma unroll
-                    for (int r = 0; r < 2; r++)
+        for (int o = 1; o < TPR; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+        if (tid % TPR == 0) rexp[r] = t_exponent(m);
+        __syncthreads();
 #pragma unroll
-                        for (int i = 0; i < NI; i++) {
-                            float v = acc[m][r][g * NI + i];
+        for (int i = 0; i < CPT; i++) ae[i] = rexp[(lane + i * 64) >> 2];
+    }
+    uint8_t *mine = lds + wave * STAGE;
+    auto one = [&](int step, Step &p) {
 #pragma unroll
-                            for (int s = 0; s < WK; s++)
-                                if (s != g) v += js[at(g, s, r, i)];
-                            const int k = g * NI + i;
-                            put(32 * m + 8 * (k >> 2) + 4 * (lane >> 5) + (k & 3), r, v);
-                        }
+        for (int i = 0; i < CPT; i++) {
+            if (16 * i >= live) continue;   // (rows that are not kept: whatever LDS holds)
+            const int c = lane + i * 64;
+            half8v hv, lv;
+            t_split8(af[i], KIND != COLI_KIND_FP4, ae[i], hv, lv);
+            *(half8v *)(mine + ((c & 3) * BM + (c >> 2)) * 16) = hv;
+            *(half8v *)(mine + ((4 + (c & 3)) * BM + (c >> 2)) * 16) = lv;
+        }
+        load_a(step + W);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the wave's other lanes' chunks
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const uint32_t d[2][2] = {{p.w[0][2 * h], p.w[0][2 * h + 1]}, {p.w[1][2 * h], p.w[1][2 * h + 1]}};
+            t_products<KIND, 1>(d, p.s[h], p.s2[h], nc, mine, lane, acc[h]);
+        }
+        load_w(step + PD * W, p);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // read before the next step's writes
+    };
+    for (int step = k0 + wave; step < k1; step += PD * W) {
+        one(step, st[0]);
+        if (step + W < k1) one(step + W, st[1]);
+    }
+    // wave w finishes registers 2 w, 2 w + 1 of both operands r
+    float *js = (float *)lds;
+    const int c0 = 128 * q + 32 * (lane >> 3 & 1) + 8 * (lane >> 4 & 1) + (lane & 7);
+    float *out = a.out + ((size_t)blockIdx.z * a.S + row0) * a.I;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const int E = a.ge[4 * q + 2 * h + (lane >> 3 & 1)];
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < 2; r++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) js[((r * 16 + i) * W + wave) * 64 + lane] = acc[h][0][r][i];
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int i = 2 * wave + u, row = 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                float v = js[(r * 16 + i) * W * 64 + lane];
+#pragma unroll
+                for (int s = 1; s < W; s++) v += js[((r * 16 + i) * W + s) * 64 + lane];
+                const int c = c0 + 64 * h + 16 * r;
+                if (row < live && c < a.I) out[(size_t)row * a.I + c] = ldexpf(v, E + rexp[row]);
+            }
         }
     }
+}
+
+// dy of fewer than four columns as rows of four.
+__global__ void coli_t_pad(const float *__restrict__ dy, float *__restrict__ to, int S, int O) {
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < 4 * S) to[i] = (i & 3) < O ? dy[(size_t)(i >> 2) * O + (i & 3)] : 0.0f;
 }
 
 // Sum of the K splits, in order.
@@ -421,14 +543,14 @@ int build_t_scales(DevCtx *ctx, ColiCudaTensor *t, bool update_only) {
 }
 
 template <int KIND>
-static void launch_gemm_t(const GemmTArgs &a, int mt, hipStream_t st) {
-    const int rb = (a.S + 32 * mt - 1) / (32 * mt);
-    if (mt == 4)
-        hipLaunchKernelGGL((coli_gemm_t<KIND, 4, 4, 2, false>), dim3((a.nq + 1) / 2, rb, a.splits), dim3(512), 0, st, a);
-    else if (mt == 2)
-        hipLaunchKernelGGL((coli_gemm_t<KIND, 2, 2, 4, true>), dim3(a.nq, rb, a.splits), dim3(512), 0, st, a);
+static void launch_gemm_t(const GemmTArgs &a, bool few, hipStream_t st) {
+    const dim3 grid(a.nq, (a.S + 31) / 32, a.splits);
+    if (few && a.O % 4 == 0)
+        hipLaunchKernelGGL((coli_gemm_t_few<KIND, false>), grid, dim3(512), 0, st, a);
+    else if (few)
+        hipLaunchKernelGGL((coli_gemm_t_few<KIND, true>), grid, dim3(512), 0, st, a);
     else
-        hipLaunchKernelGGL((coli_gemm_t<KIND, 1, 2, 4, true>), dim3(a.nq, rb, a.splits), dim3(512), 0, st, a);
+        hipLaunchKernelGGL((coli_gemm_t<KIND, 4, 4, 2>), dim3((a.nq + 1) / 2, (a.S + 127) / 128, a.splits), dim3(512), 0, st, a);
 }
 
 // K splits of many rows: the modelled time, in steps of 32 rows of W. A
@@ -456,32 +578,37 @@ int gemm_t_plan(DevCtx *ctx, ColiCudaTensor *t, const float *dy, int S, GemmTPla
     *g = GemmTPlan{};
     if (t->kind == COLI_KIND_GENERIC) return 1;
     if (!t->sct && !build_t_scales(ctx, t, false)) return 0;
-    const int noct = t_octets(t), steps = noct / 4, mt = S <= 32 ? 1 : S <= 64 ? 2 : 4;
-    const bool few = mt < 4;
+    const int noct = t_octets(t), steps = noct / 4;
+    const bool few = S <= COLI_T_FEW;
     const size_t Sp = few ? 0 : ((size_t)S + 127) & ~(size_t)127, fb = (size_t)noct * Sp * 16;
     const int cus = ctx->cu_count ? ctx->cu_count : 256;
-    const long blocks = (long)((S + 32 * mt - 1) / (32 * mt)) * (few ? t->nq : (t->nq + 1) / 2);
-    int splits = few ? (int)std::max(1L, std::min((2L * cus + blocks - 1) / blocks, (long)std::max(1, steps / 8)))
-                     : t_splits(t, S, cus, blocks, steps);
+    const long blocks = few ? (long)((S + 31) / 32) * t->nq : (long)((S + 127) / 128) * ((t->nq + 1) / 2);
+    // few rows: a workgroup a CU, a step for each of its waves at least
+    int splits = few ? (int)std::max(1L, std::min((long)cus / blocks, (long)steps / 8)) : t_splits(t, S, cus, blocks, steps);
     const int per = (steps + splits - 1) / splits;
     splits = (steps + per - 1) / per;
     const size_t eb = (Sp * sizeof(int) + 255) & ~(size_t)255;
     const size_t pb = splits > 1 ? (size_t)splits * S * t->I * sizeof(float) : 0;
-    if (2 * fb + eb + pb && !reserve_kept(ctx, &ctx->gt, 2 * fb + eb + pb, 0)) return 0;
+    const size_t db = t->O < 4 ? (size_t)S * 16 : 0;
+    if (2 * fb + eb + pb + db && !reserve_kept(ctx, &ctx->gt, 2 * fb + eb + pb + db, 0)) return 0;
     uint8_t *p = (uint8_t *)ctx->gt.p;
-    g->mt = mt;
     g->splits = splits;
     g->per = per;
     g->part = (float *)(p + 2 * fb + eb);
     g->parts = splits > 1 ? splits : 0;
     ColiTPrepArgs &a = g->prep;
     a.dy = dy;
+    if (db) {   // (the kernels load four columns at a time)
+        a.dy = (float *)(p + 2 * fb + eb + pb);
+        hipLaunchKernelGGL(coli_t_pad, dim3((4 * S + 255) / 256), dim3(256), 0, ctx->stream, dy, (float *)a.dy, S, t->O);
+        if (!hip_check(hipGetLastError(), "gradient rows padding")) return 0;
+    }
     a.hi = (_Float16 *)p;
     a.lo = (_Float16 *)(p + fb);
     a.exps = (int *)(p + 2 * fb);
     a.Sp = Sp;
     a.S = S;
-    a.K = t->O;
+    a.K = std::max(4, t->O);
     a.noct = noct;
     a.int4 = t->kind != COLI_KIND_FP4;
     a.nblocks = few ? 0 : (S + 3) / 4;
@@ -509,8 +636,8 @@ int gemm_t_run(DevCtx *ctx, ColiCudaTensor *t, float *dx, const float *dy, int S
     a.lo = g.prep.lo;
     a.exps = g.prep.exps;
     a.Sp = g.prep.Sp;
-    a.dy = dy;
-    a.O = t->O;
+    a.dy = g.prep.dy;
+    a.O = g.prep.K;
     a.nrt = t->nrt;
     a.nq = t->nq;
     a.noct = g.prep.noct;
@@ -519,9 +646,9 @@ int gemm_t_run(DevCtx *ctx, ColiCudaTensor *t, float *dx, const float *dy, int S
     a.splits = g.splits;
     a.per = g.per;
     a.out = g.parts ? g.part : dx;
-    if (t->kind == COLI_KIND_I4_H) launch_gemm_t<COLI_KIND_I4_H>(a, g.mt, st);
-    else if (t->kind == COLI_KIND_I4_F) launch_gemm_t<COLI_KIND_I4_F>(a, g.mt, st);
-    else launch_gemm_t<COLI_KIND_FP4>(a, g.mt, st);
+    if (t->kind == COLI_KIND_I4_H) launch_gemm_t<COLI_KIND_I4_H>(a, S <= COLI_T_FEW, st);
+    else if (t->kind == COLI_KIND_I4_F) launch_gemm_t<COLI_KIND_I4_F>(a, S <= COLI_T_FEW, st);
+    else launch_gemm_t<COLI_KIND_FP4>(a, S <= COLI_T_FEW, st);
     if (!hip_check(hipGetLastError(), "input gradient")) return 0;
     if (!with_join || !g.parts) return 1;
     const size_t n = (size_t)S * t->I;

@@ -387,12 +387,15 @@ __global__ __launch_bounds__(64 * W) void coli_lora_shrink(LoraRows w, LoraSide<
     // columns past the last whole step: the last split, 32 a wave (the factors'
     // padding is zero, the row is read as zero past N)
     if (sp == s.splits - 1) {
-        const float *xr = s.x + (size_t)rows[min(m, n - 1)] * s.N + 8 * kq;
+        const float *xr = s.x + (size_t)rows[min(m, n - 1)] * s.N;
         const T *vr = vs + (size_t)m * s.Np + 8 * kq;
         for (int c = STEP * full + 32 * wave; c < s.N; c += 32 * W) {
             float xv[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) xv[j] = c + 8 * kq + j < s.N ? xr[c + j] : 0.0f;
+            for (int j = 0; j < 8; j++) {
+                const float t = xr[min(c + 8 * kq + j, s.N - 1)];
+                xv[j] = c + 8 * kq + j < s.N ? t : 0.0f;
+            }
             Raw8<T> v[NR];
 #pragma unroll
             for (int r = 0; r < NR; r++) v[r].load(vr + (size_t)16 * r * s.Np + c);
@@ -471,16 +474,16 @@ __device__ __forceinline__ float lora_h(const float *h, int splits, size_t pitch
 // rows, added to y (JOIN: to the sum of y's partial sums, also in rows without
 // an adapter). Factors and y are requested before h is joined.
 template <typename T, bool JOIN>
-__global__ __launch_bounds__(256) void coli_lora_expand(LoraRows w, LoraSide<T> s, int Rp) {
-    extern __shared__ float hs[];   // [16][Rp + 1]
+__device__ __forceinline__ void lora_expand_block(const LoraRows &w, const LoraSide<T> &s, int Rp, int tile, int cb, float *hs) {
+    // hs: [16][Rp + 1]
     __shared__ int rows[COLI_LORA_TILE];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, kq = lane >> 4;
     int slot = 0;
-    const int n = lora_tile<JOIN>(w, blockIdx.x, rows, slot);
+    const int n = lora_tile<JOIN>(w, tile, rows, slot);
     if (n == 0) return;   // (uniform over the workgroup)
     const bool none = slot < 0;
     if (none) slot = 0;
-    const int c0 = blockIdx.y * 512 + wave * 128, c = c0 + 8 * m;
+    const int c0 = cb * 512 + wave * 128, c = c0 + 8 * m;
     const T *vr = s.v + (size_t)slot * Rp * s.Np + (size_t)kq * s.Np + min(c, s.Np - 8);
     Raw8<T> v[4];
 #pragma unroll
@@ -494,27 +497,21 @@ __global__ __launch_bounds__(256) void coli_lora_expand(LoraRows w, LoraSide<T> 
 #pragma unroll
     for (int i = 0; i < 4; i++) yr[i] = (JOIN ? s.part : s.out) + (size_t)rows[min(4 * kq + i, n - 1)] * s.N + c;
     f4u y[4][2];
-    auto load_y = [&](f4u (&v)[4][2]) {
-        if (whole) {
+    // (a lane whose eight columns pass N loads h instead, which has as many, and
+    // adds its columns one by one at the end: see row4 for why not here)
+    auto load_y = [&](int p, f4u (&v)[4][2]) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                v[i][0] = *GPTR(f4u, yr[i]);
-                v[i][1] = *GPTR(f4u, yr[i] + 4);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < 8; j++) v[i][j >> 2][j & 3] = c + j < s.N ? yr[i][j] : 0.0f;
+        for (int i = 0; i < 4; i++) {
+            const float *q = whole ? yr[i] + (size_t)p * w.S * s.N : s.h;
+            v[i][0] = *GPTR(f4u, q);
+            v[i][1] = *GPTR(f4u, q + 4);
         }
     };
-    load_y(y);
+    load_y(0, y);
     if constexpr (JOIN) {
         for (int p = 1; p < s.parts; p++) {
             f4u z[4][2];
-#pragma unroll
-            for (int i = 0; i < 4; i++) yr[i] += (size_t)w.S * s.N;
-            load_y(z);
+            load_y(p, z);
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -524,7 +521,7 @@ __global__ __launch_bounds__(256) void coli_lora_expand(LoraRows w, LoraSide<T> 
     for (int e = threadIdx.x; e < 16 * r16; e += 256) {
         const int row = e / r16, r = e - row * r16;
         // (past the rank: zeros, also where a row of infinities shrank to NaN)
-        const int hr = s.sorted ? w.tile[blockIdx.x].y + min(row, n - 1) : rows[min(row, n - 1)];
+        const int hr = s.sorted ? w.tile[tile].y + min(row, n - 1) : rows[min(row, n - 1)];
         const float hv = lora_h(s.h + (size_t)hr * Rp + min(r, rank - 1), s.splits, (size_t)w.S * Rp);
         hs[row * (Rp + 1) + r] = row < n && r < rank ? meta.scale * hv : 0.0f;
     }
@@ -552,21 +549,25 @@ __global__ __launch_bounds__(256) void coli_lora_expand(LoraRows w, LoraSide<T> 
         const int row = 4 * kq + i;
         if (row >= n || c >= s.N) continue;
         float *to = s.out + (size_t)rows[row] * s.N + c;
-        f4u y0 = y[i][0], y1 = y[i][1];
-        if (rank) {
+        if (whole) {
+            f4u y0 = y[i][0], y1 = y[i][1];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                y0[j] += acc[j][i];
+                y0[j] += acc[j][i];   // (rank 0: the sums of no products, 0)
                 y1[j] += acc[4 + j][i];
             }
-        }
-        if (whole) {
             *(f4u *)to = y0;
             *(f4u *)(to + 4) = y1;
         } else {
+            float t[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) t[j] = yr[i][min(j, s.N - 1 - c)];
+            for (int p = 1; JOIN && p < s.parts; p++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) t[j] += yr[i][(size_t)p * w.S * s.N + min(j, s.N - 1 - c)];
 #pragma unroll
             for (int j = 0; j < 8; j++)
-                if (c + j < s.N) to[j] = j < 4 ? y0[j & 3] : y1[j & 3];
+                if (c + j < s.N) to[j] = t[j] + acc[j][i];
         }
     }
 }
@@ -580,22 +581,22 @@ __global__ __launch_bounds__(256) void coli_lora_expand(LoraRows w, LoraSide<T> 
 // stored transposed, [slots][N][max_rank]. Every element is written, zeros
 // where a slot has no rows or rank.
 template <typename T, int NR, int W>
-__global__ __launch_bounds__(64 * W) void coli_lora_outer(LoraRows w, LoraSide<T> s0, LoraSide<T> s1, int Rp, int max_rank) {
+__device__ __forceinline__ void lora_outer_block(const LoraRows &w, const LoraSide<T> &s0, const LoraSide<T> &s1, int Rp,
+                                                 int max_rank, int cb, int sr, bool side1) {
     constexpr int RW = W > 8 ? 8 : W;   // waves of the LDS join
     constexpr bool LIST = W > 4;        // beyond COLI_LORA_BALLOT rows
     __shared__ int rows[COLI_LORA_BALLOT];
     __shared__ float hl[LIST ? 1 : COLI_LORA_BALLOT][LIST ? 1 : 16 * NR + 1];
     __shared__ float red[RW][64][17];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, kq = lane >> 4;
-    const int nrp = (Rp / 16 + NR - 1) / NR, slot = blockIdx.y / nrp, rt0 = (blockIdx.y - slot * nrp) * NR;
-    const bool side1 = blockIdx.z != 0;
+    const int nrp = (Rp / 16 + NR - 1) / NR, slot = sr / nrp, rt0 = (sr - slot * nrp) * NR;
     // (h of one side meets the rows of the other)
     const float *x = side1 ? s1.x : s0.x;
     const int N = side1 ? s1.N : s0.N;
     const float *h = (side1 ? s0.h : s1.h) + 16 * rt0;
     const int splits = side1 ? s0.splits : s1.splits;
     float *out = side1 ? s1.out : s0.out;
-    const int c0 = blockIdx.x * 64, c = c0 + 4 * m;
+    const int c0 = cb * 64, c = c0 + 4 * m;
     if (c0 >= N) return;
     const LoraMeta meta = w.meta[slot];
     const int rank = min(meta.rank, Rp);
@@ -626,9 +627,8 @@ __global__ __launch_bounds__(64 * W) void coli_lora_outer(LoraRows w, LoraSide<T
     for (int r = 0; r < NR; r++)
 #pragma unroll
         for (int j = 0; j < 4; j++) acc[r][j] = (floatx4){0.f, 0.f, 0.f, 0.f};
-    const bool whole = c + 4 <= N;
     struct Step {
-        f4u x[4];
+        floatx4 x[4];
         float h[4][NR];
     };
     auto numbers = [&](int p0, int (&rw)[4]) {
@@ -638,24 +638,19 @@ __global__ __launch_bounds__(64 * W) void coli_lora_outer(LoraRows w, LoraSide<T
     auto load = [&](int p0, const int (&rw)[4], Step &st) {
 #pragma unroll
         for (int u = 0; u < 4; u++) {
-            const float *xr = x + (size_t)rw[u] * N + c;
-            if (whole) {
-                st.x[u] = *GPTR(f4u, xr);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; j++) st.x[u][j] = c + j < N ? xr[j] : 0.0f;
-            }
+            st.x[u] = row4<true>(x + (size_t)rw[u] * N, c, N);   // (columns past N: not kept)
 #pragma unroll
             for (int r = 0; r < NR; r++) {
                 const int p = min(p0 + 4 * u + kq, cnt - 1);
                 if constexpr (LIST) st.h[u][r] = h[(size_t)(first + p) * Rp + 16 * r + m];
                 else st.h[u][r] = hl[p][16 * r + m];
             }
-            if (p0 + 4 * u + kq >= cnt) {
-                st.x[u] = (f4u){0.f, 0.f, 0.f, 0.f};
+            // (rows past the slot's: zeros on both sides, whatever the clamped row holds)
+            const bool live = p0 + 4 * u + kq < cnt;
 #pragma unroll
-                for (int r = 0; r < NR; r++) st.h[u][r] = 0.0f;
-            }
+            for (int j = 0; j < 4; j++) st.x[u][j] = live ? st.x[u][j] : 0.0f;
+#pragma unroll
+            for (int r = 0; r < NR; r++) st.h[u][r] = live ? st.h[u][r] : 0.0f;
         }
     };
     int p0 = 16 * wave;
@@ -720,6 +715,30 @@ __global__ __launch_bounds__(64 * W) void coli_lora_outer(LoraRows w, LoraSide<T
             if (k < max_rank && c0 + col < N)
                 out[side1 ? ((size_t)slot * N + c0 + col) * max_rank + k : ((size_t)slot * max_rank + k) * N + c0 + col] = v;
         }
+    }
+}
+
+template <typename T, bool JOIN>
+__global__ __launch_bounds__(256) void coli_lora_expand(LoraRows w, LoraSide<T> s, int Rp) {
+    extern __shared__ float hs[];
+    lora_expand_block<T, JOIN>(w, s, Rp, blockIdx.x, blockIdx.y, hs);
+}
+template <typename T, int NR>
+__global__ __launch_bounds__(1024) void coli_lora_outer(LoraRows w, LoraSide<T> s0, LoraSide<T> s1, int Rp, int max_rank) {
+    lora_outer_block<T, NR, 16>(w, s0, s1, Rp, max_rank, blockIdx.x, blockIdx.y, blockIdx.z != 0);
+}
+// Up to COLI_LORA_BALLOT rows both run in one launch, the expand's workgroups
+// (ne; none without dx) first.
+template <typename T, int NR, bool JOIN>
+__global__ __launch_bounds__(256) void coli_lora_finish(LoraRows w, LoraSide<T> s0, LoraSide<T> s1, LoraSide<T> e, int Rp,
+                                                        int max_rank, int ne, int tiles, int cols) {
+    extern __shared__ float hs[];
+    const int b = blockIdx.x;
+    if (b < ne) {
+        lora_expand_block<T, JOIN>(w, e, Rp, b % tiles, b / tiles, hs);
+    } else {
+        const int o = b - ne, half = (int)(gridDim.x - ne) / 2, r = o % half;
+        lora_outer_block<T, NR, 4>(w, s0, s1, Rp, max_rank, r % cols, r / cols, o >= half);
     }
 }
 
@@ -810,21 +829,37 @@ static int launch_expand(DevCtx *ctx, const ColiHipLora *l, const LoraRows &w, c
     return hip_check(hipGetLastError(), "adapter expand");
 }
 
+// Adapter gradients and, with e, the expand: one launch up to COLI_LORA_BALLOT rows.
 template <typename T>
-static int launch_outer(DevCtx *ctx, const ColiHipLora *l, const LoraRows &w, const LoraSide<T> &s0, const LoraSide<T> &s1) {
-    const int nrt = l->Rp / 16, cols = (std::max(l->I, l->O) + 63) / 64, nr = nrt >= 4 ? 4 : nrt;
-#define COLI_OUTER(NR, W)                                                                                           hipLaunchKernelGGL((coli_lora_outer<T, NR, W>), dim3(cols, l->slots *(nrt / nr), 2), dim3(64 * W), 0,                                ctx->stream, w, s0, s1, l->Rp, l->max_rank)
+static int launch_outer(DevCtx *ctx, const ColiHipLora *l, const LoraRows &w, const LoraSide<T> &s0, const LoraSide<T> &s1,
+                        const LoraSide<T> *e) {
+    const int nrt = l->Rp / 16, cols = (std::max(l->I, l->O) + 63) / 64, nr = nrt >= 4 ? 4 : nrt, ny = l->slots * (nrt / nr);
     if (w.S <= COLI_LORA_BALLOT) {
-        if (nr == 1) COLI_OUTER(1, 4);
-        else if (nr == 2) COLI_OUTER(2, 4);
-        else COLI_OUTER(4, 4);
-    } else {
-        if (nr == 1) COLI_OUTER(1, 16);
-        else if (nr == 2) COLI_OUTER(2, 16);
-        else COLI_OUTER(4, 16);
+        const int tiles = lora_tiles(w.S, l->slots), ne = e ? tiles * ((e->Np + 511) / 512) : 0;
+        const size_t shm = (size_t)16 * (l->Rp + 1) * sizeof(float);
+#define COLI_FINISH(NR, JOIN)                                                                                    \
+    hipLaunchKernelGGL((coli_lora_finish<T, NR, JOIN>), dim3(ne + 2 * cols * ny), dim3(256), shm, ctx->stream, w, s0, \
+                       s1, e ? *e : s0, l->Rp, l->max_rank, ne, tiles, cols)
+#define COLI_FINISH_NR(JOIN)            \
+    if (nr == 1) COLI_FINISH(1, JOIN);      \
+    else if (nr == 2) COLI_FINISH(2, JOIN); \
+    else COLI_FINISH(4, JOIN)
+        if (e && e->parts) {
+            COLI_FINISH_NR(true);
+        } else {
+            COLI_FINISH_NR(false);
+        }
+#undef COLI_FINISH_NR
+#undef COLI_FINISH
+        return hip_check(hipGetLastError(), "adapter gradients");
     }
+#define COLI_OUTER(NR) \
+    hipLaunchKernelGGL((coli_lora_outer<T, NR>), dim3(cols, ny, 2), dim3(1024), 0, ctx->stream, w, s0, s1, l->Rp, l->max_rank)
+    if (nr == 1) COLI_OUTER(1);
+    else if (nr == 2) COLI_OUTER(2);
+    else COLI_OUTER(4);
 #undef COLI_OUTER
-    return hip_check(hipGetLastError(), "adapter gradients");
+    return hip_check(hipGetLastError(), "adapter gradients") && (!e || launch_expand<T>(ctx, l, w, *e));
 }
 
 template <typename T>
@@ -867,15 +902,14 @@ static int lora_backward(DevCtx *ctx, ColiCudaTensor *t, const ColiHipLora *l, c
         sb.h = j.to[1];
         sa.splits = sb.splits = 1;
     }
-    if (!launch_outer<T>(ctx, l, w, sa, sb)) return 0;
-    if (!dx) return 1;
+    if (!dx) return launch_outer<T>(ctx, l, w, sa, sb, nullptr);
     LoraSide<T> e = lora_side<T>(l, false, nullptr, sb.h, dx, sb.splits);
     e.sorted = !few;
     if (plan.parts) {   // the expand joins the K splits
         e.part = plan.part;
         e.parts = plan.parts;
     }
-    return gemm_t_run(ctx, t, dx, dy, S, plan, few, !e.parts) && launch_expand<T>(ctx, l, w, e);
+    return gemm_t_run(ctx, t, dx, dy, S, plan, few, !e.parts) && launch_outer<T>(ctx, l, w, sa, sb, &e);
 }
 
 // ---------------------------------------------------------------------------
@@ -895,7 +929,7 @@ extern "C" void coli_hip_lora_free(ColiHipLora *l) {
 }
 
 extern "C" int coli_hip_lora_create(ColiHipLora **out, int device, int I, int O, int slots, int max_rank, int dtype) {
-    if (!out || I < 1 || O < 1 || I > (1 << 20) || O > (1 << 20) || slots < 1 || slots > COLI_LORA_MAX_SLOTS ||
+    if (!out || I < 4 || O < 4 || I > (1 << 20) || O > (1 << 20) || slots < 1 || slots > COLI_LORA_MAX_SLOTS ||
         max_rank < 1 || max_rank > COLI_LORA_MAX_RANK || dtype < 0 || dtype > 2)
         return 0;
     DevCtx *ctx = ctx_of(device);

@@ -136,7 +136,8 @@ int coli_hip_pipe_gemm_noalloc(ColiCudaTensor *tensor, float *y_dev, const float
 
 /* A bank of low-rank adapters for one projection of width I -> O: slot a holds
  * A [rank, I], B [O, rank] and a scale. dtype of the factors: 0 f32, 1 fp16,
- * 2 bf16. slots <= 1024, max_rank <= 256. Slots start empty. */
+ * 2 bf16. I and O at least 4 (and at most 2^20), slots <= 1024, max_rank <= 256.
+ * Slots start empty. */
 typedef struct ColiHipLora ColiHipLora;
 int coli_hip_lora_create(ColiHipLora **lora, int device, int I, int O, int slots, int max_rank, int dtype);
 void coli_hip_lora_free(ColiHipLora *lora);

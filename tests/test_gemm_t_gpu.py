@@ -24,7 +24,7 @@ def tol(kind, O):
 # O and I around the tiles (16 rows, 128 columns) and the K steps (32 rows),
 # rows around the tile heights 32 / 64 / 128 and the K splits
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("O,I,S", [(1, 1, 1), (16, 128, 1), (17, 33, 2), (33, 129, 5), (100, 200, 16), (31, 64, 31),
+@pytest.mark.parametrize("O,I,S", [(1, 1, 1), (2, 40, 70), (3, 200, 9), (5, 128, 64), (16, 128, 1), (17, 33, 2), (33, 129, 5), (100, 200, 16), (31, 64, 31),
                                    (96, 256, 32), (48, 130, 33), (640, 384, 64), (200, 515, 65), (1040, 260, 128),
                                    (64, 128, 129), (2049, 131, 20), (300, 1000, 300)])
 def test_matches_dense(session, kind, O, I, S):

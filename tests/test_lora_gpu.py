@@ -98,7 +98,8 @@ class Case:
 
 
 SHAPES = [  # kind, O, I, S, slots, rank, dtype, pattern
-    ("i4h", 1, 1, 1, 1, 1, 0, "0"),
+    ("i4h", 4, 5, 1, 1, 1, 0, "0"),
+    ("i4f", 7, 6, 70, 2, 3, 1, "mixed"),
     ("i4h", 64, 96, 1, 1, 8, 1, "0"),
     ("fp4", 200, 130, 1, 3, 16, 2, "1"),
     ("i4f", 33, 65, 5, 4, 5, 0, "mixed"),
@@ -319,7 +320,7 @@ def test_two_projections_in_sequence(session):
 def test_refusals(session):
     b = session.b
     bank = C.c_void_p()
-    for args in ((0, 0, 8, 1, 1, 0), (0, 8, 0, 1, 1, 0), (0, 8, 8, 0, 1, 0), (0, 8, 8, 1025, 1, 0), (0, 8, 8, 1, 0, 0),
+    for args in ((0, 3, 8, 1, 1, 0), (0, 8, 3, 1, 1, 0), (0, (1 << 20) + 1, 8, 1, 1, 0), (0, 8, (1 << 20) + 1, 1, 1, 0), (0, 8, 8, 0, 1, 0), (0, 8, 8, 1025, 1, 0), (0, 8, 8, 1, 0, 0),
                  (0, 8, 8, 1, 257, 0), (0, 8, 8, 1, 1, 3), (0, 8, 8, 1, 1, -1), (9, 8, 8, 1, 1, 0)):
         assert not b.hip_lora_create(C.byref(bank), *args) and not bank
     with Case(session, 50, "i4h", 32, 64, 4, 2, 4, 0, "0") as c, Case(session, 51, "i4h", 64, 32, 4, 2, 4, 0, "0") as o:
