@@ -745,18 +745,45 @@ __global__ __launch_bounds__(256) void coli_lora_finish(LoraRows w, LoraSide<T> 
 // ---------------------------------------------------------------------------
 // launches
 // ---------------------------------------------------------------------------
-// Column splits of one side's shrink: workgroups of `cols` columns such that
-// all of them are about two a CU (four waves each up to COLI_LORA_BALLOT rows:
-// at least a step a wave; eight waves beyond, at most `most` splits).
-static int shrink_splits(const DevCtx *ctx, int S, long columns, int N, long most) {
-    const int cus = ctx->cu_count ? ctx->cu_count : 256;
-    const bool few = S <= COLI_LORA_BALLOT;
-    const long cols = std::max(few ? 256L : 512L, columns / (2 * cus));
-    return (int)std::max(1L, std::min((N + cols / 2) / cols, few ? 16L : most));
+// Column splits of one side's shrink; `groups` workgroups without splits, over
+// both sides if there are two, `columns` the columns that they take together.
+// Up to COLI_LORA_BALLOT rows (four waves) workgroups of at least a step a wave,
+// about two a CU. Beyond (eight waves, whose LDS mostly leaves a CU room for
+// one): one side by the rounds of workgroups, each with a fixed part of about
+// 2900 columns' time (1024 x 14336, rank 64, 69 tiles, the whole call: 1, 2, 3,
+// 4, 6, 8 splits 352, 316, 306, 325, 314, 322 us); two sides, whose splits
+// differ, as many as fit into one round if that leaves each side some (the
+// adapter gradients of 512 x 4096 x 4096, rank 64: 43 us against 49 for two
+// rounds' worth), else two rounds' worth (2048 x 4096 x 14336, rank 32: 106
+// against 117).
+static int shrink_splits(const DevCtx *ctx, int S, long groups, long columns, int N, bool two) {
+    const long cus = ctx->cu_count ? ctx->cu_count : 256;
+    if (S <= COLI_LORA_BALLOT) {
+        const long cols = std::max(256L, columns / (2 * cus));
+        return (int)std::max(1L, std::min((N + cols / 2) / cols, two ? 4L : 16L));
+    }
+    if (two) {
+        const long cols = std::max(512L, columns / (2 * groups <= cus ? cus : 2 * cus));
+        return (int)std::max(1L, std::min((2 * groups <= cus ? N : N + cols / 2) / cols, 4L));
+    }
+    long best = 1, least = 0;
+    for (long s = 1; s <= 8 && s * 512 <= std::max(512, N); s++) {
+        const long t = (groups * s + cus - 1) / cus * (N / s + 2900);
+        if (s == 1 || t < least) {
+            least = t;
+            best = s;
+        }
+    }
+    return (int)best;
 }
 
 static int lora_tiles(int S, int slots) {
     return S <= COLI_LORA_BALLOT ? S : S / COLI_LORA_TILE + std::min(S, slots + 1);
+}
+
+// Shrink workgroups of one side without splits.
+static long lora_groups(int S, const ColiHipLora *l) {
+    return (long)lora_tiles(S, l->slots) * (l->Rp >= 64 ? l->Rp / 64 : 1);
 }
 
 // The rows' grouping, and (beyond COLI_LORA_BALLOT rows) the launch that makes it.
@@ -866,7 +893,8 @@ template <typename T>
 static int lora_forward(DevCtx *ctx, ColiCudaTensor *t, const ColiHipLora *l, float *y, const float *x, int S,
                         const int *slot_dev) {
     LoraRows w;
-    const int splits = shrink_splits(ctx, S, (long)lora_tiles(S, l->slots) * l->I, l->I, 8);
+    const long groups = lora_groups(S, l);
+    const int splits = shrink_splits(ctx, S, groups, groups * l->I, l->I, false);
     if (!reserve_kept(ctx, &ctx->lora_h, (size_t)splits * S * l->Rp * sizeof(float), 0) ||
         !lora_rows(ctx, l, slot_dev, S, &w))
         return 0;
@@ -882,8 +910,9 @@ template <typename T>
 static int lora_backward(DevCtx *ctx, ColiCudaTensor *t, const ColiHipLora *l, const float *x, const float *dy, int S,
                          const int *slot_dev, float *dx, float *da, float *db) {
     LoraRows w;
-    const long columns = (long)lora_tiles(S, l->slots) * (l->I + l->O);
-    const int spa = shrink_splits(ctx, S, columns, l->I, 4), spb = shrink_splits(ctx, S, columns, l->O, 4);
+    const long groups = lora_groups(S, l), columns = groups * (l->I + l->O);
+    const int spa = shrink_splits(ctx, S, 2 * groups, columns, l->I, true);
+    const int spb = shrink_splits(ctx, S, 2 * groups, columns, l->O, true);
     const bool few = S <= COLI_LORA_BALLOT;
     const size_t hn = (size_t)S * l->Rp;
     if (!reserve_kept(ctx, &ctx->lora_h, (spa + spb + (few ? 0 : 2)) * hn * sizeof(float), 0) ||
