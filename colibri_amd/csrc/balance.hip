@@ -590,7 +590,8 @@ extern "C" int coli_hip_balance_grad_dev(int device, const float *logits, const 
                                          const int *counts, const int *rows, float *dlogits) {
     if (fault_injected()) return 0;
     if (!logits || !dloss || !counts || !rows || !dlogits || (!offsets && n != 1) ||
-        !balance_shape_ok(n, T, E, route_mode))
+        !balance_shape_ok(n, T, E, route_mode) ||
+        (dlogits != logits && ranges_overlap(dlogits, (size_t)T * E * 4, logits, (size_t)T * E * 4)))
         return 0;
     DevCtx *ctx = ctx_of(device);
     if (!bind_ctx(ctx)) return 0;

@@ -326,23 +326,23 @@ __device__ __forceinline__ int t_exponent(float m) {
 }
 
 // [octet of K][row][8]: a step's operand is contiguous over the rows. Only for
-// more than 64 rows: fewer are converted by the product itself.
+// coli_gemm_t: coli_gemm_t_few converts the rows itself.
 //
 // Four rows a workgroup, thread (row = t % 4, octet t / 4 of each 256), so
 // that loads read 512 and stores write 64 contiguous bytes; a row of up to
 // 16384 columns is read once.
 #define COLI_T_SLOTS 8   // octets a thread holds
-template <bool ODD> __device__ __forceinline__ void t_prep_block(const ColiTPrepArgs &a, int blk, float (*wmax)[4]) {
+template <bool ODD, int NS> __device__ __forceinline__ void t_prep_block(const ColiTPrepArgs &a, int blk, float (*wmax)[4]) {
     const int tid = threadIdx.x, lane = tid & 63, r = tid & 3, o0 = tid >> 2, row = blk * 4 + r;
     const float *xr = a.dy + (size_t)min(row, a.S - 1) * a.K;
-    float v[COLI_T_SLOTS][8], m = 0.0f;
+    float v[NS][8], m = 0.0f;
 #pragma unroll
-    for (int s = 0; s < COLI_T_SLOTS; s++) t_load8<ODD>(xr, o0 + 256 * s, a.K, v[s]);
+    for (int s = 0; s < NS; s++) t_load8<ODD>(xr, o0 + 256 * s, a.K, v[s]);
 #pragma unroll
-    for (int s = 0; s < COLI_T_SLOTS; s++)
+    for (int s = 0; s < NS; s++)
 #pragma unroll
         for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(v[s][i]));
-    for (int o = o0 + 256 * COLI_T_SLOTS; o < a.noct; o += 256) {
+    for (int o = o0 + 256 * NS; o < a.noct; o += 256) {
         float u[8];
         t_load8<ODD>(xr, o, a.K, u);
 #pragma unroll
@@ -364,18 +364,24 @@ template <bool ODD> __device__ __forceinline__ void t_prep_block(const ColiTPrep
         *(half8v *)(a.lo + ((size_t)o * a.Sp + row) * 8) = l;
     };
 #pragma unroll
-    for (int s = 0; s < COLI_T_SLOTS; s++)
+    for (int s = 0; s < NS; s++)
         if (o0 + 256 * s < a.noct) put(o0 + 256 * s, v[s]);
-    for (int o = o0 + 256 * COLI_T_SLOTS; o < a.noct; o += 256) {
+    for (int o = o0 + 256 * NS; o < a.noct; o += 256) {
         float u[8];
         t_load8<ODD>(xr, o, a.K, u);
         put(o, u);
     }
 }
+template <bool ODD> __device__ __forceinline__ void t_prep_slots(const ColiTPrepArgs &a, int blk, float (*wmax)[4]) {
+    if (a.noct <= 256) t_prep_block<ODD, 1>(a, blk, wmax);
+    else if (a.noct <= 512) t_prep_block<ODD, 2>(a, blk, wmax);
+    else if (a.noct <= 1024) t_prep_block<ODD, 4>(a, blk, wmax);
+    else t_prep_block<ODD, COLI_T_SLOTS>(a, blk, wmax);
+}
 __device__ __forceinline__ void coli_t_prep_block(const ColiTPrepArgs &a, int blk) {
     __shared__ float wmax[16][4];
-    if (a.K % 4 == 0) t_prep_block<false>(a, blk, wmax);
-    else t_prep_block<true>(a, blk, wmax);
+    if (a.K % 4 == 0) t_prep_slots<false>(a, blk, wmax);
+    else t_prep_slots<true>(a, blk, wmax);
 }
 
 // ---------------------------------------------------------------------------

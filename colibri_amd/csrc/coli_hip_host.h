@@ -187,6 +187,7 @@ int gemm_prepared(DevCtx *ctx, ColiCudaTensor *t, float *y_dev, const float *x_d
 // dx, else left in part [parts][S][I] where parts is not 0).
 struct GemmTPlan {
     ColiTPrepArgs prep;
+    bool few;
     int splits, per;
     float *part;
     int parts;
@@ -194,6 +195,10 @@ struct GemmTPlan {
 int gemm_t_plan(DevCtx *ctx, ColiCudaTensor *t, const float *dy, int S, GemmTPlan *plan);
 int gemm_t_run(DevCtx *ctx, ColiCudaTensor *t, float *dx, const float *dy, int S, const GemmTPlan &plan, bool with_prep,
                bool with_join);
+// Do the ranges share a byte (outputs that would overwrite a call's inputs)?
+inline bool ranges_overlap(const void *a, size_t na, const void *b, size_t nb) {
+    return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
+}
 int build_t_scales(DevCtx *ctx, ColiCudaTensor *t, bool update_only);
 // Counts and balance loss over router logits given as nch column-chunk
 // partials, chstride floats apart (balance.hip).

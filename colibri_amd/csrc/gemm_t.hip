@@ -27,6 +27,8 @@
 #include "coli_hip_ext.h"
 
 #include <algorithm>
+#include <cstdlib>
+#include <cstring>
 
 // ---------------------------------------------------------------------------
 // scales by column group
@@ -87,18 +89,14 @@ __global__ __launch_bounds__(1024) void coli_t_prep_rows(ColiTPrepArgs a) { coli
 // ---------------------------------------------------------------------------
 // the product
 // ---------------------------------------------------------------------------
-// Rows that convert dy inside the product (measured, product and build: 64 rows
-// of 4096 x 14336 int4 45 us, on the many-row kernel 52).
-#define COLI_T_FEW 64
-
 struct GemmTArgs {
     const uint8_t *w;            // tiles [nrt][nq]
     const _Float16 *sct;
     const int *ge;               // [4 nq]
-    const _Float16 *hi, *lo;     // [noct][Sp][8] (many rows)
+    const _Float16 *hi, *lo;     // [noct][Sp][8] (coli_gemm_t)
     const int *exps;             // [S]
     size_t Sp;
-    const float *dy;             // [S][O] (few rows)
+    const float *dy;             // [S][O] (coli_gemm_t_few)
     int O;                       // its columns, at least 4
     int nrt, nq, noct, I, S;
     int splits, per;             // K split: steps of 32 rows of W each
@@ -322,14 +320,14 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void coli_gemm_t(GemmTArgs a) {
     }
 }
 
-// Up to 64 rows: workgroup (tile quad, 32 rows, K split), eight waves that take
-// its K steps in turn, each with all 128 columns and its own copy of the step's
+// Few rows or a small W (t_plan): workgroup (tile quad, 32 rows, K split), eight
+// waves that take its K steps in turn, each with all 128 columns and its own copy of the step's
 // dy: read as f32 and converted on its way into the wave's LDS, under the
 // exponent of the row's part in this split (the splits' sums are f32 already).
 // No launch builds operands, and no barrier holds the waves together before
 // their sums are joined. Bound by the VALU (transpose, unpack and conversion,
 // about 450 instructions a step of 4096 weights); a 64-row form spilled its
-// accumulators, so 33 to 64 rows read and unpack the weights twice.
+// accumulators, so every 32 rows read and unpack the weights again.
 template <int KIND, bool ODD>
 __global__ __launch_bounds__(512, 2) void coli_gemm_t_few(GemmTArgs a) {
     constexpr int BM = 32, W = 8, CPT = 4 * BM / 64, STAGE = 8 * BM * 16, PD = 2;
@@ -553,22 +551,44 @@ static void launch_gemm_t(const GemmTArgs &a, bool few, hipStream_t st) {
         hipLaunchKernelGGL((coli_gemm_t<KIND, 4, 4, 2>), dim3((a.nq + 1) / 2, (a.S + 127) / 128, a.splits), dim3(512), 0, st, a);
 }
 
-// K splits of many rows: the modelled time, in steps of 32 rows of W. A
-// workgroup (eight waves of about 240 registers) has a CU to itself, so rounds
-// of workgroups, each about eight steps longer than its products; a split adds
-// its sums written and read again, and a launch to join them. A step takes 1.4
-// us with three products (int4), 0.9 with two (measured, all CUs busy: 2048 x
-// 4096 x 14336 and 512 x 7168 x 2048). Splits measured: 512 x 4096 x 14336 2 /
-// 4 / 8: 285 / 196 / 213 us; 512 x 7168 x 2048 MXFP4 1 / 2 / 3: 83 / 65 / 85.
-static int t_splits(const ColiCudaTensor *t, int S, int cus, long blocks, int steps) {
-    const double step = t->kind == COLI_KIND_FP4 ? 0.9 : 1.4, mb = (double)S * t->I * 4e-6;
-    int best = 1;
-    double least = 1e30;
+// Which kernel, and its K splits, by the modelled time in us. A workgroup of
+// either (eight waves of about 200 registers) has a CU to itself, so rounds of
+// workgroups; a split adds its sums written and read again, and a launch to
+// join them.
+//   coli_gemm_t: 128 rows and two quads a workgroup, a step of 32 rows of W 1.4
+//   us with three products (int4), 0.9 with two (all CUs busy: 2048 x 4096 x
+//   14336 and 512 x 7168 x 2048), about eight steps before the first; the dy
+//   operands' build 7 us and its bytes. Splits measured: 512 x 4096 x 14336 2 /
+//   4 / 8: 285 / 196 / 213 us; 512 x 7168 x 2048 MXFP4 1 / 2 / 3: 83 / 65 / 85.
+//   coli_gemm_t_few: eight steps, one a wave, 2.5 us (2.1 with two products),
+//   and 8 us. Up to 32 rows it is the faster one at every size; more, while its
+//   workgroups fit one round. Both measured, rows x I x O, few / many: int4 160
+//   x 6400 x 2176 28 / 42 us, 192 49 / 43; 64 x 14336 x 4096 48 / 67, 66 78 /
+//   62; 512 x 768 x 1920 18 / 36; MXFP4 128 x 7168 x 2048 21 / 34, 192 40 / 40;
+//   192 x 2048 x 7168 38 / 43, 320 61 / 52.
+struct TPlan {
+    bool few;
+    int splits;
+};
+static TPlan t_plan(const ColiCudaTensor *t, int S, int cus, int steps) {
+    const bool fp4 = t->kind == COLI_KIND_FP4;
+    const double mb = (double)S * t->I * 4e-6;
+    auto join = [&](int s) { return s > 1 ? (s + 1) * mb / 4 + 3 : 0.0; };
+    auto rounds = [&](long blocks) { return (double)((blocks + cus - 1) / cus); };
+    const long fb = (long)((S + 31) / 32) * t->nq, mbk = (long)((S + 127) / 128) * ((t->nq + 1) / 2);
+    // few: a workgroup a CU, a step for each of its waves at least
+    TPlan best = {true, (int)std::max(1L, std::min((long)cus / fb, (long)steps / 8))};
+    double least = 8 + (fp4 ? 2.1 : 2.5) * rounds(fb * best.splits) * ((steps + 8 * best.splits - 1) / (8 * best.splits)) + join(best.splits);
+    const double prep = 7 + (double)S * t->O * 8e-6 / 4;
+    int force = 0;   // COLI_HIP_GEMM_T=few|many pins the kernel (tuning and tests)
+    if (const char *e = std::getenv("COLI_HIP_GEMM_T")) force = std::strcmp(e, "few") == 0 ? 1 : (std::strcmp(e, "many") == 0 ? -1 : 0);
+    if (force > 0) return best;
+    if (force < 0) least = 1e30;
     for (int s = 1; s <= 32 && s * 8 <= std::max(8, steps); s++) {
-        const double us = step * (double)((blocks * s + cus - 1) / cus) * ((steps + s - 1) / s + 8) + (s > 1 ? (s + 1) * mb / 4 + 3 : 0);
+        const double us = prep + (fp4 ? 0.9 : 1.4) * rounds(mbk * s) * ((steps + s - 1) / s + 8) + join(s);
         if (us < least) {
             least = us;
-            best = s;
+            best = {false, s};
         }
     }
     return best;
@@ -579,12 +599,10 @@ int gemm_t_plan(DevCtx *ctx, ColiCudaTensor *t, const float *dy, int S, GemmTPla
     if (t->kind == COLI_KIND_GENERIC) return 1;
     if (!t->sct && !build_t_scales(ctx, t, false)) return 0;
     const int noct = t_octets(t), steps = noct / 4;
-    const bool few = S <= COLI_T_FEW;
+    const TPlan pl = t_plan(t, S, ctx->cu_count ? ctx->cu_count : 256, steps);
+    const bool few = pl.few;
     const size_t Sp = few ? 0 : ((size_t)S + 127) & ~(size_t)127, fb = (size_t)noct * Sp * 16;
-    const int cus = ctx->cu_count ? ctx->cu_count : 256;
-    const long blocks = few ? (long)((S + 31) / 32) * t->nq : (long)((S + 127) / 128) * ((t->nq + 1) / 2);
-    // few rows: a workgroup a CU, a step for each of its waves at least
-    int splits = few ? (int)std::max(1L, std::min((long)cus / blocks, (long)steps / 8)) : t_splits(t, S, cus, blocks, steps);
+    int splits = pl.splits;
     const int per = (steps + splits - 1) / splits;
     splits = (steps + per - 1) / per;
     const size_t eb = (Sp * sizeof(int) + 255) & ~(size_t)255;
@@ -592,6 +610,7 @@ int gemm_t_plan(DevCtx *ctx, ColiCudaTensor *t, const float *dy, int S, GemmTPla
     const size_t db = t->O < 4 ? (size_t)S * 16 : 0;
     if (2 * fb + eb + pb + db && !reserve_kept(ctx, &ctx->gt, 2 * fb + eb + pb + db, 0)) return 0;
     uint8_t *p = (uint8_t *)ctx->gt.p;
+    g->few = few;
     g->splits = splits;
     g->per = per;
     g->part = (float *)(p + 2 * fb + eb);
@@ -646,9 +665,9 @@ int gemm_t_run(DevCtx *ctx, ColiCudaTensor *t, float *dx, const float *dy, int S
     a.splits = g.splits;
     a.per = g.per;
     a.out = g.parts ? g.part : dx;
-    if (t->kind == COLI_KIND_I4_H) launch_gemm_t<COLI_KIND_I4_H>(a, S <= COLI_T_FEW, st);
-    else if (t->kind == COLI_KIND_I4_F) launch_gemm_t<COLI_KIND_I4_F>(a, S <= COLI_T_FEW, st);
-    else launch_gemm_t<COLI_KIND_FP4>(a, S <= COLI_T_FEW, st);
+    if (t->kind == COLI_KIND_I4_H) launch_gemm_t<COLI_KIND_I4_H>(a, g.few, st);
+    else if (t->kind == COLI_KIND_I4_F) launch_gemm_t<COLI_KIND_I4_F>(a, g.few, st);
+    else launch_gemm_t<COLI_KIND_FP4>(a, g.few, st);
     if (!hip_check(hipGetLastError(), "input gradient")) return 0;
     if (!with_join || !g.parts) return 1;
     const size_t n = (size_t)S * t->I;
@@ -658,7 +677,9 @@ int gemm_t_run(DevCtx *ctx, ColiCudaTensor *t, float *dx, const float *dy, int S
 
 extern "C" int coli_hip_gemm_t_dev(ColiCudaTensor *t, float *dx_dev, const float *dy_dev, int S) {
     if (fault_injected()) return 0;
-    if (!tensor_computable(t) || !dx_dev || !dy_dev || S < 1 || S > COLI_GRAD_MAX_ROWS) return 0;
+    if (!tensor_computable(t) || !dx_dev || !dy_dev || S < 1 || S > COLI_GRAD_MAX_ROWS ||
+        ranges_overlap(dx_dev, (size_t)S * t->I * 4, dy_dev, (size_t)S * t->O * 4))
+        return 0;
     DevCtx *ctx = ctx_of(t->device);
     if (!bind_ctx(ctx)) return 0;
     GemmTPlan g;

@@ -86,6 +86,31 @@ def test_matches_definition(session, mode, shape):
     check(session, z, idx, keff, mask, off, mode, T)
 
 
+@pytest.mark.parametrize("T", [30, 300])
+@pytest.mark.parametrize("E", [1, 2, 3, 4, 5, 65, 127, 129, 257, 258, 385, 386, 513, 515, 769, 1023])
+def test_odd_numbers_of_experts(session, E, T):
+    """Widths at which the last columns are loaded moved back, one at a time, or not at all."""
+    rng = np.random.default_rng(E + T)
+    z, idx = routed(rng, T, E, min(E, 3))
+    check(session, z, idx, None, (rng.random(T) < 0.7).astype(np.uint8), np.array([1, T // 2, T - 1], np.int32), (0, 1, 3)[E % 3])
+
+
+@pytest.mark.parametrize("E", [48, 130])
+def test_gradient_in_place(session, E):
+    """dlogits may be the logits themselves; not a part of them moved by some elements."""
+    b = session.b
+    rng = np.random.default_rng(E)
+    T, off = 500, np.array([0, 7, 200, 490], np.int32)
+    z, idx = routed(rng, T, E, 4)
+    one = np.ones(3, np.float32)
+    loss, counts, rows, dz = run(session, z, idx, None, None, off, 1, one, z, 3)
+    with Bufs(b) as d:
+        pz, po, pd, pc, pr = d.up(z), d.up(off), d.up(one), d.up(counts), d.up(rows)
+        assert not b.hip_balance_grad_dev(0, pz, None, po, 3, T - 1, E, 1, pd, pc, pr, pz + 4 * E)
+        assert b.hip_balance_grad_dev(0, pz, None, po, 3, T, E, 1, pd, pc, pr, pz)
+        assert np.array_equal(d.down(pz, (T, E)).view(np.uint32), dz.view(np.uint32))
+
+
 @pytest.mark.parametrize("T", [40, 400])
 @pytest.mark.parametrize("mode", [0, 1, 3])
 def test_masked_places(session, mode, T):

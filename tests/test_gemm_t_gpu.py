@@ -37,6 +37,34 @@ def test_matches_dense(session, kind, O, I, S):
         session.free(h)
 
 
+@pytest.mark.parametrize("pin", ["few", "many"])
+@pytest.mark.parametrize("kind", ["i4h", "i4f", "fp4"])
+@pytest.mark.parametrize("O,I,S", [(1, 1, 1), (5, 131, 33), (200, 300, 64), (64, 512, 128), (700, 70, 129), (1030, 400, 260)])
+def test_both_kernels_at_any_size(session, monkeypatch, pin, kind, O, I, S):
+    """The kernel that converts its rows itself and the one that reads them built, pinned."""
+    monkeypatch.setenv("COLI_HIP_GEMM_T", pin)
+    test_matches_dense(session, kind, O, I, S)
+
+
+@pytest.mark.parametrize("S,pin", [(700, "few"), (4096, "many")])
+def test_rows_choose_the_kernel(session, S, pin):
+    """By the modelled times (2000 x 2044 on 256 CUs, us: 700 rows two rounds of
+    few, 8 + 2 x 8 x 2.5 = 48, five splits of the other 29 + 12 + 10 = 51; 4096
+    rows eight rounds, 168, against 99 + 23 = 122): bitwise the pinned kernel."""
+    rng = np.random.default_rng(29)
+    O, I = 2000, 2044
+    h, w = matrix(session, rng, "i4h", O, I)
+    try:
+        dy = rng.standard_normal((S, O)).astype(np.float32)
+        got = run(session, h, dy, I)
+        close(got, dy.astype(np.float64) @ w, np.abs(dy).astype(np.float64) @ np.abs(w), gemm_tol(O))
+        with pytest.MonkeyPatch.context() as m:
+            m.setenv("COLI_HIP_GEMM_T", pin)
+            assert np.array_equal(run(session, h, dy, I).view(np.uint32), got.view(np.uint32))
+    finally:
+        session.free(h)
+
+
 def test_one_hot_rows_read_the_matrix(session):
     """dy = e_o gives row o of W: every weight at its place, as exact as its
     fp16 hi + lo: 3 x 2^-22 of an f32 scale's weight (see gemm_tol), else exact
@@ -189,7 +217,11 @@ def test_refusals(session):
             assert not b.hip_gemm_t_dev(None, p, p, 1)
             assert not b.hip_gemm_t_dev(h, None, p, 1)
             assert not b.hip_gemm_t_dev(h, p, None, 1)
-            assert not b.hip_gemm_t_dev(h, p, p, 0)
-            assert not b.hip_gemm_t_dev(h, p, p, 65536)
+            q = d.up(np.zeros((2, 32), np.float32))
+            assert not b.hip_gemm_t_dev(h, p, q, 0)
+            assert not b.hip_gemm_t_dev(h, p, q, 65536)
+            for dx, dy in ((q, q), (q, q + 128), (q + 4, q)):   # dx over dy
+                assert not b.hip_gemm_t_dev(h, dx, dy, 2 if dx != dy else 1)
+            assert b.hip_gemm_t_dev(h, q, q + 128, 1)           # next to it
     finally:
         session.free(h)

@@ -112,6 +112,7 @@ SHAPES = [  # kind, O, I, S, slots, rank, dtype, pattern
     ("fp4", 130, 384, 257, 1, 256, 1, "0"),
     ("i4h", 128, 128, 1000, 600, 4, 2, "mixed"),   # more slots than the sort has threads
     ("i4h", 96, 2050, 130, 4, 128, 0, "-1"),       # no row has an adapter
+    ("gen", 70, 120, 90, 3, 12, 0, "mixed"),
 ]
 
 
@@ -127,6 +128,15 @@ def test_gradients(session, shape):
         c.check_grads(want_dx=SHAPES.index(shape) % 4 != 3)
 
 
+@pytest.mark.parametrize("pin", ["few", "many"])
+@pytest.mark.parametrize("shape", [("i4h", 200, 300, 40, 3, 16, 1, "mixed"), ("fp4", 515, 260, 150, 4, 24, 2, "runs"),
+                                   ("i4f", 300, 129, 300, 2, 70, 0, "mixed")], ids=lambda s: "-".join(map(str, s)))
+def test_gradients_with_either_product(session, monkeypatch, shape, pin):
+    monkeypatch.setenv("COLI_HIP_GEMM_T", pin)
+    with Case(session, 300 + shape[3], *shape) as c:
+        c.check_grads()
+
+
 def test_rows_without_an_adapter_keep_the_projection(session):
     """Slots outside the bank or empty: bitwise coli_cuda_pipe_gemm."""
     for S in (7, 90):
@@ -139,19 +149,16 @@ def test_rows_without_an_adapter_keep_the_projection(session):
             assert none.any() and np.array_equal(got[none].view(np.uint32), plain[none].view(np.uint32))
 
 
-def test_a_row_does_not_depend_on_its_batch(session):
-    """A request's delta is the same bits alone, in a batch and in a long list."""
+def test_forward_repeats_bitwise(session):
     with Case(session, 32, "fp4", 192, 320, 200, 3, 16, 2, "mixed") as c:
         d, S, O = c.d, c.S, c.O
         px, ps = d.up(c.x), d.up(c.slot)
-        py, p0 = d.up(np.zeros((S, O), np.float32)), d.up(np.zeros((S, O), np.float32))
+        py = d.up(np.zeros((S, O), np.float32))
         assert c.b.hip_lora_gemm_dev(c.h, c.bank, py, px, S, ps)
         whole = d.down(py, (S, O))
         again = d.up(np.zeros((S, O), np.float32))
         assert c.b.hip_lora_gemm_dev(c.h, c.bank, again, px, S, ps)
         assert np.array_equal(whole.view(np.uint32), d.down(again, (S, O)).view(np.uint32))
-        del p0
-
 
 def test_gradients_repeat_bitwise(session):
     with Case(session, 33, "i4h", 144, 272, 300, 3, 24, 1, "mixed") as c:
@@ -326,11 +333,16 @@ def test_refusals(session):
     with Case(session, 50, "i4h", 32, 64, 4, 2, 4, 0, "0") as c, Case(session, 51, "i4h", 64, 32, 4, 2, 4, 0, "0") as o:
         d = c.d
         px, py, ps = d.up(c.x), d.up(c.dy), d.up(c.slot)
-        pa, pb = d.up(np.zeros((2, 4, 64), np.float32)), d.up(np.zeros((2, 32, 4), np.float32))
+        pa, pb, pdx = (d.up(np.zeros(n, np.float32)) for n in ((2, 4, 64), (2, 32, 4), (4, 64)))
         ok = (c.h, c.bank, py, px, 4, ps)
+        assert not c.b.hip_lora_gemm_dev(c.h, c.bank, px + 4 * 63, px, 4, ps)
         for k, bad in ((0, None), (1, None), (2, None), (3, None), (4, 0), (4, 65536), (5, None), (1, o.bank)):
             assert not b.hip_lora_gemm_dev(*(ok[:k] + (bad,) + ok[k + 1:])), (k, bad)
-        ok = (c.h, c.bank, px, py, 4, ps, px, pa, pb)
+        ok = (c.h, c.bank, px, py, 4, ps, pdx, pa, pb)
+        assert c.b.hip_lora_grad_dev(*ok)
+        # a gradient over its inputs or over another one
+        for k, bad in ((6, px), (6, py), (7, px), (8, py), (6, pa), (8, pa + 16)):
+            assert not b.hip_lora_grad_dev(*(ok[:k] + (bad,) + ok[k + 1:])), (k, bad)
         for k, bad in ((0, None), (1, None), (2, None), (3, None), (4, 0), (5, None), (7, None), (8, None), (1, o.bank)):
             assert not b.hip_lora_grad_dev(*(ok[:k] + (bad,) + ok[k + 1:])), (k, bad)
         for slot, a, bb, r in ((-1, pa, pb, 1), (2, pa, pb, 1), (0, None, pb, 1), (0, pa, None, 1), (0, pa, pb, 5),
