@@ -390,8 +390,12 @@ __device__ __forceinline__ void coli_t_prep_block(const ColiTPrepArgs &a, int bl
 // the build beside other work.
 // ---------------------------------------------------------------------------
 #define COLI_PREP_SLOTS 8
-// Block `blk` of the build (every thread of a 256-thread block calls it).
-__device__ __forceinline__ void prep_frag_block(const ColiPrepArgs &a, int blk) {
+// Block `blk` of the build, by 256 threads; of a workgroup of TH, each 256 take a
+// block (every thread calls it, and all of them with a block that exists).
+template <int TH = 256> __device__ __forceinline__ void prep_frag_block(const ColiPrepArgs &a, int blk) {
+    const int tid = TH == 256 ? threadIdx.x : threadIdx.x & 255;
+    const int sub = TH == 256 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+    if constexpr (TH != 256) blk = __builtin_amdgcn_readfirstlane(blk);
     const float *__restrict__ x = a.x;
     const int *__restrict__ src_row = a.src_row, *__restrict__ nrows_dev = a.nrows_dev;
     _Float16 *__restrict__ hi = a.hi, *__restrict__ lo = a.lo;
@@ -420,12 +424,12 @@ __device__ __forceinline__ void prep_frag_block(const ColiPrepArgs &a, int blk) 
     float v[COLI_PREP_SLOTS][8];
     float m = 0.0f;
 #pragma unroll
-    for (int i = 0; i < COLI_PREP_SLOTS; i++) load_slot(threadIdx.x + 256 * i, v[i]);
+    for (int i = 0; i < COLI_PREP_SLOTS; i++) load_slot(tid + 256 * i, v[i]);
 #pragma unroll
     for (int i = 0; i < COLI_PREP_SLOTS; i++)
 #pragma unroll
         for (int t = 0; t < 8; t++) m = fmaxf(m, fabsf(v[i][t]));
-    for (int slot = threadIdx.x + 256 * COLI_PREP_SLOTS; slot < nslot; slot += 256) {
+    for (int slot = tid + 256 * COLI_PREP_SLOTS; slot < nslot; slot += 256) {
         float u[8];
         load_slot(slot, u);
 #pragma unroll
@@ -433,16 +437,16 @@ __device__ __forceinline__ void prep_frag_block(const ColiPrepArgs &a, int blk) 
     }
 #pragma unroll
     for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-    __shared__ float wmax[4];
+    __shared__ float wmax[TH / 64];
     if ((threadIdx.x & 63) == 0) wmax[threadIdx.x >> 6] = m;
     __syncthreads();
-    m = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
+    m = fmaxf(fmaxf(wmax[4 * sub], wmax[4 * sub + 1]), fmaxf(wmax[4 * sub + 2], wmax[4 * sub + 3]));
     int E = 0;
     if (m > 0.0f && isfinite(m)) {
         frexpf(m, &E);
         E -= 15;
     }
-    if (threadIdx.x == 0 && chunk == 0) exp2out[r] = E;
+    if (tid == 0 && chunk == 0) exp2out[r] = E;
     bool any = false;
     auto convert = [&](int slot, const float (&u)[8]) {
         if (slot >= nslot) return;
@@ -462,10 +466,10 @@ __device__ __forceinline__ void prep_frag_block(const ColiPrepArgs &a, int blk) 
     };
 #pragma unroll
     for (int i = 0; i < COLI_PREP_SLOTS; i++)
-        if (i % nchunk == chunk) convert(threadIdx.x + 256 * i, v[i]);
+        if (i % nchunk == chunk) convert(tid + 256 * i, v[i]);
     for (int i = COLI_PREP_SLOTS; 256 * i < nslot; i++) {
         if (i % nchunk != chunk) continue;
-        const int slot = threadIdx.x + 256 * i;
+        const int slot = tid + 256 * i;
         float u[8];
         load_slot(slot, u);
         convert(slot, u);

@@ -193,8 +193,7 @@ struct GemmTPlan {
     int parts;
 };
 int gemm_t_plan(DevCtx *ctx, ColiCudaTensor *t, const float *dy, int S, GemmTPlan *plan);
-int gemm_t_run(DevCtx *ctx, ColiCudaTensor *t, float *dx, const float *dy, int S, const GemmTPlan &plan, bool with_prep,
-               bool with_join);
+int gemm_t_run(DevCtx *ctx, ColiCudaTensor *t, float *dx, const float *dy, int S, const GemmTPlan &plan, bool with_join);
 // Do the ranges share a byte (outputs that would overwrite a call's inputs)?
 inline bool ranges_overlap(const void *a, size_t na, const void *b, size_t nb) {
     return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;

@@ -634,8 +634,7 @@ int gemm_t_plan(DevCtx *ctx, ColiCudaTensor *t, const float *dy, int S, GemmTPla
     return 1;
 }
 
-int gemm_t_run(DevCtx *ctx, ColiCudaTensor *t, float *dx, const float *dy, int S, const GemmTPlan &g, bool with_prep,
-               bool with_join) {
+int gemm_t_run(DevCtx *ctx, ColiCudaTensor *t, float *dx, const float *dy, int S, const GemmTPlan &g, bool with_join) {
     forget_emitted(ctx, dx, (size_t)S * t->I * sizeof(float));
     hipStream_t st = ctx->stream;
     if (t->kind == COLI_KIND_GENERIC) {
@@ -643,7 +642,7 @@ int gemm_t_run(DevCtx *ctx, ColiCudaTensor *t, float *dx, const float *dy, int S
                            t->ng_src, t->I, t->O, dy, dx);
         return hip_check(hipGetLastError(), "generic gradient");
     }
-    if (with_prep && g.prep.nblocks) {
+    if (g.prep.nblocks) {
         hipLaunchKernelGGL(coli_t_prep_rows, dim3(g.prep.nblocks), dim3(1024), 0, st, g.prep);
         if (!hip_check(hipGetLastError(), "gradient rows")) return 0;
     }
@@ -683,5 +682,5 @@ extern "C" int coli_hip_gemm_t_dev(ColiCudaTensor *t, float *dx_dev, const float
     DevCtx *ctx = ctx_of(t->device);
     if (!bind_ctx(ctx)) return 0;
     GemmTPlan g;
-    return gemm_t_plan(ctx, t, dy_dev, S, &g) && gemm_t_run(ctx, t, dx_dev, dy_dev, S, g, true, true);
+    return gemm_t_plan(ctx, t, dy_dev, S, &g) && gemm_t_run(ctx, t, dx_dev, dy_dev, S, g, true);
 }

@@ -166,10 +166,18 @@ __device__ __forceinline__ int lora_tile(const LoraRows &w, int t, int *rows, in
 
 // Stable counting sort of the rows by slot: NW waves count and then place a
 // run of rows each, 64 at a time, so a slot's rows keep their order (the sums
-// over them do not depend on timing).
+// over them do not depend on timing). One workgroup, a few us of one CU: the
+// workgroups past it build the product's row operands meanwhile (`ride` the
+// forward's, else `tride` the input gradient's, which takes 1024 threads).
 template <int NW>
-__global__ __launch_bounds__(64 * NW) void coli_lora_sort(LoraRows w) {
+__global__ __launch_bounds__(64 * NW) void coli_lora_sort(LoraRows w, ColiPrepArgs ride, ColiTPrepArgs tride) {
     extern __shared__ int cnt[];   // [NW][slots + 1]
+    if (blockIdx.x) {
+        const int b = blockIdx.x - 1;
+        if (ride.nblocks) prep_frag_block<64 * NW>(ride, min(b * (NW / 4) + ((int)threadIdx.x >> 8), ride.nblocks - 1));
+        else if constexpr (NW == 16) coli_t_prep_block(tride, b);
+        return;
+    }
     __shared__ int wsum[NW][2];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nsl = w.slots + 1;
     const int per = ((w.S + NW - 1) / NW + 63) & ~63, r0 = wave * per, r1 = min(w.S, r0 + per);
@@ -430,11 +438,11 @@ struct LoraJoin {
     float *to[2];
     int splits[2];
     const int *perm;
-    int S, Rp, nblocks;          // nblocks workgroups of 1024 threads a side
+    int S, Rp, nblocks;          // nblocks workgroups a side
 };
-__device__ __forceinline__ void lora_join_block(const LoraJoin &j, int b) {
-    const int side = b >= j.nblocks, r4 = j.Rp / 4;
-    const size_t e = (size_t)(b - side * j.nblocks) * 1024 + threadIdx.x, p = e / r4, n = (size_t)j.S * r4;
+__global__ __launch_bounds__(256) void coli_lora_join(LoraJoin j) {
+    const int b = blockIdx.x, side = b >= j.nblocks, r4 = j.Rp / 4;
+    const size_t e = (size_t)(b - side * j.nblocks) * 256 + threadIdx.x, p = e / r4, n = (size_t)j.S * r4;
     if (e >= n) return;
     const floatx4 *h = (const floatx4 *)(side ? j.h[1] : j.h[0]) + (size_t)j.perm[p] * r4 + e % r4;
     const int splits = side ? j.splits[1] : j.splits[0];
@@ -448,12 +456,6 @@ __device__ __forceinline__ void lora_join_block(const LoraJoin &j, int b) {
     ((floatx4 *)(side ? j.to[1] : j.to[0]))[e] = v;
 }
 
-// The join, with the input gradient's operand build (gemm_t.hip) beside it.
-__global__ __launch_bounds__(1024) void coli_lora_join(LoraJoin j, ColiTPrepArgs prep) {
-    const int b = blockIdx.x;
-    if (b < 2 * j.nblocks) lora_join_block(j, b);
-    else coli_t_prep_block(prep, b - 2 * j.nblocks);
-}
 
 // An element of h: the column splits joined in order, eight requested at once.
 __device__ __forceinline__ float lora_h(const float *h, int splits, size_t pitch) {
@@ -786,8 +788,10 @@ static long lora_groups(int S, const ColiHipLora *l) {
     return (long)lora_tiles(S, l->slots) * (l->Rp >= 64 ? l->Rp / 64 : 1);
 }
 
-// The rows' grouping, and (beyond COLI_LORA_BALLOT rows) the launch that makes it.
-static int lora_rows(DevCtx *ctx, const ColiHipLora *l, const int *slot_dev, int S, LoraRows *w) {
+// The rows' grouping, and (beyond COLI_LORA_BALLOT rows) the launch that makes
+// it; what it took along of the operand builds has nblocks 0 afterwards.
+static int lora_rows(DevCtx *ctx, const ColiHipLora *l, const int *slot_dev, int S, LoraRows *w, ColiPrepArgs *ride,
+                     ColiTPrepArgs *tride) {
     *w = LoraRows{};
     w->slot = slot_dev;
     w->meta = l->meta;
@@ -804,10 +808,16 @@ static int lora_rows(DevCtx *ctx, const ColiHipLora *l, const int *slot_dev, int
     w->ntile = (int *)(p + tb + rb + pb);
     // (a counter for each wave and slot: about 32 KiB of LDS at most)
     const size_t bins = (size_t)l->slots + 1;
-    if (l->slots <= 512)
-        hipLaunchKernelGGL((coli_lora_sort<16>), dim3(1), dim3(1024), 16 * bins * sizeof(int), ctx->stream, *w);
-    else
-        hipLaunchKernelGGL((coli_lora_sort<8>), dim3(1), dim3(512), 8 * bins * sizeof(int), ctx->stream, *w);
+    const int rb2 = (ride->nblocks + 1) / 2, rb4 = (ride->nblocks + 3) / 4;
+    if (l->slots <= 512) {
+        hipLaunchKernelGGL((coli_lora_sort<16>), dim3(1 + (ride->nblocks ? rb4 : tride->nblocks)), dim3(1024),
+                           16 * bins * sizeof(int), ctx->stream, *w, *ride, *tride);
+        tride->nblocks = 0;
+    } else {
+        hipLaunchKernelGGL((coli_lora_sort<8>), dim3(1 + rb2), dim3(512), 8 * bins * sizeof(int), ctx->stream, *w, *ride,
+                           ColiTPrepArgs{});
+    }
+    ride->nblocks = 0;
     return hip_check(hipGetLastError(), "adapter rows");
 }
 
@@ -825,7 +835,7 @@ static LoraSide<T> lora_side(const ColiHipLora *l, bool b, const float *x, float
 }
 
 // Up to COLI_LORA_BALLOT rows the launch also runs `ride`; beyond, its
-// workgroups have eight waves and the projection launches that build itself.
+// workgroups have eight waves and the sort has run it.
 template <typename T>
 static int launch_shrink(DevCtx *ctx, const ColiHipLora *l, const LoraRows &w, const LoraSide<T> &s0,
                          const LoraSide<T> &s1, int sides, const ColiPrepArgs &ride) {
@@ -895,14 +905,14 @@ static int lora_forward(DevCtx *ctx, ColiCudaTensor *t, const ColiHipLora *l, fl
     LoraRows w;
     const long groups = lora_groups(S, l);
     const int splits = shrink_splits(ctx, S, groups, groups * l->I, l->I, false);
+    ColiPrepArgs ride = {};
+    ColiTPrepArgs none = {};
     if (!reserve_kept(ctx, &ctx->lora_h, (size_t)splits * S * l->Rp * sizeof(float), 0) ||
-        !lora_rows(ctx, l, slot_dev, S, &w))
+        !gemm_prep_beside(ctx, t, x, S, &ride) || !lora_rows(ctx, l, slot_dev, S, &w, &ride, &none))
         return 0;
     float *h = (float *)ctx->lora_h.p;
     const LoraSide<T> a = lora_side<T>(l, false, x, h, nullptr, splits);
     const LoraSide<T> b = lora_side<T>(l, true, nullptr, h, y, splits);
-    ColiPrepArgs ride = {};
-    if (!gemm_prep_beside(ctx, t, x, S, S <= COLI_LORA_BALLOT ? &ride : nullptr)) return 0;
     return launch_shrink<T>(ctx, l, w, a, a, 1, ride) && gemm_prepared(ctx, t, y, x, S) && launch_expand<T>(ctx, l, w, b);
 }
 
@@ -915,17 +925,17 @@ static int lora_backward(DevCtx *ctx, ColiCudaTensor *t, const ColiHipLora *l, c
     const int spb = shrink_splits(ctx, S, 2 * groups, columns, l->O, true);
     const bool few = S <= COLI_LORA_BALLOT;
     const size_t hn = (size_t)S * l->Rp;
+    GemmTPlan plan = {};
+    ColiPrepArgs none = {};
     if (!reserve_kept(ctx, &ctx->lora_h, (spa + spb + (few ? 0 : 2)) * hn * sizeof(float), 0) ||
-        !lora_rows(ctx, l, slot_dev, S, &w))
+        (dx && !gemm_t_plan(ctx, t, dy, S, &plan)) || !lora_rows(ctx, l, slot_dev, S, &w, &none, &plan.prep))
         return 0;
     float *h0 = (float *)ctx->lora_h.p, *h1 = h0 + spa * hn;
     LoraSide<T> sa = lora_side<T>(l, false, x, h0, da, spa), sb = lora_side<T>(l, true, dy, h1, db, spb);
-    GemmTPlan plan = {};
-    if (dx && !gemm_t_plan(ctx, t, dy, S, &plan)) return 0;
     if (!launch_shrink<T>(ctx, l, w, sa, sb, 2, ColiPrepArgs{})) return 0;
     if (!few) {
-        LoraJoin j = {{h0, h1}, {h1 + spb * hn, h1 + (spb + 1) * hn}, {spa, spb}, w.perm, S, l->Rp, (int)((hn / 4 + 1023) / 1024)};
-        hipLaunchKernelGGL(coli_lora_join, dim3(2 * j.nblocks + plan.prep.nblocks), dim3(1024), 0, ctx->stream, j, plan.prep);
+        LoraJoin j = {{h0, h1}, {h1 + spb * hn, h1 + (spb + 1) * hn}, {spa, spb}, w.perm, S, l->Rp, (int)((hn / 4 + 255) / 256)};
+        hipLaunchKernelGGL(coli_lora_join, dim3(2 * j.nblocks), dim3(256), 0, ctx->stream, j);
         if (!hip_check(hipGetLastError(), "adapter rows join")) return 0;
         sa.h = j.to[0];
         sb.h = j.to[1];
@@ -938,7 +948,7 @@ static int lora_backward(DevCtx *ctx, ColiCudaTensor *t, const ColiHipLora *l, c
         e.part = plan.part;
         e.parts = plan.parts;
     }
-    return gemm_t_run(ctx, t, dx, dy, S, plan, few, !e.parts) && launch_outer<T>(ctx, l, w, sa, sb, &e);
+    return gemm_t_run(ctx, t, dx, dy, S, plan, !e.parts) && launch_outer<T>(ctx, l, w, sa, sb, &e);
 }
 
 // ---------------------------------------------------------------------------
