@@ -108,7 +108,9 @@ int reserve_kept(DevCtx *ctx, DevBuf *b, size_t bytes, int zero) {
     const size_t want = std::max(bytes, 2 * b->cap) + 256;
     void *p = nullptr;
     if (!hip_check(hipMalloc(&p, want), "workspace allocation")) return 0;
-    if (zero && !hip_check(hipMemset(p, 0, want), "workspace clear")) {
+    // (the clear runs on the null stream, which the backend's does not wait for)
+    if (zero && (!hip_check(hipMemset(p, 0, want), "workspace clear") ||
+                 !hip_check(hipDeviceSynchronize(), "workspace clear"))) {
         (void)hipFree(p);
         return 0;
     }

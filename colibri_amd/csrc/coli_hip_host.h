@@ -34,7 +34,7 @@
 #define COLI_PIECES 32
 
 // Outgrown workspaces a device keeps (each at least doubles its buffer).
-#define COLI_OUTGROWN 256
+#define COLI_OUTGROWN 1024
 
 struct DevBuf {
     void *p = nullptr;

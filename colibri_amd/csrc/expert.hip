@@ -190,8 +190,8 @@ static int flush_frags_into(DevCtx *ctx, FragSet &f, int *flag, const void *zero
     size_t halves = (size_t)nrows * ngp * 32;
     if (ws) {
         if (halves * 2 > f.hi.cap || halves * 2 > f.lo.cap || (size_t)nrows * sizeof(int) > f.exp.cap) return 0;
-    } else if (!reserve(ctx, &f.hi, halves * 2, 0) || !reserve(ctx, &f.lo, halves * 2, 0) ||
-               !reserve(ctx, &f.exp, (size_t)nrows * sizeof(int), 0)) {
+    } else if (!reserve_kept(ctx, &f.hi, halves * 2, 0) || !reserve_kept(ctx, &f.lo, halves * 2, 0) ||
+               !reserve_kept(ctx, &f.exp, (size_t)nrows * sizeof(int), 0)) {
         return 0;
     }
     f.gen = f.gen == 0x7fffffff ? 1 : f.gen + 1;
@@ -283,8 +283,8 @@ int run_gemv(DevCtx *ctx, int kind, bool dual, const ColiProb *probs_dev, int np
                              part_bytes, inst);
                 return 0;
             }
-        } else if (!reserve(ctx, &ctx->partial, part_bytes, 0) ||
-                   !reserve(ctx, &ctx->split_cnt, inst * sizeof(int), 1)) {
+        } else if (!reserve_kept(ctx, &ctx->partial, part_bytes, 0) ||
+                   !reserve_kept(ctx, &ctx->split_cnt, inst * sizeof(int), 1)) {
             return 0;
         }
     }
@@ -362,8 +362,8 @@ int run_gemv(DevCtx *ctx, int kind, bool dual, const ColiProb *probs_dev, int np
         FragSet &e = ctx->frag[emit->set];
         const int rows_pad = (max_rows + 15) / 16 * 16;
         const size_t halves = (size_t)max_rows * O;
-        if (!reserve(ctx, &e.hi, halves * 2, 0) || !reserve(ctx, &e.lo, halves * 2, 0) ||
-            !reserve(ctx, &e.gexp, (size_t)(O / 128) * rows_pad * 4, 0))
+        if (!reserve_kept(ctx, &e.hi, halves * 2, 0) || !reserve_kept(ctx, &e.lo, halves * 2, 0) ||
+            !reserve_kept(ctx, &e.gexp, (size_t)(O / 128) * rows_pad * 4, 0))
             return 0;
         e.pending = false;
         e.px = nullptr;
@@ -513,7 +513,7 @@ int run_gemm(DevCtx *ctx, int kind, bool dual, const ColiProb *probs_dev, int np
                   &a.splits);
         a.part_rows = split_rows;
         if (a.splits > 1) {
-            if (!reserve(ctx, &ctx->partial, (size_t)a.splits * split_rows * cols * sizeof(float), 0)) return 0;
+            if (!reserve_kept(ctx, &ctx->partial, (size_t)a.splits * split_rows * cols * sizeof(float), 0)) return 0;
             a.partial = (float *)ctx->partial.p;
         }
     }
@@ -531,7 +531,7 @@ int run_gemm(DevCtx *ctx, int kind, bool dual, const ColiProb *probs_dev, int np
     if (a.segq < a.qps && inline_prob->nrows > COLI_GM_ROWS) {
         const size_t item = (size_t)a.splits * a.rb_per_prob * ((a.qps - 1) / a.segq) * COLI_GM_SUMS * sizeof(float);
         if (a.splits == 1) step = (int)std::max((size_t)1, std::min((size_t)n_mt, ((size_t)512 << 20) / item));
-        if (!reserve(ctx, &ctx->sums, step * item, 0)) return 0;
+        if (!reserve_kept(ctx, &ctx->sums, step * item, 0)) return 0;
         a.sums = (float *)ctx->sums.p;
     }
     for (int i = 0; i < n_mt; i += step) {
@@ -1134,8 +1134,8 @@ static int idot_dev(DevCtx *ctx, ColiCudaTensor *t, float *y_dev, const float *x
     const int set = frag_set_of(t->kind, false), ngp = ngp_of(t->I);
     FragSet &f = ctx->frag[set];
     const size_t halves = (size_t)S * ngp * 32;
-    if (!reserve(ctx, &f.hi, halves * 2, 0) || !reserve(ctx, &f.lo, halves * 2, 0) ||
-        !reserve(ctx, &f.exp, (size_t)S * sizeof(int), 0) || !reserve(ctx, &ctx->idot_y, (size_t)S * t->O * 4, 0) ||
+    if (!reserve_kept(ctx, &f.hi, halves * 2, 0) || !reserve_kept(ctx, &f.lo, halves * 2, 0) ||
+        !reserve_kept(ctx, &f.exp, (size_t)S * sizeof(int), 0) || !reserve(ctx, &ctx->idot_y, (size_t)S * t->O * 4, 0) ||
         !reserve(ctx, &ctx->idot_sx, (size_t)S * 4, 0))
         return 0;
     // hi parts only: the GEMVs over this set never read its lo buffer

@@ -294,6 +294,45 @@ def test_graph_replays(session, S):
                 o.check_grads()
 
 
+def test_graph_outlives_larger_products(session):
+    """A captured forward and backward after larger eager calls of the same
+    storage kind, which outgrow every buffer that the captured launches hold
+    (row operands, partial sums of GEMV and GEMM, counters, adapter rows)."""
+    b = session.b
+    with Case(session, 45, "i4h", 304, 640, 90, 3, 16, 1, "mixed") as c, \
+            Case(session, 46, "i4h", 256, 8192, 6, 3, 16, 1, "mixed") as few, \
+            Case(session, 47, "i4h", 2048, 2304, 1500, 5, 48, 1, "mixed") as o:
+        d, outs = c.d, []
+        graphs = []
+        for k in (few, c):
+            px, pdy, ps = k.d.up(k.x), k.d.up(k.dy), k.d.up(k.slot)
+            py, pdx = k.d.up(np.zeros((k.S, k.O), np.float32)), k.d.up(np.zeros((k.S, k.I), np.float32))
+            pda, pdb = k.d.up(np.zeros((3, 16, k.I), np.float32)), k.d.up(np.zeros((3, k.O, 16), np.float32))
+
+            def step():
+                assert b.hip_lora_gemm_dev(k.h, k.bank, py, px, k.S, ps)
+                assert b.hip_lora_grad_dev(k.h, k.bank, px, pdy, k.S, ps, pdx, pda, pdb)
+
+            step()
+            sizes = ((py, (k.S, k.O)), (pdx, (k.S, k.I)), (pda, (3, 16, k.I)), (pdb, (3, k.O, 16)))
+            eager = [d.down(p, n) for p, n in sizes]
+            with hiprt.Graph(b.hip_stream(0)) as g:
+                step()
+            graphs.append((g, sizes, eager))
+        o.check_forward()
+        o.check_grads()
+        outs = [o.d.up(np.zeros((1500, 2048), np.float32)) for _ in range(4)]
+        for rep in range(3):
+            for g, sizes, eager in graphs:
+                for p, n in sizes:
+                    assert b.hip_fill_random_u8(0, p, int(np.prod(n)) * 4, 7 + rep)
+                g.launch()
+                for (p, n), want in zip(sizes, eager):
+                    assert np.array_equal(d.down(p, n).view(np.uint32), want.view(np.uint32)), (rep, n)
+            px = outs[rep]
+            assert b.cuda_pipe_gemm(o.h, px, o.d.up(o.x), 1500 - rep)
+
+
 def test_two_projections_in_sequence(session):
     """A two-layer feed-forward with adapters on both projections, forward and backward in one queue."""
     b = session.b
