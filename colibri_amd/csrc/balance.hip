@@ -15,6 +15,13 @@
 // 4 l), at most sixteen columns a lane, so a wave runs four rows at once up to
 // 256 experts, and the reductions of a row are lane permutes on the VALU. All sums are f32,
 // the counts integers; they are joined in a fixed order (no float atomics).
+//
+// Measured, 65536 rows of 384 experts: softmax and sigmoid forward 26 us with the
+// join's 7 (101 MB of logits, 20 us of them at 5 TB/s), backward 35 us (201 MB,
+// 5.7 TB/s, the logits partly cached); sqrt-softplus, whose four hardware
+// functions an element meet the bytes, 36 and 40 us. Rows a workgroup, forward
+// (mode 0): 16 / 32 / 64 / 128: 36 / 29 / 26 / 26 us; backward 34 to 36 us for
+// all of them. 64 rows of 64 experts: one workgroup, 6.7 us, latency.
 #include "coli_hip_host.h"
 #include "coli_device.h"
 

@@ -17,9 +17,15 @@
 //   * A weight enters as n sc 2^-Eg in fp16 hi + lo, Eg the exponent of its
 //     column group's largest scale (exact for MXFP4, whose lo is zero and left
 //     out, and for int4 with fp16 scales; to 3 x 2^-22 with f32 scales, which
-//     enter as two fp16); dy as fp16 hi + lo under its row's exponent (2^-22). hi hi + hi lo + lo hi are summed in f32. The scales
-//     are kept a second time per tensor, by column group with eight rows' worth
-//     in 16 bytes (coli_t_scales, made on first use).
+//     enter as two fp16); dy as fp16 hi + lo under its row's exponent (2^-22).
+//     hi hi + hi lo + lo hi are summed in f32. The scales are kept a second time
+//     per tensor, by column group with eight rows' worth in 16 bytes
+//     (coli_t_scales, made on first use).
+//
+// Many rows are bound by the matrix units: 2048 x 4096 x 14336 int4, three
+// products, 600 us, 1.2 PFLOP/s of fp16 products (an 8192^3 library product:
+// 1.07); 512 rows 187 us with the join (7 us) and the build of dy's operands
+// (16 us, 59 MB at 3.8 TB/s) to come. Few rows: see coli_gemm_t_few.
 #include "coli_hip_host.h"
 #include "coli_device.h"
 
@@ -327,7 +333,9 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void coli_gemm_t(GemmTArgs a) {
 // No launch builds operands, and no barrier holds the waves together before
 // their sums are joined. Bound by the VALU (transpose, unpack and conversion,
 // about 450 instructions a step of 4096 weights); a 64-row form spilled its
-// accumulators, so every 32 rows read and unpack the weights again.
+// accumulators, so every 32 rows read and unpack the weights again. Measured: 16
+// rows of 7168 x 2048 MXFP4 (8.4 MB) 8.7 us and the join 2.8; 64 of 14336 x 4096
+// int4 46 us (33 MB).
 template <int KIND, bool ODD>
 __global__ __launch_bounds__(512, 2) void coli_gemm_t_few(GemmTArgs a) {
     constexpr int BM = 32, W = 8, CPT = 4 * BM / 64, STAGE = 8 * BM * 16, PD = 2;
