@@ -89,8 +89,9 @@ struct DevCtx {
     FragSet frag[4];                   // 0/1: inputs (int4 / fp4 order), 2/3: hidden rows
     int dense_set[2] = {0, 1};         // set the next coli_hip_gemm_run_dev reads, per order (gemm_prep)
     DevBuf pipe[COLI_PIPE_SLOTS];
-    // workspaces of the adapter, input-gradient and balance entry points
-    // (reserve_kept: outgrown ones live until shutdown)
+    // workspaces of the adapter, input-gradient and balance entry points; these,
+    // the fragments, partial, split_cnt and sums grow by reserve_kept: outgrown
+    // ones live until shutdown
     DevBuf lora_h, lora_list, gt, bal, bal_cnt;
     void *outgrown[COLI_OUTGROWN] = {};
     int n_outgrown = 0;
@@ -179,12 +180,12 @@ int tensor_computable(const ColiCudaTensor *t);
 int gemm_dev(DevCtx *ctx, ColiCudaTensor *t, float *y_dev, const float *x_dev, int S);
 // gemm_dev in two halves: the rows' fragment build, if the product will read
 // fragments, as launch arguments for a launch that runs it beside other work
-// (a null: left for gemm_prepared to launch), then the product.
+// (nblocks 0: nothing to run), then the product.
 int gemm_prep_beside(DevCtx *ctx, ColiCudaTensor *t, const float *x_dev, int S, ColiPrepArgs *a);
 int gemm_prepared(DevCtx *ctx, ColiCudaTensor *t, float *y_dev, const float *x_dev, int S);
-// dx = dy W: the decomposition, then the launches (with_prep: the rows' operands
-// too, where plan.prep.nblocks asks for them; with_join: the K splits' sums into
-// dx, else left in part [parts][S][I] where parts is not 0).
+// dx = dy W: the decomposition, then the launches (the rows' operands too while
+// plan.prep.nblocks is not 0, so a launch that has built them clears it; with_join:
+// the K splits' sums into dx, else left in part [parts][S][I] where parts is not 0).
 struct GemmTPlan {
     ColiTPrepArgs prep;
     bool few;

@@ -1051,10 +1051,9 @@ int gemm_dev(DevCtx *ctx, ColiCudaTensor *t, float *y_dev, const float *x_dev, i
 }
 
 int gemm_prep_beside(DevCtx *ctx, ColiCudaTensor *t, const float *x_dev, int S, ColiPrepArgs *a) {
-    if (a) a->nblocks = 0;
+    a->nblocks = 0;
     if (t->kind == COLI_KIND_GENERIC) return 1;
     if (!gemm_prep(ctx, t, x_dev, S)) return 0;
-    if (!a) return 1;
     const int set = ctx->dense_set[t->kind == COLI_KIND_FP4 ? 1 : 0];
     if (!dense_on_gemm(ctx, t, S)) {
         // (the plan run_gemv makes for one matrix)

@@ -250,7 +250,8 @@ def test_graph_replays(session, T):
 
 
 @pytest.mark.parametrize("mode,S,E,K,D", [(0, 1, 64, 8, 2048), (0, 9, 64, 8, 256), (2, 5, 128, 8, 1536), (1, 70, 33, 4, 640),
-                                          (3, 300, 96, 6, 384)])
+                                          (3, 300, 96, 6, 384), (2, 1, 256, 8, 1024), (0, 1, 128, 8, 512),
+                                          (3, 1, 40, 4, 384), (0, 64, 64, 8, 256), (1, 65, 64, 8, 256), (0, 2, 16, 2, 256)])
 def test_last_forward_of_a_layer(session, mode, S, E, K, D):
     """Counts and loss of the layer's own router after a forward."""
     rng = np.random.default_rng(S + E)
