@@ -114,15 +114,16 @@ __global__ __launch_bounds__(256) void coli_lora_set(const T *__restrict__ a, co
     __shared__ T tile[64][66];
     const int nb = blockIdx.x - na, no = Op / 64, o0 = (nb % no) * 64, r0 = (nb / no) * 64;
     const int nr = min(64, Rp - r0);   // 16, 32 or 64: a wave's lanes cover 64 / nr rows of B
+    const int sh = nr == 16 ? 4 : nr == 32 ? 5 : 6;
     T v[16];
 #pragma unroll
     for (int k = 0; k < 16; k++) {
-        const int e = tid + 256 * k, o = o0 + e / nr, r = r0 + e % nr;
+        const int e = tid + 256 * k, o = o0 + (e >> sh), r = r0 + (e & (nr - 1));
         v[k] = e < 64 * nr && o < O && r < rank ? b[(size_t)o * rank + r] : T{};
     }
 #pragma unroll
     for (int k = 0; k < 16; k++)
-        if (tid + 256 * k < 64 * nr) tile[(tid + 256 * k) / nr][(tid + 256 * k) % nr] = v[k];
+        if (tid + 256 * k < 64 * nr) tile[(tid + 256 * k) >> sh][(tid + 256 * k) & (nr - 1)] = v[k];
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < 16; k++) {
@@ -512,22 +513,18 @@ __device__ __forceinline__ void lora_expand_block(const LoraRows &w, const LoraS
     const bool whole = c + 8 <= s.N;
     const float *yr[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) yr[i] = (JOIN ? s.part : s.out) + (size_t)rows[min(4 * kq + i, n - 1)] * s.N + c;
-    f4u y[4][2];
-    // (a lane whose eight columns pass N loads h instead, which has as many, and
-    // adds its columns one by one at the end: see row4 for why not here)
-    auto load_y = [&](int p, f4u (&v)[4][2]) {
+    for (int i = 0; i < 4; i++) yr[i] = (JOIN ? s.part : s.out) + (size_t)rows[min(4 * kq + i, n - 1)] * s.N;
+    floatx4 y[4][2];
+    auto load_y = [&](int p, floatx4 (&v)[4][2]) {   // (columns past N: not kept)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float *q = whole ? yr[i] + (size_t)p * w.S * s.N : s.h;
-            v[i][0] = *GPTR(f4u, q);
-            v[i][1] = *GPTR(f4u, q + 4);
-        }
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) v[i][e] = row4<true>(yr[i] + (size_t)p * w.S * s.N, c + 4 * e, s.N);
     };
     load_y(0, y);
     if constexpr (JOIN) {
         for (int p = 1; p < s.parts; p++) {
-            f4u z[4][2];
+            floatx4 z[4][2];
             load_y(p, z);
 #pragma unroll
             for (int i = 0; i < 4; i++)
@@ -566,25 +563,16 @@ __device__ __forceinline__ void lora_expand_block(const LoraRows &w, const LoraS
         const int row = 4 * kq + i;
         if (row >= n || c >= s.N) continue;
         float *to = s.out + (size_t)rows[row] * s.N + c;
+        floatx4 t[2];
+#pragma unroll
+        for (int j = 0; j < 8; j++) t[j >> 2][j & 3] = y[i][j >> 2][j & 3] + acc[j][i];   // (rank 0: the sums of no products, 0)
         if (whole) {
-            f4u y0 = y[i][0], y1 = y[i][1];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                y0[j] += acc[j][i];   // (rank 0: the sums of no products, 0)
-                y1[j] += acc[4 + j][i];
-            }
-            *(f4u *)to = y0;
-            *(f4u *)(to + 4) = y1;
+            *(f4u *)to = t[0];
+            *(f4u *)(to + 4) = t[1];
         } else {
-            float t[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) t[j] = yr[i][min(j, s.N - 1 - c)];
-            for (int p = 1; JOIN && p < s.parts; p++)
-#pragma unroll
-                for (int j = 0; j < 8; j++) t[j] += yr[i][(size_t)p * w.S * s.N + min(j, s.N - 1 - c)];
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (c + j < s.N) to[j] = t[j] + acc[j][i];
+            for (int j = 0; j < 7; j++)
+                if (c + j < s.N) to[j] = t[j >> 2][j & 3];
         }
     }
 }
