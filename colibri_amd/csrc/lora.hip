@@ -577,22 +577,25 @@ __device__ __forceinline__ void lora_expand_block(const LoraRows &w, const LoraS
     }
 }
 
-// outer: workgroup (64 columns, slot and NR rank tiles, side); the W waves take
-// 16 rows of the slot in turn, four MFMA steps of four rows, the next 16 rows
-// requested before this step's products and their numbers a step earlier; the
-// waves' sums are joined in LDS. h: up to COLI_LORA_BALLOT rows its column
-// splits, joined here in LDS; beyond, joined and in slot order already
-// (coli_lora_join). Side 0: dA [slots][max_rank][N]; side 1 (dB):
-// stored transposed, [slots][N][max_rank]. Every element is written, zeros
-// where a slot has no rows or rank.
-template <typename T, int NR, int W>
+// outer: workgroup (64 columns, slot and NR rank tiles, side); its W waves
+// take 16 rows of the slot in turn, four MFMA steps of four rows, the next 16
+// rows requested before this step's products and their numbers a step earlier;
+// the waves' sums are joined in LDS. Four waves, several workgroups a CU, so that
+// one's products run beside another's first loads and its join: with 16 / 8 / 4
+// waves the adapter gradients of 1024 x 14336 x 4096, rank 64, 8 slots, take 135 /
+// 114 / 107 us, of 2048 x 4096 x 14336, rank 32, 4 slots, 105 / 92 / 90; sixteen
+// where the workgroups leave CUs idle (512 x 7168 x 2048, one slot: this kernel
+// 9.0 us against 11.0). h: up to COLI_LORA_BALLOT rows
+// its column splits, joined here in LDS; beyond (LIST), joined and in slot order
+// already (coli_lora_join). Side 0: dA [slots][max_rank][N]; side 1 (dB): stored
+// transposed, [slots][N][max_rank]. Every element is written, zeros where a slot
+// has no rows or rank.
+template <typename T, int NR, int W, bool LIST>
 __device__ __forceinline__ void lora_outer_block(const LoraRows &w, const LoraSide<T> &s0, const LoraSide<T> &s1, int Rp,
                                                  int max_rank, int cb, int sr, bool side1) {
-    constexpr int RW = W > 8 ? 8 : W;   // waves of the LDS join
-    constexpr bool LIST = W > 4;        // beyond COLI_LORA_BALLOT rows
     __shared__ int rows[COLI_LORA_BALLOT];
     __shared__ float hl[LIST ? 1 : COLI_LORA_BALLOT][LIST ? 1 : 16 * NR + 1];
-    __shared__ float red[RW][64][17];
+    __shared__ float red[W][64][17];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, kq = lane >> 4;
     const int nrp = (Rp / 16 + NR - 1) / NR, slot = sr / nrp, rt0 = (sr - slot * nrp) * NR;
     // (h of one side meets the rows of the other)
@@ -684,36 +687,20 @@ __device__ __forceinline__ void lora_outer_block(const LoraRows &w, const LoraSi
     for (int r = 0; r < NR; r++) {
         __syncthreads();
         // lane (m, kq): columns 4 m + j, ranks 4 kq + i
-        if (W > RW && wave >= RW) {
 #pragma unroll
-            for (int q = 0; q < NR; q++)
-                if (q == r)
+        for (int q = 0; q < NR; q++)
+            if (q == r)
 #pragma unroll
-                    for (int j = 0; j < 4; j++)
+                for (int j = 0; j < 4; j++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) red[wave - RW][lane][4 * i + j] = acc[q][j][i];
-        }
-        if (W > RW) __syncthreads();
-        if (wave < RW) {
-#pragma unroll
-            for (int q = 0; q < NR; q++)
-                if (q == r)
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            float v = acc[q][j][i];
-                            if (W > RW) v += red[wave][lane][4 * i + j];
-                            red[wave][lane][4 * i + j] = v;
-                        }
-        }
+                    for (int i = 0; i < 4; i++) red[wave][lane][4 * i + j] = acc[q][j][i];
         __syncthreads();
         for (int e = threadIdx.x; e < 1024; e += 64 * W) {
             const int rk = side1 ? e & 15 : e >> 6, col = side1 ? e >> 4 : e & 63;
             const int ln = (col >> 2) + 16 * (rk >> 2), at = 4 * (rk & 3) + (col & 3);
             float v = red[0][ln][at];
 #pragma unroll
-            for (int q = 1; q < RW; q++) v += red[q][ln][at];
+            for (int q = 1; q < W; q++) v += red[q][ln][at];
             const int k = 16 * (rt0 + r) + rk;
             // (past the rank: zeros, also where a row of infinities shrank to NaN)
             v = k < rank ? v * meta.scale : 0.0f;
@@ -728,9 +715,9 @@ __global__ __launch_bounds__(256) void coli_lora_expand(LoraRows w, LoraSide<T> 
     extern __shared__ float hs[];
     lora_expand_block<T, JOIN>(w, s, Rp, blockIdx.x, blockIdx.y, hs);
 }
-template <typename T, int NR>
-__global__ __launch_bounds__(1024) void coli_lora_outer(LoraRows w, LoraSide<T> s0, LoraSide<T> s1, int Rp, int max_rank) {
-    lora_outer_block<T, NR, 16>(w, s0, s1, Rp, max_rank, blockIdx.x, blockIdx.y, blockIdx.z != 0);
+template <typename T, int NR, int W>
+__global__ __launch_bounds__(64 * W) void coli_lora_outer(LoraRows w, LoraSide<T> s0, LoraSide<T> s1, int Rp, int max_rank) {
+    lora_outer_block<T, NR, W, true>(w, s0, s1, Rp, max_rank, blockIdx.x, blockIdx.y, blockIdx.z != 0);
 }
 // Up to COLI_LORA_BALLOT rows both run in one launch, the expand's workgroups
 // (ne; none without dx) first.
@@ -743,7 +730,7 @@ __global__ __launch_bounds__(256) void coli_lora_finish(LoraRows w, LoraSide<T> 
         lora_expand_block<T, JOIN>(w, e, Rp, b % tiles, b / tiles, hs);
     } else {
         const int o = b - ne, half = (int)(gridDim.x - ne) / 2, r = o % half;
-        lora_outer_block<T, NR, 4>(w, s0, s1, Rp, max_rank, r % cols, r / cols, o >= half);
+        lora_outer_block<T, NR, 4, false>(w, s0, s1, Rp, max_rank, r % cols, r / cols, o >= half);
     }
 }
 
@@ -869,37 +856,50 @@ static int launch_expand(DevCtx *ctx, const ColiHipLora *l, const LoraRows &w, c
     return hip_check(hipGetLastError(), "adapter expand");
 }
 
-// Adapter gradients and, with e, the expand: one launch up to COLI_LORA_BALLOT rows.
+// Up to COLI_LORA_BALLOT rows: adapter gradients and, with e, the expand.
 template <typename T>
-static int launch_outer(DevCtx *ctx, const ColiHipLora *l, const LoraRows &w, const LoraSide<T> &s0, const LoraSide<T> &s1,
-                        const LoraSide<T> *e) {
+static int launch_finish(DevCtx *ctx, const ColiHipLora *l, const LoraRows &w, const LoraSide<T> &s0, const LoraSide<T> &s1,
+                         const LoraSide<T> *e) {
     const int nrt = l->Rp / 16, cols = (std::max(l->I, l->O) + 63) / 64, nr = nrt >= 4 ? 4 : nrt, ny = l->slots * (nrt / nr);
-    if (w.S <= COLI_LORA_BALLOT) {
-        const int tiles = lora_tiles(w.S, l->slots), ne = e ? tiles * ((e->Np + 511) / 512) : 0;
-        const size_t shm = (size_t)16 * (l->Rp + 1) * sizeof(float);
+    const int tiles = lora_tiles(w.S, l->slots), ne = e ? tiles * ((e->Np + 511) / 512) : 0;
+    const size_t shm = (size_t)16 * (l->Rp + 1) * sizeof(float);
 #define COLI_FINISH(NR, JOIN)                                                                                    \
     hipLaunchKernelGGL((coli_lora_finish<T, NR, JOIN>), dim3(ne + 2 * cols * ny), dim3(256), shm, ctx->stream, w, s0, \
                        s1, e ? *e : s0, l->Rp, l->max_rank, ne, tiles, cols)
-#define COLI_FINISH_NR(JOIN)            \
+#define COLI_FINISH_NR(JOIN)                \
     if (nr == 1) COLI_FINISH(1, JOIN);      \
     else if (nr == 2) COLI_FINISH(2, JOIN); \
     else COLI_FINISH(4, JOIN)
-        if (e && e->parts) {
-            COLI_FINISH_NR(true);
-        } else {
-            COLI_FINISH_NR(false);
-        }
+    if (e && e->parts) {
+        COLI_FINISH_NR(true);
+    } else {
+        COLI_FINISH_NR(false);
+    }
 #undef COLI_FINISH_NR
 #undef COLI_FINISH
-        return hip_check(hipGetLastError(), "adapter gradients");
+    return hip_check(hipGetLastError(), "adapter gradients");
+}
+
+// Beyond: adapter gradients alone.
+template <typename T>
+static int launch_outer(DevCtx *ctx, const ColiHipLora *l, const LoraRows &w, const LoraSide<T> &s0, const LoraSide<T> &s1) {
+    const int nrt = l->Rp / 16, cols = (std::max(l->I, l->O) + 63) / 64, nr = nrt >= 4 ? 4 : nrt, ny = l->slots * (nrt / nr);
+    const long live = (long)((l->I + 63) / 64 + (l->O + 63) / 64) * ny;
+#define COLI_OUTER(NR, W)                                                                                            \
+    hipLaunchKernelGGL((coli_lora_outer<T, NR, W>), dim3(cols, ny, 2), dim3(64 * W), 0, ctx->stream, w, s0, s1, l->Rp, \
+                       l->max_rank)
+#define COLI_OUTER_NR(W)               \
+    if (nr == 1) COLI_OUTER(1, W);     \
+    else if (nr == 2) COLI_OUTER(2, W); \
+    else COLI_OUTER(4, W)
+    if (live <= (ctx->cu_count ? ctx->cu_count : 256)) {
+        COLI_OUTER_NR(16);
+    } else {
+        COLI_OUTER_NR(4);
     }
-#define COLI_OUTER(NR) \
-    hipLaunchKernelGGL((coli_lora_outer<T, NR>), dim3(cols, ny, 2), dim3(1024), 0, ctx->stream, w, s0, s1, l->Rp, l->max_rank)
-    if (nr == 1) COLI_OUTER(1);
-    else if (nr == 2) COLI_OUTER(2);
-    else COLI_OUTER(4);
+#undef COLI_OUTER_NR
 #undef COLI_OUTER
-    return hip_check(hipGetLastError(), "adapter gradients") && (!e || launch_expand<T>(ctx, l, w, *e));
+    return hip_check(hipGetLastError(), "adapter gradients");
 }
 
 template <typename T>
@@ -944,14 +944,18 @@ static int lora_backward(DevCtx *ctx, ColiCudaTensor *t, const ColiHipLora *l, c
         sb.h = j.to[1];
         sa.splits = sb.splits = 1;
     }
-    if (!dx) return launch_outer<T>(ctx, l, w, sa, sb, nullptr);
+    // (beyond COLI_LORA_BALLOT rows ahead of the product, which drives the rows out
+    // of the caches)
+    if (!few && !launch_outer<T>(ctx, l, w, sa, sb)) return 0;
+    if (!dx) return !few || launch_finish<T>(ctx, l, w, sa, sb, nullptr);
     LoraSide<T> e = lora_side<T>(l, false, nullptr, sb.h, dx, sb.splits);
     e.sorted = !few;
     if (plan.parts) {   // the expand joins the K splits
         e.part = plan.part;
         e.parts = plan.parts;
     }
-    return gemm_t_run(ctx, t, dx, dy, S, plan, !e.parts) && launch_outer<T>(ctx, l, w, sa, sb, &e);
+    return gemm_t_run(ctx, t, dx, dy, S, plan, !e.parts) &&
+           (few ? launch_finish<T>(ctx, l, w, sa, sb, &e) : launch_expand<T>(ctx, l, w, e));
 }
 
 // ---------------------------------------------------------------------------
