@@ -21,8 +21,8 @@
 // a launch (2 to 3 us) and of its few dependent loads up to 64. Measured (bf16
 // factors; MI355X, a large copy 4.7 TB/s):
 //   2048 rows, 4096 -> 14336, rank 32: both shrinks of the backward 40 us (151
-//     MB, 3.7 TB/s), outer 64 us (the same rows again, 2.3 TB/s), expand 56 us
-//     forward (235 MB, 4.2 TB/s) and 25 us backward (67 MB)
+//     MB, 3.7 TB/s), outer 52 us (the same rows again, 2.9 TB/s), expand 53 us
+//     forward (235 MB, 4.4 TB/s) and 21 us backward (67 MB)
 //   1024 rows, 14336 -> 4096, rank 64: shrink 39 us (59 MB, one step of 64 MFMAs
 //     a wave at a time), expand 21 us
 //   16 rows of 16 adapters, 7168 -> 2048, rank 32: 6.2 and 5.6 us
