@@ -831,7 +831,9 @@ static int launch_shrink(DevCtx *ctx, const ColiHipLora *l, const LoraRows &w, c
                          const LoraSide<T> &s1, int sides, const ColiPrepArgs &ride) {
     const int tiles = lora_tiles(w.S, l->slots), nrt = l->Rp / 16, sp = std::max(s0.splits, sides > 1 ? s1.splits : 1);
     const int nr = nrt >= 4 ? 4 : nrt, nz = nrt / nr, nown = tiles * sp * sides * nz;
-#define COLI_SHRINK(NR, W)                                                                                            hipLaunchKernelGGL((coli_lora_shrink<T, NR, W>), dim3(nown + ride.nblocks), dim3(64 * W), 0,                               ctx->stream, w, s0, s1, l->Rp, nz, tiles, sp, nown, ride)
+#define COLI_SHRINK(NR, W)                                                                                        \
+    hipLaunchKernelGGL((coli_lora_shrink<T, NR, W>), dim3(nown + ride.nblocks), dim3(64 * W), 0, ctx->stream, w, s0, \
+                       s1, l->Rp, nz, tiles, sp, nown, ride)
     if (w.S <= COLI_LORA_BALLOT) {
         if (nr == 1) COLI_SHRINK(1, 4);
         else if (nr == 2) COLI_SHRINK(2, 4);

@@ -130,7 +130,8 @@ def test_gradients(session, shape):
 
 @pytest.mark.parametrize("pin", ["few", "many"])
 @pytest.mark.parametrize("shape", [("i4h", 200, 300, 40, 3, 16, 1, "mixed"), ("fp4", 515, 260, 150, 4, 24, 2, "runs"),
-                                   ("i4f", 300, 129, 300, 2, 70, 0, "mixed")], ids=lambda s: "-".join(map(str, s)))
+                                   ("i4f", 300, 129, 300, 2, 70, 0, "mixed"),
+                                   ("i4h", 130, 140, 400, 600, 4, 2, "mixed")], ids=lambda s: "-".join(map(str, s)))
 def test_gradients_with_either_product(session, monkeypatch, shape, pin):
     monkeypatch.setenv("COLI_HIP_GEMM_T", pin)
     with Case(session, 300 + shape[3], *shape) as c:
