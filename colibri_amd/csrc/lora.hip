@@ -11,8 +11,9 @@
 //   expand  Y[s][n]  += scale sum_r h[s][r] V[r][n]  (B h, A^T dh)
 //   outer   G[r][n]   = scale sum_s h[s][r] X[s][n]  (dA, dB)
 // on v_mfma_f32_16x16x4_f32: the adapters' products are a few hundredths of
-// the projection's, so f32 operands cost nothing that the rows' bytes do not
-// hide, and need neither splitting nor exponents. Rows of one slot are
+// the projection's, and f32 operands need neither splitting nor exponents; the
+// shrink of bf16 factors alone, where they are most of the time at high ranks,
+// splits x into three bf16 (shrink_products). Rows of one slot are
 // gathered 16 at a time into an MFMA tile: up to 64 rows each workgroup finds
 // its tile with one ballot over the rows' slots, beyond it a one-workgroup
 // stable counting sort lists them. Sums run in a fixed order.
@@ -20,12 +21,12 @@
 // All three are bound by the rows' bytes once there are many, by the latency of
 // a launch (2 to 3 us) and of its few dependent loads up to 64. Measured (bf16
 // factors; MI355X, a large copy 4.7 TB/s):
-//   2048 rows, 4096 -> 14336, rank 32: both shrinks of the backward 40 us (151
-//     MB, 3.7 TB/s), outer 52 us (the same rows again, 2.9 TB/s), expand 53 us
+//   2048 rows, 4096 -> 14336, rank 32: both shrinks of the backward 38 us (151
+//     MB, 4.0 TB/s), outer 52 us (the same rows again, 2.9 TB/s), expand 53 us
 //     forward (235 MB, 4.4 TB/s) and 21 us backward (67 MB)
-//   1024 rows, 14336 -> 4096, rank 64: shrink 39 us (59 MB, one step of 64 MFMAs
-//     a wave at a time), expand 21 us
-//   16 rows of 16 adapters, 7168 -> 2048, rank 32: 6.2 and 5.6 us
+//   1024 rows, 14336 -> 4096, rank 64: shrink 22 us (59 MB; on f32 MFMAs 39),
+//     expand 21 us
+//   16 rows of 16 adapters, 7168 -> 2048, rank 32: 5.4 and 5.6 us
 //   one row, 4096 -> 14336, rank 16: 4.4 and 4.2 us beside a projection of 10
 // up to 64 rows the gradients' outer and the expand are one launch
 // (coli_lora_finish), and the projection's row operands are built in the
@@ -298,6 +299,45 @@ template <typename T> struct LoraSide {
     int sorted;                  // h rows are in slot order (coli_lora_join), not the call's
 };
 
+// acc[r] += x v[r] over the lane's eight columns and its neighbours', 32 in all.
+// bf16 factors: x as three bf16 (truncated, 8 bits each: exact) on
+// v_mfma_f32_16x16x32_bf16, three MFMAs of 16 cycles where f32 takes eight of 32,
+// and the factors need no conversion (adapters beside 1024 x 14336, rank 64: 30 ->
+// 20 us; all gradients of 2048 x 4096 x 14336, rank 32: 90 -> 83). fp16 and f32
+// factors would have to be split as well, 32 and 44 VALU instructions for eight,
+// which takes the gain. f32 sums either way.
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+template <typename T, int NR>
+__device__ __forceinline__ void shrink_products(const float (&x)[8], const Raw8<T> (&v)[NR], floatx4 (&acc)[NR]) {
+    if constexpr (__is_same(T, bf16_t)) {
+        u32x4 part[3];
+        float rest[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) rest[j] = x[j];
+#pragma unroll
+        for (int p = 0; p < 3; p++)
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                const uint32_t a = __float_as_uint(rest[j]), b = __float_as_uint(rest[j + 1]);
+                part[p][j / 2] = __builtin_amdgcn_perm(b, a, 0x07060302u);   // the upper halves
+                rest[j] -= __uint_as_float(a & 0xffff0000u);
+                rest[j + 1] -= __uint_as_float(b & 0xffff0000u);
+            }
+#pragma unroll
+        for (int p = 2; p >= 0; p--)
+#pragma unroll
+            for (int r = 0; r < NR; r++)
+                acc[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, part[p]),
+                                                                 __builtin_bit_cast(bf16x8, v[r].w), acc[r], 0, 0, 0);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+#pragma unroll
+            for (int r = 0; r < NR; r++)
+                acc[r] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], v[r].get(j), acc[r], 0, 0, 0);
+    }
+}
+
 // shrink: workgroup (tile, column split, NR rank tiles of one side). The W
 // waves take COLS columns in turn: a lane loads 16 bytes of a row of x or of
 // the factor, neighbours next to each other (lanes of one MFMA operand lie in
@@ -388,10 +428,13 @@ __global__ __launch_bounds__(64 * W) void coli_lora_shrink(LoraRows w, LoraSide<
 #pragma unroll
         for (int u = 0; u < STEP / 32; u++) {
             // columns 32 u + 8 kq + 0..7
-            floatx4 x[2];
+            float x[8];
 #pragma unroll
-            for (int e = 0; e < 2; e++)
-                x[e] = *(const floatx4 *)(mine + (m * G::XP + ((8 * u + 2 * kq + e) ^ (m & (G::XP - 1)))) * 16);
+            for (int e = 0; e < 2; e++) {
+                const floatx4 t = *(const floatx4 *)(mine + (m * G::XP + ((8 * u + 2 * kq + e) ^ (m & (G::XP - 1)))) * 16);
+#pragma unroll
+                for (int j = 0; j < 4; j++) x[4 * e + j] = t[j];
+            }
             Raw8<T> v[NR];
 #pragma unroll
             for (int r = 0; r < NR; r++) {
@@ -400,11 +443,7 @@ __global__ __launch_bounds__(64 * W) void coli_lora_shrink(LoraRows w, LoraSide<
                 if constexpr (sizeof(T) == 4) v[r].set(piece(8 * u + 2 * kq), piece(8 * u + 2 * kq + 1));
                 else v[r].set(piece(4 * u + kq));
             }
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-#pragma unroll
-                for (int r = 0; r < NR; r++)
-                    acc[r] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j >> 2][j & 3], v[r].get(j), acc[r], 0, 0, 0);
+            shrink_products<T, NR>(x, v, acc);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // read before the next step's writes
     }
@@ -423,10 +462,7 @@ __global__ __launch_bounds__(64 * W) void coli_lora_shrink(LoraRows w, LoraSide<
             Raw8<T> v[NR];
 #pragma unroll
             for (int r = 0; r < NR; r++) v[r].load(vr + (size_t)16 * r * s.Np + c);
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-#pragma unroll
-                for (int r = 0; r < NR; r++) acc[r] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[j], v[r].get(j), acc[r], 0, 0, 0);
+            shrink_products<T, NR>(xv, v, acc);
         }
     }
     for (int r = 0; r < NR; r++) {
