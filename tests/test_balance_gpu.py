@@ -303,3 +303,24 @@ def test_refusals(session):
             assert not b.hip_balance_grad_dev(*(ok[:k] + (bad,) + ok[k + 1:])), (k, bad)
         assert not b.hip_balance_grad_dev(0, p, None, None, 2, 4, 8, 0, p, p, p, p)
         assert not b.hip_moe_last_balance_dev(None, None, None, 1, p, p, p)
+
+
+@pytest.mark.parametrize("n", [1023, 1024, 5000])
+@pytest.mark.parametrize("mode", [0, 3])
+def test_many_sequences(session, mode, n):
+    """Offsets held in LDS up to 1023 sequences, read from memory beyond."""
+    rng = np.random.default_rng(n + mode)
+    T, E, K = 6001, 20, 2
+    z, idx = routed(rng, T, E, K)
+    off = np.concatenate(([3], np.sort(rng.integers(3, T - 4, n - 1)), [T - 4])).astype(np.int32)
+    check(session, z, idx, None, (rng.random(T) < 0.9).astype(np.uint8), off, mode, n)
+
+
+@pytest.mark.parametrize("E,off", [(130, [0, 2900, 3000]), (130, [7, 900, 2990]), (1000, [0, 1, 3000])])
+def test_long_sequences_joined_by_columns(session, E, off):
+    """Sequences of so many rows that the join takes 64 columns a workgroup; the
+    last to arrive adds the pieces of the loss, also on a second call."""
+    rng = np.random.default_rng(E + off[1])
+    z, idx = routed(rng, 3000, E, 4)
+    for mode in (0, 1):
+        check(session, z, idx, None, None, np.asarray(off, np.int32), mode)

@@ -225,3 +225,12 @@ def test_refusals(session):
             assert b.hip_gemm_t_dev(h, q, q + 128, 1)           # next to it
     finally:
         session.free(h)
+
+
+@pytest.mark.parametrize("kind", ["i4h", "i4f", "fp4"])
+@pytest.mark.parametrize("O", [2050, 4100, 9001, 16500])
+def test_built_rows_of_many_columns(session, monkeypatch, kind, O):
+    """Rows of dy that the build holds in two, four or eight slots a thread, and
+    beyond 16384 columns reads a second time."""
+    monkeypatch.setenv("COLI_HIP_GEMM_T", "many")
+    test_matches_dense(session, kind, O, 70, 3)

@@ -402,3 +402,20 @@ def test_fault_injection(session, monkeypatch):
         monkeypatch.delenv("COLI_GPU_FAIL_AFTER")
         assert (d.down(py, (4, 32)) == 7.0).all()
         c.check_forward()
+
+
+HIGH_RANK = [  # bf16 factors split beside four rank tiles, eight waves a workgroup; rows of more than 2048 columns
+    ("i4h", 300, 2333, 130, 4, 64, 2, "mixed"),
+    ("fp4", 260, 2304, 120, 3, 70, 2, "runs"),
+    ("i4h", 2051, 330, 100, 3, 64, 2, "mixed"),
+    ("fp4", 4100, 260, 70, 2, 70, 1, "mixed"),
+]
+
+
+@pytest.mark.parametrize("shape", HIGH_RANK, ids=lambda s: "-".join(map(str, s)))
+def test_high_ranks_of_many_rows(session, monkeypatch, shape):
+    with Case(session, 400 + HIGH_RANK.index(shape), *shape) as c:
+        c.check_forward()
+        c.check_grads()
+        monkeypatch.setenv("COLI_HIP_GEMM_T", "many")   # (the sort builds dy's operands)
+        c.check_grads()
