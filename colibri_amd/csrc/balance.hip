@@ -35,8 +35,8 @@
 
 struct BalanceArgs {
     const float *z;            // [nch][T][E]: logits, or column-chunk partials added in chunk order
-    size_t chstride;
     int nch;
+    const int *state;          // null, or a MoE layer's state, which holds T and z
     const int *idx, *keff;     // [T][K], [T] or null
     const uint8_t *mask;       // [T] or null
     const int *off;            // [n + 1] or null: one sequence of all rows
@@ -92,6 +92,13 @@ template <int L> __device__ __forceinline__ int bal_sumi(int v) {
     return v;
 }
 
+// T and z of the layer's last forward (0 rows: none has run).
+__device__ __forceinline__ void bal_last(BalanceArgs &a) {
+    if (!a.state) return;
+    a.T = a.state[4];
+    a.z = *(const float *const *)(a.state + 6);
+}
+
 // Columns that every E taking this form has (nv_of): its blocks up to there are whole.
 template <int L, int NV> constexpr int bal_whole() {
     return L == 16 ? (NV == 1 ? 0 : 32 * NV) : L == 32 ? (NV == 3 ? 256 : 384) : 512;
@@ -128,7 +135,7 @@ __device__ __forceinline__ void bal_load(const BalanceArgs &a, int row, int l, f
     for (int ch = 1; ch < a.nch; ch++)
 #pragma unroll
         for (int i = 0; i < NV; i++) {
-            const floatx4 t = block(zr + (size_t)ch * a.chstride, i);
+            const floatx4 t = block(zr + (size_t)ch * a.T * a.E, i);
 #pragma unroll
             for (int k = 0; k < 4; k++) v[4 * i + k] += t[k];
         }
@@ -235,10 +242,11 @@ __global__ __launch_bounds__(SINGLE ? 1024 : 256, 4) void coli_balance_rows(Bala
     __shared__ int seg_n[2], s_off[COLI_BAL_OFF];
     __shared__ float wsum[W];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l = lane % L, g = lane / L;
+    bal_last(a);
     const int b = blockIdx.x, r0 = b * a.R, r1 = min(a.T, r0 + a.R);
     float v[4 * NV];
     int have = 0;   // the step whose rows v holds
-    bal_load<L, NV, ROW>(a, min(r0 + RW * wave + g, r1 - 1), l, v);
+    if (r0 < r1) bal_load<L, NV, ROW>(a, min(r0 + RW * wave + g, r1 - 1), l, v);
     if constexpr (SINGLE) {
         for (int e = tid; e < a.n * a.E; e += NT) a.counts[e] = 0;
         for (int i = tid; i < a.n; i += NT) {
@@ -246,6 +254,7 @@ __global__ __launch_bounds__(SINGLE ? 1024 : 256, 4) void coli_balance_rows(Bala
             a.rows[i] = 0;
         }
     }
+    if (r0 >= r1) return;   // (fewer rows than the launch allows for)
     int i = bal_first(a, r0, s_off);
     const BalOff off = {s_off, a.off, a.n, a.T};
     if (!a.off || SINGLE) __syncthreads();
@@ -352,6 +361,7 @@ __global__ __launch_bounds__(1024) void coli_balance_join(BalanceArgs a) {
     __shared__ int sn[G][2];
     __shared__ float wsum[16];
     const int i = blockIdx.x, eb = blockIdx.y, neb = gridDim.y, tid = threadIdx.x, l = tid % L, g = tid / L;
+    bal_last(a);
     const BalOff off = {nullptr, a.off, COLI_BAL_OFF, a.T};
     const int lo = off.get(i), hi = off.get(i + 1);
     const int b0 = lo / a.R, b1 = hi > lo ? (hi - 1) / a.R : b0 - 1;
@@ -518,14 +528,14 @@ static bool balance_shape_ok(int n, int T, int E, int mode) {
            mode <= 3;
 }
 
-int run_balance(DevCtx *ctx, const float *z, int nch, size_t chstride, const int *idx, const int *keff,
-                const uint8_t *mask, const int *off, int n, int T, int E, int K, int mode, float *loss, int *counts,
-                int *rows) {
+int run_balance(DevCtx *ctx, const float *z, int nch, const int *idx, const int *keff, const uint8_t *mask,
+                const int *off, int n, int T, int E, int K, int mode, float *loss, int *counts, int *rows,
+                const BalanceLast *last) {
     if (!balance_shape_ok(n, T, E, mode) || K < 1 || K > 64 || K > E) return 0;
     BalanceArgs a = {};
     a.z = z;
     a.nch = nch;
-    a.chstride = chstride;
+    a.state = last ? last->state : nullptr;
     a.idx = idx;
     a.keff = keff;
     a.mask = mask;
@@ -541,17 +551,18 @@ int run_balance(DevCtx *ctx, const float *z, int nch, size_t chstride, const int
     forget_emitted(ctx, counts, (size_t)n * E * sizeof(int));
     forget_emitted(ctx, rows, (size_t)n * sizeof(int));
     hipStream_t st = ctx->stream;
+    const int most = last ? last->max_rows : T;   // rows that the launches must hold for
     // up to four steps of one workgroup: one launch, loss included
     if (T <= (E <= 256 ? 256 : E <= 512 ? 128 : 64) && n <= 64) {
-        a.R = T;
+        a.R = most;
 #define COLI_BAL_ONE(L, NV, M, ROW) hipLaunchKernelGGL((coli_balance_rows<L, NV, M, ROW, true>), dim3(1), dim3(1024), 0, st, a)
         COLI_BAL_CALL(mode, COLI_BAL_ONE)
 #undef COLI_BAL_ONE
         return hip_check(hipGetLastError(), "balance");
     }
     // 16 rows a step of a workgroup; about 1024 workgroups once there are rows for them
-    a.R = std::max(16, (T + 1023) / 1024 + 15 & ~15);
-    const int nb = (T + a.R - 1) / a.R;
+    a.R = std::max(16, (most + 1023) / 1024 + 15 & ~15);
+    const int nb = (most + a.R - 1) / a.R;
     const size_t slots = (size_t)nb + n;
     a.Ep = (E + 63) / 64 * 64;
     // slots of a sequence: few, one workgroup adds all its columns; many, one for each 64
@@ -589,7 +600,7 @@ extern "C" int coli_hip_balance_dev(int device, const float *logits, const int *
     if (!logits || !idx || !loss || !counts || !rows || (!offsets && n != 1)) return 0;
     DevCtx *ctx = ctx_of(device);
     if (!bind_ctx(ctx)) return 0;
-    return run_balance(ctx, logits, 1, 0, idx, keff, mask, offsets, n, T, E, K, route_mode, loss, counts, rows);
+    return run_balance(ctx, logits, 1, idx, keff, mask, offsets, n, T, E, K, route_mode, loss, counts, rows);
 }
 
 extern "C" int coli_hip_balance_grad_dev(int device, const float *logits, const unsigned char *mask,

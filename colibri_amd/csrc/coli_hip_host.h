@@ -200,11 +200,17 @@ inline bool ranges_overlap(const void *a, size_t na, const void *b, size_t nb) {
     return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
 }
 int build_t_scales(DevCtx *ctx, ColiCudaTensor *t, bool update_only);
-// Counts and balance loss over router logits given as nch column-chunk
-// partials, chstride floats apart (balance.hip).
-int run_balance(DevCtx *ctx, const float *z, int nch, size_t chstride, const int *idx, const int *keff,
-                const uint8_t *mask, const int *off, int n, int T, int E, int K, int mode, float *loss, int *counts,
-                int *rows);
+// Counts and balance loss (balance.hip) over logits [T][E]; with `last`, over the
+// nch column-chunk partials [T][E] of the forward of a MoE layer that ran last
+// before the launch, whose rows and partials are in its state on the device (T is then
+// a guess of the rows, at most max_rows).
+struct BalanceLast {
+    const int *state;
+    int max_rows;
+};
+int run_balance(DevCtx *ctx, const float *z, int nch, const int *idx, const int *keff, const uint8_t *mask,
+                const int *off, int n, int T, int E, int K, int mode, float *loss, int *counts, int *rows,
+                const BalanceLast *last = nullptr);
 
 // Expert path runner (expert.hip): one shared routine behind expert_group,
 // issue, expert_mlp, resident_issue and the MoE layer.

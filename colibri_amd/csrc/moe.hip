@@ -42,18 +42,30 @@ struct ColiHipMoe {
     int kind;                 // storage kind shared by every expert matrix
     std::vector<const ColiCudaTensor *> mats;   // every expert matrix (e8_fold is read per forward)
     int S_cap;
-    int S_last = 0;           // rows of the last forward
+    int S_last = 0;           // rows of the forward queued or captured last (0: it failed, or there was none)
     float *rw = nullptr, *rb = nullptr;
     ColiProb *tab = nullptr;  // [E (+1 shared)][2]: dual template, down template
-    // per-forward state (device)
+    // what the last forward leaves of its routing (device), at one address for
+    // the layer's life: coli_hip_moe_last_* find there what ran last, whether
+    // a call queued it or a graph's replay
+    int *idx = nullptr, *keff = nullptr, *uniq = nullptr;
+    int *state = nullptr;     // [COLI_MOE_STATE], see moe_put_state
+    // per-forward buffers (device)
     float *logits = nullptr, *wsel = nullptr, *h = nullptr, *y = nullptr;
-    int *idx = nullptr, *keff = nullptr;
-    int *state = nullptr;     // [0] problems, [1] packed rows, [2] union size, [3] GEMM row tiles
-    int *uniq = nullptr, *xrows = nullptr, *slotrow = nullptr, *mt = nullptr;
+    int *xrows = nullptr, *slotrow = nullptr, *mt = nullptr;
     ColiProb *pdual = nullptr, *pdown = nullptr;
     int *route_cnt = nullptr;   // arrival counter of coli_moe_route (zero between launches)
     bool route_cnt_dirty = false;   // a forward failed part-way: clear the counter before the next
 };
+
+// A forward's state: [0] problems, [1] packed rows, [2] union size, [3] GEMM row
+// tiles, [4] rows, [6..7] where its router partials lie.
+#define COLI_MOE_STATE 8
+__device__ __forceinline__ void moe_put_state(int *state, int np, int rows, int nu, int tiles, int S, const float *logits) {
+    *(int4 *)state = make_int4(np, rows, nu, tiles);
+    state[4] = S;
+    *(const float **)(state + 6) = logits;
+}
 
 // ---------------------------------------------------------------------------
 // union + descriptor build, one block (decode and small batches;
@@ -73,7 +85,8 @@ __device__ __forceinline__ void moe_union_body(const int *idx, const int *keff, 
                                                const ColiProb *__restrict__ tab, ColiProb *__restrict__ pdual,
                                                ColiProb *__restrict__ pdown, int *__restrict__ uniq,
                                                int *__restrict__ xrows, int *__restrict__ slotrow,
-                                               int *__restrict__ mt, int *__restrict__ state, int *sm) {
+                                               int *__restrict__ mt, int *__restrict__ state, const float *logits,
+                                               int *sm) {
     constexpr int tile = COLI_GM_TILE;   // (decode and small batches: at most 64 rows an expert, one tile either way)
     // first [E] | cnt [E] | cur [E] | rank [E] | order [E + 1] | off [E + 2] | toff [E + 2]
     int *first = sm, *cnt = first + E, *cur = cnt + E, *rank = cur + E, *order = rank + E, *off = order + E + 1,
@@ -202,12 +215,7 @@ __device__ __forceinline__ void moe_union_body(const int *idx, const int *keff, 
         pdown[j] = dn;
         for (int q = 0; q * tile < c; q++) mt[toff[j] + q] = j << 16 | q;
     }
-    if (threadIdx.x == 0) {
-        state[0] = np;
-        state[1] = off[np];
-        state[2] = nu;
-        state[3] = toff[np];
-    }
+    if (threadIdx.x == 0) moe_put_state(state, np, off[np], nu, toff[np], S, logits);
 }
 
 // ints of the selection / union work area (LDS) of E experts; the decode
@@ -222,8 +230,8 @@ __device__ __forceinline__ void moe_union_wave(const int *idx, const int *keff, 
                                                const ColiProb *__restrict__ tab, ColiProb *__restrict__ pdual,
                                                ColiProb *__restrict__ pdown, int *__restrict__ uniq,
                                                int *__restrict__ xrows, int *__restrict__ slotrow,
-                                               int *__restrict__ mt, int *__restrict__ state, int lane,
-                                               int shared_row = -1) {
+                                               int *__restrict__ mt, int *__restrict__ state, const float *logits,
+                                               int lane, int shared_row = -1) {
     const int n = S * K;
     const int t = lane / K, kk = lane - t * K;
     int e = -1;
@@ -288,12 +296,7 @@ __device__ __forceinline__ void moe_union_wave(const int *idx, const int *keff, 
             mt[nu] = nu << 16;
         }
     }
-    if (lane == 0) {
-        state[0] = np;
-        state[1] = rows_routed + (has_shared ? S : 0);
-        state[2] = nu;
-        state[3] = np;
-    }
+    if (lane == 0) moe_put_state(state, np, rows_routed + (has_shared ? S : 0), nu, np, S, logits);
 }
 
 // The union of up to COLI_MOE_MAX_SEL selections (prefill) by one 1024-thread
@@ -308,7 +311,8 @@ __global__ __launch_bounds__(1024) void coli_moe_union(const int *__restrict__ i
                                                        const ColiProb *__restrict__ tab, ColiProb *__restrict__ pdual,
                                                        ColiProb *__restrict__ pdown, int *__restrict__ uniq,
                                                        int *__restrict__ xrows, int *__restrict__ slotrow,
-                                                       int *__restrict__ mt, int *__restrict__ state, int tile) {
+                                                       int *__restrict__ mt, int *__restrict__ state,
+                                                       const float *logits, int tile) {
     // first [E, padded to 4] | cnt [E] | off [E] by expert | order [E]
     extern __shared__ __attribute__((aligned(16))) int sm_union[];
     const int E4 = (E + 3) & ~3;
@@ -418,12 +422,7 @@ __global__ __launch_bounds__(1024) void coli_moe_union(const int *__restrict__ i
             xrows[row] = i / K;
             slotrow[i] = row;
         }
-    if (tid == 0) {
-        state[0] = np;
-        state[1] = rows + (has_shared ? S : 0);
-        state[2] = nu;
-        state[3] = tiles + sh_tiles;
-    }
+    if (tid == 0) moe_put_state(state, np, rows + (has_shared ? S : 0), nu, tiles + sh_tiles, S, logits);
 }
 
 // ---------------------------------------------------------------------------
@@ -499,10 +498,10 @@ __global__ __launch_bounds__(256) void coli_moe_select_union(const float *__rest
     __syncthreads();
     if (S * K <= 64) {   // decode: the one-wave union
         if (wave == 0) moe_union_wave(sidx, skeff, S, K, E, has_shared, small ? stab : tab, pdual, pdown, uniq, xrows,
-                                      slotrow, mt, state, lane);
+                                      slotrow, mt, state, part, lane);
         return;
     }
-    moe_union_body(sidx, skeff, S, K, E, has_shared, tab, pdual, pdown, uniq, xrows, slotrow, mt, state, work);
+    moe_union_body(sidx, skeff, S, K, E, has_shared, tab, pdual, pdown, uniq, xrows, slotrow, mt, state, part, work);
 }
 
 // ---------------------------------------------------------------------------
@@ -553,10 +552,10 @@ __global__ __launch_bounds__(256) void coli_moe_route(const float *__restrict__ 
     __syncthreads();
     if (S * K <= 64) {
         if (wave == 0) moe_union_wave(sidx, skeff, S, K, E, has_shared, stab, pdual, pdown, uniq, xrows, slotrow, mt,
-                                      state, lane);
+                                      state, part, lane);
         return;
     }
-    moe_union_body(sidx, skeff, S, K, E, has_shared, tab, pdual, pdown, uniq, xrows, slotrow, mt, state, work);
+    moe_union_body(sidx, skeff, S, K, E, has_shared, tab, pdual, pdown, uniq, xrows, slotrow, mt, state, part, work);
 }
 
 // ---------------------------------------------------------------------------
@@ -1086,7 +1085,8 @@ __global__ __launch_bounds__(64 * W) void coli_moe_select_union_sh(
                               (float *)work, stage, cand, nval, selb, sidx, skeff, true, wave, lane);
     __syncthreads();
     if (wave == 0)
-        moe_union_wave(sidx, skeff, 1, K, E, 1, stab, pdual, pdown, uniq, xrows, slotrow, mt, state, lane, K);
+        moe_union_wave(sidx, skeff, 1, K, E, 1, stab, pdual, pdown, uniq, xrows, slotrow, mt, state, part, lane,
+                       K);
 }
 
 // ---------------------------------------------------------------------------
@@ -1127,7 +1127,7 @@ __global__ __launch_bounds__(64 * W) void coli_moe_route_dual1(
                                     psel, 0, lane, sidx, skeff, first);
     __syncthreads();
     if (first && wave == 0)
-        moe_union_wave(sidx, skeff, 1, K, E, has_shared, stab, pdual, pdown, uniq, xrows, slotrow, mt, state, lane);
+        moe_union_wave(sidx, skeff, 1, K, E, has_shared, stab, pdual, pdown, uniq, xrows, slotrow, mt, state, part, lane);
     const int ke = skeff[0];
     int e;
     if (p < ke) e = sidx[p];
@@ -1227,7 +1227,12 @@ extern "C" int coli_hip_moe_create(ColiHipMoe **out, int device, const ColiHipMo
              hip_check(hipMemcpy(m->tab, tab.data(), tab.size() * sizeof(ColiProb), hipMemcpyHostToDevice),
                     "expert table upload") &&
              hip_check(hipMalloc((void **)&m->route_cnt, sizeof(int)), "routing counter") &&
-             hip_check(hipMemset(m->route_cnt, 0, sizeof(int)), "routing counter clear");
+             hip_check(hipMemset(m->route_cnt, 0, sizeof(int)), "routing counter clear") &&
+             hip_check(hipMalloc((void **)&m->idx, (size_t)std::min(COLI_MOE_MAX_ROWS * c.K, COLI_MOE_MAX_SEL) * 4), "selections") &&
+             hip_check(hipMalloc((void **)&m->keff, COLI_MOE_MAX_ROWS * 4), "selections") &&
+             hip_check(hipMalloc((void **)&m->uniq, (size_t)c.E * 4), "union") &&
+             hip_check(hipMalloc((void **)&m->state, COLI_MOE_STATE * sizeof(int)), "union") &&
+             hip_check(coli_launch_zero_i32(m->state, COLI_MOE_STATE, ctx->stream), "union clear");
     if (ok && router_bias)
         ok = hip_check(hipMalloc((void **)&m->rb, (size_t)c.E * sizeof(float)), "router bias") &&
              hip_check(hipMemcpy(m->rb, router_bias, (size_t)c.E * sizeof(float), hipMemcpyHostToDevice),
@@ -1267,8 +1272,7 @@ static int moe_reserve(DevCtx *ctx, ColiHipMoe *m, int S) {
     if (!hip_check(hipStreamSynchronize(ctx->stream), "moe reserve sync")) return 0;
     const ColiHipMoeConfig &c = m->cfg;
     const int P = moe_problems(c, S), rows = moe_rows(c, S);
-    void **bufs[] = {(void **)&m->logits, (void **)&m->wsel, (void **)&m->h, (void **)&m->y, (void **)&m->idx,
-                     (void **)&m->keff, (void **)&m->state, (void **)&m->uniq, (void **)&m->xrows,
+    void **bufs[] = {(void **)&m->logits, (void **)&m->wsel, (void **)&m->h, (void **)&m->y, (void **)&m->xrows,
                      (void **)&m->slotrow, (void **)&m->mt, (void **)&m->pdual, (void **)&m->pdown};
     for (void **b : bufs)
         if (*b) {
@@ -1276,10 +1280,10 @@ static int moe_reserve(DevCtx *ctx, ColiHipMoe *m, int S) {
             *b = nullptr;
         }
     const size_t sizes[] = {(size_t)coli_router_chunks(c.D) * S * c.E * 4, (size_t)S * c.K * 4,
-                            (size_t)rows * c.I * 4, (size_t)rows * c.D * 4, (size_t)S * c.K * 4, (size_t)S * 4, 16,
-                            (size_t)c.E * 4, (size_t)rows * 4, (size_t)S * c.K * 4, (size_t)moe_tiles(c, S, COLI_GM_ROWS) * 4,
-                            (size_t)P * sizeof(ColiProb), (size_t)P * sizeof(ColiProb)};
-    for (int i = 0; i < 13; i++)
+                            (size_t)rows * c.I * 4, (size_t)rows * c.D * 4, (size_t)rows * 4, (size_t)S * c.K * 4,
+                            (size_t)moe_tiles(c, S, COLI_GM_ROWS) * 4, (size_t)P * sizeof(ColiProb),
+                            (size_t)P * sizeof(ColiProb)};
+    for (int i = 0; i < 9; i++)
         if (!hip_check(hipMalloc(bufs[i], sizes[i]), "moe buffers")) return 0;
     m->S_cap = S;
     return 1;
@@ -1560,7 +1564,7 @@ static int moe_forward_impl(ColiHipMoe *m, DevCtx *ctx, const float *x_dev, floa
         // 4. union
         const size_t ush = (size_t)(4 * c.E + 3) * sizeof(int);
         hipLaunchKernelGGL(coli_moe_union, dim3(1), dim3(1024), ush, st, m->idx, m->keff, S, c.K, c.E, c.has_shared,
-                           m->tab, m->pdual, m->pdown, m->uniq, m->xrows, m->slotrow, m->mt, m->state, tile);
+                           m->tab, m->pdual, m->pdown, m->uniq, m->xrows, m->slotrow, m->mt, m->state, m->logits, tile);
         if (!hip_check(hipGetLastError(), "moe union")) return 0;
     }
     // 5. gate/up + SwiGLU over the union, 6. hidden fragments, 7. down
@@ -1658,7 +1662,7 @@ extern "C" int coli_hip_moe_forward(ColiHipMoe *m, const float *x, float *out, i
 }
 
 extern "C" int coli_hip_moe_last_union(ColiHipMoe *m, int *nu, int *uniq) {
-    if (!m || !nu || !m->state) return 0;
+    if (!m || !nu || !m->S_cap) return 0;
     DevCtx *ctx = ctx_of(m->device);
     if (!bind_ctx(ctx) || !hip_check(hipStreamSynchronize(ctx->stream), "union sync")) return 0;
     int st[3];
@@ -1670,8 +1674,10 @@ extern "C" int coli_hip_moe_last_union(ColiHipMoe *m, int *nu, int *uniq) {
     return 1;
 }
 
-// The router's logits, indices and counts of live selections are still where
-// the last forward left them.
+// The router's partials and selections are still where the last forward left
+// them. Which one that was only the device knows (a graph's replay passes no
+// host code), so the kernels take its rows and partials from `state`; S_last
+// picks their form.
 extern "C" int coli_hip_moe_last_balance_dev(ColiHipMoe *m, const unsigned char *mask, const int *offsets, int n,
                                              float *loss, int *counts, int *rows) {
     if (fault_injected()) return 0;
@@ -1679,6 +1685,7 @@ extern "C" int coli_hip_moe_last_balance_dev(ColiHipMoe *m, const unsigned char 
     DevCtx *ctx = ctx_of(m->device);
     if (!bind_ctx(ctx)) return 0;
     const ColiHipMoeConfig &c = m->cfg;
-    return run_balance(ctx, m->logits, coli_router_chunks(c.D), (size_t)m->S_last * c.E, m->idx, m->keff, mask, offsets,
-                       n, m->S_last, c.E, c.K, c.route_mode, loss, counts, rows);
+    const BalanceLast last = {m->state, std::min(COLI_MOE_MAX_ROWS, COLI_MOE_MAX_SEL / c.K)};
+    return run_balance(ctx, nullptr, coli_router_chunks(c.D), m->idx, m->keff, mask, offsets, n, m->S_last, c.E, c.K,
+                       c.route_mode, loss, counts, rows, &last);
 }

@@ -187,7 +187,10 @@ int coli_hip_balance_grad_dev(int device, const float *logits, const unsigned ch
                               int T, int E, int route_mode, const float *dloss, const int *counts, const int *rows,
                               float *dlogits);
 /* coli_hip_balance_dev over the last forward of a MoE layer (its rows, its own
- * router logits, selections and route mode). Refused before the first one. */
+ * router logits, selections and route mode): the one that ran last on the
+ * stream before this call, queued by a call or by a graph's replay. mask and
+ * offsets are for that forward's rows. Refused before the first forward and
+ * after one that failed. */
 int coli_hip_moe_last_balance_dev(ColiHipMoe *moe, const unsigned char *mask, const int *offsets, int n, float *loss,
                                   int *counts, int *rows);
 

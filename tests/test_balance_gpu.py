@@ -324,3 +324,91 @@ def test_long_sequences_joined_by_columns(session, E, off):
     z, idx = routed(rng, 3000, E, 4)
     for mode in (0, 1):
         check(session, z, idx, None, None, np.asarray(off, np.int32), mode)
+
+
+class LayerOf:
+    """A MoE layer of `E` random experts with its router, and the routing of S rows by the host forward."""
+
+    def __init__(self, session, mode, E, K, D, rows, seed):
+        self.session, self.b, self.mode, self.E, self.K, self.D = session, session.b, mode, E, K, D
+        rng = np.random.default_rng(seed)
+        layer = Layer(rng, 4, D, 128, E, shared=False)
+        self.x, self.W, bias = make_router_inputs(rng, rows, D, E, K, mode, bias=mode != 0)
+        self.hs = layer.upload(session)
+        self.m = C.c_void_p()
+        (g, _a), (u, _b), (w, _c) = (tensor_array([t[k] for t in self.hs[:E]]) for k in range(3))
+        cfg = ColiHipMoeConfig(D, 128, E, K, mode, 1, 0.0, 1.0, 0)
+        assert self.b.hip_moe_create(C.byref(self.m), 0, C.byref(cfg), f32p(self.W), None if bias is None else f32p(bias),
+                                     g, u, w, None, None, None)
+        self.d = Bufs(self.b)
+        self.px, self.py = self.d.up(self.x), self.d.up(np.zeros_like(self.x))
+        self.pl, self.pc, self.pr = self.d.up(np.zeros(1, np.float32)), self.d.up(np.zeros(E, np.int32)), self.d.up(np.zeros(1, np.int32))
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.b.hip_moe_free(self.m)
+        for t in self.hs:
+            for h in t:
+                self.session.free(h)
+        self.d.__exit__()
+
+    def forward(self, S, at=0):
+        """S rows from row `at` on."""
+        assert self.b.hip_moe_forward_dev(self.m, self.px + 4 * at * self.D, self.py, S)
+
+    def balance(self):
+        return self.b.hip_moe_last_balance_dev(self.m, None, None, 1, self.pl, self.pc, self.pr)
+
+    def routing(self, S, at=0):
+        out, idx = np.zeros((S, self.D), np.float32), np.zeros((S, self.K), np.int32)
+        wt, keff = np.zeros((S, self.K), np.float32), np.zeros(S, np.int32)
+        x = np.ascontiguousarray(self.x[at: at + S])
+        assert self.b.hip_moe_forward(self.m, f32p(x), f32p(out), S, i32p(idx), f32p(wt), i32p(keff))
+        return idx, keff
+
+    def check(self, S, routing, at=0):
+        """What the last call of balance() left is that of these S rows."""
+        loss, counts, rows = self.d.down(self.pl, (1,)), self.d.down(self.pc, (1, self.E), np.int32), self.d.down(self.pr, (1,), np.int32)
+        x = self.x[at: at + S].astype(np.float64)
+        z = x @ self.W.astype(np.float64).T
+        rl, rc, rr, _, _ = balance(z, routing[0], routing[1], None, None, self.E, self.mode)
+        assert np.array_equal(rows, rr) and np.array_equal(counts, rc), (S, rows, rr)
+        dz = ((np.abs(x) @ np.abs(self.W).astype(np.float64).T).max() * (2 * self.D + 16)) * 2.0 ** -24
+        assert (np.abs(loss - rl) <= (p_tol(z) + (S / 16 + 96) * 2.0 ** -24 + 2 * dz) * rl).all()
+
+
+# one-token forms (gate/up that selects for itself; the shared overlap is not
+# taken without a shared expert), the one-launch routing, the selection by four
+# waves and the separate union
+@pytest.mark.parametrize("mode,E,K,D,few", [(0, 64, 8, 2048, 1), (0, 64, 8, 256, 5), (2, 96, 8, 1536, 9), (3, 40, 4, 384, 70)])
+def test_last_forward_after_replays(session, mode, E, K, D, few):
+    """The last forward is the last one that ran: a replayed graph's, also where
+    another number of rows was queued or captured after the graph was."""
+    with LayerOf(session, mode, E, K, D, 300, E + few) as o:
+        ref = {S: o.routing(S) for S in (300, few)}
+        o.forward(300)
+        assert o.balance()                          # (workspaces)
+        graphs = {}
+        for S in (few, 300):
+            with hiprt.Graph(o.b.hip_stream(0)) as graphs[S]:
+                o.forward(S)
+        with hiprt.Graph(o.b.hip_stream(0)) as alone:
+            assert o.balance()
+        for rep in range(2):
+            for S in (few, 300):
+                other = few + 300 - S
+                graphs[S].launch()                  # (300 rows captured last)
+                assert o.balance()
+                o.check(S, ref[S])
+                o.forward(other)
+                graphs[S].launch()                  # (the other number queued last)
+                assert o.balance()
+                o.check(S, ref[S])
+                o.b.hip_fill_random_u8(0, o.pc, 4 * E, rep + 1)
+                alone.launch()
+                o.check(S, ref[S])
+                o.forward(other)
+                alone.launch()
+                o.check(other, ref[other])
