@@ -33,7 +33,8 @@
 #define COLI_PIECE_BYTES ((size_t)512 << 10)
 #define COLI_PIECES 32
 
-// Outgrown workspaces a device keeps (each at least doubles its buffer).
+// Outgrown workspaces a device keeps (each growth at least doubles its buffer,
+// unless memory is short).
 #define COLI_OUTGROWN 1024
 
 struct DevBuf {
@@ -89,9 +90,11 @@ struct DevCtx {
     FragSet frag[4];                   // 0/1: inputs (int4 / fp4 order), 2/3: hidden rows
     int dense_set[2] = {0, 1};         // set the next coli_hip_gemm_run_dev reads, per order (gemm_prep)
     DevBuf pipe[COLI_PIPE_SLOTS];
+    bool stream_out = false;           // the caller has the stream and may capture it
+    bool captured = false;             // some call's launches have gone into a graph
     // workspaces of the adapter, input-gradient and balance entry points; these,
-    // the fragments, partial, split_cnt and sums grow by reserve_kept: outgrown
-    // ones live until shutdown
+    // the fragments, partial, split_cnt and sums grow by reserve_kept: where a
+    // graph may hold them, outgrown ones live until shutdown
     DevBuf lora_h, lora_list, gt, bal, bal_cnt;
     void *outgrown[COLI_OUTGROWN] = {};
     int n_outgrown = 0;

@@ -1,0 +1,67 @@
+"""Device memory that the shared workspaces hold, measured in a process of its
+own (what other tests have captured or allocated does not count there)."""
+import json
+import os
+import subprocess
+import sys
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+CHILD = """
+import ctypes as C, json, sys
+import numpy as np
+sys.path[:0] = [{root!r}, {root!r} + "/tests"]
+from colibri_amd import hiprt
+from colibri_amd.backend import Session
+from quant_util import rand_mxfp4
+
+I, O, ROWS = 16384, 64, 4000
+q4, e8 = rand_mxfp4(np.random.default_rng(0), O, I)
+
+
+def held(sizes, capture):
+    s = Session(0)
+    b = s.b
+    free, total = C.c_size_t(), C.c_size_t()
+    h = s.upload_mxfp4(q4, e8, I, O)
+    x, y = b.cuda_pipe_alloc(0, ROWS * I * 4), b.cuda_pipe_alloc(0, ROWS * O * 4)
+
+    def left():
+        assert b.cuda_pipe_sync(0) and b.cuda_mem_info(0, C.byref(free), C.byref(total))
+        return free.value
+
+    assert b.cuda_pipe_gemm(h, y, x, 1)
+    if capture:
+        with hiprt.Graph(b.hip_stream(0)):
+            assert b.cuda_pipe_gemm(h, y, x, 1)
+    before = left()
+    for S in sizes:
+        assert b.cuda_pipe_gemm(h, y, x, S)
+    out = before - left()
+    for p in (x, y):
+        b.cuda_pipe_free(0, p)
+    s.free(h)
+    s.close()
+    return out
+
+
+slowly = list(range(500, ROWS, 25)) + [ROWS]
+print(json.dumps([held([ROWS], False), held(slowly, False), held(slowly, True)]))
+"""
+
+
+def test_growing_calls_hold_what_the_largest_needs():
+    """A prefill that grows by 25 rows at a time: workspaces a quarter larger than
+    the largest call's, as one call of that size takes (the outgrown ones are
+    freed). Where a graph has been captured they are kept, and so doubled at each
+    growth: less than four times the largest call's."""
+    r = subprocess.run([sys.executable, "-c", CHILD.format(root=ROOT)], capture_output=True, text=True, timeout=110)
+    assert r.returncode == 0, r.stderr[-2000:]
+    once, grown, kept = json.loads(r.stdout.strip().splitlines()[-1])
+    rows = 4000 * 16384 * 4     # fp16 hi + lo
+    assert rows <= once <= 1.25 * rows + (96 << 20)
+    assert grown <= 1.25 * rows + (96 << 20), (once, grown)
+    assert kept <= 4 * once, (once, kept)
