@@ -36,6 +36,11 @@
 #define COLI_MOE_MAX_ROWS 2048
 #define COLI_MOE_MAX_SEL 16384
 
+// Per-forward buffers, and how many outgrown ones a layer keeps (growths double
+// the rows, unless memory is short).
+#define COLI_MOE_BUFS 9
+#define COLI_MOE_OUTGROWN (64 * COLI_MOE_BUFS)
+
 struct ColiHipMoe {
     int device;
     ColiHipMoeConfig cfg;
@@ -54,6 +59,8 @@ struct ColiHipMoe {
     float *logits = nullptr, *wsel = nullptr, *h = nullptr, *y = nullptr;
     int *xrows = nullptr, *slotrow = nullptr, *mt = nullptr;
     ColiProb *pdual = nullptr, *pdown = nullptr;
+    void *outgrown[COLI_MOE_OUTGROWN] = {};   // per-forward buffers that a captured graph may hold
+    int n_outgrown = 0;
     int *route_cnt = nullptr;   // arrival counter of coli_moe_route (zero between launches)
     bool route_cnt_dirty = false;   // a forward failed part-way: clear the counter before the next
 };
@@ -1182,6 +1189,7 @@ extern "C" void coli_hip_moe_free(ColiHipMoe *m) {
                     m->uniq, m->xrows, m->slotrow, m->mt, m->pdual, m->pdown, m->route_cnt};
     for (void *p : bufs)
         if (p) (void)hipFree(p);
+    for (int i = 0; i < m->n_outgrown; i++) (void)hipFree(m->outgrown[i]);
     delete m;
 }
 
@@ -1266,27 +1274,47 @@ static int moe_tile_rows(const DevCtx *ctx, const ColiHipMoeConfig &c, int S) {
     return items * ((c.I + 127) / 128) <= 2 * cus ? COLI_GM_ROWS : COLI_GM_TILE;
 }
 
-// Per-forward buffers for up to S rows (allocated once per growth of S).
+// Per-forward buffers for up to S rows (allocated once per growth of S). Once
+// calls on the device have been captured a graph may hold them, so outgrown ones
+// stay until the layer is freed, and a growth doubles the rows; else they are
+// freed first.
 static int moe_reserve(DevCtx *ctx, ColiHipMoe *m, int S) {
     if (S <= m->S_cap) return 1;
-    if (!hip_check(hipStreamSynchronize(ctx->stream), "moe reserve sync")) return 0;
     const ColiHipMoeConfig &c = m->cfg;
-    const int P = moe_problems(c, S), rows = moe_rows(c, S);
-    void **bufs[] = {(void **)&m->logits, (void **)&m->wsel, (void **)&m->h, (void **)&m->y, (void **)&m->xrows,
-                     (void **)&m->slotrow, (void **)&m->mt, (void **)&m->pdual, (void **)&m->pdown};
-    for (void **b : bufs)
-        if (*b) {
+    constexpr int NB = COLI_MOE_BUFS;
+    void **bufs[NB] = {(void **)&m->logits, (void **)&m->wsel, (void **)&m->h, (void **)&m->y, (void **)&m->xrows,
+                       (void **)&m->slotrow, (void **)&m->mt, (void **)&m->pdual, (void **)&m->pdown};
+    const int had = m->S_cap;
+    const bool keep = had && ctx->captured;
+    if (keep && m->n_outgrown + NB > COLI_MOE_OUTGROWN) return 0;
+    if (had && !keep) {
+        if (!hip_check(hipStreamSynchronize(ctx->stream), "moe reserve sync")) return 0;
+        m->S_cap = 0;
+        for (void **b : bufs) {
             (void)hipFree(*b);
             *b = nullptr;
         }
-    const size_t sizes[] = {(size_t)coli_router_chunks(c.D) * S * c.E * 4, (size_t)S * c.K * 4,
-                            (size_t)rows * c.I * 4, (size_t)rows * c.D * 4, (size_t)rows * 4, (size_t)S * c.K * 4,
-                            (size_t)moe_tiles(c, S, COLI_GM_ROWS) * 4, (size_t)P * sizeof(ColiProb),
-                            (size_t)P * sizeof(ColiProb)};
-    for (int i = 0; i < 9; i++)
-        if (!hip_check(hipMalloc(bufs[i], sizes[i]), "moe buffers")) return 0;
-    m->S_cap = S;
-    return 1;
+    }
+    for (int rows : {std::max(S, keep ? std::min(2 * had, std::min(COLI_MOE_MAX_ROWS, COLI_MOE_MAX_SEL / c.K)) : 0), S}) {
+        const size_t R = moe_rows(c, rows), P = moe_problems(c, rows);
+        const size_t sizes[NB] = {(size_t)coli_router_chunks(c.D) * rows * c.E * 4, (size_t)rows * c.K * 4, R * c.I * 4,
+                                  R * c.D * 4, R * 4, (size_t)rows * c.K * 4,
+                                  (size_t)moe_tiles(c, rows, COLI_GM_ROWS) * 4, P * sizeof(ColiProb), P * sizeof(ColiProb)};
+        void *p[NB] = {};
+        int n = 0;
+        while (n < NB && hipMalloc(&p[n], sizes[n]) == hipSuccess) n++;
+        if (n == NB) {
+            for (int i = 0; i < NB; i++) {
+                if (keep) m->outgrown[m->n_outgrown++] = *bufs[i];
+                *bufs[i] = p[i];
+            }
+            m->S_cap = rows;
+            return 1;
+        }
+        (void)hipGetLastError();
+        while (n) (void)hipFree(p[--n]);
+    }
+    return hip_check(hipErrorOutOfMemory, "moe buffers");
 }
 
 // COLI_HIP_FUSED_ROUTE=0 runs the router, selection and union as three

@@ -102,7 +102,8 @@ void coli_hip_moe_free(ColiHipMoe *moe);
 /* Device-resident forward of S <= 2048 rows (decode, verification or
  * prefill; S * K <= 16384): x_dev [S, D] f32 -> out_dev [S, D] f32,
  * asynchronous on the backend stream (no host sync, no allocation after the
- * first call at a given S). Up to 32 rows the experts run the tiled GEMV,
+ * first call at a given S; a captured forward stays valid when later ones have
+ * more rows). Up to 32 rows the experts run the tiled GEMV,
  * beyond it the grouped GEMM. */
 int coli_hip_moe_forward_dev(ColiHipMoe *moe, const float *x_dev, float *out_dev, int S);
 

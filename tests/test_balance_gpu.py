@@ -412,3 +412,43 @@ def test_last_forward_after_replays(session, mode, E, K, D, few):
                 o.forward(other)
                 alone.launch()
                 o.check(other, ref[other])
+
+
+@pytest.mark.parametrize("mode,E,K,D,S", [(0, 64, 8, 2048, 1), (2, 96, 8, 384, 9), (1, 40, 4, 256, 70)])
+def test_graphs_outlive_larger_forwards(session, mode, E, K, D, S):
+    """A captured forward with its balance, and a balance captured alone, after
+    forwards of more rows have outgrown the layer's buffers; the union read back
+    is the replayed forward's."""
+    b = session.b
+    with LayerOf(session, mode, E, K, D, 300, E + S) as o:
+        small, large = o.routing(S), None
+
+        def outputs():
+            return [o.d.down(p, n, np.uint32) for p, n in ((o.py, (S, D)), (o.pl, (1,)), (o.pc, (E,)), (o.pr, (1,)))]
+
+        o.forward(S)
+        assert o.balance()
+        eager = outputs()
+        with hiprt.Graph(b.hip_stream(0)) as both:
+            o.forward(S)
+            assert o.balance()
+        with hiprt.Graph(b.hip_stream(0)) as alone:
+            assert o.balance()
+        nu, uniq = C.c_int(), np.zeros(E, np.int32)
+        for rep, rows in enumerate((S + 1, 130, 300)):   # (each needs larger buffers)
+            large = o.routing(rows)
+            alone.launch()
+            o.check(rows, large)
+            for p, n in ((o.py, S * D), (o.pl, 1), (o.pc, E), (o.pr, 1)):
+                assert b.hip_fill_random_u8(0, p, 4 * n, rep + 1)
+            both.launch()
+            for u, v in zip(outputs(), eager):
+                assert np.array_equal(u, v), rep
+            assert b.hip_moe_last_union(o.m, C.byref(nu), i32p(uniq))
+            seen = [e for t in range(S) for e in small[0][t, : small[1][t]]]
+            assert list(uniq[: nu.value]) == list(dict.fromkeys(seen))
+            alone.launch()
+            o.check(S, small)
+            o.forward(rows)
+            assert o.balance()
+            o.check(rows, large)
