@@ -544,7 +544,9 @@ extern "C" void coli_cuda_tensor_free(ColiCudaTensor *t) {
     std::free(t);
 }
 
-extern "C" size_t coli_cuda_tensor_bytes(const ColiCudaTensor *t) { return t ? t->w_bytes + t->sc_bytes : 0; }
+extern "C" size_t coli_cuda_tensor_bytes(const ColiCudaTensor *t) {
+    return t ? t->w_bytes + t->sc_bytes + t->sct_bytes : 0;
+}
 extern "C" int coli_cuda_tensor_device(const ColiCudaTensor *t) { return t ? t->device : -1; }
 extern "C" size_t coli_hip_tensor_stream_bytes(const ColiCudaTensor *t) { return t ? t->w_bytes + t->sc_bytes : 0; }
 extern "C" int coli_hip_tensor_kind(const ColiCudaTensor *t) { return t ? t->kind : -1; }

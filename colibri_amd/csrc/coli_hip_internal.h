@@ -48,6 +48,7 @@ struct ColiCudaTensor {
     void *sc_unit;               // fmt=2 int8-activation path: unit group scales (made on first use)
     void *sct;                   // input gradients: scales by column group (made on first use, see gemm_t.hip)
     int *sct_ge;                 // their column groups' exponents [4 nq], in the same allocation
+    size_t sct_bytes;            // of that allocation
     int e8_fold;                 // MXFP4: every e8m0 byte in [114, 140], so each e2m1 value times its
                                  // scale is a normal fp16 (the GEMM folds the scale into the operand)
 };

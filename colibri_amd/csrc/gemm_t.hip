@@ -537,6 +537,9 @@ int build_t_scales(DevCtx *ctx, ColiCudaTensor *t, bool update_only) {
         const size_t sb = (size_t)planes * t->nq * 4 * noct * 16;
         if (!hip_check(hipMalloc(&t->sct, sb + (size_t)t->nq * 4 * sizeof(int)), "transposed scales")) return 0;
         t->sct_ge = (int *)((uint8_t *)t->sct + sb);
+        t->sct_bytes = sb + (size_t)t->nq * 4 * sizeof(int);
+        t->accounted += t->sct_bytes;
+        ctx->tensor_bytes += t->sct_bytes;
     }
 #define COLI_TS(KD)                                                                                            \
     hipLaunchKernelGGL((coli_t_scales<KD>), dim3(t->nq), dim3(256), 0, ctx->stream, t->sc, t->nrt, t->nq, noct, \

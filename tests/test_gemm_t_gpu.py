@@ -1,5 +1,7 @@
 """coli_hip_gemm_t_dev (dx = dy W over resident quantized weights) against a
 64-bit product with the dequantized matrix."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -234,3 +236,28 @@ def test_built_rows_of_many_columns(session, monkeypatch, kind, O):
     beyond 16384 columns reads a second time."""
     monkeypatch.setenv("COLI_HIP_GEMM_T", "many")
     test_matches_dense(session, kind, O, 70, 3)
+
+
+def test_scales_are_counted(session):
+    """The second copy of the scales is in the tensor's bytes and the device's statistics while it is held."""
+    b = session.b
+    n, byt = C.c_size_t(), C.c_size_t()
+
+    def stats():
+        b.cuda_stats(0, C.byref(n), C.byref(byt))
+        return byt.value
+
+    rng = np.random.default_rng(2)
+    O, I = 200, 300
+    for kind, planes in (("i4h", 1), ("i4f", 2), ("fp4", 1)):
+        start = stats()
+        h, _ = matrix(session, rng, kind, O, I)
+        loaded, own = stats(), b.cuda_tensor_bytes(h)
+        run(session, h, np.ones((2, O), np.float32), I)
+        # tile quads of 128 columns, four groups each, an exponent a group; rows by 32
+        extra = planes * 3 * 4 * 28 * 16 + 3 * 4 * 4
+        assert stats() - loaded == extra and b.cuda_tensor_bytes(h) - own == extra
+        run(session, h, np.ones((2, O), np.float32), I)
+        assert stats() - loaded == extra
+        session.free(h)
+        assert stats() == start
