@@ -533,13 +533,15 @@ static int t_octets(const ColiCudaTensor *t) { return (t->nrt + 1) / 2 * 4; }
 int build_t_scales(DevCtx *ctx, ColiCudaTensor *t, bool update_only) {
     if (t->kind == COLI_KIND_GENERIC || (update_only && !t->sct)) return 1;
     const int noct = t_octets(t), planes = t->kind == COLI_KIND_I4_F ? 2 : 1;
-    if (!t->sct) {
-        const size_t sb = (size_t)planes * t->nq * 4 * noct * 16;
-        if (!hip_check(hipMalloc(&t->sct, sb + (size_t)t->nq * 4 * sizeof(int)), "transposed scales")) return 0;
+    const size_t sb = (size_t)planes * t->nq * 4 * noct * 16, bytes = sb + (size_t)t->nq * 4 * sizeof(int);
+    const bool first = !t->sct;
+    if (first) {
+        // laid out by a graph they would be missing in every call before its replay
+        hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+        if (!hip_check(hipStreamIsCapturing(ctx->stream, &cap), "transposed scales") || cap != hipStreamCaptureStatusNone)
+            return 0;
+        if (!hip_check(hipMalloc(&t->sct, bytes), "transposed scales")) return 0;
         t->sct_ge = (int *)((uint8_t *)t->sct + sb);
-        t->sct_bytes = sb + (size_t)t->nq * 4 * sizeof(int);
-        t->accounted += t->sct_bytes;
-        ctx->tensor_bytes += t->sct_bytes;
     }
 #define COLI_TS(KD)                                                                                            \
     hipLaunchKernelGGL((coli_t_scales<KD>), dim3(t->nq), dim3(256), 0, ctx->stream, t->sc, t->nrt, t->nq, noct, \
@@ -548,7 +550,16 @@ int build_t_scales(DevCtx *ctx, ColiCudaTensor *t, bool update_only) {
     else if (t->kind == COLI_KIND_I4_F) COLI_TS(COLI_KIND_I4_F);
     else COLI_TS(COLI_KIND_FP4);
 #undef COLI_TS
-    return hip_check(hipGetLastError(), "transposed scales");
+    const int ok = hip_check(hipGetLastError(), "transposed scales");
+    if (first && ok) {
+        t->sct_bytes = bytes;
+        t->accounted += bytes;
+        ctx->tensor_bytes += bytes;
+    } else if (first) {
+        (void)hipFree(t->sct);
+        t->sct = nullptr;
+    }
+    return ok;
 }
 
 template <int KIND>

@@ -160,7 +160,8 @@ int coli_hip_lora_grad_dev(ColiCudaTensor *tensor, ColiHipLora *lora, const floa
 /* Input gradient of coli_cuda_pipe_gemm: dx[S, I] = dy[S, O] W. dx must not
  * overlap dy. The first call on a tensor also lays out its scales a second
  * time (counted in the tensor's bytes and the device's statistics from then on;
- * freed with it; kept current by coli_cuda_tensor_update). */
+ * freed with it; kept current by coli_cuda_tensor_update), so it is refused
+ * under capture, like the first coli_hip_lora_grad_dev with a dx. */
 int coli_hip_gemm_t_dev(ColiCudaTensor *tensor, float *dx_dev, const float *dy_dev, int S);
 
 /* ---- load balance of routed rows -------------------------------------------

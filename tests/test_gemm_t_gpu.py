@@ -261,3 +261,29 @@ def test_scales_are_counted(session):
         assert stats() - loaded == extra
         session.free(h)
         assert stats() == start
+
+
+def test_first_gradient_is_not_captured(session):
+    """Under capture a tensor's first gradient, which lays out its scales, is
+    refused; the capture goes on, and calls outside it are right."""
+    b = session.b
+    rng = np.random.default_rng(43)
+    O, I, S = 96, 160, 5
+    h, w = matrix(session, rng, "i4h", O, I)
+    try:
+        dy = rng.standard_normal((S, O)).astype(np.float32)
+        with Bufs(b) as d:
+            py, px, pz = d.up(dy), d.up(np.zeros((S, I), np.float32)), d.up(np.zeros((S, O), np.float32))
+            assert b.cuda_pipe_gemm(h, pz, px, S)
+            with hiprt.Graph(b.hip_stream(0)) as g:
+                assert not b.hip_gemm_t_dev(h, px, py, S)
+                assert b.cuda_pipe_gemm(h, pz, px, S)
+            want = dy.astype(np.float64) @ w
+            mag = np.abs(dy).astype(np.float64) @ np.abs(w)
+            for _ in range(2):
+                assert b.hip_gemm_t_dev(h, px, py, S)
+                close(d.down(px, (S, I)), want, mag, gemm_tol(O))
+                g.launch()
+            assert np.isfinite(d.down(pz, (S, O))).all()
+    finally:
+        session.free(h)
