@@ -29,6 +29,7 @@
 #include "coli_hip_ext.h"
 
 #include <algorithm>
+#include <initializer_list>
 
 #define COLI_BAL_MAX_SEQS 16384
 #define COLI_BAL_MAX_ROWS (1 << 24)
@@ -528,10 +529,27 @@ static bool balance_shape_ok(int n, int T, int E, int mode) {
            mode <= 3;
 }
 
+// The first `outs` ranges share no byte with each other nor with the others (null: absent).
+struct Range {
+    const void *p;
+    size_t n;
+};
+static bool outputs_apart(std::initializer_list<Range> r, size_t outs) {
+    const Range *v = r.begin();
+    for (size_t i = 0; i < outs; i++)
+        for (size_t j = i + 1; j < r.size(); j++)
+            if (v[j].p && ranges_overlap(v[i].p, v[i].n, v[j].p, v[j].n)) return false;
+    return true;
+}
+
 int run_balance(DevCtx *ctx, const float *z, int nch, const int *idx, const int *keff, const uint8_t *mask,
                 const int *off, int n, int T, int E, int K, int mode, float *loss, int *counts, int *rows,
                 const BalanceLast *last) {
-    if (!balance_shape_ok(n, T, E, mode) || K < 1 || K > 64 || K > E) return 0;
+    const size_t rows4 = (size_t)T * 4;
+    if (!balance_shape_ok(n, T, E, mode) || K < 1 || K > 64 || K > E ||
+        !outputs_apart({{loss, (size_t)n * 4}, {counts, (size_t)n * E * 4}, {rows, (size_t)n * 4}, {z, rows4 * E}, {idx, rows4 * K},
+                        {keff, rows4}, {mask, last ? 1 : (size_t)T}, {off, (size_t)(n + 1) * 4}}, 3))
+        return 0;   // (last: the mask may be shorter than the guess)
     BalanceArgs a = {};
     a.z = z;
     a.nch = nch;
@@ -609,7 +627,9 @@ extern "C" int coli_hip_balance_grad_dev(int device, const float *logits, const 
     if (fault_injected()) return 0;
     if (!logits || !dloss || !counts || !rows || !dlogits || (!offsets && n != 1) ||
         !balance_shape_ok(n, T, E, route_mode) ||
-        (dlogits != logits && ranges_overlap(dlogits, (size_t)T * E * 4, logits, (size_t)T * E * 4)))
+        (dlogits != logits && ranges_overlap(dlogits, (size_t)T * E * 4, logits, (size_t)T * E * 4)) ||
+        !outputs_apart({{dlogits, (size_t)T * E * 4}, {mask, (size_t)T}, {offsets, (size_t)(n + 1) * 4}, {dloss, (size_t)n * 4},
+                        {counts, (size_t)n * E * 4}, {rows, (size_t)n * 4}}, 1))
         return 0;
     DevCtx *ctx = ctx_of(device);
     if (!bind_ctx(ctx)) return 0;

@@ -1074,7 +1074,9 @@ extern "C" int coli_hip_lora_gemm_dev(ColiCudaTensor *t, ColiHipLora *l, float *
     if (fault_injected()) return 0;
     if (!y_dev || !x_dev || !slot_dev) return 0;
     DevCtx *ctx = lora_ctx(t, l, S);
-    if (!ctx || ranges_overlap(y_dev, (size_t)S * t->O * 4, x_dev, (size_t)S * t->I * 4)) return 0;
+    const size_t yb = (size_t)S * t->O * 4;
+    if (!ctx || ranges_overlap(y_dev, yb, x_dev, (size_t)S * t->I * 4) || ranges_overlap(y_dev, yb, slot_dev, (size_t)S * 4))
+        return 0;
     switch (l->dtype) {
     case 0: return lora_forward<float>(ctx, t, l, y_dev, x_dev, S, slot_dev);
     case 1: return lora_forward<_Float16>(ctx, t, l, y_dev, x_dev, S, slot_dev);
@@ -1089,11 +1091,11 @@ extern "C" int coli_hip_lora_grad_dev(ColiCudaTensor *t, ColiHipLora *l, const f
     DevCtx *ctx = lora_ctx(t, l, S);
     if (!ctx) return 0;
     // the inputs are read until the last launch: no output lies over one, or over another output
-    const void *at[5] = {dx_dev, da_dev, db_dev, x_dev, dy_dev};
-    const size_t rank = (size_t)l->slots * l->max_rank * 4, n[5] = {(size_t)S * t->I * 4, rank * t->I, rank * t->O,
-                                                                   (size_t)S * t->I * 4, (size_t)S * t->O * 4};
+    const void *at[6] = {dx_dev, da_dev, db_dev, x_dev, dy_dev, slot_dev};
+    const size_t rank = (size_t)l->slots * l->max_rank * 4;
+    const size_t n[6] = {(size_t)S * t->I * 4, rank * t->I, rank * t->O, (size_t)S * t->I * 4, (size_t)S * t->O * 4, (size_t)S * 4};
     for (int i = 0; i < 3; i++)
-        for (int j = i + 1; j < 5; j++)
+        for (int j = i + 1; j < 6; j++)
             if (at[i] && ranges_overlap(at[i], n[i], at[j], n[j])) return 0;
     forget_emitted(ctx, da_dev, (size_t)l->slots * l->max_rank * l->I * sizeof(float));
     forget_emitted(ctx, db_dev, (size_t)l->slots * l->max_rank * l->O * sizeof(float));

@@ -148,13 +148,13 @@ void coli_hip_lora_free(ColiHipLora *lora);
 int coli_hip_lora_set_dev(ColiHipLora *lora, int slot, const void *a_dev, const void *b_dev, int rank, float scale);
 /* y[s] = W x[s] + scale_a B_a (A_a x[s]) with a = slot_dev[s]: the projection
  * of coli_cuda_pipe_gemm and each row's adapter in one call. A slot number
- * outside the bank, or of an empty slot: no adapter. y must not overlap x. */
+ * outside the bank, or of an empty slot: no adapter. y must not overlap x or slot_dev. */
 int coli_hip_lora_gemm_dev(ColiCudaTensor *tensor, ColiHipLora *lora, float *y_dev, const float *x_dev, int S,
                            const int *slot_dev);
 /* Gradients of that call from dy [S, O]: dx [S, I] (NULL: not wanted), and for
  * every slot of the bank da [slots, max_rank, I] and db [slots, O, max_rank]
  * (written whole: zeros past a slot's rank and where no row has the slot). None
- * of them may overlap x, dy or another. */
+ * of them may overlap an input or another. */
 int coli_hip_lora_grad_dev(ColiCudaTensor *tensor, ColiHipLora *lora, const float *x_dev, const float *dy_dev, int S,
                            const int *slot_dev, float *dx_dev, float *da_dev, float *db_dev);
 /* Input gradient of coli_cuda_pipe_gemm: dx[S, I] = dy[S, O] W. dx must not
@@ -179,13 +179,14 @@ int coli_hip_gemm_t_dev(ColiCudaTensor *tensor, float *dx_dev, const float *dy_d
  * and n_i its rows:
  *   counts[i, e] = c_e, rows[i] = n_i,
  *   loss[i] = sum_e (E c_e / C) (1 / n_i) sum_t p[t, e]      (0 where C or n_i is 0)
- * 1.0 is balance (top-K of equal loads). E <= 1024, K <= min(64, E), n <= 16384, T <= 2^24. */
+ * 1.0 is balance (top-K of equal loads). E <= 1024, K <= min(64, E), n <= 16384, T <= 2^24. No
+ * output may overlap an input or another output. */
 int coli_hip_balance_dev(int device, const float *logits, const int *idx, const int *keff, const unsigned char *mask,
                          const int *offsets, int n, int T, int E, int K, int route_mode, float *loss, int *counts,
                          int *rows);
 /* dlogits [T, E] from dloss [n] and the forward's counts and rows (the counts
  * carry no gradient). Masked rows get zeros; rows of no sequence are left as
- * they were. dlogits may be logits. */
+ * they were. dlogits may be logits, and must not overlap any other input. */
 int coli_hip_balance_grad_dev(int device, const float *logits, const unsigned char *mask, const int *offsets, int n,
                               int T, int E, int route_mode, const float *dloss, const int *counts, const int *rows,
                               float *dlogits);

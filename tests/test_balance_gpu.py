@@ -452,3 +452,26 @@ def test_graphs_outlive_larger_forwards(session, mode, E, K, D, S):
             o.forward(rows)
             assert o.balance()
             o.check(rows, large)
+
+
+def test_outputs_over_inputs_are_refused(session):
+    b = session.b
+    T, E, K, n = 40, 8, 2, 2
+    with Bufs(b) as d:
+        z, idx, keff, mask = d.up(np.zeros((T, E), np.float32)), d.up(np.zeros((T, K), np.int32)), d.up(np.zeros(T, np.int32)), d.up(np.ones(T, np.uint8))
+        off = d.up(np.array([0, 20, 40], np.int32))
+        loss, counts, rows, dl = d.up(np.zeros(n, np.float32)), d.up(np.zeros((n, E), np.int32)), d.up(np.zeros(n, np.int32)), d.up(np.zeros(n, np.float32))
+        dz = d.up(np.zeros((T, E), np.float32))
+        ok = (0, z, idx, keff, mask, off, n, T, E, K, 0, loss, counts, rows)
+        assert b.hip_balance_dev(*ok)
+        for k, size in ((11, 4 * n), (12, 4 * n * E), (13, 4 * n)):
+            for p, nb in ((z, 4 * T * E), (idx, 4 * T * K), (keff, 4 * T), (mask, T), (off, 4 * (n + 1))):
+                for bad in (p, p + nb - 4, p - size + 4):
+                    assert not b.hip_balance_dev(*(ok[:k] + (bad,) + ok[k + 1:])), (k, bad)
+        for k, bad in ((11, counts + 4 * n * E - 4), (12, rows), (13, loss + 4)):
+            assert not b.hip_balance_dev(*(ok[:k] + (bad,) + ok[k + 1:])), (k, bad)
+        ok = (0, z, mask, off, n, T, E, 0, dl, counts, rows, dz)
+        assert b.hip_balance_grad_dev(*ok)
+        for p, nb in ((mask, T), (off, 4 * (n + 1)), (dl, 4 * n), (counts, 4 * n * E), (rows, 4 * n)):
+            for bad in (p, p + nb - 4, p - 4 * T * E + 4):
+                assert not b.hip_balance_grad_dev(*(ok[:11] + (bad,))), bad

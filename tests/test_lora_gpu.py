@@ -419,3 +419,19 @@ def test_high_ranks_of_many_rows(session, monkeypatch, shape):
         c.check_grads()
         monkeypatch.setenv("COLI_HIP_GEMM_T", "many")   # (the sort builds dy's operands)
         c.check_grads()
+
+
+def test_outputs_over_the_slots_are_refused(session):
+    """The rows' slots are read by the last launch too."""
+    b = session.b
+    with Case(session, 53, "i4h", 32, 64, 20, 2, 4, 0, "0") as c:
+        d = c.d
+        px, py, ps = d.up(c.x), d.up(c.dy), d.up(c.slot)
+        pa, pb, pdx = (d.up(np.zeros(n, np.float32)) for n in ((2, 4, 64), (2, 32, 4), (20, 64)))
+        for bad in (ps, ps + 4 * 19, ps - 4 * 20 * 32 + 4):
+            assert not b.hip_lora_gemm_dev(c.h, c.bank, bad, px, 20, ps)
+        ok = (c.h, c.bank, px, py, 20, ps, pdx, pa, pb)
+        for k, size in ((6, 4 * 20 * 64), (7, 4 * 2 * 4 * 64), (8, 4 * 2 * 32 * 4)):
+            for bad in (ps, ps + 4 * 19, ps - size + 4):
+                assert not b.hip_lora_grad_dev(*(ok[:k] + (bad,) + ok[k + 1:])), (k, bad)
+        assert b.hip_lora_grad_dev(*ok) and b.hip_lora_gemm_dev(c.h, c.bank, py, px, 20, ps)
