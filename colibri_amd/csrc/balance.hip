@@ -151,10 +151,15 @@ __device__ __forceinline__ void bal_load(const BalanceArgs &a, int row, int l, f
 // v: the row's logits in; out, scores whose sum over the row (`sum`) they are to
 // be divided by: p = v / sum. GRAD: v u'(z) instead, and ws = sum_e w_e v_e, so
 // that the row is held once. The hardware's exp2, log2, rcp and rsq (1 ulp each)
-// are used: a p is off by a few 2^-23. Scores so small that their sum would lose
-// bits (every z below about -27) go by their logarithm instead, where both u are
-// linear to within f32: z, or z / 2 in mode 3. A row of nothing but -inf has
-// p = 0.
+// are used, and their rounded arguments count for more the farther a logit lies:
+// a p is off by up to about (|z| + 8) 2^-23 of itself (z under the row's maximum
+// in mode 0; at z = -20 the library's expf is off by one 2^-23). A score below 2^-126
+// is zero. So scores so small that others of the row would be lost beside them, or
+// their sum lose bits, go by their logarithm instead, under the row's maximum, where
+// both u are linear to within f32: z where all of them are below about -27, z / 2 in
+// mode 3 below about -16 (its softplus leaves the normal range at -87, where a
+// score e^(z / 2) would still be 2^-24 of the row's at -54).
+// A row of nothing but -inf has p = 0.
 template <int L, int NV, int MODE, int ROW, bool GRAD>
 __device__ __forceinline__ void bal_scores(const BalanceArgs &a, int row, int l, const float *w, float (&v)[4 * NV],
                                            float &sum, float &ws) {
@@ -187,7 +192,7 @@ __device__ __forceinline__ void bal_scores(const BalanceArgs &a, int row, int l,
         }
     }
     if (MODE) sum = bal_sum<L>(sum);
-    if (MODE == 0 || sum < 1e-12f) {
+    if (MODE == 0 || sum < (MODE == 3 ? 3e-4f : 1e-12f)) {
         if (MODE) bal_load<L, NV, ROW>(a, row, l, v);
         float m = -INFINITY;
 #pragma unroll

@@ -475,3 +475,20 @@ def test_outputs_over_inputs_are_refused(session):
         for p, nb in ((mask, T), (off, 4 * (n + 1)), (dl, 4 * n), (counts, 4 * n * E), (rows, 4 * n)):
             for bad in (p, p + nb - 4, p - 4 * T * E + 4):
                 assert not b.hip_balance_grad_dev(*(ok[:11] + (bad,))), bad
+
+
+@pytest.mark.parametrize("mode", [0, 1, 3])
+def test_small_scores_beside_larger_ones(session, mode):
+    """Rows whose largest logit is far below zero and whose others lie farther:
+    each score keeps its own relative accuracy while it is above 2^-126."""
+    rng = np.random.default_rng(60 + mode)
+    T, E = 40, 24
+    z, idx = routed(rng, T, E, 4)
+    if mode == 3:   # rows of -50 at most (scores of 1e-11) down to -100, and of -20 down to -84
+        z[:20] = -50.0 - 50.0 * rng.random((20, E))
+        z[20:] = -20.0 - 64.0 * rng.random((20, E))
+    else:           # from -20 down to -84: softmax's 64 under its maximum
+        z[:, 0] = -20.0
+        z[:, 1:] = -20.0 - 64.0 * rng.random((T, E - 1))
+    z = z.astype(np.float32)
+    check(session, z, idx, None, None, np.array([0, 10, 40], np.int32), mode)
