@@ -15,11 +15,16 @@
 //     + l % 8 in register r, rows 8 (l / 32) + 0..7: the B operand of
 //     v_mfma_f32_32x32x16_f16. About 1.3 instructions a weight, no LDS.
 //   * A weight enters as n sc 2^-Eg in fp16 hi + lo, Eg the exponent of its
-//     column group's largest scale (exact for MXFP4, whose lo is zero and left
-//     out, and for int4 with fp16 scales; to 3 x 2^-22 with f32 scales, which
-//     enter as two fp16); dy as fp16 hi + lo under its row's exponent (2^-22).
-//     hi hi + hi lo + lo hi are summed in f32. The scales are kept a second time
-//     per tensor, by column group with eight rows' worth in 16 bytes
+//     column group's largest scale over all rows of W (it must be one: the sum
+//     over the rows is taken before it is applied); dy as fp16 hi + lo under its
+//     row's exponent (2^-22). hi hi + hi lo + lo hi are summed in f32. Weights of
+//     MXFP4 (lo is zero and left out) and of fp16 scales are exact while their
+//     scale is within 2^-35 and 2^-22 of that largest one; f32 scales enter as two
+//     fp16, to 3 x 2^-22 within 2^-11 of it. Smaller scales lose places to fp16's
+//     least one: a weight is off by at most 8 x 2^-32 of the largest scale (MXFP4
+//     7 x 2^-37) beside that, and zero where its scale is below. The forward, which
+//     applies scales to results, does not lose them. The scales are kept a second
+//     time per tensor, by column group with eight rows' worth in 16 bytes
 //     (coli_t_scales, made on first use).
 //
 // Many rows are bound by the matrix units: 2048 x 4096 x 14336 int4, three

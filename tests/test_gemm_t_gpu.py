@@ -287,3 +287,47 @@ def test_first_gradient_is_not_captured(session):
             assert np.isfinite(d.down(pz, (S, O))).all()
     finally:
         session.free(h)
+
+
+def spread_tol(kind, w, smax):
+    """Error of a weight beyond its 6 x 2^-22 (gemm_tol): what fp16 cannot hold
+    of a scale far below its column group's largest, which lies in [2^11, 2^12)
+    there (MXFP4: at 2^12). int4: a scale, the odd rows' over 16, is rounded to
+    2^-25, so by 2^-21 / 2^11 of the largest, times a nibble of at most 8, and
+    lo to 2^-25 once more. MXFP4: e8m0 scales are powers of two, held down to
+    2^-24, so at most 2^-25 / 2^12 of the largest is lost, times 6, and the
+    product is rounded to 2^-25."""
+    return 6 * 2.0 ** -22 * np.abs(w) + (7 * 2.0 ** -37 if kind == "fp4" else 8 * 2.0 ** -32 + 2.0 ** -36) * smax
+
+
+@pytest.mark.parametrize("pin", ["few", "many"])
+@pytest.mark.parametrize("kind", ["i4h", "i4f", "fp4"])
+def test_weights_of_small_scales(session, monkeypatch, kind, pin):
+    """One-hot rows of dy read weights whose scales lie 2^-16, 2^-30 and 2^-45
+    below the column group's largest: off by no more than the bound under it."""
+    monkeypatch.setenv("COLI_HIP_GEMM_T", pin)
+    rng = np.random.default_rng(41)
+    O, I = 80, 200
+    down = np.array([0, 16, 30, 45])[np.arange(O) // 3 % 4]
+    if kind == "fp4":
+        q4, e8 = rand_mxfp4(rng, O, I)
+        e8 = (e8 - down[:, None]).astype(np.uint8)
+        h, w, s = session.upload_mxfp4(q4, e8, I, O), deq_mxfp4(q4, e8, I), 2.0 ** (e8.astype(np.float64) - 127)
+    else:
+        q4, sc = rand_i4(rng, O, I, 32, fp16_scales=False)
+        sc = ((0.5 + sc) * 2.0 ** -down[:, None]).astype(np.float32)
+        if kind == "i4h":   # (2^-30 and 2^-45 are below fp16: zero scales)
+            sc = sc.astype(np.float16).astype(np.float32)
+        h, w, s = session.upload(q4, sc, 4, I, O, 32), deq_i4(q4, sc, I, 32), sc.astype(np.float64)
+    try:
+        assert session.b.hip_tensor_kind(h) == ("i4h", "i4f", "fp4").index(kind)
+        got = run(session, h, np.eye(O, dtype=np.float32), I)
+        smax = np.repeat(s.max(0), 32)[None, :I]
+        err = np.abs(got.astype(np.float64) - w)
+        # (a result is rounded to f32: within the 6 x 2^-22)
+        assert (err <= spread_tol(kind, w, smax)).all(), float((err / spread_tol(kind, w, smax)).max())
+        # nothing is lost where the scales are within the range that fp16 holds whole
+        exact = down <= {"i4h": 16, "i4f": -1, "fp4": 30}[kind]
+        assert not err[exact].any()
+    finally:
+        session.free(h)
