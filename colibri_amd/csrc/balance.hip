@@ -252,7 +252,8 @@ __global__ __launch_bounds__(SINGLE ? 1024 : 256, 4) void coli_balance_rows(Bala
     const int b = blockIdx.x, r0 = b * a.R, r1 = min(a.T, r0 + a.R);
     float v[4 * NV];
     int have = 0;   // the step whose rows v holds
-    if (r0 < r1) bal_load<L, NV, ROW>(a, min(r0 + RW * wave + g, r1 - 1), l, v);
+    const bool none = a.state && r0 >= r1;   // fewer rows than the launch allows for
+    if (!none) bal_load<L, NV, ROW>(a, min(r0 + RW * wave + g, r1 - 1), l, v);
     if constexpr (SINGLE) {
         for (int e = tid; e < a.n * a.E; e += NT) a.counts[e] = 0;
         for (int i = tid; i < a.n; i += NT) {
@@ -260,7 +261,7 @@ __global__ __launch_bounds__(SINGLE ? 1024 : 256, 4) void coli_balance_rows(Bala
             a.rows[i] = 0;
         }
     }
-    if (r0 >= r1) return;   // (fewer rows than the launch allows for)
+    if (none) return;
     int i = bal_first(a, r0, s_off);
     const BalOff off = {s_off, a.off, a.n, a.T};
     if (!a.off || SINGLE) __syncthreads();
