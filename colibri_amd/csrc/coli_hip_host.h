@@ -93,8 +93,8 @@ struct DevCtx {
     bool stream_out = false;           // the caller has the stream and may capture it
     bool captured = false;             // some call's launches have gone into a graph
     // workspaces of the adapter, input-gradient and balance entry points; these,
-    // the fragments, partial, split_cnt and sums grow by reserve_kept: where a
-    // graph may hold them, outgrown ones live until shutdown
+    // the fragments, partial, split_cnt, sums, qdq, idot_y and idot_sx grow by
+    // reserve_kept: where a graph may hold them, outgrown ones live until shutdown
     DevBuf lora_h, lora_list, gt, bal, bal_cnt;
     void *outgrown[COLI_OUTGROWN] = {};
     int n_outgrown = 0;

@@ -224,7 +224,8 @@ int make_frags8(DevCtx *ctx, int set, const float *x, int ld, int nrows, int K, 
                 const int *nrows_dev) {
     FragSet &f = ctx->frag[set];
     const int nq = (K + 127) / 128, np = coli_mx_pieces();
-    if (!reserve(ctx, &f.p8, (size_t)np * nrows * nq * 128, 0) || !reserve(ctx, &f.s8, (size_t)np * nrows * nq * 4, 0))
+    if (!reserve_kept(ctx, &f.p8, (size_t)np * nrows * nq * 128, 0) ||
+        !reserve_kept(ctx, &f.s8, (size_t)np * nrows * nq * 4, 0))
         return 0;
     f.prow = nrows;
     int *flag = (int *)ctx->flags.p + 8 + set;
@@ -1134,8 +1135,8 @@ static int idot_dev(DevCtx *ctx, ColiCudaTensor *t, float *y_dev, const float *x
     FragSet &f = ctx->frag[set];
     const size_t halves = (size_t)S * ngp * 32;
     if (!reserve_kept(ctx, &f.hi, halves * 2, 0) || !reserve_kept(ctx, &f.lo, halves * 2, 0) ||
-        !reserve_kept(ctx, &f.exp, (size_t)S * sizeof(int), 0) || !reserve(ctx, &ctx->idot_y, (size_t)S * t->O * 4, 0) ||
-        !reserve(ctx, &ctx->idot_sx, (size_t)S * 4, 0))
+        !reserve_kept(ctx, &f.exp, (size_t)S * sizeof(int), 0) || !reserve_kept(ctx, &ctx->idot_y, (size_t)S * t->O * 4, 0) ||
+        !reserve_kept(ctx, &ctx->idot_sx, (size_t)S * 4, 0))
         return 0;
     // hi parts only: the GEMVs over this set never read its lo buffer
     f.pending = false;
@@ -1174,7 +1175,7 @@ static int gemm_host(DevCtx *ctx, ColiCudaTensor *t, float *y, const float *x, i
     const float *xin = (const float *)ctx->x.p;
     // qdq 1: e4m3 per 128 (native_quant contract); 2: int8 per 32 (matmul_mxfp4_i8)
     if (qdq == 1 || (qdq == 2 && t->I % 32 == 0)) {
-        if (!reserve(ctx, &ctx->qdq, xb, 0) ||
+        if (!reserve_kept(ctx, &ctx->qdq, xb, 0) ||
             !hip_check(qdq == 1 ? coli_launch_qdq_e4m3(xin, (float *)ctx->qdq.p, S, t->I, ctx->stream)
                              : coli_launch_qdq_i8(xin, (float *)ctx->qdq.p, S, t->I, ctx->stream),
                     "activation qdq"))
@@ -1277,7 +1278,7 @@ extern "C" int coli_hip_fp4_matmul_i8_dev(ColiCudaTensor *t, float *y_dev, const
     if (!bind_ctx(ctx)) return 0;
     if (t->I % 32) return gemm_dev(ctx, t, y_dev, x_dev, S);
     size_t xb = (size_t)S * t->I * sizeof(float);
-    if (!reserve(ctx, &ctx->qdq, xb, 0) ||
+    if (!reserve_kept(ctx, &ctx->qdq, xb, 0) ||
         !hip_check(coli_launch_qdq_i8(x_dev, (float *)ctx->qdq.p, S, t->I, ctx->stream), "activation qdq"))
         return 0;
     return gemm_dev(ctx, t, y_dev, (const float *)ctx->qdq.p, S);
@@ -1297,7 +1298,7 @@ extern "C" int coli_hip_fp4_matmul_qdq_dev(ColiCudaTensor *t, float *y_dev, cons
     DevCtx *ctx = ctx_of(t->device);
     if (!bind_ctx(ctx)) return 0;
     size_t xb = (size_t)S * t->I * sizeof(float);
-    if (!reserve(ctx, &ctx->qdq, xb, 0) ||
+    if (!reserve_kept(ctx, &ctx->qdq, xb, 0) ||
         !hip_check(coli_launch_qdq_e4m3(x_dev, (float *)ctx->qdq.p, S, t->I, ctx->stream), "activation qdq"))
         return 0;
     return gemm_dev(ctx, t, y_dev, (const float *)ctx->qdq.p, S);

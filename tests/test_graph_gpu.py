@@ -173,3 +173,72 @@ def test_gemm_rows_graph_replays_match_eager(session, monkeypatch, fmt, O, I, S)
     memory by tall tiles, K splits with their reduction, and short tiles."""
     monkeypatch.setenv("COLI_HIP_GEMV", "gemm")
     test_gemm_graph_replays_match_eager(session, fmt, O, I, S)
+
+
+@pytest.mark.parametrize("call", ["idot", "qdq", "i8"])
+def test_graphs_outlive_larger_activation_buffers(session, call):
+    """A captured call that quantizes its activations, after larger calls have
+    outgrown the buffers that it holds them in."""
+    b = session.b
+    rng = np.random.default_rng(71)
+    O, I, S, most = 256, 512, 3, 400
+    if call == "idot":
+        q, s = rand_i4(rng, O, I, 0)
+        h = session.upload(q, s, 2, I, O)
+    else:
+        h = session.upload_mxfp4(*rand_mxfp4(rng, O, I), I, O)
+    fn = {"idot": b.hip_matmul_i4_idot_dev, "qdq": b.hip_fp4_matmul_qdq_dev, "i8": b.hip_fp4_matmul_i8_dev}[call]
+    xd, yd = _dev(b, rng.standard_normal((most, I)).astype(np.float32)), b.cuda_pipe_alloc(0, S * O * 4)
+    zd = b.cuda_pipe_alloc(0, most * O * 4)
+    try:
+        assert fn(h, yd, xd, S)
+        hiprt.device_sync()
+        eager = _get(b, yd, (S, O))
+        with hiprt.Graph(b.hip_stream(0)) as g:
+            assert fn(h, yd, xd, S)
+        for rep in range(3):
+            assert fn(h, zd, xd, 100 * (rep + 2))
+            b.hip_fill_random_u8(0, yd, S * O * 4, 7 + rep)
+            g.launch()
+            hiprt.device_sync()
+            assert np.array_equal(_get(b, yd, (S, O)).view(np.uint32), eager.view(np.uint32)), rep
+    finally:
+        for p in (xd, yd, zd):
+            b.cuda_pipe_free(0, p)
+        session.free(h)
+
+
+def test_graph_outlives_larger_block_scaled_forwards(session, monkeypatch):
+    """The same for a layer on the opt-in block-scaled GEMM, whose activation
+    pieces the later forwards outgrow with the layer's own buffers."""
+    monkeypatch.setenv("COLI_HIP_MX", "1")
+    b = session.b
+    rng = np.random.default_rng(72)
+    D, I, E, K, S, most = 256, 128, 16, 4, 40, 300
+    layer = Layer(rng, 7, D, I, E, shared=False)
+    x, W, bias = make_router_inputs(rng, most, D, E, K, 1, bias=True)
+    hs = layer.upload(session)
+    m, xd, yd = C.c_void_p(), _dev(b, x), b.cuda_pipe_alloc(0, most * D * 4)
+    try:
+        (gt, _a), (up, _b), (dn, _c) = (tensor_array([t[k] for t in hs[:E]]) for k in range(3))
+        cfg = ColiHipMoeConfig(D, I, E, K, 1, 1, 0.0, 1.0, 0)
+        assert b.hip_moe_create(C.byref(m), 0, C.byref(cfg), f32p(W), f32p(bias), gt, up, dn, None, None, None)
+        assert b.hip_moe_forward_dev(m, xd, yd, S)
+        hiprt.device_sync()
+        eager = _get(b, yd, (S, D))
+        with hiprt.Graph(b.hip_stream(0)) as g:
+            assert b.hip_moe_forward_dev(m, xd, yd, S)
+        for rep in range(3):
+            assert b.hip_moe_forward_dev(m, xd, yd, 100 * (rep + 1))
+            b.hip_fill_random_u8(0, yd, S * D * 4, 7 + rep)
+            g.launch()
+            hiprt.device_sync()
+            assert np.array_equal(_get(b, yd, (S, D)).view(np.uint32), eager.view(np.uint32)), rep
+    finally:
+        if m:
+            b.hip_moe_free(m)
+        for p in (xd, yd):
+            b.cuda_pipe_free(0, p)
+        for t in hs:
+            for h in t:
+                session.free(h)
