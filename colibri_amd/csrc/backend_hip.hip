@@ -235,11 +235,8 @@ extern "C" void coli_cuda_shutdown(void) {
                           &ctx->gt, &ctx->bal, &ctx->bal_cnt};
         for (DevBuf *b : bufs) free_buf(b);
         for (int k = 0; k < ctx->n_outgrown; k++) (void)hipFree(ctx->outgrown[k]);
-        for (int f = 0; f < 4; f++) {
-            free_buf(&ctx->frag[f].hi);
-            free_buf(&ctx->frag[f].lo);
-            free_buf(&ctx->frag[f].exp);
-        }
+        for (FragSet &f : ctx->frag)
+            for (DevBuf *b : {&f.hi, &f.lo, &f.exp, &f.gexp, &f.p8, &f.s8}) free_buf(b);
         for (int s = 0; s < COLI_PIPE_SLOTS; s++) free_buf(&ctx->pipe[s]);
         if (ctx->host_x.h) (void)hipHostFree(ctx->host_x.h);
         if (ctx->host_y.h) (void)hipHostFree(ctx->host_y.h);
