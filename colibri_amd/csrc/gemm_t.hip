@@ -27,10 +27,13 @@
 //     time per tensor, by column group with eight rows' worth in 16 bytes
 //     (coli_t_scales, made on first use).
 //
-// Many rows are bound by the matrix units: 2048 x 4096 x 14336 int4, three
-// products, 600 us, 1.2 PFLOP/s of fp16 products (an 8192^3 library product:
-// 1.07); 512 rows 187 us with the join (7 us) and the build of dy's operands
-// (16 us, 59 MB at 3.8 TB/s) to come. Few rows: see coli_gemm_t_few.
+// Many rows run at the rate of a large library product: 2048 x 4096 x 14336
+// int4, three products, 600 us, 1.2 PFLOP/s of fp16 products (8192^3 by the
+// library: 1.07), the matrix units busy for 54 % of the cycles, waves waiting for
+// a third of theirs; 512 rows 187 us with the join (7 us) and the build of dy's
+// operands (16 us, 59 MB at 3.8 TB/s) to come. f32 scales (a second plane of them)
+// take 3 to 6 % longer: whole calls of 512 rows 183 us against 177. Few rows: see
+// coli_gemm_t_few.
 #include "coli_hip_host.h"
 #include "coli_device.h"
 
@@ -204,10 +207,8 @@ __device__ __forceinline__ void t_products(const uint32_t (&d)[2][2], const half
 // Many rows: workgroup (64 WN columns, 32 MT rows, K split); WK wave groups
 // share its K steps (32 rows of W: two row tiles) and are joined in LDS at the
 // end. A step's dy octets are staged in LDS (two buffers), the weights and
-// scales of the next step are requested before this one's products. Bound by
-// the matrix cores: int4 runs three products, at 2048 x 4096 x 14336 617 us or
-// 1.17 PFLOP/s of fp16 (the library's large fp16 product: 1.07 on the same
-// card); with one wave group, one wave a SIMD, 686 us.
+// scales of the next step are requested before this one's products. 2048 x 4096
+// x 14336 int4: 600 us; with one wave group, one wave a SIMD, 686 us.
 template <int KIND, int MT, int WN, int WK>
 __global__ __launch_bounds__(64 * WN * WK, 2) void coli_gemm_t(GemmTArgs a) {
     constexpr int BM = 32 * MT, NT = 64 * WN, CH = 8 * BM;   // 16-byte chunks of a step: 2 parts x 4 octets x BM rows
@@ -336,11 +337,12 @@ __global__ __launch_bounds__(64 * WN * WK, 2) void coli_gemm_t(GemmTArgs a) {
 // dy: read as f32 and converted on its way into the wave's LDS, under the
 // exponent of the row's part in this split (the splits' sums are f32 already).
 // No launch builds operands, and no barrier holds the waves together before
-// their sums are joined. Bound by the VALU (transpose, unpack and conversion,
-// about 450 instructions a step of 4096 weights); a 64-row form spilled its
-// accumulators, so every 32 rows read and unpack the weights again. Measured: 16
-// rows of 7168 x 2048 MXFP4 (8.4 MB) 8.7 us and the join 2.8; 64 of 14336 x 4096
-// int4 46 us (33 MB).
+// their sums are joined. Transpose, unpack and conversion are about 450 VALU
+// instructions a step of 4096 weights: 64 rows of 14336 x 4096 int4 (33 MB) take
+// 46 us, the busy CUs' VALU issuing for 62 % of their cycles and waves waiting for
+// 40 % of theirs; 16 rows of 7168 x 2048 MXFP4 (8.4 MB) 8.7 us and the join 2.8,
+// latency. A 64-row form spilled its accumulators, so every 32 rows read and
+// unpack the weights again.
 template <int KIND, bool ODD>
 __global__ __launch_bounds__(512, 2) void coli_gemm_t_few(GemmTArgs a) {
     constexpr int BM = 32, W = 8, CPT = 4 * BM / 64, STAGE = 8 * BM * 16, PD = 2;

@@ -11,8 +11,8 @@
 //   expand  Y[s][n]  += scale sum_r h[s][r] V[r][n]  (B h, A^T dh)
 //   outer   G[r][n]   = scale sum_s h[s][r] X[s][n]  (dA, dB)
 // on v_mfma_f32_16x16x4_f32: the adapters' products are a few hundredths of
-// the projection's, and f32 operands need neither splitting nor exponents; the
-// shrink of bf16 factors alone, where they are most of the time at high ranks,
+// the projection's, and f32 operands need neither splitting nor exponents; only
+// the shrink of bf16 factors, where f32 MFMAs are most of the time at high ranks,
 // splits x into three bf16 (shrink_products). Rows of one slot are
 // gathered 16 at a time into an MFMA tile: up to 64 rows each workgroup finds
 // its tile with one ballot over the rows' slots, beyond it a one-workgroup
@@ -24,8 +24,8 @@
 //   2048 rows, 4096 -> 14336, rank 32: both shrinks of the backward 38 us (151
 //     MB, 4.0 TB/s), outer 52 us (the same rows again, 2.9 TB/s), expand 53 us
 //     forward (235 MB, 4.4 TB/s) and 21 us backward (67 MB)
-//   1024 rows, 14336 -> 4096, rank 64: shrink 22 us (59 MB; on f32 MFMAs 39),
-//     expand 21 us
+//   1024 rows, 14336 -> 4096, rank 64: shrink 22 us (89 MB; fp16 and f32 factors,
+//     on f32 MFMAs, 40 and 41), expand 21 us
 //   16 rows of 16 adapters, 7168 -> 2048, rank 32: 5.4 and 5.6 us
 //   one row, 4096 -> 14336, rank 16: 4.4 and 4.2 us beside a projection of 10
 // up to 64 rows the gradients' outer and the expand are one launch
@@ -300,12 +300,15 @@ template <typename T> struct LoraSide {
 };
 
 // acc[r] += x v[r] over the lane's eight columns and its neighbours', 32 in all.
-// bf16 factors: x as three bf16 (truncated, 8 bits each: exact) on
-// v_mfma_f32_16x16x32_bf16, three MFMAs of 16 cycles where f32 takes eight of 32,
-// and the factors need no conversion (adapters beside 1024 x 14336, rank 64: 30 ->
-// 20 us; all gradients of 2048 x 4096 x 14336, rank 32: 90 -> 83). fp16 and f32
-// factors would have to be split as well, 32 and 44 VALU instructions for eight,
-// which takes the gain. f32 sums either way.
+// bf16 factors: x as three bf16 (truncated, 8 bits each: exact for finite x, but
+// for what lies below 2^-126; an infinity becomes NaN, as in the projection's own
+// operands) on v_mfma_f32_16x16x32_bf16, three MFMAs of 16 cycles where f32 takes
+// eight of 32, and the factors need no conversion (1024 x 14336, rank 64: 22 us
+// against the 40 of fp16 factors; all gradients of 2048 x 4096 x 14336, rank 32:
+// 90 -> 83). fp16 and f32 factors would have to be split as well: here, 32 and 44
+// VALU instructions for eight of them, which takes the gain; once, when the bank
+// is written, for two and three times their bytes in bf16, which is not built. f32
+// sums either way.
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 template <typename T, int NR>
 __device__ __forceinline__ void shrink_products(const float (&x)[8], const Raw8<T> (&v)[NR], floatx4 (&acc)[NR]) {

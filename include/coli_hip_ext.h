@@ -158,13 +158,15 @@ int coli_hip_lora_gemm_dev(ColiCudaTensor *tensor, ColiHipLora *lora, float *y_d
 int coli_hip_lora_grad_dev(ColiCudaTensor *tensor, ColiHipLora *lora, const float *x_dev, const float *dy_dev, int S,
                            const int *slot_dev, float *dx_dev, float *da_dev, float *db_dev);
 /* Input gradient of coli_cuda_pipe_gemm: dx[S, I] = dy[S, O] W. dx must not
- * overlap dy. The scales of 32 columns are held under the largest of them over all
- * O rows: a weight is off by at most 2^-28 of that scale (MXFP4: 2^-34) beside
- * 2^-20 of itself, so rows of W whose scales lie farther below count as zero. (So
- * too for the dx of coli_hip_lora_grad_dev.) The first call on a tensor also lays out its scales a second
- * time (counted in the tensor's bytes and the device's statistics from then on;
- * freed with it; kept current by coli_cuda_tensor_update), so it is refused
- * under capture, like the first coli_hip_lora_grad_dev with a dx. */
+ * overlap dy. The scales of 32 columns are held under the largest of them over
+ * all O rows: a weight is off by at most 2^-28 of that scale (MXFP4: 2^-34)
+ * beside 2^-20 of itself, so rows of W whose scales lie farther below count as
+ * zero. (So too for the dx of coli_hip_lora_grad_dev.)
+ * The first call on a tensor also lays out its scales a second time: 190 us with
+ * the allocation for 14336 x 4096, as long as the product of 512 rows. They count
+ * in the tensor's bytes and the device's statistics from then on, are freed with
+ * it and kept current by coli_cuda_tensor_update. That first call (or the first
+ * coli_hip_lora_grad_dev with a dx) is refused under capture. */
 int coli_hip_gemm_t_dev(ColiCudaTensor *tensor, float *dx_dev, const float *dy_dev, int S);
 
 /* ---- load balance of routed rows -------------------------------------------
