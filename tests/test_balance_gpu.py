@@ -492,3 +492,33 @@ def test_small_scores_beside_larger_ones(session, mode):
         z[:, 1:] = -20.0 - 64.0 * rng.random((T, E - 1))
     z = z.astype(np.float32)
     check(session, z, idx, None, None, np.array([0, 10, 40], np.int32), mode)
+
+
+@pytest.mark.parametrize("S", [5, 300])
+def test_forward_captured_before_any_ran(session, S):
+    """A layer whose only forward has been captured (in the mode that lets it
+    allocate) and not replayed yet: no rows, then the replay's."""
+    b = session.b
+    with LayerOf(session, 1, 40, 4, 256, 300, 90) as warm, LayerOf(session, 1, 40, 4, 256, 300, 91) as o, \
+            LayerOf(session, 1, 40, 4, 256, 300, 91) as ref:
+        warm.forward(S)
+        assert warm.balance() and not o.balance()
+        lib, st = hiprt.lib(), b.hip_stream(0)
+        graph, ex = C.c_void_p(), C.c_void_p()
+        hiprt.device_sync()
+        hiprt.check(lib.hipStreamBeginCapture(st, 2), "capture")
+        ok = b.hip_moe_forward_dev(o.m, o.px, o.py, S)
+        hiprt.check(lib.hipStreamEndCapture(st, C.byref(graph)), "capture end")
+        hiprt.check(lib.hipGraphInstantiate(C.byref(ex), graph, None, None, 0), "instantiate")
+        try:
+            assert ok and b.hip_fill_random_u8(0, o.pc, 4 * 40, 1) and o.balance()
+            assert not o.d.down(o.pc, (40,), np.int32).any() and not o.d.down(o.pr, (1,), np.int32).any()
+            assert not o.d.down(o.pl, (1,)).any()
+            for _ in range(2):
+                hiprt.check(lib.hipGraphLaunch(ex, st), "replay")
+                assert o.balance()
+                o.check(S, ref.routing(S))
+        finally:
+            hiprt.device_sync()
+            lib.hipGraphExecDestroy(ex)
+            lib.hipGraphDestroy(graph)
