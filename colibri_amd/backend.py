@@ -114,6 +114,17 @@ _SIGS = {
     "coli_hip_gemm_t_dev": ([_tp, _vp, _vp, _i], _i),
     "coli_hip_balance_dev": ([_i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp], _i),
     "coli_hip_balance_grad_dev": ([_i, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp], _i),
+    "coli_hip_dispatch_dev": ([_i, _vp, _vp, _vp, _i, _i, _i, _vp, _sz, _vp, _vp, _vp, _vp], _i),
+    "coli_hip_combine_dev": ([_i, _vp, _i, _vp, _vp, _i, _i, _i, _i, _vp], _i),
+    "coli_hip_combine_grad_dev": ([_i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp], _i),
+    "coli_hip_mxfp4_quantize_dev": ([_i, _vp, _i, _i, _i, _vp, _vp], _i),
+    "coli_hip_mxfp4_dequantize_dev": ([_i, _vp, _vp, _i, _i, _vp, _i], _i),
+    "coli_hip_tensor_quantize_mxfp4": ([_tpp, _vp, _i, _i, _i, _i], _i),
+    "coli_hip_fp4_matmul_a4": ([_tp, _f, _f, _i], _i),
+    "coli_hip_fp4_matmul_a4_dev": ([_tp, _vp, _vp, _i], _i),
+    "coli_hip_experts_create": ([C.POINTER(_vp), _i, _i, _tpp, _tpp, C.c_float], _i),
+    "coli_hip_experts_free": ([_vp], None),
+    "coli_hip_experts_a4_dev": ([_vp, _vp, _vp, _i, _vp, _i, _vp, _i], _i),
     "coli_hip_stream": ([_i], _vp),
     "coli_hip_tensor_upload_from_device": ([_tpp, _vp, _f, _u8, _i, _i, _i, _i, _i], _i),
     "coli_hip_fill_random_u8": ([_i, _vp, _sz, C.c_ulonglong], _i),

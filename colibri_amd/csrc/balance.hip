@@ -536,19 +536,6 @@ static bool balance_shape_ok(int n, int T, int E, int mode) {
            mode <= 3;
 }
 
-// The first `outs` ranges share no byte with each other nor with the others (null: absent).
-struct Range {
-    const void *p;
-    size_t n;
-};
-static bool outputs_apart(std::initializer_list<Range> r, size_t outs) {
-    const Range *v = r.begin();
-    for (size_t i = 0; i < outs; i++)
-        for (size_t j = i + 1; j < r.size(); j++)
-            if (v[j].p && ranges_overlap(v[i].p, v[i].n, v[j].p, v[j].n)) return false;
-    return true;
-}
-
 int run_balance(DevCtx *ctx, const float *z, int nch, const int *idx, const int *keff, const uint8_t *mask,
                 const int *off, int n, int T, int E, int K, int mode, float *loss, int *counts, int *rows,
                 const BalanceLast *last) {

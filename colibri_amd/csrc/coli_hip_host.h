@@ -5,6 +5,8 @@
 
 #include <stdint.h>
 
+#include <initializer_list>
+
 #define COLI_PIPE_SLOTS 27
 // Batches larger than this run the grouped GEMM instead of the GEMV.
 #define COLI_GEMM_MIN_ROWS 32
@@ -96,6 +98,7 @@ struct DevCtx {
     // the fragments, partial, split_cnt, sums, qdq, idot_y and idot_sx grow by
     // reserve_kept: where a graph may hold them, outgrown ones live until shutdown
     DevBuf lora_h, lora_list, gt, bal, bal_cnt;
+    DevBuf sort_hist, fp4_x, fp4_items;   // of the sorted-rows and 4-bit entry points, likewise
     void *outgrown[COLI_OUTGROWN] = {};
     int n_outgrown = 0;
     // pinned staging
@@ -178,9 +181,10 @@ hipError_t coli_launch_weighted_sum_rows(float *out, const float *y, const float
 hipError_t coli_launch_sum_slots(float *dst, const float *slots, int n, int D, hipStream_t st);
 }
 
-// single-matrix products (expert.hip, gemm_t.hip)
+// single-matrix products (expert.hip, gemm_t.hip, fp4.hip)
 int tensor_computable(const ColiCudaTensor *t);
 int gemm_dev(DevCtx *ctx, ColiCudaTensor *t, float *y_dev, const float *x_dev, int S);
+int matmul_a4_dev(DevCtx *ctx, ColiCudaTensor *t, float *y_dev, const float *x_dev, int S);   // fp4.hip
 // gemm_dev in two halves: the rows' fragment build, if the product will read
 // fragments, as launch arguments for a launch that runs it beside other work
 // (nblocks 0: nothing to run), then the product.
@@ -201,6 +205,18 @@ int gemm_t_run(DevCtx *ctx, ColiCudaTensor *t, float *dx, const float *dy, int S
 // Do the ranges share a byte (outputs that would overwrite a call's inputs)?
 inline bool ranges_overlap(const void *a, size_t na, const void *b, size_t nb) {
     return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
+}
+// The first `outs` ranges share no byte with each other nor with the others (null: absent).
+struct Range {
+    const void *p;
+    size_t n;
+};
+inline bool outputs_apart(std::initializer_list<Range> r, size_t outs) {
+    const Range *v = r.begin();
+    for (size_t i = 0; i < outs; i++)
+        for (size_t j = i + 1; j < r.size(); j++)
+            if (v[i].p && v[j].p && ranges_overlap(v[i].p, v[i].n, v[j].p, v[j].n)) return false;
+    return true;
 }
 int build_t_scales(DevCtx *ctx, ColiCudaTensor *t, bool update_only);
 // Counts and balance loss (balance.hip) over logits [T][E]; with `last`, over the

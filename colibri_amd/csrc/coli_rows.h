@@ -1,0 +1,41 @@
+// coli_rows.h -- rows of f32, fp16 or bf16 that start at any address their type
+// allows (shared by sorted.hip and fp4.hip).
+#pragma once
+
+#include "coli_device.h"
+
+typedef uint32_t u32x4a1 __attribute__((ext_vector_type(4), aligned(1)));   // 16 bytes at any address
+typedef uint32_t u32a1 __attribute__((aligned(1)));
+
+// N elements from p on as f32, and back, rounded to nearest even: 16 bytes a load.
+template <typename T, int N> __device__ __forceinline__ void el_load(const T *p, float (&f)[N]) {
+    constexpr int V = 16 / sizeof(T);
+    if constexpr (N % V) {
+#pragma unroll
+        for (int i = 0; i < N; i++) f[i] = (float)*GPTR(T, p + i);
+    } else {
+        struct Raw { T e[V]; };
+#pragma unroll
+        for (int k = 0; k < N; k += V) {
+            const Raw r = __builtin_bit_cast(Raw, (u32x4)*GPTR(u32x4a1, p + k));
+#pragma unroll
+            for (int i = 0; i < V; i++) f[k + i] = (float)r.e[i];
+        }
+    }
+}
+template <typename T, int N> __device__ __forceinline__ void el_store(T *p, const float (&f)[N]) {
+    constexpr int V = 16 / sizeof(T);
+    if constexpr (N % V) {
+#pragma unroll
+        for (int i = 0; i < N; i++) p[i] = (T)f[i];
+    } else {
+        struct Raw { T e[V]; };
+#pragma unroll
+        for (int k = 0; k < N; k += V) {
+            Raw r;
+#pragma unroll
+            for (int i = 0; i < V; i++) r.e[i] = (T)f[k + i];
+            *(u32x4a1 *)(p + k) = __builtin_bit_cast(u32x4, r);
+        }
+    }
+}

@@ -1173,7 +1173,8 @@ static int gemm_host(DevCtx *ctx, ColiCudaTensor *t, float *y, const float *x, i
     if (!hip_check(hipMemcpyAsync(ctx->x.p, ctx->host_x.h, xb, hipMemcpyHostToDevice, ctx->stream), "input upload"))
         return 0;
     const float *xin = (const float *)ctx->x.p;
-    // qdq 1: e4m3 per 128 (native_quant contract); 2: int8 per 32 (matmul_mxfp4_i8)
+    // qdq 1: e4m3 per 128 (native_quant contract); 2: int8 per 32 (matmul_mxfp4_i8);
+    // 3: int8 per row; 4: MXFP4
     if (qdq == 1 || (qdq == 2 && t->I % 32 == 0)) {
         if (!reserve_kept(ctx, &ctx->qdq, xb, 0) ||
             !hip_check(qdq == 1 ? coli_launch_qdq_e4m3(xin, (float *)ctx->qdq.p, S, t->I, ctx->stream)
@@ -1182,7 +1183,9 @@ static int gemm_host(DevCtx *ctx, ColiCudaTensor *t, float *y, const float *x, i
             return 0;
         xin = (const float *)ctx->qdq.p;
     }
-    if (!(qdq == 3 ? idot_dev(ctx, t, (float *)ctx->y.p, xin, S) : gemm_dev(ctx, t, (float *)ctx->y.p, xin, S)) ||
+    if (!(qdq == 3   ? idot_dev(ctx, t, (float *)ctx->y.p, xin, S)
+          : qdq == 4 ? matmul_a4_dev(ctx, t, (float *)ctx->y.p, xin, S)
+                     : gemm_dev(ctx, t, (float *)ctx->y.p, xin, S)) ||
         !hip_check(hipMemcpyAsync(ctx->host_y.h, ctx->y.p, yb, hipMemcpyDeviceToHost, ctx->stream), "output download") ||
         !hip_check(hipStreamSynchronize(ctx->stream), "gemm synchronize"))
         return 0;
@@ -1282,6 +1285,14 @@ extern "C" int coli_hip_fp4_matmul_i8_dev(ColiCudaTensor *t, float *y_dev, const
         !hip_check(coli_launch_qdq_i8(x_dev, (float *)ctx->qdq.p, S, t->I, ctx->stream), "activation qdq"))
         return 0;
     return gemm_dev(ctx, t, y_dev, (const float *)ctx->qdq.p, S);
+}
+
+extern "C" int coli_hip_fp4_matmul_a4(ColiCudaTensor *t, float *y, const float *x, int S) {
+    if (fault_injected()) return 0;
+    if (!t || t->kind != COLI_KIND_FP4 || !y || !x || S < 1) return 0;
+    DevCtx *ctx = ctx_of(t->device);
+    if (!bind_ctx(ctx)) return 0;
+    return gemm_host(ctx, t, y, x, S, 4);
 }
 
 extern "C" int coli_hip_fp4_matmul_qdq(ColiCudaTensor *t, float *y, const float *x, int S) {

@@ -203,6 +203,83 @@ int coli_hip_balance_grad_dev(int device, const float *logits, const unsigned ch
 int coli_hip_moe_last_balance_dev(ColiHipMoe *moe, const unsigned char *mask, const int *offsets, int n, float *loss,
                                   int *counts, int *rows);
 
+/* ---- rows sorted by expert, and back ---------------------------------------
+ * What lies between a router and the experts: for experts on other devices
+ * (the sorted rows are what is sent), and for tuning through them. Device
+ * pointers, contiguous, asynchronous on the device's stream; workspaces and
+ * captures as above. No atomics on floating values: the same call gives the same
+ * bits. No output may overlap an input or another output. None has a counterpart
+ * in the reference.
+ *
+ * Sort the live selections of T rows by expert: idx [T, K], of which the first
+ * keff[t] are live (NULL: all K), none of a row whose mask byte is 0 (NULL: all
+ * rows count), nor one outside 0..E-1. Selection s = t K + k; the order is by
+ * expert, then by s.
+ *   offsets [E + 1]: expert e has the sorted rows [offsets[e], offsets[e + 1])
+ *   src [T K]:       the selection of each sorted row
+ *   pos [T, K]:      the sorted row of each selection, -1 where it is not live
+ *   xs [T K, row_bytes]: the rows, xs[r] = x[src[r] / K], x [T, row_bytes]: of any
+ *                    type (x and xs NULL: not wanted)
+ * src and xs behind the last live selection are left as they were. Gradient of x:
+ * coli_hip_combine_dev of xs's, without weights. T from 0 to 2^23, E <= 1024, K <=
+ * 64, T K <= 2^30, rows of up to 64 MiB. */
+int coli_hip_dispatch_dev(int device, const int *idx, const int *keff, const unsigned char *mask, int T, int E, int K,
+                          const void *x, size_t row_bytes, int *offsets, int *src, int *pos, void *xs);
+/* out[t] = sum_k w[t, k] ys[pos[t, k]] over the places pos [T, K] within 0..N-1
+ * (others count for nothing, whatever their weight); w [T, K] f32 (NULL: ones), ys
+ * [N, D] and out [T, D] of dtype 0 f32, 1 fp16, 2 bf16. Summed in f32 in the order
+ * of k, rounded once. Rows of ys that no place names are not looked at. */
+int coli_hip_combine_dev(int device, const void *ys, int dtype, const int *pos, const float *w, int T, int K, int N,
+                         int D, void *out);
+/* Its gradients from dout [T, D]: dys[pos[t, k]] = w[t, k] dout[t] (rows that no
+ * place names are left as they were) and dw[t, k] = <dout[t], ys[pos[t, k]]> (0
+ * where the place is outside), the product in f32. dys or dw NULL: not wanted (ys may be
+ * NULL without dw). No row may be named twice where dys is wanted. */
+int coli_hip_combine_grad_dev(int device, const void *ys, int dtype, const int *pos, const float *w, const void *dout,
+                              int T, int K, int N, int D, void *dys, float *dw);
+
+/* ---- MXFP4: quantization, and products of 4-bit rows ------------------------
+ * Device pointers, asynchronous on the stream, workspaces and captures as above.
+ * None has a counterpart in the reference.
+ *
+ * x [rows, cols] of dtype 0 f32, 1 fp16, 2 bf16 to the native MXFP4 bytes of
+ * coli_hip_tensor_upload_mxfp4: q4 [rows, ceil(cols / 2)], e8 [rows, ceil(cols /
+ * 32)]. The scale of 32 columns is the smallest power of two, 2^-126 at least, that
+ * holds their largest magnitude within 6 (the rule of the e4m3 path: nothing
+ * saturates); a block of zeros has scale 1; one with an infinity or NaN has byte
+ * 255 and codes 0, which is NaN to whatever reads it. Codes are the nearest, ties to the
+ * even code. Zero-row calls succeed. */
+int coli_hip_mxfp4_quantize_dev(int device, const void *x, int dtype, int rows, int cols, unsigned char *q4,
+                                unsigned char *e8);
+/* y [rows, cols] from such bytes: code times scale, rounded once to dtype (byte
+ * 0 is scale 0, byte 255 infinity, as in the products with f32 rows). */
+int coli_hip_mxfp4_dequantize_dev(int device, const unsigned char *q4, const unsigned char *e8, int rows, int cols,
+                                  void *y, int dtype);
+/* A resident MXFP4 tensor [O, I] quantized from weights on the device (a fresh
+ * handle only; synchronous, as the uploads). The weights must be complete. */
+int coli_hip_tensor_quantize_mxfp4(ColiCudaTensor **tensor, const void *weights_dev, int dtype, int I, int O, int device);
+/* y[S, O] = Q(x) W^T with Q the quantizer above (a row's 32-column blocks) and W a
+ * resident MXFP4 tensor, on the fp4 matrix units: exact products, f32 sums. A scale
+ * byte of 255 is NaN here, 0 is 2^-127. Host pointers (synchronous) / device pointers
+ * (asynchronous; y must not overlap x). The gradient that passes it (straight through
+ * Q) is coli_hip_gemm_t_dev. */
+int coli_hip_fp4_matmul_a4(ColiCudaTensor *tensor, float *y, const float *x, int S);
+int coli_hip_fp4_matmul_a4_dev(ColiCudaTensor *tensor, float *y_dev, const float *x_dev, int S);
+/* The experts' matrices for that product over sorted rows: E <= 1024 resident
+ * MXFP4 tensors [O, I] of one shape on one device; with ups a second one each,
+ * and silu(gate) * up as the result (swiglu_limit > 0: the clamped form). The
+ * tensors must outlive the set. */
+typedef struct ColiHipExperts ColiHipExperts;
+int coli_hip_experts_create(ColiHipExperts **experts, int device, int E, ColiCudaTensor *const *gates,
+                            ColiCudaTensor *const *ups, float swiglu_limit);
+void coli_hip_experts_free(ColiHipExperts *experts);
+/* y[r] = W_e Q(x row of r) for the sorted rows offsets[e] <= r < offsets[e + 1] (ascending;
+ * taken within 0..N) of y [N, O]; other rows of y are left as they were. The row is
+ * x[src[r] / K] with src (of coli_hip_dispatch_dev: the rows need not be copied), x[r]
+ * without; x is [rows, I], a row outside it counts as zeros. N and rows from 0 on. */
+int coli_hip_experts_a4_dev(ColiHipExperts *experts, float *y, const float *x, int rows, const int *src, int K,
+                            const int *offsets, int N);
+
 /* ---- plumbing for benchmarks and tests ----------------------------------- */
 /* coli_cuda_pipe_gemm in two halves, so a timer can bracket the GEMV kernel
  * alone: prep names the activations x_dev[S, I] for the tensor's storage

@@ -1,0 +1,502 @@
+"""MXFP4 on the device: the quantizer and its way back, products of 4-bit rows with
+one resident matrix and with the experts' over sorted rows, against 64-bit
+references."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from colibri_amd import hiprt
+from colibri_amd.backend import f32p, tensor_array
+from mx_ref import combine, mx_quant, pack, plan, silu
+from op_util import Bufs, bits
+from quant_util import deq_mxfp4, mx4_scale, rand_i4, rand_mxfp4, E2M1, nibbles
+
+pytestmark = pytest.mark.gpu
+
+
+def product_tol(I):
+    """Products of codes and scales are exact; the sums are f32: ceil(I / 128) MFMAs
+    that add 128 products to the running sum, and joins of at most 32 parts. Each is
+    allowed two units in the last place of the terms' magnitudes (2 x 2^-23)."""
+    return ((I + 127) // 128 + 32) * 2.0 ** -22
+
+
+def act(rng, S, I):
+    """Rows whose columns differ in size."""
+    return (rng.standard_normal((S, I)) * np.exp(rng.standard_normal(I))).astype(np.float32)
+
+
+def quantize(b, raw, dtype, extra=3):
+    rows, cols = raw.shape
+    qb, eb = rows * ((cols + 1) // 2), rows * ((cols + 31) // 32)
+    with Bufs(b) as d:
+        q4, e8 = d.up(np.full(qb + extra, 0xA5, np.uint8)), d.up(np.full(eb + extra, 0xA5, np.uint8))
+        assert b.hip_mxfp4_quantize_dev(0, d.up(raw), dtype, rows, cols, q4, e8)
+        q, e = d.down(q4, qb + extra, np.uint8), d.down(e8, eb + extra, np.uint8)
+    assert (q[qb:] == 0xA5).all() and (e[eb:] == 0xA5).all()
+    return q[:qb].reshape(rows, -1), e[:eb].reshape(rows, -1)
+
+
+def check_quantize(b, x, dtype):
+    raw, val = bits(dtype, x)
+    q, e = quantize(b, raw, dtype)
+    codes, byte, _ = mx_quant(val)
+    assert np.array_equal(e, byte)
+    bad = np.repeat(byte == 255, 32, 1)[:, :x.shape[1]]
+    assert np.array_equal(q, pack(np.where(bad, 0, codes)))
+
+
+# around the octets (8), a block (32), a lane's last octet, rows of one workgroup
+# (256 octets) and beyond
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 2), (2, 7), (5, 8), (4, 9), (70, 31), (3, 32), (9, 33), (2, 63), (5, 100), (37, 999),
+                                       (300, 64), (3, 2048), (2, 2050), (2, 4111), (1, 16500)])
+def test_quantize(session, dtype, rows, cols):
+    rng = np.random.default_rng(rows * 7 + cols + dtype)
+    check_quantize(session.b, rng.standard_normal((rows, cols)) * np.exp(2 * rng.standard_normal((rows, 1))), dtype)
+
+
+def test_quantize_borders(session):
+    """Every border between two codes and its neighbours, under every scale, both signs."""
+    mids = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])
+    f = np.float32
+    near = np.concatenate([mids, np.nextafter(mids.astype(f), f(0)), np.nextafter(mids.astype(f), f(9)), [6.0, 0.0, -0.0]])
+    row = np.concatenate([near, -near[:8]])
+    assert len(row) == 32
+    e = np.arange(1, 254)[:, None] - 127.0
+    with np.errstate(under="ignore"):
+        x = (row[None, :] * 2.0 ** e).astype(np.float32)
+    check_quantize(session.b, x, 0)
+
+
+def test_quantize_scale_borders(session):
+    """A block's largest magnitude at 6 times a power of two and next to it, over the whole range of f32, subnormals too."""
+    f = np.float32
+    with np.errstate(over="ignore", under="ignore"):
+        top = (1.5 * 2.0 ** np.arange(-149, 128)).astype(f)
+        top = np.concatenate([top, np.nextafter(top, f(0)), np.nextafter(top, f(np.inf)), [f(2.0 ** -149), f(np.finfo(f).max), f(0)]])
+    rng = np.random.default_rng(1)
+    x = (rng.uniform(-1, 1, (len(top), 32)) * top[:, None].astype(np.float64)).astype(f)
+    x[:, 5] = top
+    check_quantize(session.b, x, 0)
+
+
+def test_quantize_every_bf16_and_f16(session):
+    rng = np.random.default_rng(2)
+    u = rng.permutation(np.arange(65536).astype(np.uint16)).reshape(32, 2048)
+    v = (u.astype(np.uint32) << 16).view(np.float32)
+    q, e = quantize(session.b, u, 2)
+    codes, byte, _ = mx_quant(v)
+    assert np.array_equal(e, byte) and np.array_equal(q, pack(np.where(np.repeat(byte == 255, 32, 1), 0, codes)))
+    # blocks of one exponent: no value is lost below its neighbours
+    for dtype, raw, val in ((2, np.arange(65536).astype(np.uint16), None), (1, np.arange(65536).astype(np.uint16).view(np.float16), None)):
+        raw = raw.reshape(64, 1024)
+        val = (raw.astype(np.uint32) << 16).view(np.float32) if dtype == 2 else raw.astype(np.float32)
+        q, e = quantize(session.b, raw, dtype)
+        codes, byte, _ = mx_quant(val)
+        assert np.array_equal(e, byte) and np.array_equal(q, pack(np.where(np.repeat(byte == 255, 32, 1), 0, codes)))
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 2), (2, 6), (2, 7), (5, 8), (4, 9), (70, 31), (9, 33), (37, 999), (300, 64), (2, 2050), (1, 16500)])
+def test_dequantize(session, dtype, rows, cols):
+    """Codes times scales, one rounding: exact in f32 (2^-127 and up), to half a step in the others. Bytes 0 and 255 too."""
+    rng = np.random.default_rng(rows + cols)
+    q4, e8 = rand_mxfp4(rng, rows, cols, 100, 140)
+    e8.reshape(-1)[::5] = rng.choice([0, 1, 2, 253, 254, 255], len(e8.reshape(-1)[::5]))
+    with np.errstate(over="ignore", invalid="ignore"):
+        sc = mx4_scale(e8)[:, np.arange(cols) // 32]
+        ref = (E2M1[nibbles(q4, cols)] * sc).astype(np.float32)
+        want, _ = bits(dtype, ref)
+    with Bufs(session.b) as d:
+        y = d.up(np.full(rows * cols + 2, 7, want.dtype))
+        assert session.b.hip_mxfp4_dequantize_dev(0, d.up(q4), d.up(e8), rows, cols, y, dtype)
+        got = d.down(y, rows * cols + 2, want.dtype)
+    assert (got[-2:] == 7).all()
+    got = got[:-2].reshape(rows, cols)
+    if dtype == 2:
+        got, want = ((v.astype(np.uint32) << 16).view(np.float32) for v in (got, want))
+    nan = np.isnan(ref)
+    assert np.array_equal(np.isnan(got), nan) and np.array_equal(got[~nan], want[~nan])
+
+
+def test_no_rows(session):
+    assert session.b.hip_mxfp4_quantize_dev(0, None, 0, 0, 8, None, None)
+    assert session.b.hip_mxfp4_dequantize_dev(0, None, None, 0, 8, None, 0)
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("O,I", [(1, 1), (48, 130), (33, 999), (200, 512)])
+def test_tensor_from_device_weights(session, dtype, O, I):
+    """The resident tensor is the one that the quantizer's bytes upload to: bitwise the same products."""
+    b = session.b
+    rng = np.random.default_rng(O + I + dtype)
+    raw, val = bits(dtype, rng.standard_normal((O, I)) * 0.05)
+    codes, byte, w = mx_quant(val)
+    h, ref = C.c_void_p(), session.upload_mxfp4(pack(codes), byte, I, O)
+    try:
+        with Bufs(b) as d:
+            pw = d.up(raw)
+            assert b.cuda_pipe_sync(0)
+            assert b.hip_tensor_quantize_mxfp4(C.byref(h), pw, dtype, I, O, 0)
+            assert not b.hip_tensor_quantize_mxfp4(C.byref(h), pw, dtype, I, O, 0)
+        assert b.hip_tensor_kind(h) == 2 and b.cuda_tensor_bytes(h) == b.cuda_tensor_bytes(ref)
+        x = rng.standard_normal((3, I)).astype(np.float32)
+        assert np.array_equal(session.matmul(h, x, 7, I, O), session.matmul(ref, x, 7, I, O))
+    finally:
+        session.free(ref)
+        session.free(h)
+
+
+def matmul_a4(b, h, x, O, extra=1):
+    S = len(x)
+    with Bufs(b) as d:
+        y = d.up(np.full((S + extra, O), 7, np.float32))
+        assert b.hip_fp4_matmul_a4_dev(h, y, d.up(x), S)
+        got = d.down(y, (S + extra, O))
+    assert (got[S:] == 7).all()
+    return got[:S]
+
+
+# rows around the 16-row subtiles and the tiles, widths around the 128-column steps
+# and their pairs, outputs around the 16-row weight tiles
+@pytest.mark.parametrize("I,O,S", [(1, 1, 1), (7, 3, 2), (8, 16, 1), (31, 17, 5), (32, 33, 16), (100, 40, 17), (128, 64, 1), (129, 15, 33),
+                                   (256, 48, 64), (257, 100, 65), (384, 16, 3), (1000, 2999, 21), (999, 130, 70), (2048, 200, 128),
+                                   (1152, 96, 129), (4096, 512, 1), (4096, 300, 200), (16400, 40, 9), (640, 1040, 300), (512, 4112, 2),
+                                   (3000, 24, 1000)])
+def test_matmul(session, I, O, S):
+    rng = np.random.default_rng(I + O * 3 + S)
+    q4, e8 = rand_mxfp4(rng, O, I)
+    h, w = session.upload_mxfp4(q4, e8, I, O), deq_mxfp4(q4, e8, I)
+    try:
+        x = act(rng, S, I)
+        got = matmul_a4(session.b, h, x, O)
+        xv = mx_quant(x)[2]
+        assert (np.abs(got - xv @ w.T) <= product_tol(I) * (np.abs(xv) @ np.abs(w).T) + 1e-30).all()
+        y = np.full((S, O), 7, np.float32)
+        assert session.b.hip_fp4_matmul_a4(h, f32p(y), f32p(np.ascontiguousarray(x)), S)
+        assert np.array_equal(y, got)
+    finally:
+        session.free(h)
+
+
+def test_matmul_one_hot(session):
+    """Rows of one 6: every weight at its place, exactly; blocks of other scales beside it."""
+    rng = np.random.default_rng(3)
+    I, O = 416, 72
+    q4, e8 = rand_mxfp4(rng, O, I, 90, 160)
+    h, w = session.upload_mxfp4(q4, e8, I, O), deq_mxfp4(q4, e8, I)
+    try:
+        x = np.eye(I, dtype=np.float32) * (6 * 2.0 ** rng.integers(-20, 20, (I, 1))).astype(np.float32)
+        assert np.array_equal(matmul_a4(session.b, h, x, O), (x.astype(np.float64) @ w.T).astype(np.float32))
+    finally:
+        session.free(h)
+
+
+def test_matmul_wide_ranges(session):
+    """Scales from 2^-60 to 2^60 on both sides, zero blocks, a zero row."""
+    rng = np.random.default_rng(4)
+    I, O, S = 640, 80, 37
+    q4, e8 = rand_mxfp4(rng, O, I, 67, 187)
+    e8[:, 3] = 0
+    q4[:, 48:64] = 0
+    h, w = session.upload_mxfp4(q4, e8, I, O), deq_mxfp4(q4, e8, I)
+    try:
+        x = (rng.standard_normal((S, I)) * 2.0 ** np.repeat(rng.integers(-60, 60, (S, I // 32)), 32, 1)).astype(np.float32)
+        x[5], x[:, 64:96] = 0, 0
+        got, xv = matmul_a4(session.b, h, x, O), mx_quant(x)[2]
+        assert (np.abs(got - xv @ w.T) <= product_tol(I) * (np.abs(xv) @ np.abs(w).T)).all()
+        assert not got[5].any()
+    finally:
+        session.free(h)
+
+
+@pytest.mark.parametrize("S", [1, 4, 20, 130])
+def test_matmul_rows_do_not_mix(session, S):
+    """A row with a NaN or an infinity is NaN, the others keep their bits."""
+    rng = np.random.default_rng(5)
+    I, O = 300, 50
+    q4, e8 = rand_mxfp4(rng, O, I)
+    h = session.upload_mxfp4(q4, e8, I, O)
+    try:
+        x = act(rng, S, I)
+        clean = matmul_a4(session.b, h, x, O)
+        bad = sorted({0, S // 2, S - 1} - {0} if S > 1 else {0})
+        for k, r in enumerate(bad):
+            x[r, 299 if k else 40] = np.inf if k else np.nan
+        got = matmul_a4(session.b, h, x, O)
+        keep = np.ones(S, bool)
+        keep[bad] = False
+        assert np.isnan(got[bad]).all() and np.array_equal(got[keep], clean[keep])
+    finally:
+        session.free(h)
+
+
+class Experts:
+    """E random experts (pairs with `pair`) and their set."""
+
+    def __init__(self, session, rng, E, I, O, pair, limit=0.0):
+        self.s, self.I, self.O, self.E, self.limit = session, I, O, E, limit
+        self.h, self.w, self.set = [], [], C.c_void_p()
+        for _ in range(2 if pair else 1):
+            mats = [rand_mxfp4(rng, O, I, 117, 121) for _ in range(E)]
+            self.h.append([session.upload_mxfp4(q, e, I, O) for q, e in mats])
+            self.w.append([deq_mxfp4(q, e, I) for q, e in mats])
+        arr = [tensor_array(h) for h in self.h]
+        assert session.b.hip_experts_create(C.byref(self.set), 0, E, arr[0][0], arr[1][0] if pair else None, limit)
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.s.b.hip_experts_free(self.set)
+        for hs in self.h:
+            for h in hs:
+                self.s.free(h)
+
+    def ref(self, e, xv):
+        """(values, allowed error) of rows xv [n, I] through expert e."""
+        v = [xv @ w[e].T for w in self.w]
+        t = [product_tol(self.I) * (np.abs(xv) @ np.abs(w[e]).T) for w in self.w]
+        if len(v) == 1:
+            return v[0], t[0] + 1e-30
+        g, u = v
+        if self.limit > 0:
+            g, u = np.minimum(g, self.limit), np.clip(u, -self.limit, self.limit)
+        # |silu'| <= 1.1; exp, the division and two products: 16 roundings
+        return silu(g) * u, 1.1 * t[0] * np.abs(u) + np.abs(silu(g)) * t[1] + 1.1 * t[0] * t[1] + 2.0 ** -20 * np.abs(silu(g) * u) + 1e-30
+
+    def run(self, x, off, N, src=None, K=1, extra=2):
+        b = self.s.b
+        with Bufs(b) as d:
+            y = d.up(np.full((N + extra, self.O), 7, np.float32))
+            assert b.hip_experts_a4_dev(self.set, y, d.up(x), len(x), None if src is None else d.up(src), K, d.up(np.asarray(off, np.int32)), N)
+            return d.down(y, (N + extra, self.O))
+
+    def check(self, got, xv, off, N, rows):
+        seen = np.zeros(len(got), bool)
+        for e in range(self.E):
+            r = np.arange(max(0, off[e]), min(N, off[e + 1]))
+            if len(r):
+                seen[r] = True
+                v, tol = self.ref(e, xv[rows[r]])
+                assert (np.abs(got[r] - v) <= tol).all(), (e, np.abs(got[r] - v).max())
+        assert (got[~seen] == 7).all()
+
+
+# per expert: none, one, up to and past the tiles
+@pytest.mark.parametrize("pair", [False, True])
+@pytest.mark.parametrize("E,I,O,counts", [(1, 1, 1, [1]), (1, 128, 16, [70]), (3, 300, 40, [0, 5, 0]), (4, 257, 17, [1, 64, 0, 65]),
+                                          (5, 512, 48, [16, 17, 33, 2, 130]), (300, 64, 16, None), (2, 1000, 33, [300, 1]),
+                                          (3, 256, 272, [700, 0, 140])])
+def test_experts(session, pair, E, I, O, counts):
+    rng = np.random.default_rng(E + I + O)
+    if counts is None:
+        counts = rng.choice([0, 0, 1, 2], E)
+    off = np.concatenate([[0], np.cumsum(counts)])
+    N = int(off[-1])
+    x = act(rng, N, I)
+    with Experts(session, rng, E, I, O, pair) as ex:
+        got = ex.run(x, off, N)
+        ex.check(got, mx_quant(x)[2], off, N, np.arange(N))
+        # rows through src: bitwise the copied rows'
+        perm = rng.permutation(N).astype(np.int32)
+        inv = np.argsort(perm)
+        again = ex.run(np.ascontiguousarray(x[inv]), off, N, src=(perm * 3 + rng.integers(0, 3, N)).astype(np.int32), K=3)
+        assert np.array_equal(again, got)
+
+
+def test_experts_clamped(session):
+    rng = np.random.default_rng(7)
+    off = [0, 3, 90]
+    x = act(rng, 90, 320) * 4
+    with Experts(session, rng, 2, 320, 40, True, 1.5) as ex:
+        ex.check(ex.run(x, off, 90), mx_quant(x)[2], off, 90, np.arange(90))
+
+
+def test_experts_offsets_and_rows_outside(session):
+    """Rows before the first and behind the last offset stay as they were, offsets are taken
+    within 0..N, sources outside x are rows of zeros, and descending offsets are empty."""
+    rng = np.random.default_rng(8)
+    x = act(rng, 20, 130)
+    xv = mx_quant(x)[2]
+    with Experts(session, rng, 3, 130, 20, False) as ex:
+        for off in ([2, 9, 9, 15], [-5, 4, 1000, 2 ** 31 - 1], [0, 0, 0, 0], [-9, -3, -1, 0], [12, 4, 4, 2]):
+            ex.check(ex.run(x, off, 20), xv, np.clip(off, 0, 20), 20, np.arange(20))
+        # overlapping ranges of experts: no more tiles than there is room for, and inside y
+        got = ex.run(x, [0, 20, 0, 20], 20)
+        assert (got[20:] == 7).all()
+        src = np.arange(20, dtype=np.int32)
+        src[[0, 7, 19]] = [-1, 20, 2 ** 31 - 1]
+        got = ex.run(x, [0, 5, 12, 20], 20, src=src)
+        assert not got[[0, 7, 19]].any()
+        keep = np.setdiff1d(np.arange(20), [0, 7, 19])
+        assert np.array_equal(got[keep], ex.run(x, [0, 5, 12, 20], 20)[keep])
+        assert session.b.hip_experts_a4_dev(ex.set, None, None, 0, None, 1, None, 0)
+
+
+def route(rng, T, E, K):
+    z = rng.standard_normal((T, E))
+    idx = np.argsort(-z, 1)[:, :K].astype(np.int32)
+    w = np.exp(np.take_along_axis(z, idx, 1))
+    return idx, (w / w.sum(1, keepdims=True)).astype(np.float32)
+
+
+@pytest.mark.parametrize("T", [1, 16, 300])
+def test_layer_of_sorted_rows(session, T):
+    """Dispatch, the experts' pair, their down matrices, combine: eager and as a graph replayed
+    over changing rows, through src and over copied rows alike; and over rows that were sent in
+    4 bits (quantized, dispatched, read back): the same values to Q, under half the scale where
+    a block's largest became 3 scales."""
+    rng = np.random.default_rng(T)
+    b, (E, K, D, I) = session.b, (12, 4, 288, 160)
+    N = T * K
+    with Experts(session, rng, E, D, I, True) as up, Experts(session, rng, E, I, D, False) as down, Bufs(b) as d:
+        px, pi, pw = d.up(np.zeros((T, D), np.float32)), d.up(np.zeros((T, K), np.int32)), d.up(np.zeros((T, K), np.float32))
+        off, src, pos = (d.up(np.zeros(n, np.int32)) for n in (E + 1, N, N))
+        xs, h, ys = (d.up(np.zeros((N, n), np.float32)) for n in (D, I, D))
+        out = [d.up(np.zeros((T, D), np.float32)) for _ in range(2)]
+        q4, e8 = d.up(np.zeros((T, D // 2), np.uint8)), d.up(np.zeros((T, D // 32), np.uint8))
+        q4s, e8s = d.up(np.zeros((N, D // 2), np.uint8)), d.up(np.zeros((N, D // 32), np.uint8))
+
+        def layer(o, how):
+            if how == "src":
+                assert b.hip_dispatch_dev(0, pi, None, None, T, E, K, None, 0, off, src, pos, None)
+                assert b.hip_experts_a4_dev(up.set, h, px, T, src, K, off, N)
+            else:
+                if how == "rows":
+                    assert b.hip_dispatch_dev(0, pi, None, None, T, E, K, px, D * 4, off, src, pos, xs)
+                else:
+                    assert b.hip_mxfp4_quantize_dev(0, px, 0, T, D, q4, e8)
+                    assert b.hip_dispatch_dev(0, pi, None, None, T, E, K, q4, D // 2, off, src, pos, q4s)
+                    assert b.hip_dispatch_dev(0, pi, None, None, T, E, K, e8, D // 32, off, src, pos, e8s)
+                    assert b.hip_mxfp4_dequantize_dev(0, q4s, e8s, N, D, xs, 0)
+                assert b.hip_experts_a4_dev(up.set, h, xs, N, None, 1, off, N)
+            assert b.hip_experts_a4_dev(down.set, ys, h, N, None, 1, off, N)
+            assert b.hip_combine_dev(0, ys, 0, pos, pw, T, K, N, D, o)
+
+        layer(out[0], "src")
+        with hiprt.Graph(b.hip_stream(0)) as g:
+            layer(out[0], "src")
+        for rep in range(3):
+            x, (idx, w) = act(rng, T, D), route(rng, T, E, K)
+            for p, v in ((px, x), (pi, idx), (pw, w)):
+                d.put(p, v)
+            g.launch()
+            first = d.down(out[0], (T, D))
+            ro, rs, rp = plan(idx, None, None, E)
+            # against 64 bits from the h that the device has (its own rounding decides h's codes)
+            for how in ("sent", "rows"):
+                layer(out[1], how)
+                hd = d.down(h, (N, I))
+                up.check(np.concatenate([hd, np.full((1, I), 7, np.float32)]), mx_quant(x)[2], ro, N, rs // K)
+            assert np.array_equal(d.down(out[1], (T, D)).view(np.uint32), first.view(np.uint32))
+            hv, yv, tol = mx_quant(hd)[2], np.zeros((N, D)), np.zeros((N, D))
+            for e in range(E):
+                yv[ro[e]:ro[e + 1]], tol[ro[e]:ro[e + 1]] = down.ref(e, hv[ro[e]:ro[e + 1]])
+            ref, mag = combine(yv, rp, w, N)
+            room, _ = combine(tol, rp, np.abs(w), N)
+            assert (np.abs(first - ref) <= room + (K + 1) * 2.0 ** -24 * mag).all()
+
+
+@pytest.mark.parametrize("S", [1, 3, 40, 300])
+def test_matmul_graph_replays(session, S):
+    """Replays over changing rows with larger eager calls between (outgrown workspaces stay)."""
+    rng = np.random.default_rng(S)
+    b, (I, O) = session.b, (700, 90)
+    q4, e8 = rand_mxfp4(rng, O, I)
+    h = session.upload_mxfp4(q4, e8, I, O)
+    try:
+        with Bufs(b) as d:
+            px, y, y2 = d.up(np.zeros((S, I), np.float32)), d.up(np.zeros((S, O), np.float32)), d.up(np.zeros((S, O), np.float32))
+            assert b.hip_fp4_matmul_a4_dev(h, y, px, S)
+            with hiprt.Graph(b.hip_stream(0)) as g:
+                assert b.hip_fp4_matmul_a4_dev(h, y, px, S)
+            for rep in range(3):
+                d.put(px, act(rng, S, I))
+                g.launch()
+                matmul_a4(b, h, act(rng, 700 * (rep + 1), I), O)
+                assert b.hip_fp4_matmul_a4_dev(h, y2, px, S)
+                assert np.array_equal(d.down(y, (S, O)).view(np.uint32), d.down(y2, (S, O)).view(np.uint32))
+    finally:
+        session.free(h)
+
+
+def test_straight_through_gradient(session):
+    """dx = dy W of coli_hip_gemm_t_dev is the product's gradient for rows that Q leaves as they
+    are: the call is linear along steps that stay on such rows."""
+    rng = np.random.default_rng(9)
+    b, (I, O, S) = session.b, (96, 40, 6)
+    q4, e8 = rand_mxfp4(rng, O, I)
+    h = session.upload_mxfp4(q4, e8, I, O)
+    try:
+        grid = E2M1[:8]
+        x = rng.choice(grid, (S, I)).astype(np.float32)
+        v = rng.choice([-0.5, 0.0, 0.5], (S, I)).astype(np.float32)
+        x[:, ::32], v[:, ::32] = 6, 0                                # the block's scale stays 1
+        v[(x > 1) | (x < 0.5)] = 0                                   # x +- v are codes too
+        dy = rng.standard_normal((S, O)).astype(np.float32)
+        a, c = (matmul_a4(b, h, (x + s * v).astype(np.float32), O).astype(np.float64) for s in (1, -1))
+        with Bufs(b) as d:
+            px = d.up(np.zeros((S, I), np.float32))
+            assert b.hip_gemm_t_dev(h, px, d.up(dy), S)
+            dx = d.down(px, (S, I)).astype(np.float64)
+        w = deq_mxfp4(q4, e8, I)
+        mag = (np.abs(dy).astype(np.float64) * (np.abs(x) @ np.abs(w).T)).sum()
+        assert abs(((a - c) / 2 * dy).sum() - (dx * v).sum()) <= 2.0 ** -18 * mag
+    finally:
+        session.free(h)
+
+
+def test_refusals(session):
+    b = session.b
+    rng = np.random.default_rng(0)
+    I, O = 64, 32
+    q4, e8 = rand_mxfp4(rng, O, I)
+    h, other = session.upload_mxfp4(q4, e8, I, O), session.upload_mxfp4(*rand_mxfp4(rng, O, 96), 96, O)
+    i4, sc = rand_i4(rng, O, I, 32)
+    hi = session.upload(i4, sc, 4, I, O, 32)
+    big = 2 ** 31 - 1
+    try:
+        with Bufs(b) as d:
+            x, y, q, e = (d.up(np.zeros(4096, np.float32)) for _ in range(4))
+
+            def refused(fn, ok, changes):
+                assert fn(*ok)
+                for ch in changes:
+                    a = list(ok)
+                    for k, v in ch.items():
+                        a[k] = v
+                    assert not fn(*a), ch
+
+            refused(b.hip_mxfp4_quantize_dev, (0, x, 0, 4, 70, q, e),
+                    [{0: 5}, {0: -1}, {1: None}, {2: 3}, {2: -1}, {3: -1}, {3: big}, {4: 0}, {4: big}, {5: None}, {6: None}, {5: x}, {6: x}, {6: q}])
+            refused(b.hip_mxfp4_dequantize_dev, (0, q, e, 4, 70, y, 0),
+                    [{0: 5}, {1: None}, {2: None}, {3: -1}, {3: big}, {4: 0}, {4: big}, {5: None}, {6: 3}, {5: q}, {5: e}])
+            refused(b.hip_fp4_matmul_a4_dev, (h, y, x, 3), [{0: None}, {0: hi}, {1: None}, {2: None}, {3: 0}, {3: -1}, {3: big}, {1: x}])
+            t = C.c_void_p()
+            for a in ((None, x, 0, I, O, 0), (C.byref(h), x, 0, I, O, 0), (C.byref(t), None, 0, I, O, 0), (C.byref(t), x, 3, I, O, 0),
+                      (C.byref(t), x, 0, 0, O, 0), (C.byref(t), x, 0, I, 0, 0), (C.byref(t), x, 0, I, O, 9)):
+                assert not b.hip_tensor_quantize_mxfp4(*a) and not t
+            host = np.zeros((3, O), np.float32)
+            assert not b.hip_fp4_matmul_a4(hi, f32p(host), f32p(np.zeros((3, I), np.float32)), 3)
+            assert not b.hip_fp4_matmul_a4(h, f32p(host), f32p(np.zeros((3, I), np.float32)), 0)
+            s = C.c_void_p()
+            two, two4, mixed = tensor_array([h, h]), tensor_array([h, hi]), tensor_array([h, other])
+            gone = (C.c_void_p * 2)(h.value, None)
+            for a in ((None, 0, 2, two[0], None, 0.0), (C.byref(s), 9, 2, two[0], None, 0.0), (C.byref(s), 0, 0, two[0], None, 0.0),
+                      (C.byref(s), 0, 1025, two[0], None, 0.0), (C.byref(s), 0, 2, None, None, 0.0), (C.byref(s), 0, 2, two4[0], None, 0.0),
+                      (C.byref(s), 0, 2, two[0], two4[0], 0.0), (C.byref(s), 0, 2, mixed[0], None, 0.0), (C.byref(s), 0, 2, two[0], mixed[0], 0.0),
+                      (C.byref(s), 0, 2, C.cast(gone, C.POINTER(C.c_void_p)), None, 0.0)):
+                assert not b.hip_experts_create(*a) and not s
+            assert b.hip_experts_create(C.byref(s), 0, 2, two[0], two[0], 0.0)
+            src, off = d.up(np.zeros(8, np.int32)), d.up(np.array([0, 1, 4], np.int32))
+            refused(b.hip_experts_a4_dev, (s, y, x, 4, src, 1, off, 4),
+                    [{0: None}, {1: None}, {2: None}, {3: -1}, {3: 0}, {3: big}, {5: 0}, {6: None}, {7: -1}, {7: big}, {1: x}, {1: src}, {1: off}])
+            b.hip_experts_free(s)
+            b.hip_experts_free(None)
+            assert b.cuda_pipe_sync(0)
+    finally:
+        for t in (h, other, hi):
+            session.free(t)
