@@ -16,6 +16,8 @@
 #include <algorithm>
 #include <cstdio>
 #include <cstdlib>
+#include <cstring>
+#include <type_traits>
 #include <vector>
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
@@ -76,18 +78,24 @@ struct QuantArgs {
 };
 
 // Lanes of a row take its octets in turn, four to a block of 32. Native bytes, or
-// (OPERAND) rows of cp / 2 and cp / 32 bytes with zeros past the row's end.
+// (OPERAND) rows of cp / 2 and cp / 32 bytes with zeros past the row's end, and behind
+// the last row one of zeros.
 template <typename T, int FORM, bool OPERAND> __device__ __forceinline__ void quant_rows(const QuantArgs &a, int blk) {
     const int r = (blk << (8 - a.lpr)) + (threadIdx.x >> a.lpr);
     const int o0 = threadIdx.x & ((1 << a.lpr) - 1);
-    if (r >= a.rows) return;
-    const T *xr = (const T *)a.x + (size_t)r * a.cols;
+    if (r >= a.rows + (OPERAND ? 1 : 0)) return;
+    const bool zero = OPERAND && r == a.rows;
+    const T *xr = (const T *)a.x + (size_t)(zero ? 0 : r) * a.cols;
     const int end = OPERAND ? a.cp : (a.cols + 31) / 32 * 32;
     const size_t qs = OPERAND ? a.cp / 2 : (a.cols + 1) / 2, es = OPERAND ? a.cp / 32 : (a.cols + 31) / 32;
     for (int c = 8 * o0; c < end; c += 8 << a.lpr) {
         float v[8];
         uint32_t byte;
         row8<T, FORM>(xr, c, a.cols, v);
+        if constexpr (OPERAND) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = zero ? 0.0f : v[i];
+        }
         const uint32_t u = mx_codes(v, byte);
         uint8_t *q = a.q4 + (size_t)r * qs + c / 2;
         if (OPERAND) {
@@ -158,11 +166,10 @@ struct Fp4Args {
     int S, tile;
     int nrt, nq, O;
     int rtb;                   // row-tile blocks of an item
-    const uint8_t *xq, *xe;    // operand rows: cp / 2 codes, cp / 32 scales
+    const uint8_t *xq, *xe;    // operand rows: cp / 2 codes, cp / 32 scales; row `rows` is zeros
     int cp;
     const int *src;            // sorted row -> K x row + k (null: the row itself)
     int K, rows;
-    const uint8_t *zero;
     float *y;
     float limit;
 };
@@ -257,9 +264,9 @@ template <int NM, int R, bool DUAL, int W> __global__ __launch_bounds__(64 * W) 
             x = a.src[x];
             x = x < 0 ? -1 : x / a.K;
         }
-        const bool in = (unsigned)x < (unsigned)a.rows;
-        xq[m] = (in ? a.xq + (size_t)x * (a.cp / 2) : a.zero) + 16 * g;
-        xe[m] = in ? a.xe + (size_t)x * (a.cp / 32) : a.zero;
+        if ((unsigned)x >= (unsigned)a.rows) x = a.rows;
+        xq[m] = a.xq + (size_t)x * (a.cp / 2) + 16 * g;
+        xe[m] = a.xe + (size_t)x * (a.cp / 32);
     }
     floatx4 acc[R][NM];
 #pragma unroll
@@ -324,6 +331,278 @@ template <int NM, int R, bool DUAL, int W> __global__ __launch_bounds__(64 * W) 
         for (int i = 0; i < 4; i++)
             if (o + i < a.O) y[i] = DUAL ? swiglu_out(v[i], u[i], a.limit) : v[i];
     }
+}
+
+// Many rows: 128 rows x 16 weight tiles (DUAL: 8 gate and 8 up tiles) a workgroup of
+// four waves, each all the rows and four tiles as two operands of 32 rows on
+// v_mfma_scale_f32_32x32x64_f8f6f4: 16 MFMAs a wave and step of 128 columns, on 4 KiB of
+// weights, which go straight to registers, and 8 KiB of rows from LDS. (One wave issues
+// the 16x16x128 form every 29 cycles, four waves a SIMD every 18; the 32x32x64 form,
+// twice the work, runs at its 32 from one wave: 8.9 PFLOP/s of zeros on the card, 6.8 of
+// random codes, where 16x16x128 reaches 6.8 and 5.4.)
+// The rows come by LDS DMA two steps at a time (128 bytes of a row: a whole cache line)
+// into a ring of three stages; 16-byte pieces are stored XORed with a key of the row,
+// so that the rows of an operand read hit different banks.
+// Loads retire in order: a wave that has used the weights of a step has all the DMAs
+// requested before them, so the ring costs one barrier a stage and no wait of its own.
+// (The DMAs are buffer loads: the compiler takes global_load_lds for a flat access and
+// waits for every load in flight at the next use of any.)
+// Weights rotate through three sets of registers, one in use, one being turned, one
+// being loaded, without a copy: six steps (three stages) are written out.
+#define COLI_FP4_MANY 128
+struct FmGeom {
+    static constexpr int kRows = COLI_FP4_MANY * 128;   // a stage's codes: 256 columns
+    static constexpr int kStage = kRows + COLI_FP4_MANY * 8;
+    static constexpr int kPD = 3;
+};
+typedef __attribute__((address_space(3))) uint8_t lds_u8;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t fp4_rsrc(const void *p, uint32_t n) {
+    return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, n, 0x00020000);
+}
+__device__ __forceinline__ i32x8 fp4_op(u32x4 v) { return (i32x8){(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0}; }
+// NB: 32-row blocks
+template <int NB, bool DUAL> __device__ __forceinline__ void fp4_many(const Fp4Args &a, const Fp4Item &it, const Fp4Mat &mat,
+                                                                      int rb, lds_u8 *lds) {
+    using G = FmGeom;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 31, g = lane >> 5;
+    // operand r: two row tiles from rt[r] on (DUAL: the gate's and the up's of the same)
+    int rt[2];
+    __amdgpu_buffer_rsrc_t wr[2], sr[2];
+    uint32_t wo[2], so[2];
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+        rt[r] = DUAL ? (rb * 4 + wave) * 2 : (rb * 4 + wave) * 4 + 2 * r;
+        const int t = min(rt[r], a.nrt - 1), two = min(2, a.nrt - t);   // past the last tile it is read again
+        const size_t t0 = (size_t)t * a.nq;
+        wr[r] = fp4_rsrc(uniform_ptr(DUAL && r ? mat.w1 : mat.w0) + t0 * COLI_TILE_BYTES, two * a.nq * COLI_TILE_BYTES);
+        sr[r] = fp4_rsrc(uniform_ptr(DUAL && r ? mat.s1 : mat.s0) + t0 * 64, two * a.nq * 64);
+        const int k = min(n >> 4, two - 1) * a.nq;
+        wo[r] = k * COLI_TILE_BYTES + (32 * g + (n & 15)) * 16;   // slices 2 g and (256 bytes on) 2 g + 1 of row n
+        so[r] = k * 64 + (n & 15) * 4;
+    }
+    // operand row of the item's row r (a.rows: zeros), relative to the item's first
+    // where there is no src
+    const int base = a.src ? 0 : it.r0;
+    auto row_of = [&](int r) {
+        int x = it.r0 + min(r, it.nrows - 1);
+        if (a.src) {
+            x = a.src[x];
+            x = x < 0 ? -1 : x / a.K;
+        }
+        return (uint32_t)(((unsigned)x < (unsigned)a.rows ? x : a.rows) - base);
+    };
+    const uint32_t qs = a.cp / 2, es = a.cp / 32;
+    const __amdgpu_buffer_rsrc_t xqr = fp4_rsrc(a.xq + (size_t)base * qs, 0xffffffffu);
+    const __amdgpu_buffer_rsrc_t xer = fp4_rsrc(a.xe + (size_t)base * es, 0xffffffffu);
+    // codes: DMA k of the wave covers rows 8 (4 k + wave) .. + 7; scales: rows 32 wave + l / 2
+    uint32_t xa[NB];
+#pragma unroll
+    for (int k = 0; k < NB; k++) {
+        const int r = 8 * (4 * k + wave) + (lane >> 3);
+        xa[k] = row_of(r) * qs + 16 * ((lane & 7) ^ ((r >> 1) & 7));
+    }
+    const uint32_t xs = row_of(32 * wave + (lane >> 1)) * es + 4 * (lane & 1);
+    const int ns = a.cp / 256;
+    auto issue = [&](int s, lds_u8 *st) {
+        s = min(s, ns - 1);
+#pragma unroll
+        for (int k = 0; k < NB; k++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(xqr, (lds_void *)(st + (4 * k + wave) * 1024), 16, xa[k], s * 128, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(xer, (lds_void *)(st + G::kRows + wave * 256), 4, xs, s * 8, 0, 0);
+    };
+    // Loaded: lane (n, g) has slices 2 g, 2 g + 1 of row n, a dword of each block. Turned:
+    // its four dwords of block 2 t + g in wv[.][r][t], those that the lane 32 away had by
+    // v_permlane32_swap. Scales: shifted so that bytes 0 and 2 are blocks g, 2 + g.
+    u32x4 wv[3][2][2];
+    uint32_t ws[3][2];
+    auto load_w = [&](int p, int r, int q) {
+        q = min(q, a.nq - 1);
+        wv[p][r][0] = __builtin_amdgcn_raw_buffer_load_b128(wr[r], wo[r], q * COLI_TILE_BYTES, 0);
+        wv[p][r][1] = __builtin_amdgcn_raw_buffer_load_b128(wr[r], wo[r] + 256, q * COLI_TILE_BYTES, 0);
+        ws[p][r] = __builtin_amdgcn_raw_buffer_load_b32(sr[r], so[r], q * 64, 0);
+    };
+    auto turn = [&](int p, int r) {
+        const u32x4 x = wv[p][r][0], y = wv[p][r][1];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const auto u = __builtin_amdgcn_permlane32_swap(x[2 * t], x[2 * t + 1], false, false);
+            const auto v = __builtin_amdgcn_permlane32_swap(y[2 * t], y[2 * t + 1], false, false);
+            wv[p][r][t] = (u32x4){u[0], v[0], u[1], v[1]};
+        }
+        ws[p][r] >>= 8 * g;
+        asm("" : "+v"(ws[p][r]));   // (left alone, the shift moves to the use behind the loop's start, and its wait with it)
+    };
+    floatx16 acc[2][NB];
+#pragma unroll
+    for (int r = 0; r < 2; r++)
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) acc[r][b][i] = 0.0f;
+    // the lane's 16 bytes of a block's row n: step h, blocks 2 t + g
+    int xo[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) xo[k] = n * 128 + 16 * ((2 * k + g) ^ ((n >> 1) & 7));
+    u32x4 xv[3][2];   // the rows of this group, the next and the one after it
+    u32x2 xe[NB];     // the stage's row scales
+    int ev[2];        // this group's and the next's, shifted
+    auto read_x = [&](int p, int t, int h, int b, const lds_u8 *st) {
+        xv[p][t] = *(const __attribute__((address_space(3))) u32x4 *)(st + b * 4096 + xo[2 * h + t]);
+    };
+    auto read_e = [&](int b, const lds_u8 *st) {
+        xe[b] = *(const __attribute__((address_space(3))) u32x2 *)(st + G::kRows + (32 * b + n) * 8);
+    };
+    // Group (step h of stage s, block b of rows): four MFMAs, each with its share of the
+    // other work, in the order written here (left to the compiler, loads bunch up and
+    // operands are read right before their use: 2048 x 14336 x 4096 73 us, so 66).
+    // Beside them: reads of the rows two groups on, loads of the weights two steps on,
+    // turns of the next step's weights, and in the second step the DMAs two stages on,
+    // behind the barrier: by then every wave has the next stage's rows in and is done with
+    // the stage before this one.
+    constexpr int NG = 2 * NB;   // groups of a stage
+    auto group = [&](int s, auto kt, auto gt, lds_u8 *const *slot) {
+        constexpr int k3 = decltype(kt)::value, k = decltype(gt)::value, h = k / NB, b = k % NB, kk = 2 * k3 + h;
+        constexpr int cur = kk % 3, nxt = (kk + 1) % 3, ld = (kk + 2) % 3;
+        constexpr int gi = k3 * NG + k, p = gi % 3, pf = (gi + 2) % 3;          // row sets: this group's, that to fill
+        constexpr int fk = (k + 2) % NG, fh = fk / NB, fb = fk % NB;            // the group two on
+        constexpr int nk = (k + 1) % NG, nh = nk / NB, nb = nk % NB;            // and one on
+        const lds_u8 *fst = slot[k + 2 < NG ? k3 : (k3 + 1) % 3];
+        constexpr int every = NB / 2, r = b / every;                            // an operand of weights every so many groups
+        const int q = min(2 * s + h + 2, a.nq - 1), sd = min(s + 2, ns - 1);
+        auto mfma = [&](auto rt, auto tt) {
+            constexpr int rr = decltype(rt)::value, t = decltype(tt)::value;
+            acc[rr][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp4_op(xv[p][t]), fp4_op(wv[cur][rr][t]), acc[rr][b], 4, 4, 2 * t,
+                                                                         ev[gi & 1], 2 * t, (int)ws[cur][rr]);
+        };
+        auto dma = [&](int d) {   // d: 0 .. NB - 1 the codes, NB the scales
+            lds_u8 *st = slot[(k3 + 2) % 3];
+            if (d < NB)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(xqr, (lds_void *)(st + (4 * d + wave) * 1024), 16, xa[d], sd * 128, 0, 0);
+            else if (d == NB)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(xer, (lds_void *)(st + G::kRows + wave * 256), 4, xs, sd * 8, 0, 0);
+        };
+        using C0 = std::integral_constant<int, 0>;
+        using C1 = std::integral_constant<int, 1>;
+        if constexpr (h == 1 && b == 0) {
+            __builtin_amdgcn_s_waitcnt(0x0f76);   // vmcnt(6): all but the first step's weights, so the next stage's DMAs
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+        }
+        mfma(C0{}, C0{});
+        read_x(pf, 0, fh, fb, fst);
+        if constexpr (b % every == 0) wv[ld][r][0] = __builtin_amdgcn_raw_buffer_load_b128(wr[r], wo[r], q * COLI_TILE_BYTES, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        mfma(C1{}, C0{});
+        if constexpr (fh == 0) read_e(fb, fst);
+        if constexpr (h == 1) dma(b * (NB == 2 ? 2 : 1));
+        if constexpr (b % every == every - 1) {
+            const u32x4 x = wv[nxt][r][0], y = wv[nxt][r][1];
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const auto u = __builtin_amdgcn_permlane32_swap(x[2 * t], x[2 * t + 1], false, false);
+                const auto v = __builtin_amdgcn_permlane32_swap(y[2 * t], y[2 * t + 1], false, false);
+                wv[nxt][r][t] = (u32x4){u[0], v[0], u[1], v[1]};
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        mfma(C0{}, C1{});
+        read_x(pf, 1, fh, fb, fst);
+        if constexpr (b % every == 0) wv[ld][r][1] = __builtin_amdgcn_raw_buffer_load_b128(wr[r], wo[r] + 256, q * COLI_TILE_BYTES, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        mfma(C1{}, C1{});
+        if constexpr (b % every == 0) ws[ld][r] = __builtin_amdgcn_raw_buffer_load_b32(sr[r], so[r], q * 64, 0);
+        if constexpr (b % every == every - 1) {
+            ws[nxt][r] >>= 8 * g;
+            asm("" : "+v"(ws[nxt][r]));   // (left alone, the shift moves to its use behind the loop's start, and the wait with it)
+        }
+        if constexpr (h == 1 && (NB == 2 || b == NB - 1)) dma(NB == 2 ? 2 * b + 1 : NB);
+        ev[(gi + 1) & 1] = (int)(xe[nb][nh] >> (8 * g));
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    lds_u8 *const slot[3] = {lds, lds + G::kStage, lds + 2 * G::kStage};
+    asm volatile("" ::"v"(lds) : "memory");
+    issue(0, slot[0]);
+    issue(1, slot[1]);
+#pragma unroll
+    for (int r = 0; r < 2; r++) load_w(0, r, 0);
+#pragma unroll
+    for (int r = 0; r < 2; r++) load_w(1, r, 1);
+#pragma unroll
+    for (int r = 0; r < 2; r++) turn(0, r);
+    __builtin_amdgcn_s_waitcnt(0);   // (a builtin: the compiler counts on from it)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int k = 0; k < 2; k++) {   // (two groups: k < NB)
+        read_x(k, 0, 0, k, slot[0]);
+        read_x(k, 1, 0, k, slot[0]);
+        read_e(k, slot[0]);
+    }
+    ev[0] = (int)(xe[0][0] >> (8 * g));
+    __builtin_amdgcn_sched_barrier(0);
+    auto stage = [&](int s, auto kt) {
+        group(s, kt, std::integral_constant<int, 0>{}, slot);
+        group(s, kt, std::integral_constant<int, 1>{}, slot);
+        group(s, kt, std::integral_constant<int, 2>{}, slot);
+        group(s, kt, std::integral_constant<int, 3>{}, slot);
+        if constexpr (NB == 4) {
+            group(s, kt, std::integral_constant<int, 4>{}, slot);
+            group(s, kt, std::integral_constant<int, 5>{}, slot);
+            group(s, kt, std::integral_constant<int, 6>{}, slot);
+            group(s, kt, std::integral_constant<int, 7>{}, slot);
+        }
+    };
+    for (int s = 0;;) {
+        stage(s, std::integral_constant<int, 0>{});
+        if (++s >= ns) break;
+        stage(s, std::integral_constant<int, 1>{});
+        if (++s >= ns) break;
+        stage(s, std::integral_constant<int, 2>{});
+        if (++s >= ns) break;
+    }
+    // the last DMAs write this workgroup's LDS: none may outlive it
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    // lane (n, g), register i: row 8 (i / 4) + 4 g + i % 4 of the block, output n of the
+    // operand's 32: a store fills whole cache lines of two rows
+#pragma unroll
+    for (int r = 0; r < (DUAL ? 1 : 2); r++) {
+        const int o = 16 * rt[r] + n;
+        float *y = a.y + (size_t)it.r0 * a.O + o;
+        if (o >= a.O) continue;
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const int row = 32 * b + 8 * (i >> 2) + 4 * g + (i & 3);
+                float v = acc[r][b][i];
+                if constexpr (DUAL) v = swiglu_out(v, acc[1][b][i], a.limit);
+                if (row < it.nrows) y[(size_t)row * a.O] = v;
+            }
+    }
+}
+// Workgroups of one XCD (every eighth) take consecutive tiles, eight items' tiles of
+// one block of weights before the next block's, so that both stay in its L2.
+template <bool DUAL> __global__ __launch_bounds__(256, 2) void coli_fp4_many(Fp4Args a, int n_items) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[FmGeom::kPD * FmGeom::kStage];
+    const int n = a.mats ? min(*a.n_items, n_items) : n_items;
+    const int total = n * a.rtb, per = (total + 7) / 8, j = blockIdx.x >> 3;
+    const int id = (blockIdx.x & 7) * per + j;
+    if (j >= per || id >= total) return;
+    const int grp = id / (8 * a.rtb), in = id - grp * 8 * a.rtb, gi = min(8, n - grp * 8);
+    const int item = grp * 8 + in % gi, rb = in / gi;
+    Fp4Item it = {0, item * a.tile, 0, 0};
+    Fp4Mat mat = a.mat0;
+    if (a.mats) {
+        it = a.items[item];
+        mat = a.mats[it.mat];
+    } else {
+        it.nrows = min(a.tile, a.S - it.r0);
+    }
+    if (it.nrows <= 64) fp4_many<2, DUAL>(a, it, mat, rb, (lds_u8 *)lds);
+    else fp4_many<4, DUAL>(a, it, mat, rb, (lds_u8 *)lds);
 }
 
 // ---------------------------------------------------------------------------
@@ -411,11 +690,11 @@ extern "C" int coli_hip_tensor_quantize_mxfp4(ColiCudaTensor **tensor, const voi
 #define COLI_FP4_TILE 64
 static int fp4_prep(DevCtx *ctx, const float *x, int rows, int I, const ItemArgs *it, Fp4Args *a) {
     const int cp = (I + 255) / 256 * 256;
-    const size_t qb = ((size_t)rows * (cp / 2) + 255) & ~(size_t)255, eb = (size_t)rows * (cp / 32);
+    const size_t n = (size_t)rows + 1, qb = (n * (cp / 2) + 255) & ~(size_t)255, eb = n * (cp / 32);
     if (!reserve_kept(ctx, &ctx->fp4_x, qb + eb, 0)) return 0;
     uint8_t *p = (uint8_t *)ctx->fp4_x.p;
     const QuantArgs q = {x, p, p + qb, rows, I, cp, lanes_log2(cp)};
-    const int nblk = (rows + (256 >> q.lpr) - 1) / (256 >> q.lpr);
+    const int nblk = rows / (256 >> q.lpr) + 1;   // (a row more)
     const dim3 g(nblk + (it ? 1 : 0));
     const ItemArgs none = {};
     if (I < 8) hipLaunchKernelGGL(coli_fp4_prep<2>, g, dim3(256), 0, ctx->stream, q, it ? *it : none, nblk);
@@ -426,12 +705,28 @@ static int fp4_prep(DevCtx *ctx, const float *x, int rows, int I, const ItemArgs
     a->xe = p + qb;
     a->cp = cp;
     a->rows = rows;
-    a->zero = (const uint8_t *)ctx->zeros.p;
     return 1;
+}
+
+// Rows of an item's tile, by the rows of a matrix.
+static int fp4_tile_rows(int rows) {
+    if (const char *f = std::getenv("COLI_HIP_FP4")) {
+        if (std::strcmp(f, "few") == 0) return COLI_FP4_TILE;
+        if (std::strcmp(f, "many") == 0) return COLI_FP4_MANY;
+    }
+    return rows > 64 ? COLI_FP4_MANY : COLI_FP4_TILE;
 }
 
 // The launch over n_items items of tiles of a.tile rows.
 static int fp4_run(DevCtx *ctx, Fp4Args &a, int n_items, bool dual) {
+    if (a.tile == COLI_FP4_MANY) {
+        a.rtb = (a.nrt + (dual ? 7 : 15)) / (dual ? 8 : 16);
+        if ((int64_t)n_items * a.rtb >= (1 << 23)) return 0;
+        const dim3 g((unsigned)(n_items * a.rtb + 7) / 8 * 8);
+        if (dual) hipLaunchKernelGGL((coli_fp4_many<true>), g, dim3(256), 0, ctx->stream, a, n_items);
+        else hipLaunchKernelGGL((coli_fp4_many<false>), g, dim3(256), 0, ctx->stream, a, n_items);
+        return hip_check(hipGetLastError(), "fp4 product");
+    }
     const int W = 8;
     a.rtb = dual ? a.nrt : (a.nrt + 1) / 2;
     if ((int64_t)n_items * a.rtb * 64 * W >= ((int64_t)1 << 32)) return 0;
@@ -450,7 +745,7 @@ int matmul_a4_dev(DevCtx *ctx, ColiCudaTensor *t, float *y_dev, const float *x_d
     if (!fp4_prep(ctx, x_dev, S, t->I, nullptr, &a)) return 0;
     a.mat0 = {t->w, (const uint8_t *)t->sc, nullptr, nullptr};
     a.S = S;
-    a.tile = COLI_FP4_TILE;
+    a.tile = fp4_tile_rows(S);
     a.nrt = t->nrt;
     a.nq = t->nq;
     a.O = t->O;
@@ -538,7 +833,7 @@ extern "C" int coli_hip_experts_a4_dev(ColiHipExperts *x, float *y, const float 
     it.offsets = offsets;
     it.E = x->E;
     it.N = N;
-    it.tile = COLI_FP4_TILE;
+    it.tile = fp4_tile_rows(N / x->E);
     it.room = (int)std::min<int64_t>(N, N / it.tile + x->E);
     if (!reserve_kept(ctx, &ctx->fp4_items, 256 + (size_t)it.room * sizeof(Fp4Item), 0)) return 0;
     it.n_items = (int *)ctx->fp4_items.p;

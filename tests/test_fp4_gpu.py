@@ -181,6 +181,24 @@ def test_matmul(session, I, O, S):
         session.free(h)
 
 
+@pytest.mark.parametrize("pin", ["few", "many"])
+@pytest.mark.parametrize("I,O,S", [(1, 1, 1), (31, 17, 5), (128, 64, 1), (257, 100, 65), (600, 48, 33), (700, 300, 128), (999, 600, 130),
+                                   (1300, 270, 260), (4096, 300, 1), (900, 520, 97)])
+def test_matmul_on_both_kernels(session, monkeypatch, pin, I, O, S):
+    """The kernel of few rows and that of many, pinned, at any size."""
+    monkeypatch.setenv("COLI_HIP_FP4", pin)
+    test_matmul(session, I, O, S)
+
+
+@pytest.mark.parametrize("pin", ["few", "many"])
+@pytest.mark.parametrize("pair", [False, True])
+@pytest.mark.parametrize("E,I,O,counts", [(3, 300, 40, [0, 5, 0]), (4, 257, 17, [1, 64, 0, 65]), (5, 512, 48, [16, 17, 33, 2, 130]),
+                                          (3, 800, 272, [300, 0, 140])])
+def test_experts_on_both_kernels(session, monkeypatch, pin, pair, E, I, O, counts):
+    monkeypatch.setenv("COLI_HIP_FP4", pin)
+    test_experts(session, pair, E, I, O, counts)
+
+
 def test_matmul_one_hot(session):
     """Rows of one 6: every weight at its place, exactly; blocks of other scales beside it."""
     rng = np.random.default_rng(3)
