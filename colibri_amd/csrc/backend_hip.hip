@@ -232,7 +232,8 @@ extern "C" void coli_cuda_shutdown(void) {
                           &ctx->prob, &ctx->stage_w, &ctx->stage_s, &ctx->qdq, &ctx->flags,
                           &ctx->rslot, &ctx->rw, &ctx->tmp_tiles, &ctx->tmp_scales, &ctx->zeros,
                           &ctx->split_cnt, &ctx->idot_y, &ctx->idot_sx, &ctx->lora_h, &ctx->lora_list,
-                          &ctx->gt, &ctx->bal, &ctx->bal_cnt, &ctx->sort_hist, &ctx->fp4_x, &ctx->fp4_items};
+                          &ctx->gt, &ctx->bal, &ctx->bal_cnt, &ctx->sort_hist, &ctx->fp4_x, &ctx->fp4_items,
+                          &ctx->fp4_part};
         for (DevBuf *b : bufs) free_buf(b);
         for (int k = 0; k < ctx->n_outgrown; k++) (void)hipFree(ctx->outgrown[k]);
         for (FragSet &f : ctx->frag)

@@ -98,7 +98,7 @@ struct DevCtx {
     // the fragments, partial, split_cnt, sums, qdq, idot_y and idot_sx grow by
     // reserve_kept: where a graph may hold them, outgrown ones live until shutdown
     DevBuf lora_h, lora_list, gt, bal, bal_cnt;
-    DevBuf sort_hist, fp4_x, fp4_items;   // of the sorted-rows and 4-bit entry points, likewise
+    DevBuf sort_hist, fp4_x, fp4_items, fp4_part;   // of the sorted-rows and 4-bit entry points, likewise
     void *outgrown[COLI_OUTGROWN] = {};
     int n_outgrown = 0;
     // pinned staging

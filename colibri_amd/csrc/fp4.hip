@@ -74,21 +74,21 @@ struct QuantArgs {
     const void *x;
     uint8_t *q4, *e8;
     int rows, cols, cp;   // columns, and as written: cp (operand form, a multiple of 256) or cols
-    int lpr;              // log2 of the lanes that take a row's octets
+    int lpr, chunks;      // log2 of the lanes that take a row's octets, workgroups that share a row
 };
 
 // Lanes of a row take its octets in turn, four to a block of 32. Native bytes, or
 // (OPERAND) rows of cp / 2 and cp / 32 bytes with zeros past the row's end, and behind
 // the last row one of zeros.
 template <typename T, int FORM, bool OPERAND> __device__ __forceinline__ void quant_rows(const QuantArgs &a, int blk) {
-    const int r = (blk << (8 - a.lpr)) + (threadIdx.x >> a.lpr);
-    const int o0 = threadIdx.x & ((1 << a.lpr) - 1);
+    const int grp = blk / a.chunks, r = (grp << (8 - a.lpr)) + (threadIdx.x >> a.lpr);
+    const int o0 = ((blk - grp * a.chunks) << a.lpr) + (threadIdx.x & ((1 << a.lpr) - 1));
     if (r >= a.rows + (OPERAND ? 1 : 0)) return;
     const bool zero = OPERAND && r == a.rows;
     const T *xr = (const T *)a.x + (size_t)(zero ? 0 : r) * a.cols;
     const int end = OPERAND ? a.cp : (a.cols + 31) / 32 * 32;
     const size_t qs = OPERAND ? a.cp / 2 : (a.cols + 1) / 2, es = OPERAND ? a.cp / 32 : (a.cols + 31) / 32;
-    for (int c = 8 * o0; c < end; c += 8 << a.lpr) {
+    for (int c = 8 * o0; c < end; c += (8 << a.lpr) * a.chunks) {
         float v[8];
         uint32_t byte;
         row8<T, FORM>(xr, c, a.cols, v);
@@ -116,16 +116,16 @@ template <typename T, int FORM> __global__ __launch_bounds__(256) void coli_mx_q
 struct DequantArgs {
     const uint8_t *q4, *e8;
     void *y;
-    int rows, cols, lpr;
+    int rows, cols, lpr, chunks;
 };
 template <typename T> __global__ __launch_bounds__(256) void coli_mx_dequant(DequantArgs a) {
     typedef float float2v __attribute__((ext_vector_type(2)));
-    const int r = (blockIdx.x << (8 - a.lpr)) + (threadIdx.x >> a.lpr);
-    const int o0 = threadIdx.x & ((1 << a.lpr) - 1), qs = (a.cols + 1) / 2;
+    const int grp = blockIdx.x / a.chunks, r = (grp << (8 - a.lpr)) + (threadIdx.x >> a.lpr), qs = (a.cols + 1) / 2;
+    const int o0 = ((blockIdx.x - grp * a.chunks) << a.lpr) + (threadIdx.x & ((1 << a.lpr) - 1));
     if (r >= a.rows) return;
     const uint8_t *q = a.q4 + (size_t)r * qs, *e8 = a.e8 + (size_t)r * ((a.cols + 31) / 32);
     T *y = (T *)a.y + (size_t)r * a.cols;
-    for (int c = 8 * o0; c < a.cols; c += 8 << a.lpr) {
+    for (int c = 8 * o0; c < a.cols; c += (8 << a.lpr) * a.chunks) {
         uint32_t u;
         if (qs >= 4) {
             const int p = min(c / 2, qs - 4);
@@ -167,10 +167,14 @@ struct Fp4Args {
     int nrt, nq, O;
     int rtb;                   // row-tile blocks of an item
     const uint8_t *xq, *xe;    // operand rows: cp / 2 codes, cp / 32 scales; row `rows` is zeros
-    int cp;
+    const float *x;            // or the rows themselves, of width I (the kernel quantizes them)
+    int cp, I;
+    int splits, sps;           // K splits (many rows of one matrix): 256-column stages of each
+    float *part;               // their sums [split][S][O]
     const int *src;            // sorted row -> K x row + k (null: the row itself)
     int K, rows;
     float *y;
+    int stream;                // y past the caches (see fp4_run)
     float limit;
 };
 
@@ -230,12 +234,19 @@ __device__ __forceinline__ i32x8 fp4_tile(u32x4 x) {
     return (i32x8){(int)c[0], (int)c[1], (int)d[0], (int)d[1], 0, 0, 0, 0};
 }
 
-// Rows [0, 16 NM) of an item and R weight tiles (DUAL: the gate and the up tile) a
-// workgroup; its W waves take the 128-column steps in turn and add up in LDS, in the
-// order of the waves.
-template <int NM, int R, bool DUAL, int W> __global__ __launch_bounds__(64 * W) void coli_fp4_few(Fp4Args a) {
-    constexpr int U = 2;   // steps whose loads are requested together
+// Few rows: [0, 16 NM) of an item times R weight tiles (DUAL: the gate and the up tile) a
+// workgroup; its eight waves take the 128-column steps in turn, U of them requested
+// together, and add up in LDS, in the order of the waves. The weights' stream is the
+// bound.
+// FORM (of row8; -1: operands in memory): the workgroup quantizes the rows itself, into
+// LDS, behind its first weights' loads. That saves the operands' launch where the rows
+// are so few that 512 threads have done them before the weights are there.
+#define COLI_FP4_WAVES 8
+template <int NM, int R, bool DUAL, int FORM> __global__ __launch_bounds__(64 * COLI_FP4_WAVES) void coli_fp4_few(Fp4Args a) {
+    constexpr int W = COLI_FP4_WAVES, U = NM == 1 ? 4 : 2;
+    constexpr bool OWN = FORM >= 0;
     __shared__ floatx4 part[W][R][NM][64];
+    extern __shared__ __attribute__((aligned(16))) uint8_t xl[];   // (OWN) codes, then scales
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, g = lane >> 4;
     const int item = blockIdx.x / a.rtb, rb = blockIdx.x - item * a.rtb;
@@ -256,6 +267,7 @@ template <int NM, int R, bool DUAL, int W> __global__ __launch_bounds__(64 * W) 
         w[r] = uniform_ptr(DUAL && r ? mat.w1 : mat.w0) + t0 * COLI_TILE_BYTES;
         sc[r] = uniform_ptr(DUAL && r ? mat.s1 : mat.s0) + t0 * 64;
     }
+    const int qs = a.cp / 2, es = a.cp / 32;
     const uint8_t *xq[NM], *xe[NM];
 #pragma unroll
     for (int m = 0; m < NM; m++) {
@@ -265,29 +277,35 @@ template <int NM, int R, bool DUAL, int W> __global__ __launch_bounds__(64 * W) 
             x = x < 0 ? -1 : x / a.K;
         }
         if ((unsigned)x >= (unsigned)a.rows) x = a.rows;
-        xq[m] = a.xq + (size_t)x * (a.cp / 2) + 16 * g;
-        xe[m] = a.xe + (size_t)x * (a.cp / 32);
+        xq[m] = OWN ? xl + x * qs + 16 * g : a.xq + (size_t)x * qs + 16 * g;
+        xe[m] = OWN ? xl + a.rows * qs + x * es : a.xe + (size_t)x * es;
     }
     floatx4 acc[R][NM];
 #pragma unroll
     for (int r = 0; r < R; r++)
 #pragma unroll
         for (int m = 0; m < NM; m++) acc[r][m] = (floatx4){0.f, 0.f, 0.f, 0.f};
-    for (int q0 = wave; q0 < a.nq; q0 += W * U) {
-        u32x4 wv[U][R], xv[U][NM];
-        uint32_t ws[U][R], xs[U][NM];
+    u32x4 wv[U][R], xv[U][NM];
+    uint32_t ws[U][R], xs[U][NM];
+    auto load_w = [&](int q0) {
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int q = min(q0 + W * u, a.nq - 1);
 #pragma unroll
             for (int r = 0; r < R; r++) {
-                wv[u][r] = *GPTR(u32x4, w[r] + (size_t)q * COLI_TILE_BYTES + lane * 16);
+                wv[u][r] = __builtin_nontemporal_load(GPTR(u32x4, w[r] + (size_t)q * COLI_TILE_BYTES + lane * 16));
                 ws[u][r] = *GPTR(uint32_t, sc[r] + (size_t)q * 64 + c * 4);
             }
+        }
+    };
+    auto compute = [&](int q0) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int q = min(q0 + W * u, a.nq - 1);
 #pragma unroll
             for (int m = 0; m < NM; m++) {
-                xv[u][m] = *GPTR(u32x4, xq[m] + (size_t)q * 64);
-                xs[u][m] = *GPTR(uint32_t, xe[m] + (size_t)q * 4);
+                xv[u][m] = OWN ? *(const u32x4 *)(xq[m] + q * 64) : (u32x4)*GPTR(u32x4, xq[m] + (size_t)q * 64);
+                xs[u][m] = OWN ? *(const uint32_t *)(xe[m] + q * 4) : *GPTR(uint32_t, xe[m] + (size_t)q * 4);
             }
         }
 #pragma unroll
@@ -306,6 +324,25 @@ template <int NM, int R, bool DUAL, int W> __global__ __launch_bounds__(64 * W) 
                                                                                 (int)(xs[u][m] >> (8 * g)));
             }
         }
+    };
+    load_w(wave);
+    if constexpr (OWN) {
+        const int opr = a.cp / 8;   // octets of a row
+        for (int o = threadIdx.x; o < a.rows * opr; o += 64 * W) {
+            const int r = o / opr, k = 8 * (o - r * opr);
+            float v[8];
+            uint32_t byte;
+            row8<float, FORM>(a.x + (size_t)r * a.I, k, a.I, v);
+            const uint32_t u = mx_codes(v, byte);
+            *(uint32_t *)(xl + r * qs + k / 2) = u;
+            if ((threadIdx.x & 3) == 0) xl[a.rows * qs + r * es + k / 32] = (uint8_t)byte;
+        }
+        __syncthreads();
+    }
+    compute(wave);
+    for (int q0 = wave + W * U; q0 < a.nq; q0 += W * U) {
+        load_w(q0);
+        compute(q0);
     }
 #pragma unroll
     for (int r = 0; r < R; r++)
@@ -362,7 +399,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t fp4_rsrc(const void *p, uint32
 __device__ __forceinline__ i32x8 fp4_op(u32x4 v) { return (i32x8){(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0}; }
 // NB: 32-row blocks
 template <int NB, bool DUAL> __device__ __forceinline__ void fp4_many(const Fp4Args &a, const Fp4Item &it, const Fp4Mat &mat,
-                                                                      int rb, lds_u8 *lds) {
+                                                                      int rb, int split, lds_u8 *lds) {
     using G = FmGeom;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 31, g = lane >> 5;
@@ -403,7 +440,7 @@ template <int NB, bool DUAL> __device__ __forceinline__ void fp4_many(const Fp4A
         xa[k] = row_of(r) * qs + 16 * ((lane & 7) ^ ((r >> 1) & 7));
     }
     const uint32_t xs = row_of(32 * wave + (lane >> 1)) * es + 4 * (lane & 1);
-    const int ns = a.cp / 256;
+    const int s0 = split * a.sps, ns = min(a.cp / 256, s0 + a.sps);   // this workgroup's stages
     auto issue = [&](int s, lds_u8 *st) {
         s = min(s, ns - 1);
 #pragma unroll
@@ -523,12 +560,12 @@ template <int NB, bool DUAL> __device__ __forceinline__ void fp4_many(const Fp4A
     };
     lds_u8 *const slot[3] = {lds, lds + G::kStage, lds + 2 * G::kStage};
     asm volatile("" ::"v"(lds) : "memory");
-    issue(0, slot[0]);
-    issue(1, slot[1]);
+    issue(s0, slot[0]);
+    issue(s0 + 1, slot[1]);
 #pragma unroll
-    for (int r = 0; r < 2; r++) load_w(0, r, 0);
+    for (int r = 0; r < 2; r++) load_w(0, r, 2 * s0);
 #pragma unroll
-    for (int r = 0; r < 2; r++) load_w(1, r, 1);
+    for (int r = 0; r < 2; r++) load_w(1, r, 2 * s0 + 1);
 #pragma unroll
     for (int r = 0; r < 2; r++) turn(0, r);
     __builtin_amdgcn_s_waitcnt(0);   // (a builtin: the compiler counts on from it)
@@ -555,7 +592,7 @@ template <int NB, bool DUAL> __device__ __forceinline__ void fp4_many(const Fp4A
             group(s, kt, std::integral_constant<int, 7>{}, slot);
         }
     };
-    for (int s = 0;;) {
+    for (int s = s0;;) {
         stage(s, std::integral_constant<int, 0>{});
         if (++s >= ns) break;
         stage(s, std::integral_constant<int, 1>{});
@@ -570,7 +607,7 @@ template <int NB, bool DUAL> __device__ __forceinline__ void fp4_many(const Fp4A
 #pragma unroll
     for (int r = 0; r < (DUAL ? 1 : 2); r++) {
         const int o = 16 * rt[r] + n;
-        float *y = a.y + (size_t)it.r0 * a.O + o;
+        float *y = (a.splits > 1 ? a.part + (size_t)split * a.S * a.O : a.y) + (size_t)it.r0 * a.O + o;
         if (o >= a.O) continue;
 #pragma unroll
         for (int b = 0; b < NB; b++)
@@ -579,7 +616,9 @@ template <int NB, bool DUAL> __device__ __forceinline__ void fp4_many(const Fp4A
                 const int row = 32 * b + 8 * (i >> 2) + 4 * g + (i & 3);
                 float v = acc[r][b][i];
                 if constexpr (DUAL) v = swiglu_out(v, acc[1][b][i], a.limit);
-                if (row < it.nrows) y[(size_t)row * a.O] = v;
+                if (row >= it.nrows) continue;
+                if (a.stream) __builtin_nontemporal_store(v, y + (size_t)row * a.O);
+                else y[(size_t)row * a.O] = v;
             }
     }
 }
@@ -588,9 +627,11 @@ template <int NB, bool DUAL> __device__ __forceinline__ void fp4_many(const Fp4A
 template <bool DUAL> __global__ __launch_bounds__(256, 2) void coli_fp4_many(Fp4Args a, int n_items) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[FmGeom::kPD * FmGeom::kStage];
     const int n = a.mats ? min(*a.n_items, n_items) : n_items;
-    const int total = n * a.rtb, per = (total + 7) / 8, j = blockIdx.x >> 3;
-    const int id = (blockIdx.x & 7) * per + j;
+    const int total = n * a.rtb * a.splits, per = (total + 7) / 8, j = blockIdx.x >> 3;
+    int id = (blockIdx.x & 7) * per + j;
     if (j >= per || id >= total) return;
+    const int split = id / (n * a.rtb);
+    id -= split * n * a.rtb;
     const int grp = id / (8 * a.rtb), in = id - grp * 8 * a.rtb, gi = min(8, n - grp * 8);
     const int item = grp * 8 + in % gi, rb = in / gi;
     Fp4Item it = {0, item * a.tile, 0, 0};
@@ -601,8 +642,24 @@ template <bool DUAL> __global__ __launch_bounds__(256, 2) void coli_fp4_many(Fp4
     } else {
         it.nrows = min(a.tile, a.S - it.r0);
     }
-    if (it.nrows <= 64) fp4_many<2, DUAL>(a, it, mat, rb, (lds_u8 *)lds);
-    else fp4_many<4, DUAL>(a, it, mat, rb, (lds_u8 *)lds);
+    if (it.nrows <= 64) fp4_many<2, DUAL>(a, it, mat, rb, split, (lds_u8 *)lds);
+    else fp4_many<4, DUAL>(a, it, mat, rb, split, (lds_u8 *)lds);
+}
+
+// The K splits' sums in their order: n outputs, four a thread.
+__global__ __launch_bounds__(256) void coli_fp4_join(const float *part, int splits, size_t n, float *y) {
+    const size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i + 4 <= n) {
+        floatx4 v = {};
+        for (int p = 0; p < splits; p++) v += *GPTR(f4u, part + p * n + i);
+        *(f4u *)(y + i) = v;
+    } else {
+        for (size_t k = i; k < n; k++) {
+            float v = 0.0f;
+            for (int p = 0; p < splits; p++) v += part[p * n + k];
+            y[k] = v;
+        }
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -614,17 +671,25 @@ static int lanes_log2(int cols) {   // lanes of a row: its octets, 4 to 256
     return l;
 }
 
+// Workgroups for rows of `cols` columns: groups of rows, and where these are few a row
+// of more than 2048 columns by several (8192 rows of 7168: 55 us whole, 59 in pieces).
+static unsigned mx_grid(int rows, int cols, int lpr, int *chunks) {
+    const unsigned groups = (unsigned)((rows + (256 >> lpr) - 1) / (256 >> lpr));
+    *chunks = (int)std::max(1u, std::min((unsigned)((cols + (8 << lpr) - 1) / (8 << lpr)), 2048 / groups));
+    return groups * *chunks;
+}
+
 static size_t mx_q4_bytes(int rows, int cols) { return (size_t)rows * ((cols + 1) / 2); }
 static size_t mx_e8_bytes(int rows, int cols) { return (size_t)rows * ((cols + 31) / 32); }
 
-template <typename T> static void quant_launch(const QuantArgs &a, hipStream_t st) {
-    const dim3 g((unsigned)((a.rows + (256 >> a.lpr) - 1) / (256 >> a.lpr)));
+template <typename T> static void quant_launch(QuantArgs &a, hipStream_t st) {
+    const dim3 g(mx_grid(a.rows, a.cols, a.lpr, &a.chunks));
     if (a.cols < 8) hipLaunchKernelGGL((coli_mx_quant<T, 2>), g, dim3(256), 0, st, a);
     else if (a.cols % 8) hipLaunchKernelGGL((coli_mx_quant<T, 1>), g, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((coli_mx_quant<T, 0>), g, dim3(256), 0, st, a);
 }
 static int quantize(DevCtx *ctx, const void *x, int dtype, int rows, int cols, uint8_t *q4, uint8_t *e8) {
-    const QuantArgs a = {x, q4, e8, rows, cols, cols, lanes_log2(cols)};
+    QuantArgs a = {x, q4, e8, rows, cols, cols, lanes_log2(cols), 1};
     if (dtype == 0) quant_launch<float>(a, ctx->stream);
     else if (dtype == 1) quant_launch<_Float16>(a, ctx->stream);
     else quant_launch<__bf16>(a, ctx->stream);
@@ -660,8 +725,8 @@ extern "C" int coli_hip_mxfp4_dequantize_dev(int device, const unsigned char *q4
     if (!bind_ctx(ctx)) return 0;
     if (!rows) return 1;
     forget_emitted(ctx, y, yb);
-    const DequantArgs a = {q4, e8, y, rows, cols, lanes_log2(cols)};
-    const dim3 g((unsigned)((rows + (256 >> a.lpr) - 1) / (256 >> a.lpr)));
+    DequantArgs a = {q4, e8, y, rows, cols, lanes_log2(cols), 1};
+    const dim3 g(mx_grid(rows, cols, a.lpr, &a.chunks));
     if (dtype == 0) hipLaunchKernelGGL(coli_mx_dequant<float>, g, dim3(256), 0, ctx->stream, a);
     else if (dtype == 1) hipLaunchKernelGGL(coli_mx_dequant<_Float16>, g, dim3(256), 0, ctx->stream, a);
     else hipLaunchKernelGGL(coli_mx_dequant<__bf16>, g, dim3(256), 0, ctx->stream, a);
@@ -687,14 +752,13 @@ extern "C" int coli_hip_tensor_quantize_mxfp4(ColiCudaTensor **tensor, const voi
 }
 
 // Rows of x as operands of the products (and the items of sorted rows beside it).
-#define COLI_FP4_TILE 64
 static int fp4_prep(DevCtx *ctx, const float *x, int rows, int I, const ItemArgs *it, Fp4Args *a) {
     const int cp = (I + 255) / 256 * 256;
     const size_t n = (size_t)rows + 1, qb = (n * (cp / 2) + 255) & ~(size_t)255, eb = n * (cp / 32);
     if (!reserve_kept(ctx, &ctx->fp4_x, qb + eb, 0)) return 0;
     uint8_t *p = (uint8_t *)ctx->fp4_x.p;
-    const QuantArgs q = {x, p, p + qb, rows, I, cp, lanes_log2(cp)};
-    const int nblk = rows / (256 >> q.lpr) + 1;   // (a row more)
+    QuantArgs q = {x, p, p + qb, rows, I, cp, lanes_log2(cp), 1};
+    const int nblk = (int)mx_grid(rows + 1, cp, q.lpr, &q.chunks);
     const dim3 g(nblk + (it ? 1 : 0));
     const ItemArgs none = {};
     if (I < 8) hipLaunchKernelGGL(coli_fp4_prep<2>, g, dim3(256), 0, ctx->stream, q, it ? *it : none, nblk);
@@ -708,31 +772,105 @@ static int fp4_prep(DevCtx *ctx, const float *x, int rows, int I, const ItemArgs
     return 1;
 }
 
-// Rows of an item's tile, by the rows of a matrix.
-static int fp4_tile_rows(int rows) {
-    if (const char *f = std::getenv("COLI_HIP_FP4")) {
-        if (std::strcmp(f, "few") == 0) return COLI_FP4_TILE;
-        if (std::strcmp(f, "many") == 0) return COLI_FP4_MANY;
+// How S rows of a matrix are multiplied: rows of a tile (COLI_FP4_MANY: that kernel),
+// row tiles a workgroup of the kernel of few rows, K splits of the one of many, and
+// whether the former quantizes the rows itself.
+struct Fp4Plan {
+    int tile, R, splits;
+    bool own;
+};
+// Row tiles a workgroup: as many as leave most CUs one, since each workgroup reads all the
+// rows' operands (4096 x 14336, us with 1 / 2 / 4: 16 rows 13.9 / 11.0 / 9.7, 64 rows 37 /
+// 23 / 18; 14336 x 4096, 16 rows: 15.1 / 17.7 / 21.3).
+static int fp4_row_tiles(const DevCtx *ctx, int nrt, bool dual) {
+    int R = 1;
+    while (!dual && R < 4 && nrt / (2 * R) >= ctx->cu_count * 4 / 5) R *= 2;
+    return R;
+}
+static const char *fp4_pin(void) { return std::getenv("COLI_HIP_FP4"); }
+static Fp4Plan fp4_plan(const DevCtx *ctx, const ColiCudaTensor *t, int S) {
+    const int cp = (t->I + 255) / 256 * 256, cus = ctx->cu_count;
+    Fp4Plan p = {S <= 16 ? 16 : S <= 32 ? 32 : 64, fp4_row_tiles(ctx, t->nrt, false), 1, false};
+    // Quantizing the rows in every workgroup against a launch of their own (3 us): up to
+    // 16384 columns in all, 49152 where there is a workgroup a CU at most (14336 x 4096, 3
+    // rows: 13.9 / 14.2 us, 4096 x 14336 with four tiles a workgroup, 4 rows 8.4 / 8.9, 8
+    // rows 9.9 / 9.2; 7168 x 2048, 8 rows 10.6 / 10.6).
+    const int64_t cols = (int64_t)S * cp;
+    p.own = S <= 16 && t->I >= 8 && cols <= (t->nrt <= cus ? 49152 : 16384);
+    if (p.own)   // few columns: each workgroup's share of the work is small beside its latency
+        while (p.R > 1 && cols * (t->nrt / (p.R / 2)) <= (int64_t)4096 * 1024) p.R /= 2;
+    // The kernel of many rows, modelled in us from measurements: 8 and a stage of 256
+    // columns 0.72 (1.06 with every CU at it), each further workgroup of a CU as much
+    // again, a join of K splits 2.5 and 0.3 a MB of sums. The other: 5.5, the weights at
+    // 6.5 TB/s and the rows' operands, once for each workgroup, at 5 TB/s.
+    const int ns = cp / 256, wgs = (S + COLI_FP4_MANY - 1) / COLI_FP4_MANY * ((t->nrt + 15) / 16);
+    double best = 1e30;
+    for (int P = 1; P <= 32 && P <= ns; P *= 2) {
+        const int sps = (ns + P - 1) / P, n = wgs * P;
+        const double full = std::min(1.0, (double)n / cus);
+        const double us = 8.0 + sps * (0.72 + 0.34 * full) * std::max(1.0, (double)n / cus) +
+                          (P > 1 ? 2.5 + 0.3e-6 * 4.0 * P * (double)S * t->O : 0.0);
+        if (us < best) {
+            best = us;
+            p.splits = P;
+        }
     }
-    return rows > 64 ? COLI_FP4_MANY : COLI_FP4_TILE;
+    const int nwg = (t->nrt + p.R - 1) / p.R, all = nwg * ((S + p.tile - 1) / p.tile);
+    const double few = 5.5 + (double)t->w_bytes / 6.5e6 +
+                       0.2e-6 * nwg * (double)S * cp * 0.53 * std::max(1.0, 0.8 * cus / all);
+    const char *pin = fp4_pin();
+    if (pin ? std::strcmp(pin, "many") == 0 : S > 16 && best < few) {
+        p.tile = COLI_FP4_MANY;
+        p.own = false;
+    }
+    return p;
 }
 
-// The launch over n_items items of tiles of a.tile rows.
-static int fp4_run(DevCtx *ctx, Fp4Args &a, int n_items, bool dual) {
+template <int NM, int FORM> static void few_launch(const Fp4Args &a, dim3 g, bool dual, int R, hipStream_t st) {
+    const dim3 b(64 * COLI_FP4_WAVES);
+    const size_t own = FORM < 0 ? 0 : (size_t)a.rows * (a.cp / 2 + a.cp / 32);
+    if constexpr (FORM < 0) {   // (rows of pairs come as operands)
+        if (dual) {
+            hipLaunchKernelGGL((coli_fp4_few<NM, 2, true, FORM>), g, b, 0, st, a);
+            return;
+        }
+    }
+    if (R == 4) hipLaunchKernelGGL((coli_fp4_few<NM, 4, false, FORM>), g, b, own, st, a);
+    else if (R == 2) hipLaunchKernelGGL((coli_fp4_few<NM, 2, false, FORM>), g, b, own, st, a);
+    else hipLaunchKernelGGL((coli_fp4_few<NM, 1, false, FORM>), g, b, own, st, a);
+}
+
+// The launch over n_items items of tiles of a.tile rows, `rows` in all.
+static int fp4_run(DevCtx *ctx, Fp4Args &a, int n_items, int rows, bool dual, const Fp4Plan &plan) {
     if (a.tile == COLI_FP4_MANY) {
         a.rtb = (a.nrt + (dual ? 7 : 15)) / (dual ? 8 : 16);
-        if ((int64_t)n_items * a.rtb >= (1 << 23)) return 0;
-        const dim3 g((unsigned)(n_items * a.rtb + 7) / 8 * 8);
+        if ((int64_t)n_items * a.rtb * plan.splits >= (1 << 23)) return 0;
+        a.sps = (a.cp / 256 + plan.splits - 1) / plan.splits;
+        a.splits = (a.cp / 256 + a.sps - 1) / a.sps;
+        if (a.splits > 1 && !reserve_kept(ctx, &ctx->fp4_part, (size_t)a.splits * a.S * a.O * 4, 0)) return 0;
+        a.part = (float *)ctx->fp4_part.p;
+        // Outputs beyond half of the 256 MB cache go past it (8192 x 4096 x 14336 380 -> 290
+        // us); smaller ones may be there still when they are read (2048 rows: no difference).
+        a.stream = a.splits == 1 && (size_t)rows * a.O * 4 > ((size_t)128 << 20);
+        const dim3 g((unsigned)(n_items * a.rtb * a.splits + 7) / 8 * 8);
         if (dual) hipLaunchKernelGGL((coli_fp4_many<true>), g, dim3(256), 0, ctx->stream, a, n_items);
         else hipLaunchKernelGGL((coli_fp4_many<false>), g, dim3(256), 0, ctx->stream, a, n_items);
-        return hip_check(hipGetLastError(), "fp4 product");
+        if (!hip_check(hipGetLastError(), "fp4 product")) return 0;
+        if (a.splits > 1) {
+            const size_t n = (size_t)a.S * a.O;
+            hipLaunchKernelGGL(coli_fp4_join, dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, ctx->stream, a.part, a.splits, n, a.y);
+        }
+        return hip_check(hipGetLastError(), "fp4 join");
     }
-    const int W = 8;
-    a.rtb = dual ? a.nrt : (a.nrt + 1) / 2;
-    if ((int64_t)n_items * a.rtb * 64 * W >= ((int64_t)1 << 32)) return 0;
+    const int R = plan.R;
+    a.rtb = (a.nrt + R - 1) / R;
+    if ((int64_t)n_items * a.rtb >= (1 << 23)) return 0;
     const dim3 g((unsigned)n_items * a.rtb);
-    if (dual) hipLaunchKernelGGL((coli_fp4_few<4, 2, true, W>), g, dim3(64 * W), 0, ctx->stream, a);
-    else hipLaunchKernelGGL((coli_fp4_few<4, 2, false, W>), g, dim3(64 * W), 0, ctx->stream, a);
+    if (a.x && a.I % 8) few_launch<1, 1>(a, g, dual, R, ctx->stream);
+    else if (a.x) few_launch<1, 0>(a, g, dual, R, ctx->stream);
+    else if (a.tile <= 16) few_launch<1, -1>(a, g, dual, R, ctx->stream);
+    else if (a.tile <= 32) few_launch<2, -1>(a, g, dual, R, ctx->stream);
+    else few_launch<4, -1>(a, g, dual, R, ctx->stream);
     return hip_check(hipGetLastError(), "fp4 product");
 }
 
@@ -742,16 +880,24 @@ int matmul_a4_dev(DevCtx *ctx, ColiCudaTensor *t, float *y_dev, const float *x_d
     Fp4Args a = {};
     if (t->I > (int)COLI_FP4_MAX_I) return 0;
     forget_emitted(ctx, y_dev, (size_t)S * t->O * 4);
-    if (!fp4_prep(ctx, x_dev, S, t->I, nullptr, &a)) return 0;
+    const Fp4Plan plan = fp4_plan(ctx, t, S);
+    a.tile = plan.tile;
+    if (plan.own) {
+        a.x = x_dev;
+        a.I = t->I;
+        a.cp = (t->I + 255) / 256 * 256;
+        a.rows = S;
+    } else if (!fp4_prep(ctx, x_dev, S, t->I, nullptr, &a)) {
+        return 0;
+    }
     a.mat0 = {t->w, (const uint8_t *)t->sc, nullptr, nullptr};
     a.S = S;
-    a.tile = fp4_tile_rows(S);
     a.nrt = t->nrt;
     a.nq = t->nq;
     a.O = t->O;
     a.K = 1;
     a.y = y_dev;
-    return fp4_run(ctx, a, (S + a.tile - 1) / a.tile, false);
+    return fp4_run(ctx, a, (S + a.tile - 1) / a.tile, S, false, plan);
 }
 
 extern "C" int coli_hip_fp4_matmul_a4_dev(ColiCudaTensor *t, float *y_dev, const float *x_dev, int S) {
@@ -833,7 +979,14 @@ extern "C" int coli_hip_experts_a4_dev(ColiHipExperts *x, float *y, const float 
     it.offsets = offsets;
     it.E = x->E;
     it.N = N;
-    it.tile = fp4_tile_rows(N / x->E);
+    // Tiles by the rows of an expert, were all that have some alike (us with tiles of 16 /
+    // of 128 rows on that kernel: 64 pairs of 2048 x 1024, 256 rows 25.6 / 29.3, 512 28.5 /
+    // 30.3, 1024 41 / 31; 32 pairs of 7168 x 2048, 256 rows 90 / 96, 512 137 / 99).
+    const int mean = N / std::min(N, x->E);
+    const char *pin = fp4_pin();
+    Fp4Plan plan = {mean <= 8 ? 16 : COLI_FP4_MANY, fp4_row_tiles(ctx, x->nrt, x->dual != 0), 1, false};
+    if (pin) plan.tile = std::strcmp(pin, "many") == 0 ? COLI_FP4_MANY : mean <= 16 ? 16 : mean <= 32 ? 32 : 64;
+    it.tile = plan.tile;
     it.room = (int)std::min<int64_t>(N, N / it.tile + x->E);
     if (!reserve_kept(ctx, &ctx->fp4_items, 256 + (size_t)it.room * sizeof(Fp4Item), 0)) return 0;
     it.n_items = (int *)ctx->fp4_items.p;
@@ -851,5 +1004,5 @@ extern "C" int coli_hip_experts_a4_dev(ColiHipExperts *x, float *y, const float 
     a.K = K;
     a.y = y;
     a.limit = x->limit;
-    return fp4_run(ctx, a, it.room, x->dual != 0);
+    return fp4_run(ctx, a, it.room, N, x->dual != 0, plan);
 }
