@@ -7,8 +7,9 @@
 typedef uint32_t u32x4a1 __attribute__((ext_vector_type(4), aligned(1)));   // 16 bytes at any address
 typedef uint32_t u32a1 __attribute__((aligned(1)));
 
-// N elements from p on as f32, and back, rounded to nearest even: 16 bytes a load.
-template <typename T, int N> __device__ __forceinline__ void el_load(const T *p, float (&f)[N]) {
+// N elements from p on as f32, and back, rounded to nearest even: 16 bytes a load. NT: past
+// the caches.
+template <typename T, int N, bool NT = false> __device__ __forceinline__ void el_load(const T *p, float (&f)[N]) {
     constexpr int V = 16 / sizeof(T);
     if constexpr (N % V) {
 #pragma unroll
@@ -17,13 +18,14 @@ template <typename T, int N> __device__ __forceinline__ void el_load(const T *p,
         struct Raw { T e[V]; };
 #pragma unroll
         for (int k = 0; k < N; k += V) {
-            const Raw r = __builtin_bit_cast(Raw, (u32x4)*GPTR(u32x4a1, p + k));
+            const Raw r = __builtin_bit_cast(Raw, NT ? (u32x4)__builtin_nontemporal_load(GPTR(u32x4a1, p + k))
+                                                     : (u32x4)*GPTR(u32x4a1, p + k));
 #pragma unroll
             for (int i = 0; i < V; i++) f[k + i] = (float)r.e[i];
         }
     }
 }
-template <typename T, int N> __device__ __forceinline__ void el_store(T *p, const float (&f)[N]) {
+template <typename T, int N, bool NT = false> __device__ __forceinline__ void el_store(T *p, const float (&f)[N]) {
     constexpr int V = 16 / sizeof(T);
     if constexpr (N % V) {
 #pragma unroll
@@ -35,7 +37,8 @@ template <typename T, int N> __device__ __forceinline__ void el_store(T *p, cons
             Raw r;
 #pragma unroll
             for (int i = 0; i < V; i++) r.e[i] = (T)f[k + i];
-            *(u32x4a1 *)(p + k) = __builtin_bit_cast(u32x4, r);
+            if constexpr (NT) __builtin_nontemporal_store((u32x4a1)__builtin_bit_cast(u32x4, r), (u32x4a1 *)(p + k));
+            else *(u32x4a1 *)(p + k) = __builtin_bit_cast(u32x4, r);
         }
     }
 }

@@ -796,7 +796,7 @@ static Fp4Plan fp4_plan(const DevCtx *ctx, const ColiCudaTensor *t, int S) {
     // rows: 13.9 / 14.2 us, 4096 x 14336 with four tiles a workgroup, 4 rows 8.4 / 8.9, 8
     // rows 9.9 / 9.2; 7168 x 2048, 8 rows 10.6 / 10.6).
     const int64_t cols = (int64_t)S * cp;
-    p.own = S <= 16 && t->I >= 8 && cols <= (t->nrt <= cus ? 49152 : 16384);
+    p.own = S <= 32 && t->I >= 8 && cols <= (t->nrt <= cus ? 49152 : 16384);
     if (p.own)   // few columns: each workgroup's share of the work is small beside its latency
         while (p.R > 1 && cols * (t->nrt / (p.R / 2)) <= (int64_t)4096 * 1024) p.R /= 2;
     // The kernel of many rows, modelled in us from measurements: 8 and a stage of 256
@@ -866,8 +866,10 @@ static int fp4_run(DevCtx *ctx, Fp4Args &a, int n_items, int rows, bool dual, co
     a.rtb = (a.nrt + R - 1) / R;
     if ((int64_t)n_items * a.rtb >= (1 << 23)) return 0;
     const dim3 g((unsigned)n_items * a.rtb);
-    if (a.x && a.I % 8) few_launch<1, 1>(a, g, dual, R, ctx->stream);
-    else if (a.x) few_launch<1, 0>(a, g, dual, R, ctx->stream);
+    if (a.x && a.I % 8 && a.tile <= 16) few_launch<1, 1>(a, g, dual, R, ctx->stream);
+    else if (a.x && a.I % 8) few_launch<2, 1>(a, g, dual, R, ctx->stream);
+    else if (a.x && a.tile <= 16) few_launch<1, 0>(a, g, dual, R, ctx->stream);
+    else if (a.x) few_launch<2, 0>(a, g, dual, R, ctx->stream);
     else if (a.tile <= 16) few_launch<1, -1>(a, g, dual, R, ctx->stream);
     else if (a.tile <= 32) few_launch<2, -1>(a, g, dual, R, ctx->stream);
     else few_launch<4, -1>(a, g, dual, R, ctx->stream);

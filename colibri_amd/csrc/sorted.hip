@@ -29,6 +29,7 @@ struct SortArgs {
     size_t rb;
     int *offsets, *src, *pos, *hist;
     int per, nblk;
+    int stream;   // xs past the caches
 };
 
 // Expert of selection s, E where it is not live.
@@ -72,9 +73,13 @@ __device__ __forceinline__ void copy_piece(const SortArgs &a, int t, const int *
         return;
     }
     const size_t p = min(c, a.rb - 16);
-    const u32x4a1 v = *GPTR(u32x4a1, xr + p);
-    for (int k = 0; k < a.K; k++)
-        if (place[k] >= 0) *(u32x4a1 *)(a.xs + (size_t)place[k] * a.rb + p) = v;
+    const u32x4 v = *GPTR(u32x4a1, xr + p);
+    for (int k = 0; k < a.K; k++) {
+        if (place[k] < 0) continue;
+        u32x4a1 *to = (u32x4a1 *)(a.xs + (size_t)place[k] * a.rb + p);
+        if (a.stream) __builtin_nontemporal_store(v, to);
+        else *to = v;
+    }
 }
 
 // Few selections: one launch. A workgroup (row, piece) counts, for each of its
@@ -149,14 +154,27 @@ __global__ __launch_bounds__(1024) void coli_dispatch_place(SortArgs a) {
     const int s0 = b * a.per + wave * (a.per / 16), s1 = min(min(a.N, s0 + a.per / 16), (b + 1) * a.per);
     int *mine = at + wave * a.E;
     for (int e = tid; e < 16 * a.E; e += 1024) at[e] = 0;
+    // counts of the workgroups before this one and of all, 1024 / 2^lg threads an expert
+    __shared__ int part[2][1024];
     int before = 0, sum = 0, total;
-    if (tid < a.E)
-        for (int q = 0; q < a.nblk; q++) {
-            const int v = a.hist[q * a.E + tid];
+    const int lg = 32 - __clz(a.E - 1 | 1), e0 = tid & ((1 << lg) - 1);
+    if (e0 < a.E)
+#pragma unroll 8
+        for (int q = tid >> lg; q < a.nblk; q += 1024 >> lg) {
+            const int v = a.hist[q * a.E + e0];
             sum += v;
             before += q < b ? v : 0;
         }
-    const int first = block_scan<1024>(sum, tmp, total);   // (its barrier is behind the clear)
+    part[0][tid] = before;
+    part[1][tid] = sum;
+    __syncthreads();
+    before = sum = 0;
+    if (tid < a.E)
+        for (int q = tid; q < 1024; q += 1 << lg) {
+            before += part[0][q];
+            sum += part[1][q];
+        }
+    const int first = block_scan<1024>(sum, tmp, total);
     for (int s = s0 + lane; s < s1; s += 64) {
         const int e = sort_key(a, s);
         if (e < a.E) atomicAdd(mine + e, 1);
@@ -246,8 +264,9 @@ extern "C" int coli_hip_dispatch_dev(int device, const int *idx, const int *keff
         hipLaunchKernelGGL(coli_dispatch_few, dim3(T + 1, pieces), dim3(256), 0, st, a);
         return hip_check(hipGetLastError(), "dispatch");
     }
-    a.per = std::max(4096, (a.N + COLI_SORT_BLOCKS - 1) / COLI_SORT_BLOCKS + 1023 & ~1023);
+    a.per = std::max(1024, (a.N + COLI_SORT_BLOCKS - 1) / COLI_SORT_BLOCKS + 1023 & ~1023);
     a.nblk = (a.N + a.per - 1) / a.per;
+    a.stream = xb * K > ((size_t)128 << 20);   // more than the 256 MB cache keeps for whoever reads them next
     if (!reserve_kept(ctx, &ctx->sort_hist, (size_t)COLI_SORT_BLOCKS * COLI_SORT_MAX_E * 4, 0)) return 0;
     a.hist = (int *)ctx->sort_hist.p;
     hipLaunchKernelGGL(coli_dispatch_count, dim3(a.nblk), dim3(1024), 0, st, a);
@@ -273,7 +292,7 @@ struct CombineArgs {
 // One row t a workgroup and 256 x VE columns. The loads of up to KB selections are
 // requested together: a place that is not live reads the row of one that is (or
 // row 0) and counts zero, so no load waits behind a branch.
-template <typename T, int VE, int KB> __global__ __launch_bounds__(256) void coli_combine(CombineArgs a) {
+template <typename T, int VE, int KB, bool NT> __global__ __launch_bounds__(256) void coli_combine(CombineArgs a) {
     const int t = blockIdx.x, c0 = (blockIdx.y * 256 + threadIdx.x) * VE;
     if (c0 >= a.D) return;
     const int c = min(c0, a.D - VE);
@@ -288,7 +307,7 @@ template <typename T, int VE, int KB> __global__ __launch_bounds__(256) void col
             const int p = pos[min(k0 + i, a.K - 1)];
             const bool in = (unsigned)p < (unsigned)a.N;
             live[i] = in && k0 + i < a.K;
-            el_load<T, VE>((const T *)a.ys + (size_t)(in ? p : 0) * a.D + c, v[i]);
+            el_load<T, VE, NT>((const T *)a.ys + (size_t)(in ? p : 0) * a.D + c, v[i]);
         }
 #pragma unroll
         for (int i = 0; i < KB; i++) {
@@ -302,7 +321,7 @@ template <typename T, int VE, int KB> __global__ __launch_bounds__(256) void col
 
 // Gradients: a wave for each selection. Neighbours share the row of dout, which
 // stays cached.
-template <typename T, int VE> __global__ __launch_bounds__(256) void coli_combine_grad(CombineArgs a) {
+template <typename T, int VE, bool NT> __global__ __launch_bounds__(256) void coli_combine_grad(CombineArgs a) {
     const int64_t s = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 4 + (threadIdx.x >> 6);
     if (s >= (int64_t)a.T * a.K) return;
     const int lane = threadIdx.x & 63, t = (int)(s / a.K), p = a.pos[s];
@@ -328,7 +347,7 @@ template <typename T, int VE> __global__ __launch_bounds__(256) void coli_combin
         if (a.dys) {
 #pragma unroll
             for (int i = 0; i < VE; i++) g[i] *= f;
-            el_store<T, VE>(dy + c, g);
+            el_store<T, VE, NT>(dy + c, g);
         }
     }
     if (!a.dw) return;
@@ -342,25 +361,31 @@ static bool combine_shape_ok(int dtype, int T, int K, int N, int D) {
            (int64_t)T * K <= (1 << 30) && N >= 0 && D >= 1 && D <= (1 << 24);
 }
 
-template <typename T, int VE> static void combine_launch(const CombineArgs &a, hipStream_t st) {
+// ys (and dys) beyond half of the 256 MB cache go past it: combine of 32768 bf16 rows
+// of 7168 122 -> 117 us, its gradient 185 -> 175; smaller ones may be there still for
+// whoever reads them next.
+template <typename T, int VE> static void combine_launch(const CombineArgs &a, bool grad, hipStream_t st) {
+    const bool nt = VE > 1 && (size_t)a.N * a.D * sizeof(T) > ((size_t)128 << 20);
+    if (grad) {
+        const unsigned nw = (unsigned)(((int64_t)a.T * a.K + 3) / 4), gx = std::min(nw, 1u << 16);
+        const dim3 g(gx, (nw + gx - 1) / gx);
+        if (nt) hipLaunchKernelGGL((coli_combine_grad<T, VE, VE != 1>), g, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((coli_combine_grad<T, VE, false>), g, dim3(256), 0, st, a);
+        return;
+    }
     const dim3 g(a.T, (a.D + 256 * VE - 1) / (256 * VE));
-    if (a.K == 1) hipLaunchKernelGGL((coli_combine<T, VE, 1>), g, dim3(256), 0, st, a);
-    else if (a.K == 2) hipLaunchKernelGGL((coli_combine<T, VE, 2>), g, dim3(256), 0, st, a);
-    else if (a.K <= 4) hipLaunchKernelGGL((coli_combine<T, VE, 4>), g, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((coli_combine<T, VE, 8>), g, dim3(256), 0, st, a);
+    if (nt && a.K > 4) hipLaunchKernelGGL((coli_combine<T, VE, 8, VE != 1>), g, dim3(256), 0, st, a);
+    else if (nt && a.K > 1) hipLaunchKernelGGL((coli_combine<T, VE, 4, VE != 1>), g, dim3(256), 0, st, a);
+    else if (nt) hipLaunchKernelGGL((coli_combine<T, VE, 1, VE != 1>), g, dim3(256), 0, st, a);
+    else if (a.K == 1) hipLaunchKernelGGL((coli_combine<T, VE, 1, false>), g, dim3(256), 0, st, a);
+    else if (a.K == 2) hipLaunchKernelGGL((coli_combine<T, VE, 2, false>), g, dim3(256), 0, st, a);
+    else if (a.K <= 4) hipLaunchKernelGGL((coli_combine<T, VE, 4, false>), g, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((coli_combine<T, VE, 8, false>), g, dim3(256), 0, st, a);
 }
 template <typename T> static void combine_run(const CombineArgs &a, bool grad, hipStream_t st) {
     constexpr int V = 16 / sizeof(T);
-    const unsigned nw = (unsigned)(((int64_t)a.T * a.K + 3) / 4), gx = std::min(nw, 1u << 16);
-    const dim3 gg(gx, (nw + gx - 1) / gx);
-    if (grad) {
-        if (a.D >= V) hipLaunchKernelGGL((coli_combine_grad<T, V>), gg, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((coli_combine_grad<T, 1>), gg, dim3(256), 0, st, a);
-    } else if (a.D >= V) {
-        combine_launch<T, V>(a, st);
-    } else {
-        combine_launch<T, 1>(a, st);
-    }
+    if (a.D >= V) combine_launch<T, V>(a, grad, st);
+    else combine_launch<T, 1>(a, grad, st);
 }
 static int combine_call(DevCtx *ctx, const CombineArgs &a, int dtype, bool grad) {
     if (dtype == 0) combine_run<float>(a, grad, ctx->stream);

@@ -251,6 +251,23 @@ def test_matmul_rows_do_not_mix(session, S):
         session.free(h)
 
 
+def test_matmul_output_past_the_caches(session):
+    """More than 128 MiB of output, stored past the caches: a sample of the rows against 64 bits, and rows
+    behind the last as they were."""
+    rng = np.random.default_rng(6)
+    I, O, S = 300, 15000, 2300
+    q4, e8 = rand_mxfp4(rng, O, I)
+    h, w = session.upload_mxfp4(q4, e8, I, O), deq_mxfp4(q4, e8, I)
+    try:
+        x = act(rng, S, I)
+        got = matmul_a4(session.b, h, x, O)
+        r = np.append(np.arange(0, S, 41), S - 1)
+        xv = mx_quant(x[r])[2]
+        assert (np.abs(got[r] - xv @ w.T) <= product_tol(I) * (np.abs(xv) @ np.abs(w).T) + 1e-30).all()
+    finally:
+        session.free(h)
+
+
 class Experts:
     """E random experts (pairs with `pair`) and their set."""
 

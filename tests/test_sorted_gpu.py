@@ -265,6 +265,38 @@ def test_rounds_once_and_keeps_infinities(session):
         assert np.array_equal(d.down(out, (1, 4), np.float16), np.array([[np.inf, 1 + 2.0 ** -10, np.inf, 1]], np.float16))
 
 
+def test_rows_past_the_caches(session):
+    """Sorted rows of more than 128 MiB, which are stored and loaded past the caches: a sample of the
+    rows against 64 bits, and every row's bytes in dispatch."""
+    rng = np.random.default_rng(11)
+    b, (T, E, K, D) = session.b, (2400, 40, 8, 3600)
+    idx, keff, mask = routing(rng, T, E, K)
+    off, src, pos = plan(idx, keff, mask, E)
+    N = T * K
+    x = rng.standard_normal((T, D)).astype(np.float16)
+    w = rng.standard_normal((T, K)).astype(np.float32)
+    with Bufs(b) as d:
+        xs, out, dys = (d.up(np.full((n, D), 7, np.float16)) for n in (N, T, N))
+        dw, pp, px, pw = d.up(np.full((T, K), 7, np.float32)), d.up(np.zeros(N, np.int32)), d.up(x), d.up(w)
+        assert b.hip_dispatch_dev(0, d.up(idx), d.up(keff), d.up(mask), T, E, K, px, D * 2, d.up(off * 0), d.up(np.zeros(N, np.int32)), pp, xs)
+        assert b.hip_combine_dev(0, xs, 1, pp, pw, T, K, N, D, out)
+        assert b.hip_combine_grad_dev(0, xs, 1, pp, pw, px, T, K, N, D, dys, dw)
+        got, go, gy, gw = d.down(xs, (N, D), np.float16), d.down(out, (T, D), np.float16), d.down(dys, (N, D), np.float16), d.down(dw, (T, K))
+    n = len(src)
+    assert np.array_equal(got[:n], x[src // K]) and (got[n:] == 7).all() and (gy[n:] == 7).all()
+    xv = x.astype(np.float64)
+    for t in range(0, T, 37):
+        live = pos[t] >= 0
+        wt = w[t].astype(np.float64)[live]
+        ref, mag = wt.sum() * xv[t], np.abs(wt).sum() * np.abs(xv[t])
+        assert (np.abs(go[t] - ref) <= K * 2.0 ** -24 * mag + EPS[1] * 1.001 * np.abs(ref) + TINY[1]).all()
+        for k in np.flatnonzero(live):
+            v = float(w[t, k]) * xv[t]
+            assert (np.abs(gy[pos[t, k]] - v) <= (2.0 ** -24 + EPS[1]) * 1.001 * np.abs(v) + TINY[1]).all()
+            assert abs(gw[t, k] - (xv[t] ** 2).sum()) <= (D / 64 + 22) * 2.0 ** -24 * (xv[t] ** 2).sum()
+        assert not gw[t][~live].any()
+
+
 def test_refusals(session):
     b = session.b
     with Bufs(b) as d:
