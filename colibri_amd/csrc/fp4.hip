@@ -156,13 +156,13 @@ struct Fp4Mat {
     const uint8_t *w0, *s0, *w1, *s1;   // matrix or gate, up
 };
 struct Fp4Item {
-    int mat, r0, nrows, pad;            // rows [r0, r0 + nrows) of the output times matrix mat
+    Fp4Mat mat;
+    int r0, nrows;                      // rows [r0, r0 + nrows) of the output times mat
 };
 struct Fp4Args {
-    const Fp4Mat *mats;        // device; null: mat0, and item i is rows [i tile, ..) of S
-    Fp4Mat mat0;
-    const Fp4Item *items;
+    const Fp4Item *items;      // device; null: mat0, and item i is rows [i tile, ..) of S
     const int *n_items;
+    Fp4Mat mat0;
     int S, tile;
     int nrt, nq, O;
     int rtb;                   // row-tile blocks of an item
@@ -183,6 +183,7 @@ struct Fp4Args {
 struct ItemArgs {
     const int *offsets;
     int E, N, tile, room;
+    const Fp4Mat *mats;
     Fp4Item *items;
     int *n_items;
 };
@@ -213,7 +214,7 @@ __device__ __forceinline__ void fp4_items(const ItemArgs &a) {
         }
         __syncthreads();
         for (int i = 0; i < tiles && at + i < a.room; i++)
-            a.items[at + i] = {e, r0 + i * a.tile, min(a.tile, n - i * a.tile), 0};
+            a.items[at + i] = {a.mats[e], r0 + i * a.tile, min(a.tile, n - i * a.tile)};
     }
     if (tid == 0) *a.n_items = min(base, a.room);
 }
@@ -222,6 +223,21 @@ __device__ __forceinline__ void fp4_items(const ItemArgs &a) {
 template <int FORM> __global__ __launch_bounds__(256) void coli_fp4_prep(QuantArgs a, ItemArgs it, int nblk) {
     if (blockIdx.x == (unsigned)nblk) fp4_items(it);
     else quant_rows<float, FORM, true>(a, blockIdx.x);
+}
+
+// swiglu_out on the hardware's exp2 and reciprocal (a step of each, beside products whose
+// sums carry more): exp(-g) = 2^h (1 + l ln 2) with h + l = -g log2(e) in two parts, g's
+// whole range right to 5 x 2^-24. A tenth of the instructions of the division and expf,
+// which were a third of the time of short products (16384 rows of 2048 x 1024 pairs: 67
+// us, ?? so).
+__device__ __forceinline__ float fp4_swiglu(float g, float u, float limit) {
+    if (limit > 0.0f) {
+        g = fminf(g, limit);
+        u = fmaxf(-limit, fminf(u, limit));
+    }
+    const float h = g * -1.44269504f, l = fmaf(g, -1.44269504f, -h) + g * -1.92596303e-8f;
+    const float e = __builtin_amdgcn_exp2f(h) * fmaf(l, 0.693147181f, 1.0f);
+    return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
 }
 
 // 4x4 dword transpose across the four 16-lane rows: the stored tile gives lane (c,
@@ -250,15 +266,12 @@ template <int NM, int R, bool DUAL, int FORM> __global__ __launch_bounds__(64 * 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, g = lane >> 4;
     const int item = blockIdx.x / a.rtb, rb = blockIdx.x - item * a.rtb;
-    Fp4Item it = {0, item * a.tile, 0, 0};
-    Fp4Mat mat = a.mat0;
-    if (a.mats) {
+    Fp4Item it = {a.mat0, item * a.tile, min(a.tile, a.S - item * a.tile)};
+    if (a.items) {
         if (item >= *a.n_items) return;
         it = a.items[item];
-        mat = a.mats[it.mat];
-    } else {
-        it.nrows = min(a.tile, a.S - it.r0);
     }
+    const Fp4Mat mat = it.mat;
     const uint8_t *w[R], *sc[R];
 #pragma unroll
     for (int r = 0; r < R; r++) {
@@ -366,7 +379,7 @@ template <int NM, int R, bool DUAL, int FORM> __global__ __launch_bounds__(64 * 
         float *y = a.y + (size_t)(it.r0 + row) * a.O + o;
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            if (o + i < a.O) y[i] = DUAL ? swiglu_out(v[i], u[i], a.limit) : v[i];
+            if (o + i < a.O) y[i] = DUAL ? fp4_swiglu(v[i], u[i], a.limit) : v[i];
     }
 }
 
@@ -398,9 +411,10 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t fp4_rsrc(const void *p, uint32
 }
 __device__ __forceinline__ i32x8 fp4_op(u32x4 v) { return (i32x8){(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0}; }
 // NB: 32-row blocks
-template <int NB, bool DUAL> __device__ __forceinline__ void fp4_many(const Fp4Args &a, const Fp4Item &it, const Fp4Mat &mat,
-                                                                      int rb, int split, lds_u8 *lds) {
+template <int NB, bool DUAL> __device__ __forceinline__ void fp4_many(const Fp4Args &a, const Fp4Item &it, int rb,
+                                                                      int split, lds_u8 *lds) {
     using G = FmGeom;
+    const Fp4Mat &mat = it.mat;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 31, g = lane >> 5;
     // operand r: two row tiles from rt[r] on (DUAL: the gate's and the up's of the same)
@@ -418,6 +432,22 @@ template <int NB, bool DUAL> __device__ __forceinline__ void fp4_many(const Fp4A
         wo[r] = k * COLI_TILE_BYTES + (32 * g + (n & 15)) * 16;   // slices 2 g and (256 bytes on) 2 g + 1 of row n
         so[r] = k * 64 + (n & 15) * 4;
     }
+    const int s0 = split * a.sps, ns = min(a.cp / 256, s0 + a.sps);   // this workgroup's stages
+    // Loaded: lane (n, g) has slices 2 g, 2 g + 1 of row n, a dword of each block. Turned:
+    // its four dwords of block 2 t + g in wv[.][r][t], those that the lane 32 away had by
+    // v_permlane32_swap. Scales: shifted so that bytes 0 and 2 are blocks g, 2 + g.
+    u32x4 wv[3][2][2];
+    uint32_t ws[3][2];
+    auto load_w = [&](int p, int r, int q) {
+        q = min(q, a.nq - 1);
+        wv[p][r][0] = __builtin_amdgcn_raw_buffer_load_b128(wr[r], wo[r], q * COLI_TILE_BYTES, 0);
+        wv[p][r][1] = __builtin_amdgcn_raw_buffer_load_b128(wr[r], wo[r] + 256, q * COLI_TILE_BYTES, 0);
+        ws[p][r] = __builtin_amdgcn_raw_buffer_load_b32(sr[r], so[r], q * 64, 0);
+    };
+#pragma unroll
+    for (int r = 0; r < 2; r++) load_w(0, r, 2 * s0);   // (ahead of the rows, whose addresses are loads away)
+#pragma unroll
+    for (int r = 0; r < 2; r++) load_w(1, r, 2 * s0 + 1);
     // operand row of the item's row r (a.rows: zeros), relative to the item's first
     // where there is no src
     const int base = a.src ? 0 : it.r0;
@@ -440,24 +470,12 @@ template <int NB, bool DUAL> __device__ __forceinline__ void fp4_many(const Fp4A
         xa[k] = row_of(r) * qs + 16 * ((lane & 7) ^ ((r >> 1) & 7));
     }
     const uint32_t xs = row_of(32 * wave + (lane >> 1)) * es + 4 * (lane & 1);
-    const int s0 = split * a.sps, ns = min(a.cp / 256, s0 + a.sps);   // this workgroup's stages
     auto issue = [&](int s, lds_u8 *st) {
         s = min(s, ns - 1);
 #pragma unroll
         for (int k = 0; k < NB; k++)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(xqr, (lds_void *)(st + (4 * k + wave) * 1024), 16, xa[k], s * 128, 0, 0);
         __builtin_amdgcn_raw_ptr_buffer_load_lds(xer, (lds_void *)(st + G::kRows + wave * 256), 4, xs, s * 8, 0, 0);
-    };
-    // Loaded: lane (n, g) has slices 2 g, 2 g + 1 of row n, a dword of each block. Turned:
-    // its four dwords of block 2 t + g in wv[.][r][t], those that the lane 32 away had by
-    // v_permlane32_swap. Scales: shifted so that bytes 0 and 2 are blocks g, 2 + g.
-    u32x4 wv[3][2][2];
-    uint32_t ws[3][2];
-    auto load_w = [&](int p, int r, int q) {
-        q = min(q, a.nq - 1);
-        wv[p][r][0] = __builtin_amdgcn_raw_buffer_load_b128(wr[r], wo[r], q * COLI_TILE_BYTES, 0);
-        wv[p][r][1] = __builtin_amdgcn_raw_buffer_load_b128(wr[r], wo[r] + 256, q * COLI_TILE_BYTES, 0);
-        ws[p][r] = __builtin_amdgcn_raw_buffer_load_b32(sr[r], so[r], q * 64, 0);
     };
     auto turn = [&](int p, int r) {
         const u32x4 x = wv[p][r][0], y = wv[p][r][1];
@@ -563,10 +581,6 @@ template <int NB, bool DUAL> __device__ __forceinline__ void fp4_many(const Fp4A
     issue(s0, slot[0]);
     issue(s0 + 1, slot[1]);
 #pragma unroll
-    for (int r = 0; r < 2; r++) load_w(0, r, 2 * s0);
-#pragma unroll
-    for (int r = 0; r < 2; r++) load_w(1, r, 2 * s0 + 1);
-#pragma unroll
     for (int r = 0; r < 2; r++) turn(0, r);
     __builtin_amdgcn_s_waitcnt(0);   // (a builtin: the compiler counts on from it)
     asm volatile("" ::: "memory");
@@ -615,7 +629,7 @@ template <int NB, bool DUAL> __device__ __forceinline__ void fp4_many(const Fp4A
             for (int i = 0; i < 16; i++) {
                 const int row = 32 * b + 8 * (i >> 2) + 4 * g + (i & 3);
                 float v = acc[r][b][i];
-                if constexpr (DUAL) v = swiglu_out(v, acc[1][b][i], a.limit);
+                if constexpr (DUAL) v = fp4_swiglu(v, acc[1][b][i], a.limit);
                 if (row >= it.nrows) continue;
                 if (a.stream) __builtin_nontemporal_store(v, y + (size_t)row * a.O);
                 else y[(size_t)row * a.O] = v;
@@ -625,8 +639,8 @@ template <int NB, bool DUAL> __device__ __forceinline__ void fp4_many(const Fp4A
 // Workgroups of one XCD (every eighth) take consecutive tiles, eight items' tiles of
 // one block of weights before the next block's, so that both stay in its L2.
 template <bool DUAL> __global__ __launch_bounds__(256, 2) void coli_fp4_many(Fp4Args a, int n_items) {
-    __shared__ __attribute__((aligned(16))) uint8_t lds[FmGeom::kPD * FmGeom::kStage];
-    const int n = a.mats ? min(*a.n_items, n_items) : n_items;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];   // FmGeom::kPD stages
+    const int n = a.items ? min(*a.n_items, n_items) : n_items;
     const int total = n * a.rtb * a.splits, per = (total + 7) / 8, j = blockIdx.x >> 3;
     int id = (blockIdx.x & 7) * per + j;
     if (j >= per || id >= total) return;
@@ -634,16 +648,10 @@ template <bool DUAL> __global__ __launch_bounds__(256, 2) void coli_fp4_many(Fp4
     id -= split * n * a.rtb;
     const int grp = id / (8 * a.rtb), in = id - grp * 8 * a.rtb, gi = min(8, n - grp * 8);
     const int item = grp * 8 + in % gi, rb = in / gi;
-    Fp4Item it = {0, item * a.tile, 0, 0};
-    Fp4Mat mat = a.mat0;
-    if (a.mats) {
-        it = a.items[item];
-        mat = a.mats[it.mat];
-    } else {
-        it.nrows = min(a.tile, a.S - it.r0);
-    }
-    if (it.nrows <= 64) fp4_many<2, DUAL>(a, it, mat, rb, split, (lds_u8 *)lds);
-    else fp4_many<4, DUAL>(a, it, mat, rb, split, (lds_u8 *)lds);
+    Fp4Item it = {a.mat0, item * a.tile, min(a.tile, a.S - item * a.tile)};
+    if (a.items) it = a.items[item];
+    if (it.nrows <= 64) fp4_many<2, DUAL>(a, it, rb, split, (lds_u8 *)lds);
+    else fp4_many<4, DUAL>(a, it, rb, split, (lds_u8 *)lds);
 }
 
 // The K splits' sums in their order: n outputs, four a thread.
@@ -853,8 +861,12 @@ static int fp4_run(DevCtx *ctx, Fp4Args &a, int n_items, int rows, bool dual, co
         // us); smaller ones may be there still when they are read (2048 rows: no difference).
         a.stream = a.splits == 1 && (size_t)rows * a.O * 4 > ((size_t)128 << 20);
         const dim3 g((unsigned)(n_items * a.rtb * a.splits + 7) / 8 * 8);
-        if (dual) hipLaunchKernelGGL((coli_fp4_many<true>), g, dim3(256), 0, ctx->stream, a, n_items);
-        else hipLaunchKernelGGL((coli_fp4_many<false>), g, dim3(256), 0, ctx->stream, a, n_items);
+        // Two workgroups fit a CU; where there are no more than CUs each asks for so much LDS
+        // that it has one to itself (they were placed two to a CU beside idle ones).
+        const size_t ring = FmGeom::kPD * FmGeom::kStage;
+        const size_t shm = (int64_t)n_items * a.rtb * a.splits <= ctx->cu_count ? std::max(ring, (size_t)96 << 10) : ring;
+        if (dual) hipLaunchKernelGGL((coli_fp4_many<true>), g, dim3(256), shm, ctx->stream, a, n_items);
+        else hipLaunchKernelGGL((coli_fp4_many<false>), g, dim3(256), shm, ctx->stream, a, n_items);
         if (!hip_check(hipGetLastError(), "fp4 product")) return 0;
         if (a.splits > 1) {
             const size_t n = (size_t)a.S * a.O;
@@ -979,6 +991,7 @@ extern "C" int coli_hip_experts_a4_dev(ColiHipExperts *x, float *y, const float 
     forget_emitted(ctx, y, yb);
     ItemArgs it = {};
     it.offsets = offsets;
+    it.mats = x->mats;
     it.E = x->E;
     it.N = N;
     // Tiles by the rows of an expert, were all that have some alike (us with tiles of 16 /
@@ -995,7 +1008,6 @@ extern "C" int coli_hip_experts_a4_dev(ColiHipExperts *x, float *y, const float 
     it.items = (Fp4Item *)((uint8_t *)ctx->fp4_items.p + 256);
     Fp4Args a = {};
     if (!fp4_prep(ctx, xr, rows, x->I, &it, &a)) return 0;
-    a.mats = x->mats;
     a.items = it.items;
     a.n_items = it.n_items;
     a.tile = it.tile;
