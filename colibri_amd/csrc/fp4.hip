@@ -448,9 +448,9 @@ template <int NB, bool DUAL> __device__ __forceinline__ void fp4_many(const Fp4A
     for (int r = 0; r < 2; r++) load_w(0, r, 2 * s0);   // (ahead of the rows, whose addresses are loads away)
 #pragma unroll
     for (int r = 0; r < 2; r++) load_w(1, r, 2 * s0 + 1);
-    // operand row of the item's row r (a.rows: zeros), relative to the item's first
-    // where there is no src
-    const int base = a.src ? 0 : it.r0;
+    // operand row of the item's row r (a.rows: zeros), relative to the item's first (or
+    // the zeros) where there is no src: offsets of 32 bits, see coli_hip_experts_a4_dev
+    const int base = a.src ? 0 : min(it.r0, a.rows);
     auto row_of = [&](int r) {
         int x = it.r0 + min(r, it.nrows - 1);
         if (a.src) {
@@ -980,7 +980,7 @@ extern "C" int coli_hip_experts_create(ColiHipExperts **out, int device, int E, 
 extern "C" int coli_hip_experts_a4_dev(ColiHipExperts *x, float *y, const float *xr, int rows, const int *src, int K,
                                        const int *offsets, int N) {
     if (fault_injected()) return 0;
-    if (!x || rows < 0 || rows > COLI_MX_MAX || N < 0 || N > (1 << 30) || K < 1 || (N && (!y || !offsets || !xr || !rows)))
+    if (!x || rows < 0 || rows > COLI_MX_MAX || N < 0 || N > COLI_MX_MAX || K < 1 || (N && (!y || !offsets || !xr || !rows)))
         return 0;
     const size_t yb = (size_t)N * x->O * 4;
     if (!outputs_apart({{y, yb}, {xr, (size_t)rows * x->I * 4}, {src, (size_t)N * 4}, {offsets, (size_t)(x->E + 1) * 4}}, 1))
@@ -1000,7 +1000,10 @@ extern "C" int coli_hip_experts_a4_dev(ColiHipExperts *x, float *y, const float 
     const int mean = N / std::min(N, x->E);
     const char *pin = fp4_pin();
     Fp4Plan plan = {mean <= 8 ? 16 : COLI_FP4_MANY, fp4_row_tiles(ctx, x->nrt, x->dual != 0), 1, false};
-    if (pin) plan.tile = std::strcmp(pin, "many") == 0 ? COLI_FP4_MANY : mean <= 16 ? 16 : mean <= 32 ? 32 : 64;
+    // (that kernel's rows lie within 2 GiB of their first, so of x where src chooses them)
+    const size_t xb = ((size_t)rows + 1) * (((size_t)x->I + 255) / 256 * 128);
+    if (src && xb > ((size_t)1 << 31)) plan.tile = mean <= 16 ? 16 : 64;
+    else if (pin) plan.tile = std::strcmp(pin, "many") == 0 ? COLI_FP4_MANY : mean <= 16 ? 16 : mean <= 32 ? 32 : 64;
     it.tile = plan.tile;
     it.room = (int)std::min<int64_t>(N, N / it.tile + x->E);
     if (!reserve_kept(ctx, &ctx->fp4_items, 256 + (size_t)it.room * sizeof(Fp4Item), 0)) return 0;

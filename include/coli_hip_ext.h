@@ -248,7 +248,7 @@ int coli_hip_combine_grad_dev(int device, const void *ys, int dtype, const int *
  * holds their largest magnitude within 6 (the rule of the e4m3 path: nothing
  * saturates); a block of zeros has scale 1; one with an infinity or NaN has byte
  * 255 and codes 0, which is NaN to whatever reads it. Codes are the nearest, ties to the
- * even code. Zero-row calls succeed. */
+ * even code. rows and cols up to 2^24 - 1; without rows nothing is done. */
 int coli_hip_mxfp4_quantize_dev(int device, const void *x, int dtype, int rows, int cols, unsigned char *q4,
                                 unsigned char *e8);
 /* y [rows, cols] from such bytes: code times scale, rounded once to dtype (byte
@@ -276,7 +276,8 @@ void coli_hip_experts_free(ColiHipExperts *experts);
 /* y[r] = W_e Q(x row of r) for the sorted rows offsets[e] <= r < offsets[e + 1] (ascending;
  * taken within 0..N) of y [N, O]; other rows of y are left as they were. The row is
  * x[src[r] / K] with src (of coli_hip_dispatch_dev: the rows need not be copied), x[r]
- * without; x is [rows, I], a row outside it counts as zeros. N and rows from 0 on. */
+ * without; x is [rows, I], a row outside it counts as zeros. N and rows up to 2^24 - 1;
+ * without sorted rows (N 0) nothing is done. */
 int coli_hip_experts_a4_dev(ColiHipExperts *experts, float *y, const float *x, int rows, const int *src, int K,
                             const int *offsets, int N);
 

@@ -164,7 +164,8 @@ def matmul_a4(b, h, x, O, extra=1):
 @pytest.mark.parametrize("I,O,S", [(1, 1, 1), (7, 3, 2), (8, 16, 1), (31, 17, 5), (32, 33, 16), (100, 40, 17), (128, 64, 1), (129, 15, 33),
                                    (256, 48, 64), (257, 100, 65), (384, 16, 3), (1000, 2999, 21), (999, 130, 70), (2048, 200, 128),
                                    (1152, 96, 129), (4096, 512, 1), (4096, 300, 200), (16400, 40, 9), (640, 1040, 300), (512, 4112, 2),
-                                   (3000, 24, 1000)])
+                                   (3000, 24, 1000), (700, 14000, 21), (500, 13200, 3),
+                                   (2000, 7100, 4), (1100, 13200, 50)])
 def test_matmul(session, I, O, S):
     rng = np.random.default_rng(I + O * 3 + S)
     q4, e8 = rand_mxfp4(rng, O, I)
@@ -369,6 +370,41 @@ def test_experts_offsets_and_rows_outside(session):
         keep = np.setdiff1d(np.arange(20), [0, 7, 19])
         assert np.array_equal(got[keep], ex.run(x, [0, 5, 12, 20], 20)[keep])
         assert session.b.hip_experts_a4_dev(ex.set, None, None, 0, None, 1, None, 0)
+
+
+@pytest.mark.parametrize("pin", ["few", "many"])
+def test_experts_more_sorted_rows_than_rows(session, monkeypatch, pin):
+    """Without src the rows past x are rows of zeros, whole tiles of them too."""
+    monkeypatch.setenv("COLI_HIP_FP4", pin)
+    rng = np.random.default_rng(10)
+    I, N, rows = 200, 700, 130
+    off = [0, 100, 380, 700]
+    x = act(rng, rows, I)
+    xv = np.concatenate([mx_quant(x)[2], np.zeros((N - rows, I))])
+    with Experts(session, rng, 3, I, 40, False) as ex:
+        ex.check(ex.run(x, off, N), xv, off, N, np.arange(N))
+
+
+@pytest.mark.parametrize("pin", ["few", "many"])
+@pytest.mark.parametrize("S", [2, 70])
+def test_weights_of_scale_255_and_0(session, monkeypatch, pin, S):
+    """A scale byte of 255 makes its output NaN and no other; a byte of 0 counts as 2^-127: nothing here."""
+    monkeypatch.setenv("COLI_HIP_FP4", pin)
+    rng = np.random.default_rng(12)
+    I, O = 300, 50
+    q4, e8 = rand_mxfp4(rng, O, I)
+    e8[17, 9], e8[40, 0], e8[3, 4], e8[20, :] = 255, 255, 0, 0
+    h = session.upload_mxfp4(q4, e8, I, O)
+    try:
+        x = act(rng, S, I)
+        got = matmul_a4(session.b, h, x, O)
+    finally:
+        session.free(h)
+    bad = np.isin(np.arange(O), [17, 40])
+    w = deq_mxfp4(q4, np.where(e8 == 255, 127, e8).astype(np.uint8), I)
+    xv = mx_quant(x)[2]
+    assert np.isnan(got[:, bad]).all()
+    assert (np.abs(got - xv @ w.T) <= product_tol(I) * (np.abs(xv) @ np.abs(w).T) + 1e-30)[:, ~bad].all()
 
 
 def route(rng, T, E, K):
