@@ -16,7 +16,7 @@
 #define COLI_SORT_MAX_E 1024
 #define COLI_SORT_MAX_T (1 << 23)   // a grid of 256-thread workgroups by row
 #define COLI_SORT_MAX_K 64
-#define COLI_SORT_FEW 2048      // selections that every workgroup places by itself
+#define COLI_SORT_FEW 4096      // selections that every workgroup places by itself
 #define COLI_SORT_BLOCKS 256    // counts of at most so many workgroups are added up
 #define COLI_ROW_PIECE 4096     // bytes of a row that a workgroup moves
 
@@ -29,13 +29,16 @@ struct SortArgs {
     size_t rb;
     int *offsets, *src, *pos, *hist;
     int per, nblk;
-    int stream;   // xs past the caches
+    int stream;       // xs past the caches
+    uint32_t magic;   // ceil(2^32 / K), where selections below 2^26 are divided by it; 0: divide
 };
 
 // Expert of selection s, E where it is not live.
 __device__ __forceinline__ int sort_key(const SortArgs &a, int s) {
-    const int t = s / a.K, k = s - t * a.K, e = a.idx[s];
-    const bool live = (unsigned)e < (unsigned)a.E && (!a.keff || k < a.keff[t]) && (!a.mask || a.mask[t]);
+    const int t = a.magic ? (int)__umulhi((uint32_t)s, a.magic) : s / a.K, k = s - t * a.K, e = a.idx[s];
+    // (every load asked for: short-circuited they would wait for one another)
+    const int most = a.keff ? a.keff[t] : a.K, on = a.mask ? a.mask[t] : 1;
+    const bool live = ((unsigned)e < (unsigned)a.E) & (k < most) & (on != 0);
     return live ? e : a.E;
 }
 
@@ -86,21 +89,22 @@ __device__ __forceinline__ void copy_piece(const SortArgs &a, int t, const int *
 // row's selections, those that come before it; the row behind the last one is the
 // offsets'.
 __global__ __launch_bounds__(256) void coli_dispatch_few(SortArgs a) {
-    __shared__ int key[COLI_SORT_FEW], place[COLI_SORT_MAX_K], tmp[4];
+    __shared__ int key[COLI_SORT_FEW], place[COLI_SORT_MAX_K], cnt[COLI_SORT_MAX_K], tmp[4];
     const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     if (t == a.T) {
         if (blockIdx.y) return;
-        int *cnt = key;   // [E]
-        for (int e = tid; e < COLI_SORT_MAX_E; e += 256) cnt[e] = 0;
+        int *hist = key;   // [E]
+        for (int e = tid; e < COLI_SORT_MAX_E; e += 256) hist[e] = 0;
         __syncthreads();
+#pragma unroll 4
         for (int s = tid; s < a.N; s += 256) {
             const int e = sort_key(a, s);
-            if (e < a.E) atomicAdd(cnt + e, 1);
+            if (e < a.E) atomicAdd(hist + e, 1);
         }
         __syncthreads();
         int v[4], sum = 0, total;
 #pragma unroll
-        for (int i = 0; i < 4; i++) sum += v[i] = cnt[4 * tid + i];
+        for (int i = 0; i < 4; i++) sum += v[i] = hist[4 * tid + i];
         int at = block_scan<256>(sum, tmp, total);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -110,17 +114,29 @@ __global__ __launch_bounds__(256) void coli_dispatch_few(SortArgs a) {
         if (tid == 0) a.offsets[a.E] = total;
         return;
     }
-    for (int s = tid; s < a.N; s += 256) key[s] = sort_key(a, s);
+    // keys by expert, then selection: one number, so a place is a count of smaller ones
+#pragma unroll 4
+    for (int s = tid; s < a.N; s += 256) key[s] = sort_key(a, s) * COLI_SORT_FEW + s;
+    if (tid < a.K) cnt[tid] = 0;
     __syncthreads();
-    for (int k = wave; k < a.K; k += 4) {
-        const int me = t * a.K + k, mine = key[me];
-        int n = 0;
-        for (int s0 = 0; s0 < a.N; s0 += 64) {
-            const int s = s0 + lane, o = s < a.N ? key[s] : a.E;
-            n += __popcll(__ballot(o < mine || (o == mine && s < me)));
+    for (int k0 = 0; k0 < a.K; k0 += 8) {
+        int mine[8], n[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            mine[i] = __builtin_amdgcn_readfirstlane(key[t * a.K + min(k0 + i, a.K - 1)]);
+            n[i] = 0;
         }
-        if (lane == 0) place[k] = mine < a.E ? n : -1;
+        for (int s0 = 64 * wave; s0 < a.N; s0 += 256) {
+            const int o = s0 + lane < a.N ? key[s0 + lane] : 0x7fffffff;
+#pragma unroll
+            for (int i = 0; i < 8; i++) n[i] += __popcll(__ballot(o < mine[i]));
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (lane == 0 && k0 + i < a.K) atomicAdd(cnt + k0 + i, n[i]);
     }
+    __syncthreads();
+    if (tid < a.K) place[tid] = key[t * a.K + tid] < a.E * COLI_SORT_FEW ? cnt[tid] : -1;
     __syncthreads();
     if (blockIdx.y == 0 && tid < a.K) {
         const int p = place[tid];
@@ -250,6 +266,7 @@ extern "C" int coli_hip_dispatch_dev(int device, const int *idx, const int *keff
     a.offsets = offsets;
     a.src = src;
     a.pos = pos;
+    a.magic = K > 1 && a.N < (1 << 26) ? (uint32_t)(((1ull << 32) + K - 1) / K) : 0;
     forget_emitted(ctx, offsets, (size_t)(E + 1) * 4);
     hipStream_t st = ctx->stream;
     if (!T) {
@@ -260,7 +277,9 @@ extern "C" int coli_hip_dispatch_dev(int device, const int *idx, const int *keff
     forget_emitted(ctx, pos, n4);
     if (xs) forget_emitted(ctx, xs, xb * K);
     const unsigned pieces = x ? (unsigned)((a.rb + COLI_ROW_PIECE - 1) / COLI_ROW_PIECE) : 1;
-    if (a.N <= COLI_SORT_FEW) {
+    // (each workgroup goes through all selections: 2000 of 250 rows 7.0 us, in three launches
+    // 10.6; 4000 of 500 rows 10.6 and 10.7; 2000 of 2000 rows 11.6 and 9.7)
+    if (a.N <= COLI_SORT_FEW && (int64_t)a.N * T * pieces <= 1500000) {
         hipLaunchKernelGGL(coli_dispatch_few, dim3(T + 1, pieces), dim3(256), 0, st, a);
         return hip_check(hipGetLastError(), "dispatch");
     }

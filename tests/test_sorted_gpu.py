@@ -60,11 +60,12 @@ def check_dispatch(b, idx, keff, mask, E, x):
         assert np.array_equal(xs[:n], x[rs // K]) and (xs[n:] == 0x5A).all()
 
 
-# one launch up to 2048 selections, three beyond; widths below, at and around 16
+# one launch up to 4096 selections, three beyond; widths below, at and around 16
 # bytes and a workgroup's piece of 4096
 @pytest.mark.parametrize("T,E,K,rb", [(1, 1, 1, 1), (1, 64, 8, 8192), (3, 5, 2, 15), (7, 3, 6, 16), (16, 256, 8, 17),
                                       (33, 100, 6, 1998), (256, 256, 8, 4096), (1000, 17, 2, 4097), (2048, 9, 1, 31),
-                                      (2049, 9, 1, 33), (257, 1024, 8, 100), (683, 8, 3, 4111), (5000, 64, 8, 48),
+                                      (2049, 9, 1, 33), (257, 1024, 8, 100), (512, 1024, 8, 33), (4096, 3, 1, 20), (4097, 3, 1, 20), (586, 64, 7, 300),
+                                      (65, 64, 63, 8), (513, 1024, 8, 20), (683, 8, 3, 4111), (5000, 64, 8, 48),
                                       (64, 64, 64, 9), (20000, 1000, 6, 2), (40000, 256, 8, 4)])
 def test_dispatch(session, T, E, K, rb):
     rng = np.random.default_rng(T * 3 + E * 5 + K)
@@ -358,6 +359,6 @@ def test_graph_replays(session, T):
                     d.put(p, np.zeros(n, np.float32))
             g.launch()
             calls(outs[1])
-            check_dispatch(b, *routing(rng, 2100 + rep, 12, 2), 12, None)
+            check_dispatch(b, *routing(rng, 2100 + rep, 12, 2 + rep), 12, None)
             for p, q, n in zip(*outs, (E + 1, N, N, N * D, T * D, N * D, N)):
                 assert np.array_equal(d.down(p, n, np.uint32), d.down(q, n, np.uint32)), rep
