@@ -221,10 +221,12 @@ __device__ __forceinline__ void fp4_items(const ItemArgs &a) {
     if (tid == 0) *a.n_items = min(base, a.room);
 }
 
-// The rows' operands and, in the last workgroup (it.items), the items.
-template <int FORM> __global__ __launch_bounds__(256) void coli_fp4_prep(QuantArgs a, ItemArgs it, int nblk) {
-    if (blockIdx.x == (unsigned)nblk) fp4_items(it);
-    else quant_rows<float, FORM, true>(a, blockIdx.x);
+// The rows' operands and, in the first workgroup (it.items), the items: placed last it
+// would end after the others.
+template <int FORM> __global__ __launch_bounds__(256) void coli_fp4_prep(QuantArgs a, ItemArgs it) {
+    const int first = it.items ? 1 : 0;
+    if ((int)blockIdx.x < first) fp4_items(it);
+    else quant_rows<float, FORM, true>(a, blockIdx.x - first);
 }
 
 // swiglu_out on the hardware's exp2 and reciprocal (a step of each, beside products whose
@@ -771,9 +773,9 @@ static int fp4_prep(DevCtx *ctx, const float *x, int rows, int I, const ItemArgs
     const int nblk = (int)mx_grid(rows + 1, cp, q.lpr, &q.chunks);
     const dim3 g(nblk + (it ? 1 : 0));
     const ItemArgs none = {};
-    if (I < 8) hipLaunchKernelGGL(coli_fp4_prep<2>, g, dim3(256), 0, ctx->stream, q, it ? *it : none, nblk);
-    else if (I % 8) hipLaunchKernelGGL(coli_fp4_prep<1>, g, dim3(256), 0, ctx->stream, q, it ? *it : none, nblk);
-    else hipLaunchKernelGGL(coli_fp4_prep<0>, g, dim3(256), 0, ctx->stream, q, it ? *it : none, nblk);
+    if (I < 8) hipLaunchKernelGGL(coli_fp4_prep<2>, g, dim3(256), 0, ctx->stream, q, it ? *it : none);
+    else if (I % 8) hipLaunchKernelGGL(coli_fp4_prep<1>, g, dim3(256), 0, ctx->stream, q, it ? *it : none);
+    else hipLaunchKernelGGL(coli_fp4_prep<0>, g, dim3(256), 0, ctx->stream, q, it ? *it : none);
     if (!hip_check(hipGetLastError(), "fp4 operands")) return 0;
     a->xq = p;
     a->xe = p + qb;
