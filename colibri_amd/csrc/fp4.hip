@@ -177,6 +177,7 @@ struct Fp4Args {
     int K, rows;
     float *y;
     int stream;                // y past the caches (see fp4_run)
+    int group;                 // items of a group (coli_fp4_many)
     float limit;
 };
 
@@ -640,8 +641,11 @@ template <int NB, bool DUAL> __device__ __forceinline__ void fp4_many(const Fp4A
             }
     }
 }
-// Workgroups of one XCD (every eighth) take consecutive tiles, eight items' tiles of
-// one block of weights before the next block's, so that both stay in its L2.
+// Workgroups of one XCD (every eighth) take consecutive tiles, a group of items' tiles of
+// one block of weights before the next block's, so that both stay in its L2: eight items
+// of one matrix (one item at a time: 8192 x 8192 x 2048 100 -> 112 us), one where experts
+// have few tiles and their weights are the stream (64 pairs of 2048 x 1024, 256 rows each
+// 89 -> 85 us; 16 pairs of 7168 x 2048, 750 rows each 280 -> 287).
 template <bool DUAL> __global__ __launch_bounds__(256, 2) void coli_fp4_many(Fp4Args a, int n_items) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];   // FmGeom::kPD stages
     const int n = a.items ? min(*a.n_items, n_items) : n_items;
@@ -650,8 +654,8 @@ template <bool DUAL> __global__ __launch_bounds__(256, 2) void coli_fp4_many(Fp4
     if (j >= per || id >= total) return;
     const int split = id / (n * a.rtb);
     id -= split * n * a.rtb;
-    const int grp = id / (8 * a.rtb), in = id - grp * 8 * a.rtb, gi = min(8, n - grp * 8);
-    const int item = grp * 8 + in % gi, rb = in / gi;
+    const int grp = id / (a.group * a.rtb), in = id - grp * a.group * a.rtb, gi = min(a.group, n - grp * a.group);
+    const int item = grp * a.group + in % gi, rb = in / gi;
     Fp4Item it = {a.mat0, item * a.tile, min(a.tile, a.S - item * a.tile)};
     if (a.items) it = a.items[item];
     if (it.nrows <= 64) fp4_many<2, DUAL>(a, it, rb, split, (lds_u8 *)lds);
@@ -910,6 +914,7 @@ int matmul_a4_dev(DevCtx *ctx, ColiCudaTensor *t, float *y_dev, const float *x_d
     }
     a.mat0 = {t->w, (const uint8_t *)t->sc, nullptr, nullptr};
     a.S = S;
+    a.group = 8;
     a.nrt = t->nrt;
     a.nq = t->nq;
     a.O = t->O;
@@ -1018,6 +1023,7 @@ extern "C" int coli_hip_experts_a4_dev(ColiHipExperts *x, float *y, const float 
     a.items = it.items;
     a.n_items = it.n_items;
     a.tile = it.tile;
+    a.group = mean < 512 ? 1 : 8;
     a.nrt = x->nrt;
     a.nq = x->nq;
     a.O = x->O;
