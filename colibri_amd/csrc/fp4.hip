@@ -117,9 +117,8 @@ struct DequantArgs {
     const uint8_t *q4, *e8;
     void *y;
     int rows, cols, lpr, chunks;
-    int stream;   // y past the caches
 };
-template <typename T> __global__ __launch_bounds__(256) void coli_mx_dequant(DequantArgs a) {
+template <typename T, bool NT> __global__ __launch_bounds__(256) void coli_mx_dequant(DequantArgs a) {
     typedef float float2v __attribute__((ext_vector_type(2)));
     const int grp = blockIdx.x / a.chunks, r = (grp << (8 - a.lpr)) + (threadIdx.x >> a.lpr), qs = (a.cols + 1) / 2;
     const int o0 = ((blockIdx.x - grp * a.chunks) << a.lpr) + (threadIdx.x & ((1 << a.lpr) - 1));
@@ -141,8 +140,7 @@ template <typename T> __global__ __launch_bounds__(256) void coli_mx_dequant(Deq
 #pragma unroll
         for (int i = 0; i < 8; i++) o[i] = f[i >> 1][i & 1] * s;
         if (c + 8 <= a.cols) {
-            if (a.stream) el_store<T, 8, true>(y + c, o);
-            else el_store<T, 8>(y + c, o);
+            el_store<T, 8, NT>(y + c, o);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; i++)
@@ -176,7 +174,6 @@ struct Fp4Args {
     const int *src;            // sorted row -> K x row + k (null: the row itself)
     int K, rows;
     float *y;
-    int stream;                // y past the caches (see fp4_run)
     int group;                 // items of a group (coli_fp4_many)
     float limit;
 };
@@ -416,7 +413,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t fp4_rsrc(const void *p, uint32
 }
 __device__ __forceinline__ i32x8 fp4_op(u32x4 v) { return (i32x8){(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0}; }
 // NB: 32-row blocks
-template <int NB, bool DUAL> __device__ __forceinline__ void fp4_many(const Fp4Args &a, const Fp4Item &it, int rb,
+template <int NB, bool DUAL, bool NT> __device__ __forceinline__ void fp4_many(const Fp4Args &a, const Fp4Item &it, int rb,
                                                                       int split, lds_u8 *lds) {
     using G = FmGeom;
     const Fp4Mat &mat = it.mat;
@@ -636,7 +633,7 @@ template <int NB, bool DUAL> __device__ __forceinline__ void fp4_many(const Fp4A
                 float v = acc[r][b][i];
                 if constexpr (DUAL) v = fp4_swiglu(v, acc[1][b][i], a.limit);
                 if (row >= it.nrows) continue;
-                if (a.stream) __builtin_nontemporal_store(v, y + (size_t)row * a.O);
+                if constexpr (NT) __builtin_nontemporal_store(v, y + (size_t)row * a.O);
                 else y[(size_t)row * a.O] = v;
             }
     }
@@ -646,7 +643,9 @@ template <int NB, bool DUAL> __device__ __forceinline__ void fp4_many(const Fp4A
 // of one matrix (one item at a time: 8192 x 8192 x 2048 100 -> 112 us), one where experts
 // have few tiles and their weights are the stream (64 pairs of 2048 x 1024, 256 rows each
 // 89 -> 85 us; 16 pairs of 7168 x 2048, 750 rows each 280 -> 287).
-template <bool DUAL> __global__ __launch_bounds__(256, 2) void coli_fp4_many(Fp4Args a, int n_items) {
+// NT: y past the caches (a template's: of two stores under a branch the compiler makes one
+// and drops the hint).
+template <bool DUAL, bool NT> __global__ __launch_bounds__(256, 2) void coli_fp4_many(Fp4Args a, int n_items) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];   // FmGeom::kPD stages
     const int n = a.items ? min(*a.n_items, n_items) : n_items;
     const int total = n * a.rtb * a.splits, per = (total + 7) / 8, j = blockIdx.x >> 3;
@@ -658,8 +657,8 @@ template <bool DUAL> __global__ __launch_bounds__(256, 2) void coli_fp4_many(Fp4
     const int item = grp * a.group + in % gi, rb = in / gi;
     Fp4Item it = {a.mat0, item * a.tile, min(a.tile, a.S - item * a.tile)};
     if (a.items) it = a.items[item];
-    if (it.nrows <= 64) fp4_many<2, DUAL>(a, it, rb, split, (lds_u8 *)lds);
-    else fp4_many<4, DUAL>(a, it, rb, split, (lds_u8 *)lds);
+    if (it.nrows <= 64) fp4_many<2, DUAL, NT>(a, it, rb, split, (lds_u8 *)lds);
+    else fp4_many<4, DUAL, NT>(a, it, rb, split, (lds_u8 *)lds);
 }
 
 // The K splits' sums in their order: n outputs, four a thread.
@@ -704,6 +703,12 @@ template <typename T> static void quant_launch(QuantArgs &a, hipStream_t st) {
     else if (a.cols % 8) hipLaunchKernelGGL((coli_mx_quant<T, 1>), g, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((coli_mx_quant<T, 0>), g, dim3(256), 0, st, a);
 }
+template <typename T> static void dequant_launch(const DequantArgs &a, dim3 g, bool nt, hipStream_t st) {
+    // (f32: a lane's 32 bytes are two stores of half lines, which past the caches are
+    // written twice: 8000 rows of 14336 and back 229 -> 305 us)
+    if (nt && sizeof(T) == 2) hipLaunchKernelGGL((coli_mx_dequant<T, sizeof(T) == 2>), g, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((coli_mx_dequant<T, false>), g, dim3(256), 0, st, a);
+}
 static int quantize(DevCtx *ctx, const void *x, int dtype, int rows, int cols, uint8_t *q4, uint8_t *e8) {
     QuantArgs a = {x, q4, e8, rows, cols, cols, lanes_log2(cols), 1};
     if (dtype == 0) quant_launch<float>(a, ctx->stream);
@@ -741,11 +746,12 @@ extern "C" int coli_hip_mxfp4_dequantize_dev(int device, const unsigned char *q4
     if (!bind_ctx(ctx)) return 0;
     if (!rows) return 1;
     forget_emitted(ctx, y, yb);
-    DequantArgs a = {q4, e8, y, rows, cols, lanes_log2(cols), 1, yb > ((size_t)128 << 20)};
+    DequantArgs a = {q4, e8, y, rows, cols, lanes_log2(cols), 1};
     const dim3 g(mx_grid(rows, cols, a.lpr, &a.chunks));
-    if (dtype == 0) hipLaunchKernelGGL(coli_mx_dequant<float>, g, dim3(256), 0, ctx->stream, a);
-    else if (dtype == 1) hipLaunchKernelGGL(coli_mx_dequant<_Float16>, g, dim3(256), 0, ctx->stream, a);
-    else hipLaunchKernelGGL(coli_mx_dequant<__bf16>, g, dim3(256), 0, ctx->stream, a);
+    const bool nt = yb > ((size_t)128 << 20);   // more than the 256 MB cache keeps for whoever reads y next
+    if (dtype == 0) dequant_launch<float>(a, g, nt, ctx->stream);
+    else if (dtype == 1) dequant_launch<_Float16>(a, g, nt, ctx->stream);
+    else dequant_launch<__bf16>(a, g, nt, ctx->stream);
     return hip_check(hipGetLastError(), "mxfp4 dequantize");
 }
 
@@ -867,14 +873,13 @@ static int fp4_run(DevCtx *ctx, Fp4Args &a, int n_items, int rows, bool dual, co
         a.part = (float *)ctx->fp4_part.p;
         // Outputs beyond half of the 256 MB cache go past it (8192 x 4096 x 14336 380 -> 290
         // us); smaller ones may be there still when they are read (2048 rows: no difference).
-        a.stream = a.splits == 1 && (size_t)rows * a.O * 4 > ((size_t)128 << 20);
+        const bool nt = a.splits == 1 && (size_t)rows * a.O * 4 > ((size_t)128 << 20);
         const dim3 g((unsigned)(n_items * a.rtb * a.splits + 7) / 8 * 8);
-        // Two workgroups fit a CU; where there are no more than CUs each asks for so much LDS
-        // that it has one to itself (they were placed two to a CU beside idle ones).
-        const size_t ring = FmGeom::kPD * FmGeom::kStage;
-        const size_t shm = (int64_t)n_items * a.rtb * a.splits <= ctx->cu_count ? std::max(ring, (size_t)96 << 10) : ring;
-        if (dual) hipLaunchKernelGGL((coli_fp4_many<true>), g, dim3(256), shm, ctx->stream, a, n_items);
-        else hipLaunchKernelGGL((coli_fp4_many<false>), g, dim3(256), shm, ctx->stream, a, n_items);
+        const size_t shm = FmGeom::kPD * FmGeom::kStage;
+        if (dual && nt) hipLaunchKernelGGL((coli_fp4_many<true, true>), g, dim3(256), shm, ctx->stream, a, n_items);
+        else if (dual) hipLaunchKernelGGL((coli_fp4_many<true, false>), g, dim3(256), shm, ctx->stream, a, n_items);
+        else if (nt) hipLaunchKernelGGL((coli_fp4_many<false, true>), g, dim3(256), shm, ctx->stream, a, n_items);
+        else hipLaunchKernelGGL((coli_fp4_many<false, false>), g, dim3(256), shm, ctx->stream, a, n_items);
         if (!hip_check(hipGetLastError(), "fp4 product")) return 0;
         if (a.splits > 1) {
             const size_t n = (size_t)a.S * a.O;

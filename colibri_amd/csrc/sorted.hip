@@ -29,7 +29,6 @@ struct SortArgs {
     size_t rb;
     int *offsets, *src, *pos, *hist;
     int per, nblk;
-    int stream;       // xs past the caches
     uint32_t magic;   // ceil(2^32 / K), where selections below 2^26 are divided by it; 0: divide
 };
 
@@ -65,7 +64,9 @@ template <int NT> __device__ __forceinline__ int block_scan(int v, int *tmp, int
 
 // One piece of row t to its places: the row is read once. A piece that would pass
 // the row's end is moved back (the same bytes twice); rows below 16 bytes go by bytes.
-__device__ __forceinline__ void copy_piece(const SortArgs &a, int t, const int *place) {
+// NT: past the caches (a template's: of two stores under a branch the compiler makes one
+// and drops the hint).
+template <bool NT> __device__ __forceinline__ void copy_piece(const SortArgs &a, int t, const int *place) {
     const size_t c = (size_t)blockIdx.y * COLI_ROW_PIECE + threadIdx.x * 16;
     if (c >= a.rb) return;
     const uint8_t *xr = a.x + (size_t)t * a.rb;
@@ -80,7 +81,7 @@ __device__ __forceinline__ void copy_piece(const SortArgs &a, int t, const int *
     for (int k = 0; k < a.K; k++) {
         if (place[k] < 0) continue;
         u32x4a1 *to = (u32x4a1 *)(a.xs + (size_t)place[k] * a.rb + p);
-        if (a.stream) __builtin_nontemporal_store(v, to);
+        if constexpr (NT) __builtin_nontemporal_store((u32x4a1)v, to);
         else *to = v;
     }
 }
@@ -143,7 +144,7 @@ __global__ __launch_bounds__(256) void coli_dispatch_few(SortArgs a) {
         a.pos[t * a.K + tid] = p;
         if (p >= 0) a.src[p] = t * a.K + tid;
     }
-    if (a.x) copy_piece(a, t, place);
+    if (a.x) copy_piece<false>(a, t, place);
 }
 
 // Many selections: counts by workgroup and expert ...
@@ -230,8 +231,8 @@ __global__ __launch_bounds__(1024) void coli_dispatch_place(SortArgs a) {
     }
 }
 
-__global__ __launch_bounds__(256) void coli_dispatch_rows(SortArgs a) {
-    copy_piece(a, blockIdx.x, a.pos + (size_t)blockIdx.x * a.K);
+template <bool NT> __global__ __launch_bounds__(256) void coli_dispatch_rows(SortArgs a) {
+    copy_piece<NT>(a, blockIdx.x, a.pos + (size_t)blockIdx.x * a.K);
 }
 
 // No rows: offsets of zeros.
@@ -285,14 +286,15 @@ extern "C" int coli_hip_dispatch_dev(int device, const int *idx, const int *keff
     }
     a.per = std::max(1024, (a.N + COLI_SORT_BLOCKS - 1) / COLI_SORT_BLOCKS + 1023 & ~1023);
     a.nblk = (a.N + a.per - 1) / a.per;
-    a.stream = xb * K > ((size_t)128 << 20);   // more than the 256 MB cache keeps for whoever reads them next
     if (!reserve_kept(ctx, &ctx->sort_hist, (size_t)COLI_SORT_BLOCKS * COLI_SORT_MAX_E * 4, 0)) return 0;
     a.hist = (int *)ctx->sort_hist.p;
     hipLaunchKernelGGL(coli_dispatch_count, dim3(a.nblk), dim3(1024), 0, st, a);
     if (!hip_check(hipGetLastError(), "dispatch counts")) return 0;
     hipLaunchKernelGGL(coli_dispatch_place, dim3(a.nblk), dim3(1024), (size_t)16 * E * 4, st, a);
     if (!hip_check(hipGetLastError(), "dispatch places")) return 0;
-    if (x) hipLaunchKernelGGL(coli_dispatch_rows, dim3(T, pieces), dim3(256), 0, st, a);
+    // (sorted rows beyond half of the 256 MB cache go past it)
+    if (x && xb * K > ((size_t)128 << 20)) hipLaunchKernelGGL(coli_dispatch_rows<true>, dim3(T, pieces), dim3(256), 0, st, a);
+    else if (x) hipLaunchKernelGGL(coli_dispatch_rows<false>, dim3(T, pieces), dim3(256), 0, st, a);
     return hip_check(hipGetLastError(), "dispatch rows");
 }
 
