@@ -4,9 +4,18 @@
 // (coli_hip_mxfp4_quantize_dev, coli_hip_fp4_matmul_a4_dev, coli_hip_experts_a4_dev).
 //
 // y[r, o] = sum_b 2^(ex[r, b] + ew[o, b] - 254) sum_{k in b} cx[r, k] cw[o, k], on
-// v_mfma_scale_f32_16x16x128_f8f6f4 with both operands e2m1: the unit reads codes and
-// scales as they are stored and no conversion is left. Lane (c, g) of an operand
-// holds the 32 codes of row c's block g of the 128 columns, and their scale.
+// v_mfma_scale_f32_{16x16x128,32x32x64}_f8f6f4 with both operands e2m1: the unit reads codes
+// and scales as they are stored and no conversion is left. A lane of an operand holds the
+// 32 codes of one block of a row, and their scale. Products are exact and sums f32.
+//
+// Two kernels. coli_fp4_few streams the weights (a token through 4096 x 14336 7.6 us, 4.1
+// TB/s, what a plain read of so small a matrix reaches; the pairs that 16 rows select of
+// 256, 0.88 GB, in 130 us, 6.7 TB/s). coli_fp4_many is bound by the matrix units' power: 2048 x
+// 14336 x 4096 in 66 us, 3.6 PFLOP/s, 47 us with its loads, LDS reads and turns left out
+// (the card lowers its clock to 1.6 GHz under MFMAs of random codes); of the rest 13 us go
+// with the loads, whatever they hit: weights five steps ahead instead of two, weights that a
+// second group of waves shares, and hot lines alone change nothing.
+// coli_fp4_prep quantizes the rows ahead of them, at the rate of a copy.
 #include "coli_hip_host.h"
 #include "coli_rows.h"
 
@@ -228,10 +237,10 @@ template <int FORM> __global__ __launch_bounds__(256) void coli_fp4_prep(QuantAr
 }
 
 // swiglu_out on the hardware's exp2 and reciprocal (a step of each, beside products whose
-// sums carry more): exp(-g) = 2^h (1 + l ln 2) with h + l = -g log2(e) in two parts, g's
-// whole range right to 5 x 2^-24. A tenth of the instructions of the division and expf,
-// which were a third of the time of short products (16384 rows of 2048 x 1024 pairs: 67
-// us, ?? so).
+// sums carry more): exp(-g) = 2^h (1 + l ln 2) with h + l = -g log2(e) in two parts, right
+// to 5 x 2^-24 over g's whole range. A third of the instructions of expf and the division,
+// which a short product shows (16384 rows through 8 pairs of 2048 x 1024: 90 us, 77 so and
+// with the weights requested ahead of the rows).
 __device__ __forceinline__ float fp4_swiglu(float g, float u, float limit) {
     if (limit > 0.0f) {
         g = fminf(g, limit);
@@ -379,9 +388,17 @@ template <int NM, int R, bool DUAL, int FORM> __global__ __launch_bounds__(64 * 
         const int row = 16 * m + c, o = 16 * (DUAL ? rb : rb * R + r) + 4 * g;
         if (row >= it.nrows) continue;
         float *y = a.y + (size_t)(it.r0 + row) * a.O + o;
+        if constexpr (DUAL) {
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (o + i < a.O) y[i] = DUAL ? fp4_swiglu(v[i], u[i], a.limit) : v[i];
+            for (int i = 0; i < 4; i++) v[i] = fp4_swiglu(v[i], u[i], a.limit);
+        }
+        if (o + 4 <= a.O) {
+            *(f4u *)y = v;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 3; i++)
+                if (o + i < a.O) y[i] = v[i];
+        }
     }
 }
 
@@ -824,7 +841,8 @@ static Fp4Plan fp4_plan(const DevCtx *ctx, const ColiCudaTensor *t, int S) {
     // The kernel of many rows, modelled in us from measurements: 8 and a stage of 256
     // columns 0.72 (1.06 with every CU at it), each further workgroup of a CU as much
     // again, a join of K splits 2.5 and 0.3 a MB of sums. The other: 5.5, the weights at
-    // 6.5 TB/s and the rows' operands, once for each workgroup, at 5 TB/s.
+    // 6.5 TB/s for each tile of rows, the rows' operands, once for each workgroup, at 5
+    // TB/s, and the results at 2.5 TB/s.
     const int ns = cp / 256, wgs = (S + COLI_FP4_MANY - 1) / COLI_FP4_MANY * ((t->nrt + 15) / 16);
     double best = 1e30;
     for (int P = 1; P <= 32 && P <= ns; P *= 2) {
@@ -837,9 +855,10 @@ static Fp4Plan fp4_plan(const DevCtx *ctx, const ColiCudaTensor *t, int S) {
             p.splits = P;
         }
     }
-    const int nwg = (t->nrt + p.R - 1) / p.R, all = nwg * ((S + p.tile - 1) / p.tile);
-    const double few = 5.5 + (double)t->w_bytes / 6.5e6 +
-                       0.2e-6 * nwg * (double)S * cp * 0.53 * std::max(1.0, 0.8 * cus / all);
+    const int nwg = (t->nrt + p.R - 1) / p.R, tiles = (S + p.tile - 1) / p.tile;
+    const double few = 5.5 + tiles * (double)t->w_bytes / 6.5e6 +
+                       0.2e-6 * nwg * (double)S * cp * 0.53 * std::max(1.0, 0.8 * cus / (nwg * tiles)) +
+                       0.4e-6 * 4.0 * S * t->O;
     const char *pin = fp4_pin();
     if (pin ? std::strcmp(pin, "many") == 0 : S > 16 && best < few) {
         p.tile = COLI_FP4_MANY;
