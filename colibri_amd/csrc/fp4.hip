@@ -242,11 +242,12 @@ template <int FORM> __global__ __launch_bounds__(256) void coli_fp4_prep(QuantAr
 // which a short product shows (16384 rows through 8 pairs of 2048 x 1024: 90 us, 77 so and
 // with the weights requested ahead of the rows).
 __device__ __forceinline__ float fp4_swiglu(float g, float u, float limit) {
-    if (limit > 0.0f) {
-        g = fminf(g, limit);
-        u = fmaxf(-limit, fminf(u, limit));
+    if (limit > 0.0f) {   // (compared, not fminf: a NaN stays one)
+        g = g > limit ? limit : g;
+        u = u > limit ? limit : u < -limit ? -limit : u;
     }
-    const float h = g * -1.44269504f, l = fmaf(g, -1.44269504f, -h) + g * -1.92596303e-8f;
+    const float c = fminf(fmaxf(g, -128.0f), 128.0f);   // beyond, the sigmoid is 0 or 1 in f32
+    const float h = c * -1.44269504f, l = fmaf(c, -1.44269504f, -h) + c * -1.92596303e-8f;
     const float e = __builtin_amdgcn_exp2f(h) * fmaf(l, 0.693147181f, 1.0f);
     return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
 }
@@ -920,11 +921,12 @@ static int fp4_run(DevCtx *ctx, Fp4Args &a, int n_items, int rows, bool dual, co
     return hip_check(hipGetLastError(), "fp4 product");
 }
 
-#define COLI_FP4_MAX_I (COLI_ZERO_BYTES * 2)   // an operand row is no longer than the zeros
+#define COLI_FP4_MAX_I (1 << 21)       // a tile's operand rows lie within 2 GiB (128 MiB)
+#define COLI_FP4_MAX_ROWS (1 << 23)
 
 int matmul_a4_dev(DevCtx *ctx, ColiCudaTensor *t, float *y_dev, const float *x_dev, int S) {
     Fp4Args a = {};
-    if (t->I > (int)COLI_FP4_MAX_I) return 0;
+    if (t->I > COLI_FP4_MAX_I || S > COLI_FP4_MAX_ROWS) return 0;
     forget_emitted(ctx, y_dev, (size_t)S * t->O * 4);
     const Fp4Plan plan = fp4_plan(ctx, t, S);
     a.tile = plan.tile;
@@ -949,7 +951,7 @@ int matmul_a4_dev(DevCtx *ctx, ColiCudaTensor *t, float *y_dev, const float *x_d
 
 extern "C" int coli_hip_fp4_matmul_a4_dev(ColiCudaTensor *t, float *y_dev, const float *x_dev, int S) {
     if (fault_injected()) return 0;
-    if (!t || t->kind != COLI_KIND_FP4 || !y_dev || !x_dev || S < 1 || S > COLI_MX_MAX ||
+    if (!t || t->kind != COLI_KIND_FP4 || !y_dev || !x_dev || S < 1 || S > COLI_FP4_MAX_ROWS ||
         ranges_overlap(y_dev, (size_t)S * t->O * 4, x_dev, (size_t)S * t->I * 4))
         return 0;
     DevCtx *ctx = ctx_of(t->device);
@@ -984,7 +986,7 @@ extern "C" int coli_hip_experts_create(ColiHipExperts **out, int device, int E, 
         for (int k = 0; k < (ups ? 2 : 1); k++) {
             const ColiCudaTensor *t = k ? ups[e] : gates[e];
             if (!t || t->kind != COLI_KIND_FP4 || t->device != device || t->I != gates[0]->I || t->O != gates[0]->O ||
-                t->I > (int)COLI_FP4_MAX_I) {
+                t->I > COLI_FP4_MAX_I) {
                 std::fprintf(stderr, "[HIP] experts: expert %d is not an MXFP4 tensor of this device and shape\n", e);
                 return 0;
             }
@@ -1013,7 +1015,7 @@ extern "C" int coli_hip_experts_create(ColiHipExperts **out, int device, int E, 
 extern "C" int coli_hip_experts_a4_dev(ColiHipExperts *x, float *y, const float *xr, int rows, const int *src, int K,
                                        const int *offsets, int N) {
     if (fault_injected()) return 0;
-    if (!x || rows < 0 || rows > COLI_MX_MAX || N < 0 || N > COLI_MX_MAX || K < 1 || (N && (!y || !offsets || !xr || !rows)))
+    if (!x || rows < 0 || rows > COLI_FP4_MAX_ROWS || N < 0 || N > COLI_FP4_MAX_ROWS || K < 1 || (N && (!y || !offsets || !xr || !rows)))
         return 0;
     const size_t yb = (size_t)N * x->O * 4;
     if (!outputs_apart({{y, yb}, {xr, (size_t)rows * x->I * 4}, {src, (size_t)N * 4}, {offsets, (size_t)(x->E + 1) * 4}}, 1))

@@ -261,8 +261,8 @@ int coli_hip_tensor_quantize_mxfp4(ColiCudaTensor **tensor, const void *weights_
 /* y[S, O] = Q(x) W^T with Q the quantizer above (a row's 32-column blocks) and W a
  * resident MXFP4 tensor, on the fp4 matrix units: exact products, f32 sums. A scale
  * byte of 255 is NaN here, 0 is 2^-127. Host pointers (synchronous) / device pointers
- * (asynchronous; y must not overlap x). The gradient that passes it (straight through
- * Q) is coli_hip_gemm_t_dev. */
+ * (asynchronous; y must not overlap x). S up to 2^23, I up to 2^21. The gradient that
+ * passes it (straight through Q) is coli_hip_gemm_t_dev. */
 int coli_hip_fp4_matmul_a4(ColiCudaTensor *tensor, float *y, const float *x, int S);
 int coli_hip_fp4_matmul_a4_dev(ColiCudaTensor *tensor, float *y_dev, const float *x_dev, int S);
 /* The experts' matrices for that product over sorted rows: E <= 1024 resident
@@ -276,7 +276,7 @@ void coli_hip_experts_free(ColiHipExperts *experts);
 /* y[r] = W_e Q(x row of r) for the sorted rows offsets[e] <= r < offsets[e + 1] (ascending;
  * taken within 0..N) of y [N, O]; other rows of y are left as they were. The row is
  * x[src[r] / K] with src (of coli_hip_dispatch_dev: the rows need not be copied), x[r]
- * without; x is [rows, I], a row outside it counts as zeros. N and rows up to 2^24 - 1;
+ * without; x is [rows, I], a row outside it counts as zeros. N and rows up to 2^23;
  * without sorted rows (N 0) nothing is done. */
 int coli_hip_experts_a4_dev(ColiHipExperts *experts, float *y, const float *x, int rows, const int *src, int K,
                             const int *offsets, int N);

@@ -351,6 +351,47 @@ def test_experts_clamped(session):
         ex.check(ex.run(x, off, 90), mx_quant(x)[2], off, 90, np.arange(90))
 
 
+@pytest.mark.parametrize("pin", ["few", "many"])
+def test_swiglu_extremes(session, monkeypatch, pin):
+    """Gates from -infinity to infinity and NaN, with and without the clamp: gate and up are
+    single products here (one column of x, one weight a row), so the formula is checked alone."""
+    monkeypatch.setenv("COLI_HIP_FP4", pin)
+    O = 16
+    q4 = np.full((O, 16), 0x00, np.uint8)
+    q4[:, 0] = 2                                   # weight 1 in column 0
+    one = np.full((O, 1), 127, np.uint8)
+    two = np.full((O, 1), 128, np.uint8)
+    g, u = session.upload_mxfp4(q4, one, 32, O), session.upload_mxfp4(q4, two, 32, O)
+    x = np.zeros((26, 32), np.float32)
+    big = np.array([0, 0.5, 1, 3, 4, 6, 12, 24, 64, 96, 128, 192, 2.0 ** 60, 2.0 ** 126], np.float32)
+    x[:14, 0], x[14:25, 0], x[25, 0] = big, -big[1:12], np.nan
+    try:
+        for limit in (0.0, 1.5):
+            s = C.c_void_p()
+            (ga, _a), (ua, _b) = tensor_array([g]), tensor_array([u])
+            assert session.b.hip_experts_create(C.byref(s), 0, 1, ga, ua, limit)
+            with Bufs(session.b) as d:
+                y = d.up(np.zeros((26, O), np.float32))
+                assert session.b.hip_experts_a4_dev(s, y, d.up(x), 26, None, 1, d.up(np.array([0, 26], np.int32)), 26)
+                got = d.down(y, (26, O))
+            session.b.hip_experts_free(s)
+            a = x[:, 0].astype(np.float64)
+            b = 2 * a
+            if limit:
+                a, b = np.minimum(a, limit), np.clip(b, -limit, limit)
+            with np.errstate(over="ignore", invalid="ignore"):
+                ref = (silu(a) * b).astype(np.float32)
+            assert np.isnan(got[25]).all()
+            for r in range(25):
+                if np.isinf(ref[r]):
+                    assert (got[r] == ref[r]).all(), (r, got[r, 0])
+                else:   # 16 roundings, results below the normal range are zero
+                    assert (np.abs(got[r] - np.float64(ref[r])) <= 2.0 ** -20 * abs(float(ref[r])) + 2.0 ** -120).all(), (r, got[r, 0], ref[r])
+    finally:
+        session.free(g)
+        session.free(u)
+
+
 def test_experts_offsets_and_rows_outside(session):
     """Rows before the first and behind the last offset stay as they were, offsets are taken
     within 0..N, sources outside x are rows of zeros, and descending offsets are empty."""
@@ -471,11 +512,12 @@ def test_layer_of_sorted_rows(session, T):
             assert (np.abs(first - ref) <= room + (K + 1) * 2.0 ** -24 * mag).all()
 
 
-@pytest.mark.parametrize("S", [1, 3, 40, 300])
-def test_matmul_graph_replays(session, S):
-    """Replays over changing rows with larger eager calls between (outgrown workspaces stay)."""
+@pytest.mark.parametrize("S,I,O", [(1, 700, 90), (3, 700, 90), (40, 700, 90), (300, 700, 90), (100, 7000, 300)])
+def test_matmul_graph_replays(session, S, I, O):
+    """Replays over changing rows with larger eager calls between (outgrown workspaces stay); the
+    last size splits K."""
     rng = np.random.default_rng(S)
-    b, (I, O) = session.b, (700, 90)
+    b = session.b
     q4, e8 = rand_mxfp4(rng, O, I)
     h = session.upload_mxfp4(q4, e8, I, O)
     try:
