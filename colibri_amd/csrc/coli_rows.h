@@ -6,6 +6,7 @@
 
 typedef uint32_t u32x4a1 __attribute__((ext_vector_type(4), aligned(1)));   // 16 bytes at any address
 typedef uint32_t u32a1 __attribute__((aligned(1)));
+typedef uint16_t u16a1 __attribute__((aligned(1)));
 
 // N elements from p on as f32, and back, rounded to nearest even: 16 bytes a load. NT: past
 // the caches.

@@ -34,48 +34,51 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 // ---------------------------------------------------------------------------
 // quantization
 // ---------------------------------------------------------------------------
-// Eight elements of a row from column c on, zeros past its end, by loads that stay
-// inside the row: moved back where they would pass the end, and shifted to their
-// places again (no lane takes a branch of its own; see row4 in coli_device.h).
-// FORM 0: n % 8 == 0, 1: any n >= 8, 2: n < 8.
-template <typename T, int FORM, bool NT = false> __device__ __forceinline__ void row8(const T *xr, int c, int n, float (&v)[8]) {
+// V elements of a row from column c on, zeros past its end, by loads that stay inside
+// the row: moved back where they would pass the end, and shifted to their places again
+// (no lane takes a branch of its own; see row4 in coli_device.h).
+// FORM 0: n % V == 0, 1: any n >= V, 2: n < V.
+template <typename T, int FORM, int V, bool NT = false> __device__ __forceinline__ void row_vec(const T *xr, int c, int n, float (&v)[V]) {
     if constexpr (FORM == 2) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = (float)*GPTR(T, xr + min(c + i, n - 1));
+        for (int i = 0; i < V; i++) v[i] = (float)*GPTR(T, xr + min(c + i, n - 1));
     } else {
-        const int p = min(c, n - 8);
-        el_load<T, 8, NT>(xr + p, v);
+        const int p = min(c, n - V);
+        el_load<T, V, NT>(xr + p, v);
         if constexpr (FORM == 1) {
             const int d = c - p;
 #pragma unroll
-            for (int b = 1; b < 8; b <<= 1)
+            for (int b = 1; b < V; b <<= 1)
 #pragma unroll
-                for (int i = 0; i + b < 8; i++) v[i] = d & b ? v[i + b] : v[i];
+                for (int i = 0; i + b < V; i++) v[i] = d & b ? v[i + b] : v[i];
         }
     }
 #pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = c + i < n ? v[i] : 0.0f;
+    for (int i = 0; i < V; i++) v[i] = c + i < n ? v[i] : 0.0f;
 }
 
-// The eight codes of a lane and the scale byte of its four lanes' block. a / 6 with
+// The V codes of a lane and the scale byte of its 32 / V lanes' block. a / 6 with
 // a = m 2^e lies in (2^(e-3), 2^(e-2)] up to m = 1.5 and in (2^(e-2), 2^(e-1)) beyond,
 // so 2^ceil(log2(a / 6)) is read off a's bits: adding just under half of the mantissa's
 // range carries into the exponent beyond 1.5. The conversion divides by the scale
 // exactly and rounds once, to nearest even: no choice is left to rounding.
-__device__ __forceinline__ uint32_t mx_codes(const float (&v)[8], uint32_t &byte) {
+template <int V> __device__ __forceinline__ uint32_t mx_codes(const float (&v)[V], uint32_t &byte) {
     uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; i++) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+    for (int i = 0; i < V; i++) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
     m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xF, 0xF, false));
     m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xF, 0xF, false));
+    if constexpr (V == 4) m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x141, 0xF, 0xF, false));
     const uint32_t e = (m + 0x3fffffu) >> 23;
     byte = m == 0 ? 127u : m >= 0x7f800000u ? 255u : max(e, 3u) - 2u;
     const float scale = __uint_as_float(byte << 23);
     uint32_t u = 0;
     u = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(u, v[0], v[1], scale, 0);
     u = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(u, v[2], v[3], scale, 1);
-    u = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(u, v[4], v[5], scale, 2);
-    u = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(u, v[6], v[7], scale, 3);
+    if constexpr (V == 8) {
+        u = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(u, v[4], v[5], scale, 2);
+        u = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(u, v[6], v[7], scale, 3);
+    }
     return byte == 255u ? 0u : u;
 }
 
@@ -83,13 +86,15 @@ struct QuantArgs {
     const void *x;
     uint8_t *q4, *e8;
     int rows, cols, cp;   // columns, and as written: cp (operand form, a multiple of 256) or cols
-    int lpr, chunks;      // log2 of the lanes that take a row's octets, workgroups that share a row
+    int lpr, chunks;      // log2 of the lanes that a row has, workgroups that share a row
 };
 
-// Lanes of a row take its octets in turn, four to a block of 32. Native bytes, or
-// (OPERAND) rows of cp / 2 and cp / 32 bytes with zeros past the row's end, and behind
-// the last row one of zeros.
+// A lane takes 16 bytes of a row at a time, so that neighbours load whole cache lines
+// (8000 f32 rows of 14336 and back 227 us with 8 elements, 219 with 4).
+// Native bytes, or (OPERAND) rows of cp / 2 and cp / 32 bytes with zeros past the row's
+// end, and behind the last row one of zeros.
 template <typename T, int FORM, bool OPERAND> __device__ __forceinline__ void quant_rows(const QuantArgs &a, int blk) {
+    constexpr int V = 16 / sizeof(T);
     const int grp = blk / a.chunks, r = (grp << (8 - a.lpr)) + (threadIdx.x >> a.lpr);
     const int o0 = ((blk - grp * a.chunks) << a.lpr) + (threadIdx.x & ((1 << a.lpr) - 1));
     if (r >= a.rows + (OPERAND ? 1 : 0)) return;
@@ -97,24 +102,23 @@ template <typename T, int FORM, bool OPERAND> __device__ __forceinline__ void qu
     const T *xr = (const T *)a.x + (size_t)(zero ? 0 : r) * a.cols;
     const int end = OPERAND ? a.cp : (a.cols + 31) / 32 * 32;
     const size_t qs = OPERAND ? a.cp / 2 : (a.cols + 1) / 2, es = OPERAND ? a.cp / 32 : (a.cols + 31) / 32;
-    for (int c = 8 * o0; c < end; c += (8 << a.lpr) * a.chunks) {
-        float v[8];
+    for (int c = V * o0; c < end; c += (V << a.lpr) * a.chunks) {
+        float v[V];
         uint32_t byte;
-        row8<T, FORM, true>(xr, c, a.cols, v);   // (read once, past the caches: 8000 f32 rows of 14336 and back 264 -> 229 us)
+        row_vec<T, FORM, V, true>(xr, c, a.cols, v);   // (read once, past the caches: 8000 f32 rows of 14336 and back 264 -> 229 us)
         if constexpr (OPERAND) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = zero ? 0.0f : v[i];
+            for (int i = 0; i < V; i++) v[i] = zero ? 0.0f : v[i];
         }
-        const uint32_t u = mx_codes(v, byte);
+        const uint32_t u = mx_codes<V>(v, byte);
         uint8_t *q = a.q4 + (size_t)r * qs + c / 2;
-        if (OPERAND) {
-            *(uint32_t *)q = u;
-        } else if (c + 8 <= a.cols) {
-            *(u32a1 *)q = u;
+        if (OPERAND || c + V <= a.cols) {
+            if constexpr (V == 8) *(u32a1 *)q = u;
+            else *(u16a1 *)q = (uint16_t)u;
         } else {
             for (int i = 0; c + 2 * i < a.cols; i++) q[i] = (uint8_t)(u >> (8 * i));
         }
-        if ((threadIdx.x & 3) == 0) a.e8[(size_t)r * es + c / 32] = (uint8_t)byte;
+        if ((threadIdx.x & (32 / V - 1)) == 0) a.e8[(size_t)r * es + c / 32] = (uint8_t)byte;
     }
 }
 template <typename T, int FORM> __global__ __launch_bounds__(256) void coli_mx_quant(QuantArgs a) {
@@ -266,7 +270,7 @@ __device__ __forceinline__ i32x8 fp4_tile(u32x4 x) {
 // workgroup; its eight waves take the 128-column steps in turn, U of them requested
 // together, and add up in LDS, in the order of the waves. The weights' stream is the
 // bound.
-// FORM (of row8; -1: operands in memory): the workgroup quantizes the rows itself, into
+// FORM (of row_vec; -1: operands in memory): the workgroup quantizes the rows itself, into
 // LDS, behind its first weights' loads. That saves the operands' launch where the rows
 // are so few that 512 threads have done them before the weights are there.
 #define COLI_FP4_WAVES 8
@@ -357,8 +361,8 @@ template <int NM, int R, bool DUAL, int FORM> __global__ __launch_bounds__(64 * 
             const int r = o / opr, k = 8 * (o - r * opr);
             float v[8];
             uint32_t byte;
-            row8<float, FORM>(a.x + (size_t)r * a.I, k, a.I, v);
-            const uint32_t u = mx_codes(v, byte);
+            row_vec<float, FORM, 8>(a.x + (size_t)r * a.I, k, a.I, v);
+            const uint32_t u = mx_codes<8>(v, byte);
             *(uint32_t *)(xl + r * qs + k / 2) = u;
             if ((threadIdx.x & 3) == 0) xl[a.rows * qs + r * es + k / 32] = (uint8_t)byte;
         }
@@ -698,17 +702,17 @@ __global__ __launch_bounds__(256) void coli_fp4_join(const float *part, int spli
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-static int lanes_log2(int cols) {   // lanes of a row: its octets, 4 to 256
-    int l = 2;
-    while (l < 8 && (8 << l) < cols) l++;
+static int lanes_log2(int cols, int V) {   // lanes of a row, V columns each: a block's to 256
+    int l = V == 4 ? 3 : 2;
+    while (l < 8 && (V << l) < cols) l++;
     return l;
 }
 
 // Workgroups for rows of `cols` columns: groups of rows, and where these are few a row
-// of more than 2048 columns by several (8192 rows of 7168: 55 us whole, 59 in pieces).
-static unsigned mx_grid(int rows, int cols, int lpr, int *chunks) {
+// of more than one step of 256 lanes by several (8192 rows of 7168: 55 us whole, 59 in pieces).
+static unsigned mx_grid(int rows, int cols, int V, int lpr, int *chunks) {
     const unsigned groups = (unsigned)((rows + (256 >> lpr) - 1) / (256 >> lpr));
-    *chunks = (int)std::max(1u, std::min((unsigned)((cols + (8 << lpr) - 1) / (8 << lpr)), 2048 / groups));
+    *chunks = (int)std::max(1u, std::min((unsigned)((cols + (V << lpr) - 1) / (V << lpr)), 2048 / groups));
     return groups * *chunks;
 }
 
@@ -716,9 +720,11 @@ static size_t mx_q4_bytes(int rows, int cols) { return (size_t)rows * ((cols + 1
 static size_t mx_e8_bytes(int rows, int cols) { return (size_t)rows * ((cols + 31) / 32); }
 
 template <typename T> static void quant_launch(QuantArgs &a, hipStream_t st) {
-    const dim3 g(mx_grid(a.rows, a.cols, a.lpr, &a.chunks));
-    if (a.cols < 8) hipLaunchKernelGGL((coli_mx_quant<T, 2>), g, dim3(256), 0, st, a);
-    else if (a.cols % 8) hipLaunchKernelGGL((coli_mx_quant<T, 1>), g, dim3(256), 0, st, a);
+    constexpr int V = 16 / sizeof(T);
+    a.lpr = lanes_log2(a.cols, V);
+    const dim3 g(mx_grid(a.rows, a.cols, V, a.lpr, &a.chunks));
+    if (a.cols < V) hipLaunchKernelGGL((coli_mx_quant<T, 2>), g, dim3(256), 0, st, a);
+    else if (a.cols % V) hipLaunchKernelGGL((coli_mx_quant<T, 1>), g, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((coli_mx_quant<T, 0>), g, dim3(256), 0, st, a);
 }
 template <typename T> static void dequant_launch(const DequantArgs &a, dim3 g, bool nt, hipStream_t st) {
@@ -728,7 +734,7 @@ template <typename T> static void dequant_launch(const DequantArgs &a, dim3 g, b
     else hipLaunchKernelGGL((coli_mx_dequant<T, false>), g, dim3(256), 0, st, a);
 }
 static int quantize(DevCtx *ctx, const void *x, int dtype, int rows, int cols, uint8_t *q4, uint8_t *e8) {
-    QuantArgs a = {x, q4, e8, rows, cols, cols, lanes_log2(cols), 1};
+    QuantArgs a = {x, q4, e8, rows, cols, cols, 0, 1};
     if (dtype == 0) quant_launch<float>(a, ctx->stream);
     else if (dtype == 1) quant_launch<_Float16>(a, ctx->stream);
     else quant_launch<__bf16>(a, ctx->stream);
@@ -764,8 +770,8 @@ extern "C" int coli_hip_mxfp4_dequantize_dev(int device, const unsigned char *q4
     if (!bind_ctx(ctx)) return 0;
     if (!rows) return 1;
     forget_emitted(ctx, y, yb);
-    DequantArgs a = {q4, e8, y, rows, cols, lanes_log2(cols), 1};
-    const dim3 g(mx_grid(rows, cols, a.lpr, &a.chunks));
+    DequantArgs a = {q4, e8, y, rows, cols, lanes_log2(cols, 8), 1};
+    const dim3 g(mx_grid(rows, cols, 8, a.lpr, &a.chunks));
     const bool nt = yb > ((size_t)128 << 20);   // more than the 256 MB cache keeps for whoever reads y next
     if (dtype == 0) dequant_launch<float>(a, g, nt, ctx->stream);
     else if (dtype == 1) dequant_launch<_Float16>(a, g, nt, ctx->stream);
@@ -797,12 +803,12 @@ static int fp4_prep(DevCtx *ctx, const float *x, int rows, int I, const ItemArgs
     const size_t n = (size_t)rows + 1, qb = (n * (cp / 2) + 255) & ~(size_t)255, eb = n * (cp / 32);
     if (!reserve_kept(ctx, &ctx->fp4_x, qb + eb, 0)) return 0;
     uint8_t *p = (uint8_t *)ctx->fp4_x.p;
-    QuantArgs q = {x, p, p + qb, rows, I, cp, lanes_log2(cp), 1};
-    const int nblk = (int)mx_grid(rows + 1, cp, q.lpr, &q.chunks);
+    QuantArgs q = {x, p, p + qb, rows, I, cp, lanes_log2(cp, 4), 1};
+    const int nblk = (int)mx_grid(rows + 1, cp, 4, q.lpr, &q.chunks);
     const dim3 g(nblk + (it ? 1 : 0));
     const ItemArgs none = {};
-    if (I < 8) hipLaunchKernelGGL(coli_fp4_prep<2>, g, dim3(256), 0, ctx->stream, q, it ? *it : none);
-    else if (I % 8) hipLaunchKernelGGL(coli_fp4_prep<1>, g, dim3(256), 0, ctx->stream, q, it ? *it : none);
+    if (I < 4) hipLaunchKernelGGL(coli_fp4_prep<2>, g, dim3(256), 0, ctx->stream, q, it ? *it : none);
+    else if (I % 4) hipLaunchKernelGGL(coli_fp4_prep<1>, g, dim3(256), 0, ctx->stream, q, it ? *it : none);
     else hipLaunchKernelGGL(coli_fp4_prep<0>, g, dim3(256), 0, ctx->stream, q, it ? *it : none);
     if (!hip_check(hipGetLastError(), "fp4 operands")) return 0;
     a->xq = p;
