@@ -90,7 +90,7 @@ struct QuantArgs {
 };
 
 // A lane takes 16 bytes of a row at a time, so that neighbours load whole cache lines
-// (8000 f32 rows of 14336 and back 227 us with 8 elements, 219 with 4).
+// (8000 f32 rows of 14336 and back 227 us with 8 elements, 217 with 4).
 // Native bytes, or (OPERAND) rows of cp / 2 and cp / 32 bytes with zeros past the row's
 // end, and behind the last row one of zeros.
 template <typename T, int FORM, bool OPERAND> __device__ __forceinline__ void quant_rows(const QuantArgs &a, int blk) {
@@ -708,11 +708,15 @@ static int lanes_log2(int cols, int V) {   // lanes of a row, V columns each: a 
     return l;
 }
 
-// Workgroups for rows of `cols` columns: groups of rows, and where these are few a row
-// of more than one step of 256 lanes by several (8192 rows of 7168: 55 us whole, 59 in pieces).
+// Workgroups for rows of `cols` columns: groups of rows, and a row of more than one step
+// of 256 lanes by several: where groups are few, up to 2048 in all (8192 rows of 7168 bf16:
+// 55 us whole, 59 in pieces), and where f32 rows are many and more than six steps long
+// (operands and their product: 2048 rows of 14336 61 -> 57 us, 3000 of 7168 52.5 -> 51.8;
+// but 8000 of 4096 51 -> 52.6, 600 of 14336 30 -> 33).
 static unsigned mx_grid(int rows, int cols, int V, int lpr, int *chunks) {
-    const unsigned groups = (unsigned)((rows + (256 >> lpr) - 1) / (256 >> lpr));
-    *chunks = (int)std::max(1u, std::min((unsigned)((cols + (V << lpr) - 1) / (V << lpr)), 2048 / groups));
+    const unsigned groups = (unsigned)((rows + (256 >> lpr) - 1) / (256 >> lpr)), steps = (unsigned)((cols + (V << lpr) - 1) / (V << lpr));
+    const unsigned most = V == 4 && groups > 1024 && steps > 6 ? (8192 + groups) / groups : 2048 / groups;
+    *chunks = (int)std::max(1u, std::min(steps, most));
     return groups * *chunks;
 }
 

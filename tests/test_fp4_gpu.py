@@ -50,8 +50,8 @@ def check_quantize(b, x, dtype):
 # around the octets (8), a block (32), a lane's last octet, rows of one workgroup
 # (256 octets) and beyond
 @pytest.mark.parametrize("dtype", [0, 1, 2])
-@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 2), (2, 7), (5, 8), (4, 9), (70, 31), (3, 32), (9, 33), (2, 63), (5, 100), (37, 999),
-                                       (300, 64), (3, 2048), (2, 2050), (2, 4111), (1, 16500)])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 2), (2, 3), (6, 4), (3, 5), (2, 7), (5, 8), (4, 9), (40, 12), (70, 31), (3, 32), (9, 33), (2, 63),
+                                       (5, 100), (37, 999), (6, 1028), (300, 64), (3, 2048), (2, 2050), (2, 4111), (1, 16500), (1030, 6403)])
 def test_quantize(session, dtype, rows, cols):
     rng = np.random.default_rng(rows * 7 + cols + dtype)
     check_quantize(session.b, rng.standard_normal((rows, cols)) * np.exp(2 * rng.standard_normal((rows, 1))), dtype)
@@ -161,10 +161,10 @@ def matmul_a4(b, h, x, O, extra=1):
 
 # rows around the 16-row subtiles and the tiles, widths around the 128-column steps
 # and their pairs, outputs around the 16-row weight tiles
-@pytest.mark.parametrize("I,O,S", [(1, 1, 1), (7, 3, 2), (8, 16, 1), (31, 17, 5), (32, 33, 16), (100, 40, 17), (128, 64, 1), (129, 15, 33),
+@pytest.mark.parametrize("I,O,S", [(1, 1, 1), (3, 9, 70), (4, 9, 40), (5, 20, 40), (12, 20, 200), (7, 3, 2), (8, 16, 1), (31, 17, 5), (32, 33, 16), (100, 40, 17), (128, 64, 1), (129, 15, 33),
                                    (256, 48, 64), (257, 100, 65), (384, 16, 3), (1000, 2999, 21), (999, 130, 70), (2048, 200, 128),
                                    (1152, 96, 129), (4096, 512, 1), (4096, 300, 200), (16400, 40, 9), (640, 1040, 300), (512, 4112, 2),
-                                   (3000, 24, 1000), (700, 14000, 21), (500, 13200, 3),
+                                   (3000, 24, 1000), (7000, 16, 1100), (700, 14000, 21), (500, 13200, 3),
                                    (2000, 7100, 4), (1100, 13200, 50)])
 def test_matmul(session, I, O, S):
     rng = np.random.default_rng(I + O * 3 + S)
