@@ -242,18 +242,28 @@ template <int FORM> __global__ __launch_bounds__(256) void coli_fp4_prep(QuantAr
 
 // swiglu_out on the hardware's exp2 and reciprocal (a step of each, beside products whose
 // sums carry more): exp(-g) = 2^h (1 + l ln 2) with h + l = -g log2(e) in two parts, right
-// to 5 x 2^-24 over g's whole range. A third of the instructions of expf and the division,
-// which a short product shows (16384 rows through 8 pairs of 2048 x 1024: 90 us, 77 so and
-// with the weights requested ahead of the rows).
-__device__ __forceinline__ float fp4_swiglu(float g, float u, float limit) {
+// to 5 x 2^-24 for gates from COLI_FP4_LOW up. A third of the instructions of expf and the
+// division, which a short product shows (16384 rows through 8 pairs of 2048 x 1024: 90 us, 77
+// so and with the weights requested ahead of the rows).
+// LOW: gates below it too, whose sigmoid is exp(g) in f32 and (from -87.34 down) below the
+// normal range, where the reciprocal is 0: 2^n 2^f in two steps, the up scaled by 2^-64
+// meanwhile, so that nothing is lost that the result can hold. Where 2^-64 takes a small up out of
+// range the result is below it too: |g| exp(g) < 2^-119. Gates below -300 count as -300: the
+// result is 0 for every finite up.
+#define COLI_FP4_LOW -87.0f
+template <bool LOW> __device__ __forceinline__ float fp4_swiglu(float g, float u, float limit) {
     if (limit > 0.0f) {   // (compared, not fminf: a NaN stays one)
         g = g > limit ? limit : g;
         u = u > limit ? limit : u < -limit ? -limit : u;
     }
-    const float c = fminf(fmaxf(g, -128.0f), 128.0f);   // beyond, the sigmoid is 0 or 1 in f32
+    const float c = fminf(fmaxf(g, -128.0f), 128.0f);   // beyond, the sigmoid is 1 in f32, or 0 (LOW has it)
     const float h = c * -1.44269504f, l = fmaf(c, -1.44269504f, -h) + c * -1.92596303e-8f;
     const float e = __builtin_amdgcn_exp2f(h) * fmaf(l, 0.693147181f, 1.0f);
-    return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
+    const float y = g * __builtin_amdgcn_rcpf(1.0f + e) * u;
+    if constexpr (!LOW) return y;
+    const float d = fmaxf(g, -300.0f), n = rintf(d * 1.44269504f), f = fmaf(d, 1.44269504f, -n) + d * 1.92596303e-8f;
+    const float z = __builtin_ldexpf(d * __builtin_amdgcn_exp2f(f) * (u * 0x1p-64f), (int)n + 64);
+    return g < COLI_FP4_LOW && g > -INFINITY ? z : y;
 }
 
 // 4x4 dword transpose across the four 16-lane rows: the stored tile gives lane (c,
@@ -395,7 +405,7 @@ template <int NM, int R, bool DUAL, int FORM> __global__ __launch_bounds__(64 * 
         float *y = a.y + (size_t)(it.r0 + row) * a.O + o;
         if constexpr (DUAL) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) v[i] = fp4_swiglu(v[i], u[i], a.limit);
+            for (int i = 0; i < 4; i++) v[i] = fp4_swiglu<true>(v[i], u[i], a.limit);
         }
         if (o + 4 <= a.O) {
             *(f4u *)y = v;
@@ -642,22 +652,35 @@ template <int NB, bool DUAL, bool NT> __device__ __forceinline__ void fp4_many(c
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     // lane (n, g), register i: row 8 (i / 4) + 4 g + i % 4 of the block, output n of the
     // operand's 32: a store fills whole cache lines of two rows
+    auto store = [&](auto low) {
 #pragma unroll
-    for (int r = 0; r < (DUAL ? 1 : 2); r++) {
-        const int o = 16 * rt[r] + n;
-        float *y = (a.splits > 1 ? a.part + (size_t)split * a.S * a.O : a.y) + (size_t)it.r0 * a.O + o;
-        if (o >= a.O) continue;
+        for (int r = 0; r < (DUAL ? 1 : 2); r++) {
+            const int o = 16 * rt[r] + n;
+            float *y = (a.splits > 1 ? a.part + (size_t)split * a.S * a.O : a.y) + (size_t)it.r0 * a.O + o;
+            if (o >= a.O) continue;
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int row = 32 * b + 8 * (i >> 2) + 4 * g + (i & 3);
+                    float v = acc[r][b][i];
+                    if constexpr (DUAL) v = fp4_swiglu<decltype(low)::value>(v, acc[1][b][i], a.limit);
+                    if (row >= it.nrows) continue;
+                    if constexpr (NT) __builtin_nontemporal_store(v, y + (size_t)row * a.O);
+                    else y[(size_t)row * a.O] = v;
+                }
+        }
+    };
+    if constexpr (DUAL) {   // gates below COLI_FP4_LOW are rare: looked for by their bits, once for the wave
+        uint32_t m = 0;
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const int row = 32 * b + 8 * (i >> 2) + 4 * g + (i & 3);
-                float v = acc[r][b][i];
-                if constexpr (DUAL) v = fp4_swiglu(v, acc[1][b][i], a.limit);
-                if (row >= it.nrows) continue;
-                if constexpr (NT) __builtin_nontemporal_store(v, y + (size_t)row * a.O);
-                else y[(size_t)row * a.O] = v;
-            }
+            for (int i = 0; i < 16; i++) m = max(m, __float_as_uint(acc[0][b][i]));
+        if (__any(m > __float_as_uint(COLI_FP4_LOW))) store(std::true_type{});
+        else store(std::false_type{});
+    } else {
+        store(std::false_type{});
     }
 }
 // Workgroups of one XCD (every eighth) take consecutive tiles, a group of items' tiles of

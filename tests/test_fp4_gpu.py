@@ -392,6 +392,58 @@ def test_swiglu_extremes(session, monkeypatch, pin):
         session.free(u)
 
 
+@pytest.mark.parametrize("pin", ["few", "many"])
+def test_swiglu_of_low_gates(session, monkeypatch, pin):
+    """Gates whose sigmoid is below f32's normal range, with ups that bring the result back into it:
+    a gate is the sum of three columns, exactly, and an up has a column of its own. 16 roundings of
+    2^-24 and half the smallest step. Rows beside such gates keep their bits."""
+    monkeypatch.setenv("COLI_HIP_FP4", pin)
+    O, I = 16, 128
+    gates = [(-96, 12, -2), (-96, 12, -3), (-96, 8, 0.75), (-96, 8, 0.5), (-96, 8, 0), (-96, 8, -0.5), (-96, 8, -0.75), (-96, 8, -1),
+             (-96, 4, 0), (-96, 0, 0), (-96, -6, 0.5), (-96, -8, 0), (-128, 0, 0), (-128, -24, 2), (-192, 12, 0), (-192, -3, 0),
+             (-2.0 ** 80, 0, 0), (-96, 64, 0), (1, 0, 0), (96, -8, 0), (-1, 0, 0)]
+    ups = [1, -2.0 ** 20, 2.0 ** 60, 1.5 * 2.0 ** 126, 2.0 ** -20]
+    q = np.zeros((2, O, I // 2), np.uint8)
+    q[0, :, [0, 16, 32]] = 2                       # weight 1 in columns 0, 32 and 64
+    q[1, :, 48] = 2                                # and in 96
+    one = np.full((O, I // 32), 127, np.uint8)
+    g, u = session.upload_mxfp4(q[0], one, I, O), session.upload_mxfp4(q[1], one, I, O)
+    x = np.zeros((len(gates) * len(ups), I), np.float32)
+    for r, (gate, up) in enumerate((a, b) for b in ups for a in gates):
+        x[r, [0, 32, 64]], x[r, 96] = gate, up
+    n = len(x)
+    a, b = x[:, [0, 32, 64]].astype(np.float64).sum(1), x[:, 96].astype(np.float64)
+    assert np.array_equal(mx_quant(x)[2], x)       # every value has a code
+    s = C.c_void_p()
+    (ga, _a), (ua, _b) = tensor_array([g]), tensor_array([u])
+
+    def run(x):
+        with Bufs(session.b) as d:
+            y = d.up(np.zeros((len(x), O), np.float32))
+            assert session.b.hip_experts_a4_dev(s, y, d.up(x), len(x), None, 1, d.up(np.array([0, len(x)], np.int32)), len(x))
+            return d.down(y, (len(x), O))
+
+    try:
+        for limit in (0.0, 2.0 ** 125):
+            assert session.b.hip_experts_create(C.byref(s), 0, 1, ga, ua, limit)
+            got = run(x)
+            c = np.clip(b, -limit, limit) if limit else b
+            ref = silu(a) * c
+            over = np.abs(ref) >= 2.0 ** 128       # infinities of f32 (none of the others is near)
+            assert (got[over] == np.sign(ref[over])[:, None] * np.inf).all()
+            ref = np.where(over, 0, ref)
+            bad = (np.abs(got - ref[:, None]) > 2.0 ** -20 * np.abs(ref[:, None]) + 2.0 ** -150) & ~over[:, None]
+            assert not bad.any(), [(float(a[r]), float(c[r]), float(got[r, 0]), float(ref[r])) for r in np.flatnonzero(bad.any(1))]
+            high = np.flatnonzero(a > -64)
+            assert np.array_equal(run(np.ascontiguousarray(x[high])), got[high])
+            session.b.hip_experts_free(s)
+            s = C.c_void_p()
+    finally:
+        session.b.hip_experts_free(s)
+        session.free(g)
+        session.free(u)
+
+
 def test_experts_offsets_and_rows_outside(session):
     """Rows before the first and behind the last offset stay as they were, offsets are taken
     within 0..N, sources outside x are rows of zeros, and descending offsets are empty."""
