@@ -444,6 +444,28 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t fp4_rsrc(const void *p, uint32
     return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, n, 0x00020000);
 }
 __device__ __forceinline__ i32x8 fp4_op(u32x4 v) { return (i32x8){(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0}; }
+// The results of a wave's operands. Lane (n, g), register i: row 8 (i / 4) + 4 g + i % 4 of the
+// block, output n of the operand's 32: a store fills whole cache lines of two rows.
+template <int NB, bool DUAL, bool NT, bool LOW> __device__ __forceinline__ void fp4_store(
+    const Fp4Args &a, const Fp4Item &it, const int (&rt)[2], int split, int n, int g, const floatx16 (&acc)[2][NB]) {
+#pragma unroll
+    for (int r = 0; r < (DUAL ? 1 : 2); r++) {
+        const int o = 16 * rt[r] + n;
+        float *y = (a.splits > 1 ? a.part + (size_t)split * a.S * a.O : a.y) + (size_t)it.r0 * a.O + o;
+        if (o >= a.O) continue;
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const int row = 32 * b + 8 * (i >> 2) + 4 * g + (i & 3);
+                float v = acc[r][b][i];
+                if constexpr (DUAL) v = fp4_swiglu<LOW>(v, acc[1][b][i], a.limit);
+                if (row >= it.nrows) continue;
+                if constexpr (NT) __builtin_nontemporal_store(v, y + (size_t)row * a.O);
+                else y[(size_t)row * a.O] = v;
+            }
+    }
+}
 // NB: 32-row blocks
 template <int NB, bool DUAL, bool NT> __device__ __forceinline__ void fp4_many(const Fp4Args &a, const Fp4Item &it, int rb,
                                                                       int split, lds_u8 *lds) {
@@ -650,38 +672,18 @@ template <int NB, bool DUAL, bool NT> __device__ __forceinline__ void fp4_many(c
     }
     // the last DMAs write this workgroup's LDS: none may outlive it
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    // lane (n, g), register i: row 8 (i / 4) + 4 g + i % 4 of the block, output n of the
-    // operand's 32: a store fills whole cache lines of two rows
-    auto store = [&](auto low) {
-#pragma unroll
-        for (int r = 0; r < (DUAL ? 1 : 2); r++) {
-            const int o = 16 * rt[r] + n;
-            float *y = (a.splits > 1 ? a.part + (size_t)split * a.S * a.O : a.y) + (size_t)it.r0 * a.O + o;
-            if (o >= a.O) continue;
-#pragma unroll
-            for (int b = 0; b < NB; b++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int row = 32 * b + 8 * (i >> 2) + 4 * g + (i & 3);
-                    float v = acc[r][b][i];
-                    if constexpr (DUAL) v = fp4_swiglu<decltype(low)::value>(v, acc[1][b][i], a.limit);
-                    if (row >= it.nrows) continue;
-                    if constexpr (NT) __builtin_nontemporal_store(v, y + (size_t)row * a.O);
-                    else y[(size_t)row * a.O] = v;
-                }
-        }
-    };
     if constexpr (DUAL) {   // gates below COLI_FP4_LOW are rare: looked for by their bits, once for the wave
         uint32_t m = 0;
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
             for (int i = 0; i < 16; i++) m = max(m, __float_as_uint(acc[0][b][i]));
-        if (__any(m > __float_as_uint(COLI_FP4_LOW))) store(std::true_type{});
-        else store(std::false_type{});
-    } else {
-        store(std::false_type{});
+        if (__any(m > __float_as_uint(COLI_FP4_LOW))) {
+            fp4_store<NB, DUAL, NT, true>(a, it, rt, split, n, g, acc);
+            return;
+        }
     }
+    fp4_store<NB, DUAL, NT, false>(a, it, rt, split, n, g, acc);
 }
 // Workgroups of one XCD (every eighth) take consecutive tiles, a group of items' tiles of
 // one block of weights before the next block's, so that both stay in its L2: eight items
