@@ -189,6 +189,7 @@ struct Fp4Args {
     float *y;
     int group;                 // items of a group (coli_fp4_many)
     float limit;
+    int item0;                 // the launch's first item
 };
 
 // The items of sorted rows: tiles of `tile` rows of each expert. Offsets are taken
@@ -291,7 +292,7 @@ template <int NM, int R, bool DUAL, int FORM> __global__ __launch_bounds__(64 * 
     extern __shared__ __attribute__((aligned(16))) uint8_t xl[];   // (OWN) codes, then scales
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, g = lane >> 4;
-    const int item = blockIdx.x / a.rtb, rb = blockIdx.x - item * a.rtb;
+    const int in = blockIdx.x / a.rtb, rb = blockIdx.x - in * a.rtb, item = a.item0 + in;
     Fp4Item it = {a.mat0, item * a.tile, min(a.tile, a.S - item * a.tile)};
     if (a.items) {
         if (item >= *a.n_items) return;
@@ -694,14 +695,14 @@ template <int NB, bool DUAL, bool NT> __device__ __forceinline__ void fp4_many(c
 // and drops the hint).
 template <bool DUAL, bool NT> __global__ __launch_bounds__(256, 2) void coli_fp4_many(Fp4Args a, int n_items) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];   // FmGeom::kPD stages
-    const int n = a.items ? min(*a.n_items, n_items) : n_items;
+    const int n = a.items ? min(*a.n_items - a.item0, n_items) : n_items;   // (none left: 0 or less)
     const int total = n * a.rtb * a.splits, per = (total + 7) / 8, j = blockIdx.x >> 3;
     int id = (blockIdx.x & 7) * per + j;
     if (j >= per || id >= total) return;
     const int split = id / (n * a.rtb);
     id -= split * n * a.rtb;
     const int grp = id / (a.group * a.rtb), in = id - grp * a.group * a.rtb, gi = min(a.group, n - grp * a.group);
-    const int item = grp * a.group + in % gi, rb = in / gi;
+    const int item = a.item0 + grp * a.group + in % gi, rb = in / gi;
     Fp4Item it = {a.mat0, item * a.tile, min(a.tile, a.S - item * a.tile)};
     if (a.items) it = a.items[item];
     if (it.nrows <= 64) fp4_many<2, DUAL, NT>(a, it, rb, split, (lds_u8 *)lds);
@@ -917,11 +918,19 @@ template <int NM, int FORM> static void few_launch(const Fp4Args &a, dim3 g, boo
     else hipLaunchKernelGGL((coli_fp4_few<NM, 1, false, FORM>), g, b, own, st, a);
 }
 
-// The launch over n_items items of tiles of a.tile rows, `rows` in all.
+// Workgroups of an item, and how many items a launch takes: 2^32 threads are its limit. 0 where
+// one item has more (beyond 2^27 - 16 outputs).
+static int fp4_blocks(int nrt, bool dual, const Fp4Plan &plan, int *rtb) {
+    const int R = plan.tile == COLI_FP4_MANY ? (dual ? 8 : 16) : plan.R;
+    *rtb = (nrt + R - 1) / R;
+    return (int)(((1 << 23) - 1) / ((int64_t)*rtb * plan.splits));
+}
+
+// The launches over n_items items of tiles of a.tile rows, `rows` in all.
 static int fp4_run(DevCtx *ctx, Fp4Args &a, int n_items, int rows, bool dual, const Fp4Plan &plan) {
+    const int most = fp4_blocks(a.nrt, dual, plan, &a.rtb);
+    if (!most) return 0;
     if (a.tile == COLI_FP4_MANY) {
-        a.rtb = (a.nrt + (dual ? 7 : 15)) / (dual ? 8 : 16);
-        if ((int64_t)n_items * a.rtb * plan.splits >= (1 << 23)) return 0;
         a.sps = (a.cp / 256 + plan.splits - 1) / plan.splits;
         a.splits = (a.cp / 256 + a.sps - 1) / a.sps;
         if (a.splits > 1 && !reserve_kept(ctx, &ctx->fp4_part, (size_t)a.splits * a.S * a.O * 4, 0)) return 0;
@@ -929,13 +938,16 @@ static int fp4_run(DevCtx *ctx, Fp4Args &a, int n_items, int rows, bool dual, co
         // Outputs beyond half of the 256 MB cache go past it (8192 x 4096 x 14336 380 -> 290
         // us); smaller ones may be there still when they are read (2048 rows: no difference).
         const bool nt = a.splits == 1 && (size_t)rows * a.O * 4 > ((size_t)128 << 20);
-        const dim3 g((unsigned)(n_items * a.rtb * a.splits + 7) / 8 * 8);
         const size_t shm = FmGeom::kPD * FmGeom::kStage;
-        if (dual && nt) hipLaunchKernelGGL((coli_fp4_many<true, true>), g, dim3(256), shm, ctx->stream, a, n_items);
-        else if (dual) hipLaunchKernelGGL((coli_fp4_many<true, false>), g, dim3(256), shm, ctx->stream, a, n_items);
-        else if (nt) hipLaunchKernelGGL((coli_fp4_many<false, true>), g, dim3(256), shm, ctx->stream, a, n_items);
-        else hipLaunchKernelGGL((coli_fp4_many<false, false>), g, dim3(256), shm, ctx->stream, a, n_items);
-        if (!hip_check(hipGetLastError(), "fp4 product")) return 0;
+        for (a.item0 = 0; a.item0 < n_items; a.item0 += most) {
+            const int n = std::min(most, n_items - a.item0);
+            const dim3 g((unsigned)(n * a.rtb * a.splits + 7) / 8 * 8);
+            if (dual && nt) hipLaunchKernelGGL((coli_fp4_many<true, true>), g, dim3(256), shm, ctx->stream, a, n);
+            else if (dual) hipLaunchKernelGGL((coli_fp4_many<true, false>), g, dim3(256), shm, ctx->stream, a, n);
+            else if (nt) hipLaunchKernelGGL((coli_fp4_many<false, true>), g, dim3(256), shm, ctx->stream, a, n);
+            else hipLaunchKernelGGL((coli_fp4_many<false, false>), g, dim3(256), shm, ctx->stream, a, n);
+            if (!hip_check(hipGetLastError(), "fp4 product")) return 0;
+        }
         if (a.splits > 1) {
             const size_t n = (size_t)a.S * a.O;
             hipLaunchKernelGGL(coli_fp4_join, dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, ctx->stream, a.part, a.splits, n, a.y);
@@ -943,17 +955,18 @@ static int fp4_run(DevCtx *ctx, Fp4Args &a, int n_items, int rows, bool dual, co
         return hip_check(hipGetLastError(), "fp4 join");
     }
     const int R = plan.R;
-    a.rtb = (a.nrt + R - 1) / R;
-    if ((int64_t)n_items * a.rtb >= (1 << 23)) return 0;
-    const dim3 g((unsigned)n_items * a.rtb);
-    if (a.x && a.I % 8 && a.tile <= 16) few_launch<1, 1>(a, g, dual, R, ctx->stream);
-    else if (a.x && a.I % 8) few_launch<2, 1>(a, g, dual, R, ctx->stream);
-    else if (a.x && a.tile <= 16) few_launch<1, 0>(a, g, dual, R, ctx->stream);
-    else if (a.x) few_launch<2, 0>(a, g, dual, R, ctx->stream);
-    else if (a.tile <= 16) few_launch<1, -1>(a, g, dual, R, ctx->stream);
-    else if (a.tile <= 32) few_launch<2, -1>(a, g, dual, R, ctx->stream);
-    else few_launch<4, -1>(a, g, dual, R, ctx->stream);
-    return hip_check(hipGetLastError(), "fp4 product");
+    for (a.item0 = 0; a.item0 < n_items; a.item0 += most) {
+        const dim3 g((unsigned)std::min(most, n_items - a.item0) * a.rtb);
+        if (a.x && a.I % 8 && a.tile <= 16) few_launch<1, 1>(a, g, dual, R, ctx->stream);
+        else if (a.x && a.I % 8) few_launch<2, 1>(a, g, dual, R, ctx->stream);
+        else if (a.x && a.tile <= 16) few_launch<1, 0>(a, g, dual, R, ctx->stream);
+        else if (a.x) few_launch<2, 0>(a, g, dual, R, ctx->stream);
+        else if (a.tile <= 16) few_launch<1, -1>(a, g, dual, R, ctx->stream);
+        else if (a.tile <= 32) few_launch<2, -1>(a, g, dual, R, ctx->stream);
+        else few_launch<4, -1>(a, g, dual, R, ctx->stream);
+        if (!hip_check(hipGetLastError(), "fp4 product")) return 0;
+    }
+    return 1;
 }
 
 #define COLI_FP4_MAX_I (1 << 21)       // a tile's operand rows lie within 2 GiB (128 MiB)
@@ -962,8 +975,9 @@ static int fp4_run(DevCtx *ctx, Fp4Args &a, int n_items, int rows, bool dual, co
 int matmul_a4_dev(DevCtx *ctx, ColiCudaTensor *t, float *y_dev, const float *x_dev, int S) {
     Fp4Args a = {};
     if (t->I > COLI_FP4_MAX_I || S > COLI_FP4_MAX_ROWS) return 0;
-    forget_emitted(ctx, y_dev, (size_t)S * t->O * 4);
     const Fp4Plan plan = fp4_plan(ctx, t, S);
+    if (!fp4_blocks(t->nrt, false, plan, &a.rtb)) return 0;
+    forget_emitted(ctx, y_dev, (size_t)S * t->O * 4);
     a.tile = plan.tile;
     if (plan.own) {
         a.x = x_dev;
@@ -1058,7 +1072,6 @@ extern "C" int coli_hip_experts_a4_dev(ColiHipExperts *x, float *y, const float 
     DevCtx *ctx = ctx_of(x->device);
     if (!bind_ctx(ctx)) return 0;
     if (!N) return 1;
-    forget_emitted(ctx, y, yb);
     ItemArgs it = {};
     it.offsets = offsets;
     it.mats = x->mats;
@@ -1074,12 +1087,14 @@ extern "C" int coli_hip_experts_a4_dev(ColiHipExperts *x, float *y, const float 
     const size_t xb = ((size_t)rows + 1) * (((size_t)x->I + 255) / 256 * 128);
     if (src && xb > ((size_t)1 << 31)) plan.tile = mean <= 16 ? 16 : 64;
     else if (pin) plan.tile = std::strcmp(pin, "many") == 0 ? COLI_FP4_MANY : mean <= 16 ? 16 : mean <= 32 ? 32 : 64;
+    Fp4Args a = {};
+    if (!fp4_blocks(x->nrt, x->dual != 0, plan, &a.rtb)) return 0;
+    forget_emitted(ctx, y, yb);
     it.tile = plan.tile;
     it.room = (int)std::min<int64_t>(N, N / it.tile + x->E);
     if (!reserve_kept(ctx, &ctx->fp4_items, 256 + (size_t)it.room * sizeof(Fp4Item), 0)) return 0;
     it.n_items = (int *)ctx->fp4_items.p;
     it.items = (Fp4Item *)((uint8_t *)ctx->fp4_items.p + 256);
-    Fp4Args a = {};
     if (!fp4_prep(ctx, xr, rows, x->I, &it, &a)) return 0;
     a.items = it.items;
     a.n_items = it.n_items;

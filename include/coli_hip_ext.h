@@ -261,14 +261,14 @@ int coli_hip_tensor_quantize_mxfp4(ColiCudaTensor **tensor, const void *weights_
 /* y[S, O] = Q(x) W^T with Q the quantizer above (a row's 32-column blocks) and W a
  * resident MXFP4 tensor, on the fp4 matrix units: exact products, f32 sums. A scale
  * byte of 255 is NaN here, 0 is 2^-127. Host pointers (synchronous) / device pointers
- * (asynchronous; y must not overlap x). S up to 2^23, I up to 2^21. The gradient that
- * passes it (straight through Q) is coli_hip_gemm_t_dev. */
+ * (asynchronous; y must not overlap x). S up to 2^23, I up to 2^21, O up to 2^27 - 16. The
+ * gradient that passes it (straight through Q) is coli_hip_gemm_t_dev. */
 int coli_hip_fp4_matmul_a4(ColiCudaTensor *tensor, float *y, const float *x, int S);
 int coli_hip_fp4_matmul_a4_dev(ColiCudaTensor *tensor, float *y_dev, const float *x_dev, int S);
 /* The experts' matrices for that product over sorted rows: E <= 1024 resident
- * MXFP4 tensors [O, I] of one shape on one device; with ups a second one each,
- * and silu(gate) * up as the result (swiglu_limit > 0: the clamped form). The
- * tensors must outlive the set. */
+ * MXFP4 tensors [O, I] of one shape (I and O as above) on one device; with ups a
+ * second one each, and silu(gate) * up as the result (swiglu_limit > 0: the clamped
+ * form). The tensors must outlive the set. */
 typedef struct ColiHipExperts ColiHipExperts;
 int coli_hip_experts_create(ColiHipExperts **experts, int device, int E, ColiCudaTensor *const *gates,
                             ColiCudaTensor *const *ups, float swiglu_limit);

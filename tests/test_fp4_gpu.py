@@ -444,6 +444,67 @@ def test_swiglu_of_low_gates(session, monkeypatch, pin):
         session.free(u)
 
 
+@pytest.mark.parametrize("pin,O", [("few", 144000), ("many", 1160000)])
+def test_experts_of_more_workgroups_than_a_launch(session, monkeypatch, pin, O):
+    """1024 experts of a row each and so many outputs that their workgroups pass 2^23: rows before, at
+    and behind the place where the launches part, and the row behind the last as it was."""
+    monkeypatch.setenv("COLI_HIP_FP4", pin)
+    rng = np.random.default_rng(13)
+    E, I = 1024, 8
+    mats = [rand_mxfp4(rng, O, I) for _ in range(2)]
+    h = [session.upload_mxfp4(q, e, I, O) for q, e in mats]
+    w = [deq_mxfp4(q, e, I) for q, e in mats]
+    s = C.c_void_p()
+    (ga, _a), (ua, _b) = tensor_array([h[0]] * E), tensor_array([h[1]] * E)
+    b, x = session.b, act(rng, E, I)
+    y = b.cuda_pipe_alloc(0, (E + 1) * O * 4)
+    try:
+        assert y and b.hip_experts_create(C.byref(s), 0, E, ga, ua, 0.0)
+        with Bufs(b) as d:
+            d.put(y + E * O * 4, np.full(O, 7, np.float32))
+            assert b.hip_experts_a4_dev(s, y, d.up(x), E, None, 1, d.up(np.arange(E + 1, dtype=np.int32)), E)
+            for r in (0, 1, 500, 900, *range(920, 936), 1000, 1023):
+                got, xv = d.down(y + r * O * 4, O), mx_quant(x[r:r + 1])[2][0]
+                g, u = (v @ xv for v in w)
+                tg, tu = (product_tol(I) * (np.abs(v) @ np.abs(xv)) for v in w)
+                tol = 1.1 * tg * np.abs(u) + np.abs(silu(g)) * tu + 1.1 * tg * tu + 2.0 ** -20 * np.abs(silu(g) * u) + 1e-30
+                assert (np.abs(got - silu(g) * u) <= tol).all(), r
+            assert (d.down(y + E * O * 4, O) == 7).all()
+    finally:
+        b.hip_experts_free(s)
+        b.cuda_pipe_free(0, y)
+        for t in h:
+            session.free(t)
+
+
+def test_experts_of_rows_beyond_2_gib(session, monkeypatch):
+    """Operands of more than 2 GiB that src chooses from: the bits of the same rows copied out. Only
+    the chosen rows of x hold anything."""
+    rng = np.random.default_rng(14)
+    b, (I, rows, N, K, O) = session.b, (1 << 20, 4200, 150, 2, 20)
+    at = np.array([0, 1, 2047, 2048, 4095, 4096, 4198, 4199], np.int64)
+    xr, pick, off = act(rng, len(at), I), rng.integers(0, len(at), N), [0, 20, 150]
+    src = (at[pick] * K + rng.integers(0, K, N)).astype(np.int32)
+    src[77] = rows * K
+    x = b.cuda_pipe_alloc(0, rows * I * 4)
+    try:
+        assert x
+        with Experts(session, rng, 2, I, O, False) as ex, Bufs(b) as d:
+            for r, v in zip(at, xr):
+                d.put(x + int(r) * I * 4, v)
+            y = d.up(np.full((N + 1, O), 7, np.float32))
+            assert b.hip_experts_a4_dev(ex.set, y, x, rows, d.up(src), K, d.up(np.array(off, np.int32)), N)
+            got = d.down(y, (N + 1, O))
+            assert (got[N] == 7).all() and not got[77].any()
+            pick[77] = 0
+            monkeypatch.setenv("COLI_HIP_FP4", "few")
+            want = ex.run(xr, off, N, src=pick.astype(np.int32))[:N]
+            want[77] = 0
+            assert np.array_equal(got[:N], want) and np.abs(want).max() > 1
+    finally:
+        b.cuda_pipe_free(0, x)
+
+
 def test_experts_offsets_and_rows_outside(session):
     """Rows before the first and behind the last offset stay as they were, offsets are taken
     within 0..N, sources outside x are rows of zeros, and descending offsets are empty."""
