@@ -26,18 +26,24 @@ template <typename T, int N, bool NT = false> __device__ __forceinline__ void el
         }
     }
 }
+// One value as T. fp16 of a finished f32: left to itself the compiler folds a product into
+// v_fma_mixlo_f16 with +0 as its addend, which makes +0 of -0.
+template <typename T> __device__ __forceinline__ T el_of(float f) {
+    if constexpr (__is_same(T, _Float16)) asm("" : "+v"(f));
+    return (T)f;
+}
 template <typename T, int N, bool NT = false> __device__ __forceinline__ void el_store(T *p, const float (&f)[N]) {
     constexpr int V = 16 / sizeof(T);
     if constexpr (N % V) {
 #pragma unroll
-        for (int i = 0; i < N; i++) p[i] = (T)f[i];
+        for (int i = 0; i < N; i++) p[i] = el_of<T>(f[i]);
     } else {
         struct Raw { T e[V]; };
 #pragma unroll
         for (int k = 0; k < N; k += V) {
             Raw r;
 #pragma unroll
-            for (int i = 0; i < V; i++) r.e[i] = (T)f[k + i];
+            for (int i = 0; i < V; i++) r.e[i] = el_of<T>(f[k + i]);
             if constexpr (NT) __builtin_nontemporal_store((u32x4a1)__builtin_bit_cast(u32x4, r), (u32x4a1 *)(p + k));
             else *(u32x4a1 *)(p + k) = __builtin_bit_cast(u32x4, r);
         }

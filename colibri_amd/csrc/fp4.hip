@@ -157,7 +157,7 @@ template <typename T, bool NT> __global__ __launch_bounds__(256) void coli_mx_de
         } else {
 #pragma unroll
             for (int i = 0; i < 8; i++)
-                if (c + i < a.cols) y[c + i] = (T)o[i];
+                if (c + i < a.cols) y[c + i] = el_of<T>(o[i]);
         }
     }
 }

@@ -121,6 +121,19 @@ def test_dequantize(session, dtype, rows, cols):
     assert np.array_equal(np.isnan(got), nan) and np.array_equal(got[~nan], want[~nan])
 
 
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("rows,cols", [(3, 32), (5, 257)])
+def test_dequantize_keeps_the_sign_of_zero(session, dtype, rows, cols):
+    """Code 8 is -0 under every scale but 255, in every column."""
+    codes = (np.indices((rows, cols)).sum(0) % 3 > 0) * 8
+    e8 = np.broadcast_to(np.array([0, 1, 127, 254, 90], np.uint8)[:rows, None], (rows, (cols + 31) // 32))
+    want, _ = bits(dtype, np.where(codes == 8, -0.0, 0.0))
+    with Bufs(session.b) as d:
+        y = d.up(np.full((rows, cols), 7, want.dtype))
+        assert session.b.hip_mxfp4_dequantize_dev(0, d.up(pack(codes)), d.up(e8), rows, cols, y, dtype)
+        assert np.array_equal(d.down(y, want.nbytes, np.uint8), want.view(np.uint8).ravel())
+
+
 def test_no_rows(session):
     assert session.b.hip_mxfp4_quantize_dev(0, None, 0, 0, 8, None, None)
     assert session.b.hip_mxfp4_dequantize_dev(0, None, None, 0, 8, None, 0)

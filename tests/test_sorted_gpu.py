@@ -194,6 +194,21 @@ def test_combine_grad(session, dtype, T, E, K, D):
         assert (gy[~seen] == 7).all()
 
 
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("D", [5, 64, 999])
+def test_combine_grad_keeps_the_sign_of_zero(session, dtype, D):
+    """w dout of zeros of either sign, in every column."""
+    b, (T, K) = session.b, (3, 2)
+    v = np.where(np.indices((T, D)).sum(0) % 3 > 0, -0.0, 0.0)
+    dout, _ = bits(dtype, v)
+    w = np.array([[1, -1], [-0.5, 0.25], [2, 3]], np.float32)
+    want, _ = bits(dtype, (v[:, None] * w[:, :, None]).reshape(T * K, D))
+    with Bufs(b) as d:
+        dys = d.up(np.full((T * K, D), 7, want.dtype))
+        assert b.hip_combine_grad_dev(0, None, dtype, d.up(np.arange(T * K, dtype=np.int32)), d.up(w), d.up(dout), T, K, T * K, D, dys, None)
+        assert np.array_equal(d.down(dys, want.nbytes, np.uint8), want.view(np.uint8).ravel())
+
+
 def test_gradients_are_the_derivatives(session):
     """<dout, out> is linear in ys, in w, and (through dispatch) in x: the calls' own
     differences against the gradients, f32 roundings of both sides allowed for."""
