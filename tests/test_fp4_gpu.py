@@ -47,8 +47,8 @@ def check_quantize(b, x, dtype):
     assert np.array_equal(q, pack(np.where(bad, 0, codes)))
 
 
-# around the octets (8), a block (32), a lane's last octet, rows of one workgroup
-# (256 octets) and beyond
+# around a lane's elements (4 of f32, 8 of the others), a block (32), a lane's last ones, rows of
+# one workgroup's step (1024 and 2048 columns) and beyond
 @pytest.mark.parametrize("dtype", [0, 1, 2])
 @pytest.mark.parametrize("rows,cols", [(1, 1), (3, 2), (2, 3), (6, 4), (3, 5), (2, 7), (5, 8), (4, 9), (40, 12), (70, 31), (3, 32), (9, 33), (2, 63),
                                        (5, 100), (37, 999), (6, 1028), (300, 64), (3, 2048), (2, 2050), (2, 4111), (1, 16500), (1030, 6403)])
@@ -132,6 +132,47 @@ def test_dequantize_keeps_the_sign_of_zero(session, dtype, rows, cols):
         y = d.up(np.full((rows, cols), 7, want.dtype))
         assert session.b.hip_mxfp4_dequantize_dev(0, d.up(pack(codes)), d.up(e8), rows, cols, y, dtype)
         assert np.array_equal(d.down(y, want.nbytes, np.uint8), want.view(np.uint8).ravel())
+
+
+@pytest.mark.parametrize("dtype", [1, 2])
+def test_dequantize_past_the_caches(session, dtype):
+    """More than 128 MiB of 16-bit output, stored past the caches, of an odd width."""
+    rng = np.random.default_rng(dtype)
+    rows, cols = 9001, 7501
+    q4, e8 = rand_mxfp4(rng, rows, cols, 100, 140)
+    with Bufs(session.b) as d:
+        y = d.up(np.full(rows * cols + 2, 7, np.uint16))
+        assert session.b.hip_mxfp4_dequantize_dev(0, d.up(q4), d.up(e8), rows, cols, y, dtype)
+        got = d.down(y, rows * cols + 2, np.uint16)
+    assert (got[-2:] == 7).all()
+    r = np.append(np.arange(0, rows, 29), rows - 1)
+    with np.errstate(over="ignore"):
+        want, _ = bits(dtype, deq_mxfp4(q4[r], e8[r], cols))
+    assert np.array_equal(got[:-2].reshape(rows, cols)[r], want.view(np.uint16))
+
+
+def test_quantize_at_any_address(session):
+    """Rows from any element on and bytes from any byte on: what aligned ones give."""
+    b, (rows, cols) = session.b, (70, 999)
+    rng = np.random.default_rng(15)
+    for dtype in (0, 1, 2):
+        raw, _ = bits(dtype, rng.standard_normal((rows, cols)))
+        q, e = quantize(b, raw, dtype)
+        for k in (1, 3):
+            with Bufs(b) as d:
+                x, q4, e8 = (d.up(np.full(n + 32, 0xA5, np.uint8)) + k * m for n, m in ((raw.nbytes, raw.itemsize), (q.nbytes, 1), (e.nbytes, 1)))
+                d.put(x, raw)
+                assert b.hip_mxfp4_quantize_dev(0, x, dtype, rows, cols, q4, e8)
+                assert np.array_equal(d.down(q4, q.shape, np.uint8), q) and np.array_equal(d.down(e8, e.shape, np.uint8), e)
+                ends = [p + n for p, n in ((q4, q.nbytes), (e8, e.nbytes))]
+                y, y0 = (d.up(np.full(raw.nbytes + 32, 0xA5, np.uint8)) + n * raw.itemsize for n in (k, 0))
+                assert b.hip_mxfp4_dequantize_dev(0, q4, e8, rows, cols, y, dtype)
+                assert b.hip_mxfp4_dequantize_dev(0, d.up(q), d.up(e), rows, cols, y0, dtype)
+                assert np.array_equal(d.down(y, raw.nbytes, np.uint8), d.down(y0, raw.nbytes, np.uint8))
+                for p in (*ends, y + raw.nbytes):
+                    assert (d.down(p, 4, np.uint8) == 0xA5).all()
+                for p in (q4 - 1, e8 - 1, y - 1):
+                    assert d.down(p, 1, np.uint8)[0] == 0xA5
 
 
 def test_no_rows(session):
@@ -403,6 +444,44 @@ def test_swiglu_extremes(session, monkeypatch, pin):
     finally:
         session.free(g)
         session.free(u)
+
+
+@pytest.mark.parametrize("S,I,O", [(1, 700, 90), (3, 333, 33), (40, 700, 90), (300, 257, 530), (100, 7000, 300)])
+def test_products_at_any_address(session, S, I, O):
+    """Rows and results from any float on: the bits of those that start at 16 bytes, nothing beside them written."""
+    rng = np.random.default_rng(S)
+    b, x = session.b, act(rng, S, I)
+    off = np.array([0, S // 3, S], np.int32)
+    with Experts(session, rng, 2, I, O, True) as ex:
+        h = ex.h[0][0]
+        want, wanted = matmul_a4(b, h, x, O), ex.run(x, off, S)[:S]
+        for k in (1, 3):
+            with Bufs(b) as d:
+                px, d_off = d.up(np.zeros(S * I + 8, np.float32)) + 4 * k, d.up(np.zeros(8, np.int32)) + 4 * k
+                d.put(px, x)
+                d.put(d_off, off)
+                for one in (True, False):
+                    y = d.up(np.full(S * O + 8, 7, np.float32)) + 4 * k
+                    assert b.hip_fp4_matmul_a4_dev(h, y, px, S) if one else b.hip_experts_a4_dev(ex.set, y, px, S, None, 1, d_off, S)
+                    got = d.down(y - 4 * k, S * O + 8)
+                    assert np.array_equal(got[k:k + S * O].reshape(S, O), want if one else wanted)
+                    assert (got[:k] == 7).all() and (got[k + S * O:] == 7).all()
+
+
+def test_expert_pairs_past_the_caches(session):
+    """Pairs with more than 128 MiB of results, stored past the caches: a sample of the rows, and those behind the last."""
+    rng = np.random.default_rng(16)
+    E, I, O, counts = 3, 64, 8200, [1500, 0, 2700]
+    off = np.concatenate([[0], np.cumsum(counts)])
+    N = int(off[-1])
+    x = act(rng, N, I)
+    with Experts(session, rng, E, I, O, True) as ex:
+        got = ex.run(x, off, N)
+        assert (got[N:] == 7).all()
+        for e in (0, 2):
+            r = np.append(np.arange(off[e], off[e + 1], 31), off[e + 1] - 1)
+            v, tol = ex.ref(e, mx_quant(x[r])[2])
+            assert (np.abs(got[r] - v) <= tol).all()
 
 
 @pytest.mark.parametrize("pin", ["few", "many"])

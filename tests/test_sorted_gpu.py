@@ -111,6 +111,91 @@ def test_dispatch_many_workgroups(session):
     assert np.array_equal(pos[:T * K], want)
 
 
+@pytest.mark.parametrize("T,E,K", [(5000, 1, 1), (9000, 1, 2), (5000, 2, 1), (3000, 2, 3)])
+def test_dispatch_to_one_or_two_experts(session, T, E, K):
+    """Many selections of few experts: hundreds of threads add up one expert's counts."""
+    rng = np.random.default_rng(T + E + K)
+    check_dispatch(session.b, *routing(rng, T, E, K), E, rng.integers(0, 256, (T, 20)).astype(np.uint8))
+    check_dispatch(session.b, *routing(rng, T, E, K, False, False, False), E, None)
+
+
+# past 256 workgroups of 1024 selections, where runs get longer, and past the 2^26 that are divided by a product
+@pytest.mark.parametrize("T,E,K", [(87400, 33, 3), (7_500_000, 100, 9)])
+def test_dispatch_of_long_runs(session, T, E, K):
+    rng = np.random.default_rng(K)
+    idx = rng.integers(-1, E, (T, K), dtype=np.int32)
+    mask = (rng.random(T) >= 0.1).astype(np.uint8)
+    off, src, pos, _ = dispatch(session.b, idx, None, mask, E, None)
+    key = np.where(mask[:, None] != 0, idx, -1).ravel()
+    counts = np.bincount(key + 1, minlength=E + 1)[1:]
+    n = int(counts.sum())
+    assert np.array_equal(off[:E + 1], np.concatenate([[0], np.cumsum(counts)])) and (off[E + 1:] == 77).all()
+    # by expert, ascending within one, each live selection once
+    assert np.array_equal(key[src[:n]], np.repeat(np.arange(E, dtype=np.int32), counts)) and (src[n:] == 77).all()
+    up = np.diff(src[:n]) > 0
+    up[off[1:E][(off[1:E] > 0) & (off[1:E] < n)] - 1] = True
+    assert up.all()
+    pos = pos[:T * K]
+    assert np.array_equal(pos[src[:n]], np.arange(n, dtype=np.int32)) and ((pos >= 0) == (key >= 0)).all() and pos.min() == -1
+
+
+@pytest.mark.parametrize("T", [60, 1500])
+def test_dispatch_at_any_address(session, T):
+    """Buffers that start off 16 bytes: the rows at any byte, the rest at any four (the mask at any)."""
+    rng = np.random.default_rng(T)
+    b, (E, K, rb) = session.b, (20, 4, 4111)
+    idx, keff, mask = routing(rng, T, E, K)
+    x = rng.integers(0, 256, (T, rb)).astype(np.uint8)
+    ro, rs, rp = plan(idx, keff, mask, E)
+    n = len(rs)
+
+    def at(d, a, shift):
+        p = d.up(np.full(a.nbytes + 32, 0x5A, np.uint8))
+        d.put(p + shift, a)
+        return p + shift
+
+    for shift in (1, 7, 15):
+        with Bufs(b) as d:
+            i4 = [at(d, v, 4 * (1 + (shift + k) % 3)) for k, v in enumerate((idx, keff, np.full(E + 1, 77, np.int32), np.full(T * K, 77, np.int32),
+                                                                          np.full(T * K, 77, np.int32)))]
+            xs = at(d, np.full((T * K, rb), 0x5A, np.uint8), 16 - shift)
+            assert b.hip_dispatch_dev(0, i4[0], i4[1], at(d, mask, shift), T, E, K, at(d, x, shift), rb, *i4[2:], xs)
+            assert np.array_equal(d.down(i4[2], E + 1, np.int32), ro) and np.array_equal(d.down(i4[4], (T, K), np.int32), rp)
+            src, got = d.down(i4[3], T * K, np.int32), d.down(xs, (T * K, rb), np.uint8)
+            assert np.array_equal(src[:n], rs) and (src[n:] == 77).all()
+            assert np.array_equal(got[:n], x[rs // K]) and (got[n:] == 0x5A).all()
+            assert (d.down(xs + T * K * rb, shift, np.uint8) == 0x5A).all()
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("T,E,K,D", [(33, 100, 6, 999), (16, 16, 8, 1024)])
+def test_combine_at_any_address(session, dtype, T, E, K, D):
+    """Buffers that start at any element: the bits of those that start at 16 bytes, and nothing beside them written."""
+    rng = np.random.default_rng(D + dtype)
+    b = session.b
+    pos, N, ys, _, dout, _, w = sorted_case(rng, dtype, T, E, K, D)
+    es = ys.itemsize
+    res = []
+    for el in (0, 1, 3):
+        with Bufs(b) as d:
+            def at(a, step):
+                p = d.up(np.full(a.nbytes + 32, 7, np.uint8))
+                d.put(p + el * step, a)
+                return p + el * step
+
+            py, pd, pp, pw = at(ys, es), at(dout, es), at(pos, 4), at(w, 4)
+            out, dys, dw = at(np.zeros((T, D), ys.dtype), es), at(np.zeros((N, D), ys.dtype), es), at(np.zeros((T, K), np.float32), 4)
+            assert b.hip_combine_dev(0, py, dtype, pp, pw, T, K, N, D, out)
+            assert b.hip_combine_grad_dev(0, py, dtype, pp, pw, pd, T, K, N, D, dys, dw)
+            res.append([d.down(p, n, np.uint8) for p, n in ((out, T * D * es), (dys, N * D * es), (dw, T * K * 4))])
+            for p, n in ((out, T * D * es), (dys, N * D * es), (dw, T * K * 4)):
+                assert (d.down(p + n, 4, np.uint8) == 7).all()
+                assert el == 0 or (d.down(p - 2, 2, np.uint8) == 7).all()
+    for r in res[1:]:
+        for a, c in zip(res[0], r):
+            assert np.array_equal(a, c)
+
+
 def test_dispatch_no_rows(session):
     b = session.b
     with Bufs(b) as d:
