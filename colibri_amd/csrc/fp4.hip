@@ -244,8 +244,8 @@ template <int FORM> __global__ __launch_bounds__(256) void coli_fp4_prep(QuantAr
 // swiglu_out on the hardware's exp2 and reciprocal (a step of each, beside products whose
 // sums carry more): exp(-g) = 2^h (1 + l ln 2) with h + l = -g log2(e) in two parts, right
 // to 5 x 2^-24 for gates from COLI_FP4_LOW up. A third of the instructions of expf and the
-// division, which a short product shows (16384 rows through 8 pairs of 2048 x 1024: 90 us, 77
-// so and with the weights requested ahead of the rows).
+// division, which a short product shows (16384 rows through 8 pairs of 2048 x 1024 68.0 -> 61.8
+// us, through 64 pairs 98.0 -> 89.3).
 // LOW: gates below it too, whose sigmoid is exp(g) in f32 and (from -87.34 down) below the
 // normal range, where the reciprocal is 0: 2^n 2^f in two steps, the up scaled by 2^-64
 // meanwhile, so that nothing is lost that the result can hold. Where 2^-64 takes a small up out of
@@ -737,8 +737,9 @@ static int lanes_log2(int cols, int V) {   // lanes of a row, V columns each: a 
 // Workgroups for rows of `cols` columns: groups of rows, and a row of more than one step
 // of 256 lanes by several: where groups are few, up to 2048 in all (8192 rows of 7168 bf16:
 // 55 us whole, 59 in pieces), and where f32 rows are many and more than six steps long
-// (operands and their product: 2048 rows of 14336 61 -> 57 us, 3000 of 7168 52.5 -> 51.8;
-// but 8000 of 4096 51 -> 52.6, 600 of 14336 30 -> 33).
+// (operands and their product through 1024 outputs: 2048 rows of 14336 61 -> 57 us, 3000 of
+// 7168 52.5 -> 51.8; but 8000 of 4096 51 -> 52.6, 600 of 14336 30 -> 33. At the step, rows of
+// 14336 and back: 1024 of them, in two pieces, 28.0, 1025 in eight 29.6, whole 30.1).
 static unsigned mx_grid(int rows, int cols, int V, int lpr, int *chunks) {
     const unsigned groups = (unsigned)((rows + (256 >> lpr) - 1) / (256 >> lpr)), steps = (unsigned)((cols + (V << lpr) - 1) / (V << lpr));
     const unsigned most = V == 4 && groups > 1024 && steps > 6 ? (8192 + groups) / groups : 2048 / groups;

@@ -5,9 +5,9 @@
 // then xs[r] = x[src[r] / K]. combine: out[t] = sum_k w[t, k] ys[pos[t, k]] in f32,
 // k ascending. Its gradient: dys[pos[t, k]] = w[t, k] dout[t], dw[t, k] = <dout[t],
 // ys[pos[t, k]]>. All are bound by the rows' bytes, the small ones by their launches:
-// 8192 bf16 rows of 7168 to 35000 places 131 us (4.7 TB/s, the rate of a copy; counts and
-// places 11 of them); combine of 32768 such rows 94 us (5.6 TB/s, mostly reads), its gradient
-// 210 (5.0 TB/s); one token's rows 4.5, combine of 16 tokens 4.9, each one launch.
+// 8192 bf16 rows of 7168 to 35000 places 134 us (4.6 TB/s, nearly the rate of a copy; counts
+// and places 11 of them); combine of 32768 such rows 94 us (5.6 TB/s, mostly reads), its
+// gradient 210 (5.0 TB/s); one token's rows 4.7, combine of 16 tokens 5.0, each in one launch.
 #include "coli_hip_host.h"
 #include "coli_rows.h"
 
@@ -314,8 +314,8 @@ struct CombineArgs {
 };
 
 // One row t a workgroup and 256 x VE columns. The loads of up to KB selections are
-// requested together: a place that is not live reads the row of one that is (or
-// row 0) and counts zero, so no load waits behind a branch.
+// requested together: a place that is not live reads row 0 (one past K the last place's
+// row) and counts for nothing, so no load waits behind a branch.
 template <typename T, int VE, int KB, bool NT> __global__ __launch_bounds__(256) void coli_combine(CombineArgs a) {
     const int t = blockIdx.x, c0 = (blockIdx.y * 256 + threadIdx.x) * VE;
     if (c0 >= a.D) return;
@@ -385,9 +385,11 @@ static bool combine_shape_ok(int dtype, int T, int K, int N, int D) {
            (int64_t)T * K <= (1 << 30) && N >= 0 && D >= 1 && D <= (1 << 24);
 }
 
-// ys (and dys) beyond half of the 256 MB cache go past it: combine of 32768 bf16 rows
-// of 7168 122 -> 117 us, its gradient 185 -> 175; smaller ones may be there still for
-// whoever reads them next.
+// ys (and dys) beyond half of the 256 MB cache go past it: combine of 32768 bf16 rows of 7168
+// 107 -> 94 us. Before and behind its gradient, as a training step has it, 122 -> 94, the
+// gradient itself 185 -> 210 (it no longer finds rows of ys in the cache), the step 418 ->
+// 398. Where half of the rows are live, and so half of N's bytes, the step is 256 -> 259.
+// Smaller ones may be there still for whoever reads them next.
 template <typename T, int VE> static void combine_launch(const CombineArgs &a, bool grad, hipStream_t st) {
     const bool nt = VE > 1 && (size_t)a.N * a.D * sizeof(T) > ((size_t)128 << 20);
     if (grad) {

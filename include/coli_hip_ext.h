@@ -228,7 +228,7 @@ int coli_hip_dispatch_dev(int device, const int *idx, const int *keff, const uns
 /* out[t] = sum_k w[t, k] ys[pos[t, k]] over the places pos [T, K] within 0..N-1
  * (others count for nothing, whatever their weight); w [T, K] f32 (NULL: ones), ys
  * [N, D] and out [T, D] of dtype 0 f32, 1 fp16, 2 bf16. Summed in f32 in the order
- * of k, rounded once. Rows of ys that no place names are not looked at. */
+ * of k, rounded once. Rows of ys that no place names count for nothing. */
 int coli_hip_combine_dev(int device, const void *ys, int dtype, const int *pos, const float *w, int T, int K, int N,
                          int D, void *out);
 /* Its gradients from dout [T, D]: dys[pos[t, k]] = w[t, k] dout[t] (rows that no
@@ -276,8 +276,8 @@ void coli_hip_experts_free(ColiHipExperts *experts);
 /* y[r] = W_e Q(x row of r) for the sorted rows offsets[e] <= r < offsets[e + 1] (ascending;
  * taken within 0..N) of y [N, O]; other rows of y are left as they were. The row is
  * x[src[r] / K] with src (of coli_hip_dispatch_dev: the rows need not be copied), x[r]
- * without; x is [rows, I], a row outside it counts as zeros. N and rows up to 2^23;
- * without sorted rows (N 0) nothing is done. */
+ * without; x is [rows, I], rows at least 1, a row outside it counts as zeros. N and rows up
+ * to 2^23; without sorted rows (N 0) nothing is done. */
 int coli_hip_experts_a4_dev(ColiHipExperts *experts, float *y, const float *x, int rows, const int *src, int K,
                             const int *offsets, int N);
 

@@ -267,6 +267,28 @@ def test_matmul_one_hot(session):
         session.free(h)
 
 
+@pytest.mark.parametrize("pin", ["few", "many"])
+def test_matmul_of_every_scale(session, monkeypatch, pin):
+    """One block of weights under each scale byte from 1 to 254, rows of one power of two that brings the product
+    to 2^-140 .. 2^120: exactly, below f32's normal range too."""
+    monkeypatch.setenv("COLI_HIP_FP4", pin)
+    rng = np.random.default_rng(17)
+    O, nb = 32, 254
+    I = nb * 32
+    q4 = rng.integers(0, 256, (O, I // 2), dtype=np.uint8)
+    h = session.upload_mxfp4(q4, np.tile(np.arange(1, 255, dtype=np.uint8), (O, 1)), I, O)
+    codes = E2M1[nibbles(q4, I)][:, ::32].T
+    try:
+        for p in (-140, -126, -60, 0, 60, 120):
+            e = p - (np.arange(1, 255) - 127.0)
+            ok = (e >= -127) & (e <= 126)
+            x = np.zeros((nb, I), np.float32)
+            x[np.flatnonzero(ok), 32 * np.flatnonzero(ok)] = 2.0 ** e[ok]
+            assert np.array_equal(matmul_a4(session.b, h, x, O), np.where(ok[:, None], codes * 2.0 ** p, 0).astype(np.float32)), p
+    finally:
+        session.free(h)
+
+
 def test_matmul_wide_ranges(session):
     """Scales from 2^-60 to 2^60 on both sides, zero blocks, a zero row."""
     rng = np.random.default_rng(4)
